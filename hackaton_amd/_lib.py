@@ -73,6 +73,19 @@ SIGNATURES = {
                                    _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p]),
     "va_pack_rows": (ctypes.c_int, [_p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _i32, _p]),
     "va_unpack_rows": (ctypes.c_int, [_p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _i32, _p]),
+    "va_paged_plan_words": (ctypes.c_int, [_i32, _i64, _i32, _i32, _i32, _i32, _pi64]),
+    "va_paged_plan": (ctypes.c_int, [_p, _p, _i32, _i64, _i32, _i32, _i32, _i32, _p, _i64, _p]),
+    "va_paged_append": (ctypes.c_int, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _p, _i32,
+                                       _i32, _p, _p, _p, _i64, _i64, _i32, _i32, _i64, _i32, _i32,
+                                       _i32, _i32, _i32, _p]),
+    "va_paged_attention_workspace": (ctypes.c_int, [_i32, _i64, _i32, _i32, _i32, _i32, _pi64]),
+    "va_paged_attention": (ctypes.c_int, [_p, _p, _p, _i64, _i64, _i32, _i32, _p, _i32, _p, _i32,
+                                          _i64, _i32, _i32, _i32, _f32, _i32, _p, _p, _i64, _p]),
+    "va_pages_scratch_words": (ctypes.c_int, [_i32, _i32, _pi64]),
+    "va_pages_remap": (ctypes.c_int, [_p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _p, _p, _i32,
+                                      _i32, _p, _p, _p, _p, _p, _i64, _p]),
+    "va_pages_compact": (ctypes.c_int, [_p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _i32, _i32,
+                                        _p, _p, _p, _p, _i64, _p]),
     "va_probe_mfma": (ctypes.c_int, [_i32, _i32, _i32, _p, _p]),
     "va_probe_copy": (ctypes.c_int, [_p, _p, _i64, _i32, _p]),
 }

@@ -15,7 +15,7 @@ LIB_NAME = "libvarlen_attn.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 
 SOURCES = ["attn_fwd.hip", "attn_bwd.hip", "rope.hip", "plan_device.hip", "noalloc.hip", "probe.hip",
-           "api.cpp", "plan.cpp"]
+           "paged_attn.hip", "paged_cache.hip", "api.cpp", "paged_api.cpp", "plan.cpp"]
 ARCH = os.environ.get("VA_OFFLOAD_ARCH", "gfx950")
 
 # -packed-fp32-ops off: no packed fp32 VALU instructions are generated.

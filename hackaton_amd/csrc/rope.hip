@@ -11,6 +11,7 @@
 // row_map_kernel    the inverse of (b_idx, t_idx): which token, if any, a padded row holds.
 // pack_rows_kernel  (B, H, T, D) <-> (N, H*D) gather / scatter of whole 16-byte chunks.
 // unpack_rows_kernel  the scatter over a row map: every padded row written once, zeros included.
+// rope_paged_kernel the rotation of a step's new rows, keys and values into the pages of a cache.
 //
 // Access pattern: one wave per token. A (token, head) row of D = 128 elements is handled by 8
 // consecutive lanes; lane j of the row takes elements [8j, 8j + 8) of the first half and the
@@ -24,6 +25,7 @@
 
 #include "va_common.h"
 #include "va_kernels.h"
+#include "va_paged.h"
 
 namespace va {
 
@@ -279,6 +281,59 @@ __global__ __launch_bounds__(kRopeThreads) void rope_fwd_padded_kernel(RopeArgs 
   }
 }
 
+// A step's new rows into a paged cache: one wave per row, as above; q rows are written packed, k and v
+// rows where the page table says. A row without a place (padding, a position before the sequence,
+// past the tables or the table row, a page outside the pool) writes no key or value.
+template <int IN, int OUT>
+__global__ __launch_bounds__(kRopeThreads) void rope_paged_kernel(PagedAppendArgs a) {
+  const TokenLanes tl = token_lanes(a.n_tokens);
+  if (!tl.valid) return;
+  const int c0 = 8 * tl.j, seq = a.seq[tl.pid], pos = a.pos[tl.pid];
+  const bool placed = seq >= 0 && pos >= 0 && (a.cos_rows == 0 || pos < a.cos_rows);
+  int page = -1;
+  const int at = pos >> a.pool.page_shift, ps = 1 << a.pool.page_shift;
+  if (placed && at < a.pool.table_width)
+    page = a.pool.table[(long)seq * a.pool.table_width + at];
+  const bool in_pool = page >= 0 && page < a.pool.n_pages;
+  Tables tb;
+  if (placed) {
+    const long cb = seq * a.cos_batch_stride + pos * a.cos_seq_stride + tl.pid * a.cos_token_stride;
+    load_table8(a.cos, cb + c0, tb.cs1);
+    load_table8(a.cos, cb + HALF + c0, tb.cs2);
+    load_table8(a.sin, cb + c0, tb.sn1);
+    load_table8(a.sin, cb + HALF + c0, tb.sn2);
+  }
+  const int slots = a.heads + 2 * a.kv_heads;
+  for (int s = tl.r0; s < slots; s += 8) {
+    const bool is_q = s < a.heads, is_v = s >= a.heads + a.kv_heads;
+    const int head = is_q ? s : (is_v ? s - a.heads - a.kv_heads : s - a.heads);
+    if (!is_q && !in_pool) continue;
+    float x1[8], x2[8], y1[8], y2[8];
+    if (placed) {
+      const gcvoid x = pick3(is_q, is_v, a.q, a.k, a.v);
+      const long row = (tl.pid * (is_q ? uniform(a.heads) : uniform(a.kv_heads)) + head) * D;
+      cvt8<IN>(load_raw8<IN>(x, row + c0), x1);
+      cvt8<IN>(load_raw8<IN>(x, row + HALF + c0), x2);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float r1 = 0.f, r2 = 0.f;
+      if (placed) {
+        rope_rotate(x1[e], x2[e], tb.cs1[e], tb.cs2[e], tb.sn1[e], tb.sn2[e], r1, r2);
+        if (is_v) r1 = x1[e], r2 = x2[e];
+      }
+      y1[e] = r1;
+      y2[e] = r2;
+    }
+    const gvoid y = pick3(is_q, is_v, a.q_out, a.k_pages, a.v_pages);
+    const long stride = is_v ? uniform(a.pool.v_stride) : uniform(a.pool.k_stride);
+    const long row = is_q ? (tl.pid * a.heads + head) * D
+                          : page * stride + ((long)head * ps + (pos & (ps - 1))) * D;
+    store8<OUT>(y, row + c0, y1);
+    store8<OUT>(y, row + HALF + c0, y2);
+  }
+}
+
 // Backward, inputs: x0 = dq, x1 = dk, x2 = dv in `layout`, with `heads` heads for dq and
 // (expand ? heads : kv_heads) heads for dk/dv. Outputs y0 (N, heads*D), y1/y2 (N, kv_heads*D).
 // Row `slot`'s gradient (its first copy when expanded).
@@ -473,6 +528,19 @@ hipError_t launch_rope(const RopeArgs& a, bool fwd) {
 
 hipError_t launch_rope_fwd(const RopeArgs& a) { return launch_rope(a, true); }
 hipError_t launch_rope_bwd(const RopeArgs& a) { return launch_rope(a, false); }
+
+hipError_t launch_paged_append(const PagedAppendArgs& a) {
+  const dim3 grid((unsigned)((a.n_tokens + kTokensPerGroup - 1) / kTokensPerGroup));
+  const auto kernel =
+      a.out_dtype == kF16 ? (a.in_dtype == kF16    ? rope_paged_kernel<kF16, kF16>
+                             : a.in_dtype == kBF16 ? rope_paged_kernel<kBF16, kF16>
+                                                   : rope_paged_kernel<kF32, kF16>)
+                          : (a.in_dtype == kF16    ? rope_paged_kernel<kF16, kBF16>
+                             : a.in_dtype == kBF16 ? rope_paged_kernel<kBF16, kBF16>
+                                                   : rope_paged_kernel<kF32, kBF16>);
+  hipLaunchKernelGGL(kernel, grid, dim3(kRopeThreads), 0, a.stream, a);
+  return hipGetLastError();
+}
 
 hipError_t launch_pack_rows(const void* src, void* dst, const int32_t* b_idx, const int32_t* t_idx,
                             int64_t n_tokens, int heads, int seq, int row_bytes, int mode,

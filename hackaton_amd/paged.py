@@ -1,0 +1,442 @@
+"""A paged key/value cache for answering with the model that `packed_attention` trains: the new
+tokens of every sequence of a step are appended to pages and attend to them, one token each, a few
+drafted ones or a prompt's chunk, all in one call. Hand-written gfx950 kernels through the C ABI; the
+reference trains only and has no counterpart.
+
+    paged_plan(page_table, q_lengths, kv_lengths, n_tokens, heads, kv_heads, page_size)
+    paged_append(q, k, v, cos, sin, k_pages, v_pages, plan)
+    paged_attention(query, k_pages, v_pages, plan, scale)
+    remap_pages(pages, table, lengths, refs, parents, new_lengths)
+    compact_pages(pages, table, lengths, refs)
+    PagedCache       a pool, its page tables and the calls above on them
+
+Pages hold `page_size` rows (a power of two, 16 to 256) of every key/value head: one layer's keys are
+(n_pages, kv_heads, page_size, 128). Row t of a sequence lies in page `page_table[sequence, t //
+page_size]`, row `t % page_size`; entries outside the pool name no page. Lengths, tables and counts are
+int32 and stay on the GPU: no call reads them back, so a captured step follows them. None of the calls
+has a backward.
+"""
+
+import ctypes
+import functools
+
+import torch
+
+from . import _lib
+from ._lib import check, lib
+from .attention import _DTYPES, HEAD_DIM, _attn_dtype, _rope_strides, _stream, _tables
+
+PAGE_SIZES = (16, 32, 64, 128, 256)
+MAX_SEQUENCES = 8192  # of one step
+
+
+def _no_grad(*tensors):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError("the paged cache has no backward: call it under torch.no_grad() or "
+                           "torch.inference_mode()")
+
+
+def _one_device(*tensors):
+    device = tensors[0].device
+    for t in tensors:
+        if not t.is_cuda:
+            raise ValueError(f"the paged cache lives on the GPU only: got a tensor on {t.device}")
+        if t.device != device:
+            raise ValueError(f"tensors on {device} and {t.device}")
+    return device
+
+
+def _on_device(fn):
+    """Run `fn` with the device of its tensors current (launches and allocations go there)."""
+
+    @functools.wraps(fn)
+    def call(*args, **kwargs):
+        for t in args:
+            if isinstance(t, torch.Tensor):
+                if t.is_cuda and t.device.index != torch._C._cuda_getDevice():
+                    with torch.cuda.device(t.device):
+                        return fn(*args, **kwargs)
+                break
+        return fn(*args, **kwargs)
+
+    return call
+
+
+def _page_size(page_size):
+    if page_size not in PAGE_SIZES:
+        raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
+    return int(page_size)
+
+
+def _int32(name, t, *shape):
+    if t.dtype != torch.int32 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor, got {t.dtype}, "
+                         f"strides {t.stride()}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
+
+
+def _lengths(name, lengths, n_seqs, device):
+    """Lengths of every sequence as an int32 device tensor, from one or from a host list."""
+    if not isinstance(lengths, torch.Tensor):
+        lengths = torch.tensor([int(x) for x in lengths], dtype=torch.int32, device=device)
+    lengths = lengths.reshape(-1)
+    if lengths.dtype.is_floating_point or lengths.dtype == torch.bool:
+        raise ValueError(f"{name} must be whole numbers, got {lengths.dtype}")
+    if lengths.device != device:
+        raise ValueError(f"{name} on {lengths.device}, page_table on {device}")
+    if lengths.numel() != n_seqs:
+        raise ValueError(f"{lengths.numel()} {name} for {n_seqs} page table rows")
+    return lengths.to(torch.int32).contiguous()
+
+
+def _check_host_lengths(q_lengths, kv_lengths, n_tokens, most):
+    """Host lists are checked before anything runs; device lengths cannot be without a read."""
+    q_host = None if isinstance(q_lengths, torch.Tensor) else [int(x) for x in q_lengths]
+    kv_host = None if isinstance(kv_lengths, torch.Tensor) else [int(x) for x in kv_lengths]
+    if q_host is not None:
+        if min(q_host, default=0) < 0:
+            raise ValueError("q_lengths must not be negative")
+        if sum(q_host) > n_tokens:
+            raise ValueError(f"q_lengths sum to {sum(q_host)}, the step has {n_tokens} rows")
+    if kv_host is not None and (min(kv_host, default=0) < 0 or max(kv_host, default=0) > most):
+        raise ValueError(f"kv_lengths must lie in [0, {most}], what a page table row can name")
+    if q_host is not None and kv_host is not None:
+        if any(q > kv for q, kv in zip(q_host, kv_host)):
+            raise ValueError("kv_lengths count the new tokens too: q_lengths may not exceed them")
+
+
+@functools.lru_cache(maxsize=256)
+def _plan_sizes(n_seqs, n_tokens, heads, kv_heads, page_size, width):
+    """(int32 words of a plan, workspace bytes of an attention over it)."""
+    words, nbytes = ctypes.c_int64(), ctypes.c_int64()
+    sizes = (n_seqs, n_tokens, heads, kv_heads, page_size, width)
+    check(lib().va_paged_plan_words(*sizes, ctypes.byref(words)), "va_paged_plan_words")
+    check(lib().va_paged_attention_workspace(*sizes, ctypes.byref(nbytes)),
+          "va_paged_attention_workspace")
+    return words.value, nbytes.value
+
+
+class PagedPlan:
+    """A step's rows and work list, shared by all of its layers: made by `paged_plan`. It keeps the
+    page table and follows its entries as they are when a call runs; the lengths were read when the
+    plan was made (a captured plan reads them again in every replay)."""
+
+    __slots__ = ("page_table", "words", "n_tokens", "n_seqs", "width", "heads", "kv_heads",
+                 "page_size", "workspace_bytes", "_stream")
+
+    def _rows(self, which):
+        rows = -(-self.n_tokens // 4) * 4
+        at = -(-(self.n_seqs + 1) // 4) * 4 + which * rows
+        return self.words[at:at + self.n_tokens]
+
+    @property
+    def sequences(self):
+        """(n_tokens) int32: the sequence of every row, -1 for padding."""
+        return self._rows(0)
+
+    @property
+    def positions(self):
+        """(n_tokens) int32: the position of every row in its sequence, -1 for padding."""
+        return self._rows(1)
+
+    def _use(self):
+        """The plan's memory is used on the current stream: not handed out again before that is done."""
+        stream = _stream()
+        if stream != self._stream and not torch._C._cuda_isCurrentStreamCapturing():
+            current = torch.cuda.current_stream()
+            self.words.record_stream(current)
+            self.page_table.record_stream(current)
+        return stream
+
+
+@_on_device
+def paged_plan(page_table, q_lengths, kv_lengths, n_tokens, heads, kv_heads, page_size):
+    """The plan of a step: `q_lengths[s]` new tokens of every sequence (packed rows, one sequence
+    after the other, `n_tokens` rows in all; rows behind the last sequence are padding) and
+    `kv_lengths[s]` cached tokens with the new ones included. Both are host lists or device tensors;
+    `page_table` is (sequences, pages per sequence) int32 on the GPU. One launch."""
+    device = _one_device(page_table)
+    if page_table.dim() != 2:
+        raise ValueError(f"page_table must be (sequences, pages), got {tuple(page_table.shape)}")
+    n_seqs, width = page_table.shape
+    _int32("page_table", page_table, n_seqs, width)
+    page_size, n_tokens = _page_size(page_size), int(n_tokens)
+    _check_host_lengths(q_lengths, kv_lengths, n_tokens, width * page_size)
+    plan = PagedPlan()
+    n_words, plan.workspace_bytes = _plan_sizes(n_seqs, n_tokens, heads, kv_heads, page_size, width)
+    q_lengths = _lengths("q_lengths", q_lengths, n_seqs, device)
+    kv_lengths = _lengths("kv_lengths", kv_lengths, n_seqs, device)
+    plan.page_table, plan.n_tokens, plan.n_seqs, plan.width = page_table, n_tokens, n_seqs, width
+    plan.heads, plan.kv_heads, plan.page_size = heads, kv_heads, page_size
+    plan.words = torch.empty(n_words, dtype=torch.int32, device=device)
+    plan._stream = _stream()
+    check(lib().va_paged_plan(q_lengths.data_ptr(), kv_lengths.data_ptr(), n_seqs, n_tokens, heads,
+                              kv_heads, page_size, width, plan.words.data_ptr(), n_words,
+                              plan._stream), "va_paged_plan")
+    return plan
+
+
+def _pages_of(k_pages, v_pages, plan):
+    """(elements from one key page to the next, value page, number of pages) of one layer."""
+    shape = k_pages.shape
+    if v_pages.shape != shape or len(shape) != 4 or tuple(shape[1:]) != (
+            plan.kv_heads, plan.page_size, HEAD_DIM):
+        raise ValueError(f"pages must be (n_pages, {plan.kv_heads}, {plan.page_size}, {HEAD_DIM}), "
+                         f"got {tuple(shape)} and {tuple(v_pages.shape)}")
+    if k_pages.dtype != v_pages.dtype:
+        raise ValueError(f"keys in {k_pages.dtype}, values in {v_pages.dtype}")
+    row = (plan.page_size * HEAD_DIM, HEAD_DIM, 1)
+    strides = []
+    for pages in (k_pages, v_pages):
+        stride = pages.stride()
+        if stride[1:] != row and not (plan.kv_heads == 1 and stride[2:] == row[1:]):
+            raise ValueError(f"every page must be contiguous, got strides {stride}")
+        # (a pool of one page: its stride is free)
+        strides.append(max(stride[0], plan.kv_heads * row[0]) if shape[0] <= 1 else stride[0])
+    return strides[0], strides[1], shape[0]
+
+
+@_on_device
+def paged_append(q, k, v, cos, sin, k_pages, v_pages, plan):
+    """The step's new rows: q (n_tokens, heads * 128), k and v (n_tokens, kv_heads * 128) projections
+    in fp16, bf16 or fp32. Returns q rotated, (n_tokens, heads, 128) in the pages' type; k rotated and
+    v go into `k_pages` / `v_pages` (n_pages, kv_heads, page_size, 128) at the rows' positions, rotated
+    in fp32 and rounded once. cos / sin: (1 or sequences, T, 128) read by position, or (n_tokens, 128)
+    read by row. Rows without a place (padding, positions past the tables or in no page) write
+    nothing; padding and positions outside the cos / sin table give zeros in q."""
+    device = _one_device(q, k, v, cos, sin, k_pages, v_pages, plan.words)
+    _no_grad(q, k, v, k_pages, v_pages)
+    n, heads, kv_heads = plan.n_tokens, plan.heads, plan.kv_heads
+    if (tuple(q.shape) != (n, heads * HEAD_DIM) or tuple(k.shape) != (n, kv_heads * HEAD_DIM)
+            or v.shape != k.shape):
+        raise ValueError(f"projections must be ({n}, {heads} and {kv_heads} * {HEAD_DIM}), got "
+                         f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if not (q.dtype == k.dtype == v.dtype) or q.dtype not in _DTYPES:
+        raise ValueError(f"q, k and v must share a dtype (fp16, bf16 or fp32), got {q.dtype}, "
+                         f"{k.dtype}, {v.dtype}")
+    out_dtype = _attn_dtype(k_pages)
+    k_stride, v_stride, n_pages = _pages_of(k_pages, v_pages, plan)
+    by_row = cos.dim() == 2
+    if by_row and (tuple(cos.shape) != (n, HEAD_DIM) or sin.shape != cos.shape):
+        raise ValueError(f"cos/sin by row must be ({n}, {HEAD_DIM}), got {tuple(cos.shape)}, "
+                         f"{tuple(sin.shape)}")
+    cos, sin = _tables(cos[None] if by_row else cos, sin[None] if by_row else sin)
+    if not by_row and cos.shape[0] not in (1, plan.n_seqs):
+        raise ValueError(f"cos/sin for {cos.shape[0]} sequences, the plan has {plan.n_seqs}")
+    query = torch.empty(n, heads, HEAD_DIM, dtype=k_pages.dtype, device=device)
+    if n == 0:
+        return query
+    if cos.shape[1] == 0:
+        raise ValueError("cos/sin hold no positions")
+    batch, row = (0, 0) if by_row else _rope_strides(cos)
+    q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    check(lib().va_paged_append(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), cos.data_ptr(), sin.data_ptr(), batch, row,
+        HEAD_DIM if by_row else 0, 0 if by_row else cos.shape[1], plan.words.data_ptr(),
+        plan.page_table.data_ptr(), plan.n_seqs, plan.width, query.data_ptr(), k_pages.data_ptr(),
+        v_pages.data_ptr(), k_stride, v_stride, n_pages, plan.page_size, n, heads, kv_heads,
+        HEAD_DIM, _DTYPES[q.dtype], out_dtype, plan._use()), "va_paged_append")
+    return query
+
+
+@_on_device
+def paged_attention(query, k_pages, v_pages, plan, scale):
+    """Every new token attends to its sequence's keys at positions up to its own. query
+    (n_tokens, heads, 128) in the pages' type; returns (n_tokens, heads * 128), zeros for padding and
+    for rows that see no key. Key/value heads are shared by heads / kv_heads query heads each."""
+    _one_device(query, k_pages, v_pages, plan.words)
+    _no_grad(query, k_pages, v_pages)
+    dtype = _attn_dtype(query)
+    if k_pages.dtype != query.dtype:
+        raise ValueError(f"query in {query.dtype}, pages in {k_pages.dtype}")
+    n, heads = plan.n_tokens, plan.heads
+    if tuple(query.shape) != (n, heads, HEAD_DIM):
+        raise ValueError(f"query must be ({n}, {heads}, {HEAD_DIM}), got {tuple(query.shape)}")
+    k_stride, v_stride, n_pages = _pages_of(k_pages, v_pages, plan)
+    query = query.contiguous()
+    out = torch.empty(n, heads * HEAD_DIM, dtype=query.dtype, device=query.device)
+    if n == 0:
+        return out
+    nbytes = plan.workspace_bytes
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=query.device) if nbytes else None
+    check(lib().va_paged_attention(
+        query.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_stride, v_stride, n_pages,
+        plan.page_size, plan.page_table.data_ptr(), plan.width, plan.words.data_ptr(), plan.n_seqs,
+        n, heads, plan.kv_heads, HEAD_DIM, float(scale), dtype, out.data_ptr(),
+        ws.data_ptr() if nbytes else None, nbytes, plan._use()), "va_paged_attention")
+    return out
+
+
+# ------------------------------------------------------------------------------------------------
+# page bookkeeping
+# ------------------------------------------------------------------------------------------------
+def _pool_of(pages):
+    if pages.dim() != 6 or pages.shape[1] != 2 or pages.shape[5] != HEAD_DIM:
+        raise ValueError(f"pages must be (layers, 2, n_pages, kv_heads, page_size, {HEAD_DIM}), got "
+                         f"{tuple(pages.shape)}")
+    if not pages.is_contiguous():
+        raise ValueError(f"pages must be contiguous, got strides {pages.stride()}")
+    _attn_dtype(pages)
+    layers, _, n_pages, kv_heads, page_size, _ = pages.shape
+    return 2 * layers, n_pages, kv_heads, _page_size(page_size)
+
+
+def _state_of(table, lengths, refs, n_pages):
+    if table.dim() != 2:
+        raise ValueError(f"table must be (slots, pages), got {tuple(table.shape)}")
+    slots, width = table.shape
+    _int32("table", table, slots, width)
+    _int32("lengths", lengths, slots)
+    _int32("refs", refs, n_pages)
+    return slots, width
+
+
+@functools.lru_cache(maxsize=64)
+def _scratch_words(slots, n_pages):
+    words = ctypes.c_int64()
+    check(lib().va_pages_scratch_words(slots, n_pages, ctypes.byref(words)),
+          "va_pages_scratch_words")
+    return words.value
+
+
+@_on_device
+def remap_pages(pages, table, lengths, refs, parents=None, new_lengths=None):
+    """The page tables of the next step. Slot i goes on as slot `parents[i]` (None: every slot as
+    itself; outside the table: as nobody), cut to `new_lengths[i]` tokens or grown to them with free
+    pages (None: as long as the parent). One call forks, reorders, frees, enters, cuts back and grows
+    sequences:
+
+        fork i into j       parents[j] = i
+        free j              parents[j] = -1, new_lengths[j] = 0
+        enter n tokens      parents[j] = -1, new_lengths[j] = n
+        grow or cut         new_lengths[i]
+
+    pages (layers, 2, n_pages, kv_heads, page_size, 128); table (slots, pages per slot), lengths
+    (slots) and refs (n_pages: how often each page is held, 0 = free) int32. Returns new (table,
+    lengths, refs, shortfall). Slots share full pages; a part-filled last page stays with the lowest
+    slot that ends in it if nobody else holds it, and the others get a copy of its filled rows, in
+    every layer. Free pages are handed out in ascending order, slot after slot. shortfall (1): 0, or
+    how many pages the pool or the table rows lack, in which case nothing changes."""
+    given = [t for t in (parents, new_lengths) if t is not None]
+    device = _one_device(pages, table, lengths, refs, *given)
+    outer, n_pages, kv_heads, page_size = _pool_of(pages)
+    slots, width = _state_of(table, lengths, refs, n_pages)
+    for name, t in (("parents", parents), ("new_lengths", new_lengths)):
+        if t is not None:
+            _int32(name, t, slots)
+    out = [torch.empty_like(table), torch.empty_like(lengths), torch.empty_like(refs),
+           torch.empty(1, dtype=torch.int32, device=device)]
+    words = _scratch_words(slots, n_pages)
+    scratch = torch.empty(words, dtype=torch.int32, device=device)
+    check(lib().va_pages_remap(
+        pages.data_ptr(), outer, n_pages, kv_heads, page_size, HEAD_DIM, table.data_ptr(),
+        lengths.data_ptr(), refs.data_ptr(), None if parents is None else parents.data_ptr(),
+        None if new_lengths is None else new_lengths.data_ptr(), slots, width,
+        *(t.data_ptr() for t in out), scratch.data_ptr(), words, _stream()), "va_pages_remap")
+    return tuple(out)
+
+
+@_on_device
+def compact_pages(pages, table, lengths, refs):
+    """The live pages (refs > 0) to the front of the pool: the k-th live page at or past their number
+    moves to the k-th free page below it, in every layer. Arguments as for `remap_pages`. Returns
+    new (table, refs, live); live (1): how many pages are in use, all of them below that number."""
+    device = _one_device(pages, table, lengths, refs)
+    outer, n_pages, kv_heads, page_size = _pool_of(pages)
+    slots, width = _state_of(table, lengths, refs, n_pages)
+    out = [torch.empty_like(table), torch.empty_like(refs),
+           torch.empty(1, dtype=torch.int32, device=device)]
+    words = _scratch_words(slots, n_pages)
+    scratch = torch.empty(words, dtype=torch.int32, device=device)
+    check(lib().va_pages_compact(
+        pages.data_ptr(), outer, n_pages, kv_heads, page_size, HEAD_DIM, table.data_ptr(),
+        lengths.data_ptr(), refs.data_ptr(), slots, width, *(t.data_ptr() for t in out),
+        scratch.data_ptr(), words, _stream()), "va_pages_compact")
+    return tuple(out)
+
+
+class PagedCache:
+    """Keys and values of `layers` layers in one pool of `n_pages` pages, and up to `slots` sequences
+    of at most `max_length` tokens in it. State, all on the GPU: `pages`, `table`, `lengths`, `refs`.
+    Every call updates it in place on the current stream, so the calls of one cache belong on one
+    stream or in order across streams, and a captured step replays on the state it finds. A call
+    that lacks pages changes nothing; `check()` reports it."""
+
+    def __init__(self, layers, n_pages, page_size, kv_heads, slots, max_length,
+                 dtype=torch.float16, device="cuda"):
+        self.page_size = _page_size(page_size)
+        width = -(-int(max_length) // self.page_size)
+        self.pages = torch.empty(layers, 2, n_pages, kv_heads, page_size, HEAD_DIM, dtype=dtype,
+                                 device=device)
+        _attn_dtype(self.pages)
+        ints = {"dtype": torch.int32, "device": self.pages.device}
+        self.table = torch.full((slots, width), -1, **ints)
+        self.lengths = torch.zeros(slots, **ints)
+        self.refs = torch.zeros(n_pages, **ints)
+        self.shortfall = torch.zeros(1, **ints)
+
+    @property
+    def slots(self):
+        return self.table.shape[0]
+
+    def keys(self, layer):
+        return self.pages[layer, 0]
+
+    def values(self, layer):
+        return self.pages[layer, 1]
+
+    def _slots(self, values, fill):
+        """One int32 per slot: a device tensor as it is, or `fill` with a host dict's entries."""
+        if values is None or isinstance(values, torch.Tensor):
+            return values
+        out = list(fill)
+        for slot, value in values.items():
+            if not 0 <= slot < self.slots:
+                raise ValueError(f"slot {slot} of {self.slots}")
+            out[slot] = int(value)
+        return torch.tensor(out, dtype=torch.int32, device=self.table.device)
+
+    def remap(self, parents=None, new_lengths=None):
+        """`remap_pages` on the cache's state. parents: (slots) int32 tensor or a dict {slot: parent}
+        (the other slots go on as themselves); new_lengths: (slots) int32 tensor or None."""
+        parents = self._slots(parents, range(self.slots))
+        table, lengths, refs, shortfall = remap_pages(self.pages, self.table, self.lengths,
+                                                      self.refs, parents, new_lengths)
+        self.table.copy_(table)
+        self.lengths.copy_(lengths)
+        self.refs.copy_(refs)
+        torch.maximum(self.shortfall, shortfall, out=self.shortfall)
+
+    def fork(self, source, targets):
+        """Each slot of `targets` goes on as a copy of slot `source` (what it held is given back)."""
+        if not 0 <= source < self.slots:
+            raise ValueError(f"slot {source} of {self.slots}")
+        self.remap({t: source for t in targets})
+
+    def free(self, slots):
+        """The sequences of these slots are given up."""
+        self.remap({s: -1 for s in slots})
+
+    def step(self, q_lengths, n_tokens, heads):
+        """Room for `q_lengths[s]` new tokens of every slot, and the step's plan: `n_tokens` rows in
+        all. Where pages are lacking no slot grows and every row of the plan is padding."""
+        q = _lengths("q_lengths", q_lengths, self.slots, self.table.device).clamp(min=0)
+        before = self.lengths.clone()
+        self.remap(None, before + q)
+        return paged_plan(self.table, self.lengths - before, self.lengths, n_tokens, heads,
+                          self.pages.shape[3], self.page_size)
+
+    def compact(self):
+        """The live pages to the front of the pool; returns their number as a (1) int32 tensor."""
+        table, refs, live = compact_pages(self.pages, self.table, self.lengths, self.refs)
+        self.table.copy_(table)
+        self.refs.copy_(refs)
+        return live
+
+    def check(self):
+        """Raise if a call since the last check lacked pages (reads the GPU)."""
+        lacking = int(self.shortfall)
+        if lacking:
+            self.shortfall.zero_()
+            raise RuntimeError(f"the paged cache lacked {lacking} pages: that call changed nothing")

@@ -4,13 +4,16 @@ attention of the packed rows done by the gfx950 kernels (solution/patches.py:81-
 Calls that carry `packed=(b_idx, t_idx, batch, seq, lengths)` (a padding-free training step, as
 built by solution/packed.py:153-176) take the packed path: the q/k/v projections, then
 `packed_attention` when the rows are right padded (`lengths` is a list), otherwise the padded
-layout with the caller's mask through `qkv_rotate(padded=True)`, SDPA and `pack_rows`. Every
-other call runs the original forward unchanged.
+layout with the caller's mask through `qkv_rotate(padded=True)`, SDPA and `pack_rows`. Calls that
+carry `paged=(cache, plan)` (a serving step over a `PagedCache`: hidden rows of the step's new
+tokens, rotary tables by row) append the rows to the layer's pages and attend to them. Every other
+call runs the original forward unchanged.
 """
 
 import torch
 
 from .attention import pack_rows, packed_attention, qkv_rotate
+from .paged import paged_append, paged_attention
 
 _ORIGINAL = {}
 
@@ -25,7 +28,11 @@ def patch_qwen2_attention():
 
     def forward(self, hidden_states, position_embeddings, attention_mask, past_key_values=None,
                 **kwargs):
-        packed = kwargs.pop("packed", None)
+        packed, paged = kwargs.pop("packed", None), kwargs.pop("paged", None)
+        if paged is not None:
+            if packed is not None:
+                raise ValueError("a call is either packed or paged")
+            return _paged_forward(self, hidden_states, position_embeddings, *paged), None
         if packed is None:  # an ordinary call (generation, eval, padded batches): unchanged
             return original(self, hidden_states, position_embeddings, attention_mask,
                             past_key_values, **kwargs)
@@ -48,6 +55,19 @@ def patch_qwen2_attention():
         return self.o_proj(pack_rows(attn, b_idx, t_idx)), None
 
     cls.forward = forward
+
+
+def _paged_forward(layer, hidden_states, position_embeddings, cache, plan):
+    """The layer's rows of a serving step, (N, hidden) or (1, N, hidden): projections, append to the
+    layer's pages, attention over them, output projection."""
+    rows = hidden_states.reshape(-1, hidden_states.shape[-1])
+    cos, sin = (x.reshape(-1, x.shape[-1]) for x in position_embeddings)
+    keys, values = cache.keys(layer.layer_idx), cache.values(layer.layer_idx)
+    k, v = layer.k_proj(rows), layer.v_proj(rows)
+    q = layer.q_proj(rows)
+    query = paged_append(q, k, v, cos, sin, keys, values, plan)
+    attn = paged_attention(query, keys, values, plan, layer.scaling)
+    return layer.o_proj(attn.to(q.dtype)).reshape(hidden_states.shape)
 
 
 def unpatch_qwen2_attention():

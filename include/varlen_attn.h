@@ -288,6 +288,90 @@ int va_unpack_rows(const void* src, void* dst, const int32_t* b_idx, const int32
                    int32_t* row_map, int64_t n_tokens, int32_t batch, int32_t heads, int32_t seq,
                    int32_t head_dim, int32_t elem_bytes, void* stream);
 
+/* ---- paged key/value cache --------------------------------------------------------------------
+ * A serving program's cache: keys and values of every sequence in pages of page_size rows (a power
+ * of two, 16 to 256), found through a page table. No counterpart in the reference, which trains
+ * only (its generation goes through transformers' dense cache); the entry points follow the
+ * attention's conventions above. Layouts:
+ *   k_pages, v_pages  n_pages pages of (Hkv, page_size, 128) contiguous 16-bit elements, the pages
+ *                     k_stride / v_stride elements apart (multiples of 8, at least Hkv page_size 128)
+ *   page_table        (n_seqs, table_width) int32: row t of sequence s lies in page
+ *                     page_table[s][t / page_size], row t % page_size. Entries outside [0, n_pages)
+ *                     name no page: their rows are neither read (zero keys and values) nor written.
+ *   q_lengths, kv_lengths  (n_seqs) int32: a step's new tokens of every sequence (packed rows, one
+ *                     sequence after the other) and the cached tokens with the new ones included:
+ *                     new token j of sequence s has position kv_lengths[s] - q_lengths[s] + j.
+ *                     Both are read on the device only (a captured step follows them from replay to
+ *                     replay): negative lengths count as 0, kv_lengths end at table_width page_size,
+ *                     q_lengths where n_tokens rows are used up; rows behind the last sequence are
+ *                     padding.
+ *
+ * va_paged_plan writes the step's plan (va_paged_plan_words int32 of device memory, 16-byte aligned):
+ * the sequence and the position of every row, and the attention's work list. It depends on the
+ * lengths and sizes alone, so all layers of a step share it. n_seqs <= 8192. */
+int va_paged_plan_words(int32_t n_seqs, int64_t n_tokens, int32_t hq, int32_t hkv,
+                        int32_t page_size, int32_t table_width, int64_t* words);
+int va_paged_plan(const int32_t* q_lengths, const int32_t* kv_lengths, int32_t n_seqs,
+                  int64_t n_tokens, int32_t hq, int32_t hkv, int32_t page_size,
+                  int32_t table_width, int32_t* plan, int64_t plan_words, void* stream);
+
+/* The new rows of a step: q (N, Hq*D) rotated into q_out (N, Hq, D), k (N, Hkv*D) rotated and v cast
+ * into their pages, in fp32 and rounded once to out_dtype (VA_F16 / VA_BF16), from in_dtype
+ * projections. Row n of sequence s at position t takes row s * cos_batch_stride +
+ * t * cos_seq_stride + n * cos_token_stride of the fp32 tables (strides in elements, non-negative
+ * multiples of 4). cos_rows bounds t (0: no bound, for tables read by token): rows past it, padding
+ * rows and rows at negative positions get zero q_out and write nothing. */
+int va_paged_append(const void* q, const void* k, const void* v, const float* cos,
+                    const float* sin, int64_t cos_batch_stride, int64_t cos_seq_stride,
+                    int64_t cos_token_stride, int64_t cos_rows, const int32_t* plan,
+                    const int32_t* page_table, int32_t n_seqs, int32_t table_width, void* q_out,
+                    void* k_pages, void* v_pages, int64_t k_stride, int64_t v_stride,
+                    int32_t n_pages, int32_t page_size, int64_t n_tokens, int32_t hq,
+                    int32_t hkv, int32_t head_dim, int32_t in_dtype, int32_t out_dtype,
+                    void* stream);
+
+/* out (N, Hq, 128) = softmax(scale q k^T) v of every new token over its sequence's keys at positions
+ * up to its own; zeros for padding rows and for rows that see no key. The workspace
+ * (va_paged_attention_workspace bytes, possibly 0) holds partial results of split key ranges; calls
+ * that may overlap need one each. scale must be finite and > 0. Deterministic. */
+int va_paged_attention_workspace(int32_t n_seqs, int64_t n_tokens, int32_t hq, int32_t hkv,
+                                 int32_t page_size, int32_t table_width, int64_t* bytes);
+int va_paged_attention(const void* q, const void* k_pages, const void* v_pages, int64_t k_stride,
+                       int64_t v_stride, int32_t n_pages, int32_t page_size,
+                       const int32_t* page_table, int32_t table_width, const int32_t* plan,
+                       int32_t n_seqs, int64_t n_tokens, int32_t hq, int32_t hkv,
+                       int32_t head_dim, float scale, int32_t dtype, void* out, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+
+/* Page bookkeeping, whole on the device. `pages` holds outer (keys and values of every layer) x
+ * n_pages x (kv_heads, page_size, 128) contiguous 16-bit elements; refs (n_pages) counts the holders
+ * of each page (table rows, and whatever else the program holds pages for); lengths (n_slots) are
+ * the tokens of every table row. The outputs may not overlap the inputs. Ties go to the lowest
+ * index; table entries past a row's pages come out as -1.
+ * va_pages_remap: row i becomes parents[i]'s (outside [0, n_slots): no parent), cut to
+ * kept = min(lengths[parents[i]], new_lengths[i]) tokens and grown to new_lengths[i] (parents NULL:
+ * every row its own; new_lengths NULL: the parent's length, 0 without one) with free pages
+ * (count 0), taken in ascending order, row after row. Rows share full pages; a part-filled last page
+ * belongs to one row only: where another row holds the page too, all but the lowest row that ends
+ * in it (all of them, where a row holds it whole or the program itself does) get a copy of its
+ * kept % page_size rows in a free page. *shortfall = 0, or the number of pages that the pool or the
+ * table rows lack: then nothing changes (the outputs repeat the inputs, no page is written).
+ * va_pages_compact: with n_live = the number of pages with refs > 0, the k-th live page at or past
+ * n_live moves to the k-th free page below it; *live = n_live. lengths do not change.
+ * scratch: va_pages_scratch_words int32, contents do not matter. */
+int va_pages_scratch_words(int32_t n_slots, int32_t n_pages, int64_t* words);
+int va_pages_remap(void* pages, int64_t outer, int32_t n_pages, int32_t kv_heads,
+                   int32_t page_size, int32_t head_dim, const int32_t* table,
+                   const int32_t* lengths, const int32_t* refs, const int32_t* parents,
+                   const int32_t* new_lengths, int32_t n_slots, int32_t table_width,
+                   int32_t* table_out, int32_t* lengths_out, int32_t* refs_out,
+                   int32_t* shortfall, int32_t* scratch, int64_t scratch_words, void* stream);
+int va_pages_compact(void* pages, int64_t outer, int32_t n_pages, int32_t kv_heads,
+                     int32_t page_size, int32_t head_dim, const int32_t* table,
+                     const int32_t* lengths, const int32_t* refs, int32_t n_slots,
+                     int32_t table_width, int32_t* table_out, int32_t* refs_out, int32_t* live,
+                     int32_t* scratch, int64_t scratch_words, void* stream);
+
 /* ---- machine-ceiling probes (diagnostics) ----------------------------------------------------
  * No counterpart in the reference: the benchmark measures with them the two ceilings it quotes
  * its roofline fractions against, on the box it runs on, beside the data-sheet figures.

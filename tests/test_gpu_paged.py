@@ -1,0 +1,628 @@
+"""The paged cache on the GPU against plain 64-bit references: the attention of a step's new tokens,
+the append, the page bookkeeping, and a run of them together."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from hackaton_amd import (PagedCache, compact_pages, paged_append, paged_attention, paged_plan,
+                          remap_pages)
+from tests import paged_oracle as orc
+from tests.paged_oracle import DIM, HALF_STEP, SCALE
+
+pytestmark = pytest.mark.gpu
+
+FP16, BF16 = torch.float16, torch.bfloat16
+
+
+def banner(*what):
+    print("\n[case]", *what, flush=True)
+
+
+def ints(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def attend(query, k_pool, v_pool, table, q_lengths, kv_lengths, page_size, scale=SCALE):
+    n, heads, _ = query.shape
+    plan = paged_plan(table.cuda(), ints(q_lengths), ints(kv_lengths), n, heads, k_pool.shape[1],
+                      page_size)
+    out = paged_attention(query.cuda(), k_pool.cuda(), v_pool.cuda(), plan, scale)
+    torch.cuda.synchronize()
+    return out.view(n, heads, DIM), plan
+
+
+def check_attention(q_lengths, kv_lengths, heads, kv_heads, dtype, page_size, padding=0, **more):
+    banner("paged attention", q_lengths, kv_lengths, heads, kv_heads, dtype, page_size, more)
+    query, k, v, table = orc.paged_case(sum(kv_lengths) + heads, q_lengths, kv_lengths, heads,
+                                        kv_heads, dtype, page_size, padding, **more)
+    ref, size = orc.attention(query, k, v, table, q_lengths, kv_lengths)
+    out, plan = attend(query, k, v, table, q_lengths, kv_lengths, page_size)
+    got = out.cpu().double()
+    assert torch.isfinite(got).all()
+    excess = (got - ref).abs() - orc.attention_bound(ref, size, dtype, more.get("qk", 1.0))
+    assert float(excess.max()) <= 0, float((got - ref).abs().max())
+    again, _ = attend(query, k, v, table, q_lengths, kv_lengths, page_size)
+    assert torch.equal(out, again)
+    return out, plan
+
+
+HEADS = [(12, 2, FP16), (28, 4, BF16), (4, 4, FP16), (16, 2, BF16), (3, 1, FP16), (40, 1, BF16)]
+
+
+@pytest.mark.parametrize("page_size", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("heads,kv_heads,dtype", HEADS)
+def test_single_tokens(heads, kv_heads, dtype, page_size):
+    """One new token per sequence, caches of 1 to 1000 tokens around every tile and page border."""
+    kv = [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 511, 1000]
+    check_attention([1] * len(kv), kv, heads, kv_heads, dtype, page_size)
+
+
+@pytest.mark.parametrize("page_size", [16, 64])
+@pytest.mark.parametrize("heads,kv_heads,dtype", HEADS)
+def test_chunks_and_single_tokens_mixed(heads, kv_heads, dtype, page_size):
+    """Chunks around the row tiles' borders beside single tokens, idle sequences (no new token),
+    empty ones, a whole prompt at once, and padding rows behind the last sequence."""
+    q = [1, 0, 5, 33, 1, 0, 64, 100, 2, 3, 130, 1]
+    kv = [7, 40, 5, 300, 260, 0, 64, 165, 2, 500, 131, 77]
+    out, plan = check_attention(q, kv, heads, kv_heads, dtype, page_size, padding=5)
+    assert torch.equal(out[sum(q):], torch.zeros_like(out[sum(q):]))
+    assert plan.sequences.tolist() == [s for s, n in enumerate(q) for _ in range(n)] + [-1] * 5
+    assert plan.positions.tolist()[:sum(q)] == [k - n + j for n, k in zip(q, kv) for j in range(n)]
+
+
+@pytest.mark.parametrize("rows", range(1, 12))
+def test_few_tokens_of_odd_counts(rows):
+    """Drafted tokens: every number of rows around the single tile, over one and several key tiles."""
+    check_attention([rows, 1, rows], [rows, 70, 391 + rows], 28, 4, BF16, 16)
+    check_attention([3 * rows, rows], [3 * rows + 64, 1025], 7, 1, FP16, 32)
+
+
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+def test_long_contexts_split_over_the_card(dtype):
+    """Few rows over long caches: the key range in many parts, the last one of every size."""
+    check_attention([1, 1, 2], [20000, 8191, 16385], 12, 2, dtype, 64)
+    check_attention([40], [9000], 6, 1, dtype, 16)
+
+
+@pytest.mark.parametrize("q,kv,heads,kv_heads", [([300], [300], 12, 2), ([257, 129], [700, 129], 14, 2),
+                                                 ([200], [2300], 2, 2)])
+def test_prompt_chunks(q, kv, heads, kv_heads):
+    for dtype in (FP16, BF16):
+        check_attention(q, kv, heads, kv_heads, dtype, 32)
+
+
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+def test_peaky_scores(dtype):
+    """Queries and keys three times as large: the running maximum moves over the whole range."""
+    check_attention([1, 40, 1], [900, 350, 64], 12, 2, dtype, 16, qk=3.0)
+
+
+def test_rows_that_see_no_key_are_zero():
+    """More new tokens than the cache counts: the first ones lie before the sequence."""
+    banner("rows before the sequence")
+    q, kv = [6, 40, 3], [4, 9, 0]
+    query, k, v, table = orc.paged_case(3, q, kv, 12, 2, FP16, 16)
+    out, plan = attend(query, k, v, table, q, kv, 16)
+    ref, size = orc.attention(query, k, v, table, q, kv)
+    assert torch.isfinite(out).all()
+    assert ((out.cpu().double() - ref).abs() <= orc.attention_bound(ref, size, FP16)).all()
+    assert plan.positions.tolist()[:6] == [-2, -1, 0, 1, 2, 3]
+
+
+def test_pages_outside_the_pool_read_as_zeros():
+    banner("bad page numbers")
+    q, kv = [1, 40], [200, 300]
+    query, k, v, table = orc.paged_case(5, q, kv, 12, 2, BF16, 32)
+    table[0, 1], table[0, 4], table[1, 0], table[1, 7] = -1, k.shape[0], 1 << 30, -(1 << 31)
+    out, _ = attend(query, k, v, table, q, kv, 32)
+    ref, size = orc.attention(query, k, v, table, q, kv)
+    assert ((out.cpu().double() - ref).abs() <= orc.attention_bound(ref, size, BF16)).all()
+
+
+def test_lengths_past_their_bounds_are_cut():
+    """kv_lengths past the table row end there; q_lengths past the rows end with them; negative ones
+    count as 0."""
+    banner("lengths past their bounds")
+    q, kv = [2, 3], [50, 64]
+    query, k, v, table = orc.paged_case(6, q, kv, 12, 2, FP16, 16, width=4)
+    for q_given, kv_given in (([2, 1 << 30], [50, 64]), ([2, 3], [50, 1 << 30]), ([2, 3, -5], [50, 64, -7])):
+        rows = table if len(q_given) == 2 else torch.cat((table, table[:1]))
+        plan = paged_plan(rows.cuda(), ints(q_given), ints(kv_given), 5, 12, 2, 16)
+        out = paged_attention(query.cuda(), k.cuda(), v.cuda(), plan, SCALE).view(5, 12, DIM)
+        if q_given[1] == 1 << 30:  # the rows of the second sequence then lie before it
+            assert torch.equal(out[2:], torch.zeros_like(out[2:]))
+            continue
+        ref, size = orc.attention(query, k, v, table, q, kv)
+        assert ((out.cpu().double() - ref).abs() <= orc.attention_bound(ref, size, FP16)).all()
+
+
+@pytest.mark.parametrize("page_size", [16, 128])
+def test_pages_of_all_layers_side_by_side(page_size):
+    """A pool that keeps a page's layers together: the pages of one layer lie far apart, its keys and
+    values at different strides."""
+    banner("strided pool", page_size)
+    q, kv = [1, 50, 1], [333, 200, 16]
+    query, k, v, table = orc.paged_case(8, q, kv, 12, 2, FP16, page_size)
+    pool = torch.full((k.shape[0], 3, 2, *k.shape[1:]), math.nan, dtype=FP16, device="cuda")
+    wide = torch.full((k.shape[0], 2, *k.shape[1:]), math.nan, dtype=FP16, device="cuda")
+    pool[:, 1, 0], wide[:, 1] = k.cuda(), v.cuda()
+    plan = paged_plan(table.cuda(), q, kv, sum(q), 12, 2, page_size)
+    a = paged_attention(query.cuda(), pool[:, 1, 0], wide[:, 1], plan, SCALE)
+    b = paged_attention(query.cuda(), k.cuda(), v.cuda(), plan, SCALE)
+    assert torch.equal(a, b)
+    # queries that are a part of wider rows
+    rows = torch.randn(sum(q), 20, DIM, device="cuda").to(FP16)
+    rows[:, 4:16] = query.cuda()
+    assert torch.equal(paged_attention(rows[:, 4:16], k.cuda(), v.cuda(), plan, SCALE), b)
+
+
+def test_a_pool_past_32_bits():
+    """Pages whose byte and element offsets pass 32 bits, read by both shapes of calls and written by
+    the append, the remap's copies and the compaction."""
+    banner("pool past 32 bits")
+    page_size, kv_heads, heads = 256, 4, 28
+    n_pages = (1 << 32) // (page_size * kv_heads * DIM) + 40  # 8.6 GB of keys
+    q, kv = [1, 60], [700, 300]
+    query, k, v, table = orc.paged_case(9, q, kv, heads, kv_heads, BF16, page_size)
+    high = n_pages - k.shape[0]
+    pages = torch.empty(1, 2, n_pages, kv_heads, page_size, DIM, dtype=BF16, device="cuda")
+    pages[0, 0, high:], pages[0, 1, high:] = k.cuda(), v.cuda()
+    moved = torch.where(table >= 0, table + high, table)
+    plan = paged_plan(moved.cuda(), q, kv, sum(q), heads, kv_heads, page_size)
+    out = paged_attention(query.cuda(), pages[0, 0], pages[0, 1], plan, SCALE)
+    low, _ = attend(query, k, v, table, q, kv, page_size)
+    assert torch.equal(out.view_as(low), low)
+    refs = torch.zeros(n_pages, dtype=torch.int32)
+    refs[moved[moved >= 0].long()] = 1
+    state = [moved.cuda(), ints(kv), refs.cuda()]
+    packed, counts, live = compact_pages(pages, *state)
+    assert int(live) == int(refs.sum()) and int(packed.max()) == int(live) - 1
+    plan = paged_plan(packed, q, kv, sum(q), heads, kv_heads, page_size)
+    assert torch.equal(paged_attention(query.cuda(), pages[0, 0], pages[0, 1], plan, SCALE), out)
+    # a fork into an empty slot whose copy lands in the highest page: all others are held
+    counts = torch.ones_like(counts)
+    counts[-1] = 0
+    grown, lengths, _, short = remap_pages(pages, packed, ints([700, 0]), counts, ints([0, 0]))
+    assert int(short) == 0 and int(grown[1, 2]) == n_pages - 1
+    plan = paged_plan(grown, [1, 1], lengths, 2, heads, kv_heads, page_size)
+    rows = query[:1].cuda().expand(2, heads, DIM)
+    both = paged_attention(rows, pages[0, 0], pages[0, 1], plan, SCALE)
+    assert torch.equal(both[0], both[1]) and torch.equal(both[0], out[0])
+    proj = torch.randn(2, (heads + 2 * kv_heads) * DIM, device="cuda").to(BF16)
+    parts = proj.split([heads * DIM, kv_heads * DIM, kv_heads * DIM], 1)
+    cos, sin = torch.ones(2, DIM, device="cuda"), torch.zeros(2, DIM, device="cuda")
+    paged_append(*parts, cos, sin, pages[0, 0], pages[0, 1], plan)
+    assert torch.equal(pages[0, 1, n_pages - 1, :, 699 % page_size].reshape(-1), parts[2][1])
+    del pages
+    torch.cuda.empty_cache()
+
+
+def test_captured_steps_follow_the_lengths():
+    """Two captured graphs of the same cache: lengths, tables and queries change between the replays,
+    with eager work in between; every replay matches the eager call."""
+    banner("captured steps")
+    heads, kv_heads, ps = 12, 2, 16
+    q, kv = [1, 1, 1, 1], [1500, 33, 700, 64]
+    query, k, v, table = (x.cuda() for x in orc.paged_case(10, q, kv, heads, kv_heads, FP16, ps, 60,
+                                                           stale=0.5, width=100))
+    q_len, kv_len = ints(q), ints(kv)
+
+    def step(x):
+        plan = paged_plan(table, q_len, kv_len, 64, heads, kv_heads, ps)
+        return [paged_attention(x, k, v, plan, SCALE), paged_attention(x * 0.5, k, v, plan, SCALE)]
+
+    graphs, static = [], [query.clone(), query.clone()]
+    for x in static:
+        step(x)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step(x)
+        graphs.append((graph, got))
+    gen = torch.Generator().manual_seed(1)
+    for new, total in (([1, 1, 1, 1], kv), ([1, 40, 0, 3], [1400, 100, 700, 60]),
+                       ([0, 0, 0, 0], [1, 1, 1, 1]), ([60, 1, 1, 1], [900, 1, 2, 17])):
+        q_len.copy_(ints(new))
+        kv_len.copy_(ints(total))
+        for (graph, got), x in zip(graphs, static):
+            x.copy_(torch.randn(64, heads, DIM, generator=gen).to(FP16))
+            want = step(x)
+            for _ in range(3):
+                graph.replay()
+                torch.cuda.synchronize()
+                assert all(torch.equal(a, b) for a, b in zip(got, want)), (new, total)
+                x.mul_(1.0)  # eager work between the replays
+
+
+def test_another_stream_and_calls_at_once():
+    banner("streams")
+    q, kv = [1, 30, 1], [800, 90, 65]
+    query, k, v, table = orc.paged_case(11, q, kv, 12, 2, BF16, 16)
+    want, _ = attend(query, k, v, table, q, kv, 16)
+    dev = [x.cuda() for x in (query, k, v, table)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    for _ in range(4):
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                plan = paged_plan(dev[3], ints(q), ints(kv), sum(q), 12, 2, 16)
+                got.append(paged_attention(*dev[:3], plan, SCALE))
+    plan = paged_plan(dev[3], q, kv, sum(q), 12, 2, 16)  # made here, used there, dropped at once
+    streams[0].wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(streams[0]):
+        got.append(paged_attention(*dev[:3], plan, SCALE))
+        del plan
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want.view_as(x)) for x in got)
+
+
+# ------------------------------------------------------------------------------------------------
+# append
+# ------------------------------------------------------------------------------------------------
+def append_case(q, kv, heads, kv_heads, ps, proj, seed=0, padding=0, rows=None, per_sequence=False):
+    gen = torch.Generator().manual_seed(seed)
+    counts = [-(-x // ps) for x in kv]
+    order = torch.randperm(sum(counts) + 4, generator=gen).tolist()
+    table = np.full((len(q), max(counts + [0]) + 1), -1, dtype=np.int32)
+    for s, c in enumerate(counts):
+        for j in range(c):
+            table[s, j] = order.pop()
+    n = sum(q) + padding
+    qkv = [torch.randn(n, h * DIM, generator=gen).to(proj) for h in (heads, kv_heads, kv_heads)]
+    rows = rows or max(kv + [1])
+    angle = torch.rand(len(q) if per_sequence else 1, rows, DIM // 2, generator=gen) * 6.28
+    angle = torch.cat((angle, angle), -1)
+    return qkv, angle.cos(), angle.sin(), torch.from_numpy(table), sum(counts) + 4
+
+
+@pytest.mark.parametrize("per_sequence", [False, True])
+@pytest.mark.parametrize("proj", [FP16, BF16, torch.float32])
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+@pytest.mark.parametrize("heads,kv_heads,ps", [(12, 2, 16), (28, 4, 64), (3, 3, 256), (5, 1, 32)])
+def test_append(heads, kv_heads, ps, dtype, proj, per_sequence):
+    """q rotated, k and v in their pages; every other row of the pools left as it was. The rotation is
+    one product and one fused multiply-add in fp32 (each half a step of 2^-24) before the one rounding."""
+    banner("append", heads, kv_heads, ps, dtype, proj, per_sequence)
+    q, kv = [1, 0, 7, 40, 1, 3], [1, 50, 7, 300, 129, 20]
+    qkv, cos, sin, table, pages = append_case(q, kv, heads, kv_heads, ps, proj, heads, 2,
+                                              per_sequence=per_sequence)
+    pools = [torch.full((pages, kv_heads, ps, DIM), 7.0, dtype=dtype) for _ in range(2)]
+    dev = [x.cuda() for x in pools]
+    plan = paged_plan(table.cuda(), q, kv, sum(q) + 2, heads, kv_heads, ps)
+    got = paged_append(*(x.cuda() for x in qkv), cos.cuda(), sin.cuda(), *dev, plan).cpu()
+    assert torch.equal(got[sum(q):], torch.zeros_like(got[sum(q):]))
+    seq = [s for s, n in enumerate(q) for _ in range(n)]
+    pos = [k - n + j for n, k in zip(q, kv) for j in range(n)]
+    at = (seq if per_sequence else [0] * len(seq), pos)
+    rot = [orc.rotate(x[:sum(q)].double().view(sum(q), -1, DIM), cos[at], sin[at]) for x in qkv[:2]]
+    rot.append(qkv[2][:sum(q)].double().view(sum(q), -1, DIM))
+    # |x| cos and |x| sin in the rotation add to less than 2 * max |x|
+    slack = [2.0 ** -23 * 2 * float(x.abs().max()) for x in qkv]
+
+    def near(a, b, s):
+        return ((a.double() - b).abs() <= HALF_STEP[dtype] * b.abs() + s + 2.0 ** -25).all()
+
+    assert near(got[:sum(q)], rot[0], slack[0])
+    for which in (0, 1):
+        want, seen = pools[which].clone(), dev[which].cpu()
+        for i, (s, t) in enumerate(zip(seq, pos)):
+            page, row = int(table[s, t // ps]), t % ps
+            assert near(seen[page, :, row], rot[1 + which][i], slack[1 + which])
+            want[page, :, row] = seen[page, :, row]
+        assert torch.equal(seen, want)
+
+
+def test_append_tables_by_row_match_tables_by_position():
+    banner("append by row")
+    q, kv, ps = [3, 1, 20], [40, 9, 20], 16
+    qkv, cos, sin, table, pages = append_case(q, kv, 12, 2, ps, BF16, 4)
+    plan = paged_plan(table.cuda(), q, kv, sum(q), 12, 2, ps)
+    pos = plan.positions.long().cpu()
+    results = []
+    for tables in ((cos, sin), (cos[0, pos], sin[0, pos])):
+        dev = torch.zeros(2, pages, 2, ps, DIM, dtype=BF16, device="cuda")
+        out = paged_append(*(x.cuda() for x in qkv), *(x.cuda() for x in tables), dev[0], dev[1], plan)
+        results.append((out, dev))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_append_rows_without_a_place():
+    """Positions past the tables or before the sequence, pages outside the pool: nothing written."""
+    banner("append without a place")
+    q, kv, ps = [3, 4, 2, 2], [40, 2, 33, 31], 16
+    qkv, cos, sin, table, pages = append_case(q, kv, 12, 2, ps, FP16, 5, rows=38)
+    table[2, 1], table[2, 2], table[3, 1] = pages, -3, -1
+    dev = torch.full((2, pages, 2, ps, DIM), 3.0, dtype=FP16, device="cuda")
+    plan = paged_plan(table.cuda(), ints(q), ints(kv), sum(q), 12, 2, ps)
+    out = paged_append(*(x.cuda() for x in qkv), cos.cuda(), sin.cuda(), dev[0], dev[1], plan).cpu()
+    empty = [i for i in range(sum(q)) if not out[i].any()]
+    assert empty == [1, 2, 3, 4]  # positions 38, 39 of 38 and -2, -1
+    written = {(int(table[0, 2]), 5), (int(table[1, 0]), 0), (int(table[1, 0]), 1)}
+    changed = (dev.cpu() != 3.0).any(-1).any(2)
+    for which in (0, 1):
+        assert {tuple(x) for x in changed[which].nonzero().tolist()} == written
+
+
+# ------------------------------------------------------------------------------------------------
+# page bookkeeping
+# ------------------------------------------------------------------------------------------------
+def run_remap(table, lengths, refs, parents, new_lengths, ps, layers=2, kv_heads=2, dtype=FP16):
+    pages = torch.randn(layers, 2, len(refs), kv_heads, ps, DIM, device="cuda").to(dtype)
+    before = pages.clone()
+    width = len(table[0]) if table else 0
+    t = ints(table).reshape(len(table), width)
+    got = remap_pages(pages, t, ints(lengths), ints(refs), None if parents is None else ints(parents),
+                      None if new_lengths is None else ints(new_lengths))
+    want = orc.remap(table, lengths, refs, parents, new_lengths, ps)
+    assert [x.tolist() for x in got] == [want[0], want[1], want[2], [want[3]]]
+    for source, target, rows in want[4]:
+        before[:, :, target, :, :rows] = before[:, :, source, :, :rows]
+    assert torch.equal(pages, before)
+    again = remap_pages(pages, t, ints(lengths), ints(refs), None if parents is None else ints(parents),
+                        None if new_lengths is None else ints(new_lengths))
+    assert all(torch.equal(a, b) for a, b in zip(got, again)) and torch.equal(pages, before)
+    return want
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_remap_against_the_reference(seed):
+    rng = np.random.default_rng(seed)
+    slots, width = int(rng.integers(1, 60)), int(rng.integers(1, 20))
+    ps = int(rng.choice([16, 32, 128]))
+    pages = int(rng.integers(1, slots * width + 20))
+    banner("remap", seed, slots, width, ps, pages)
+    table, lengths, refs = orc.random_state(rng, slots, width, pages, ps, pins=seed % 4)
+    parents = rng.integers(-2, slots + 1, slots).tolist() if seed % 3 else None
+    new = [int(x) for x in rng.integers(-3, width * ps + 1, slots)]
+    if seed % 2:  # mostly small steps
+        new = [min(width * ps, (lengths[p] if 0 <= p < slots else 0) + int(rng.integers(-20, 20)))
+               for p in (parents or range(slots))]
+    run_remap(table, lengths, refs, parents, None if seed % 5 == 4 else new, ps,
+              layers=1 + seed % 3, kv_heads=1 + seed % 4, dtype=BF16 if seed % 2 else FP16)
+
+
+def test_remap_lacking_pages_changes_nothing():
+    rng = np.random.default_rng(0)
+    table, lengths, refs = orc.random_state(rng, 6, 5, 12, 16)
+    free = sum(r == 0 for r in refs)
+    grown = [min(80, x + 16 * (free // 2 + 1)) for x in lengths]
+    assert run_remap(table, lengths, refs, None, grown, 16)[3] > 0
+    assert run_remap(table, lengths, refs, None, [81] + lengths[1:], 16)[3] > 0
+    assert run_remap(table, lengths, refs, None, [(1 << 31) - 1] * 6, 16)[3] > 0
+
+
+def test_remap_of_many_slots_and_pages():
+    """More slots and pages than a work-group has threads; a fork of everything into everything."""
+    rng = np.random.default_rng(5)
+    table, lengths, refs = orc.random_state(rng, 1500, 3, 4500, 16)
+    parents = rng.integers(-1, 1500, 1500).tolist()
+    refs += [0] * 6000
+    run_remap(table, lengths, refs, parents, None, 16, layers=1, kv_heads=1)
+    run_remap(table, lengths, refs, None, [min(48, x + 1) for x in lengths], 16, layers=1, kv_heads=1)
+
+
+def test_remap_of_nothing():
+    pages = torch.zeros(1, 2, 4, 1, 16, DIM, dtype=FP16, device="cuda")
+    refs = ints([1, 0, 2, 0])
+    for table in (torch.zeros(0, 3, dtype=torch.int32, device="cuda"),
+                  torch.zeros(2, 0, dtype=torch.int32, device="cuda")):
+        lengths = torch.zeros(table.shape[0], dtype=torch.int32, device="cuda")
+        out = remap_pages(pages, table, lengths, refs)
+        assert out[0].shape == table.shape and torch.equal(out[2], refs) and int(out[3]) == 0
+        out = compact_pages(pages, table, lengths, refs)
+        assert out[1].tolist() == [1, 2, 0, 0] and int(out[2]) == 2
+    empty = torch.zeros(1, 2, 0, 1, 16, DIM, dtype=FP16, device="cuda")
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    table, lengths = ints([[-1]]), ints([0])
+    assert int(remap_pages(empty, table, lengths, none, None, ints([3]))[3]) == 1
+    assert int(compact_pages(empty, table, lengths, none)[2]) == 0
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_compact_against_the_reference(seed):
+    rng = np.random.default_rng(100 + seed)
+    slots, width = int(rng.integers(1, 40)), int(rng.integers(1, 20))
+    ps, layers = int(rng.choice([16, 64])), 1 + seed % 3
+    pages = int(rng.choice([slots * width + 1, 1500, 5000])) if seed % 2 else slots * width // 2 + 1
+    banner("compact", seed, slots, width, ps, pages)
+    table, lengths, refs = orc.random_state(rng, slots, width, pages, ps, pins=seed % 3)
+    pool = torch.randn(layers, 2, pages, 1 + seed % 2, ps, DIM, device="cuda").to(FP16)
+    before = pool.clone()
+    got = compact_pages(pool, ints(table), ints(lengths), ints(refs))
+    want = orc.compact(table, lengths, refs, ps)
+    assert [x.tolist() for x in got] == [want[0], want[1], [want[2]]]
+    for source, target in want[3]:
+        before[:, :, target] = before[:, :, source]
+    assert torch.equal(pool, before)
+
+
+# ------------------------------------------------------------------------------------------------
+# refusals
+# ------------------------------------------------------------------------------------------------
+def test_refusals():
+    q, kv = [1, 2], [40, 33]
+    query, k, v, table = (x.cuda() for x in orc.paged_case(1, q, kv, 12, 2, FP16, 16))
+    plan = paged_plan(table, q, kv, 3, 12, 2, 16)
+    for bad in ((table.long(), q, kv, 3, 12, 2, 16), (table.t(), q, kv, 3, 12, 2, 16),
+                (table, q + [1], kv, 4, 12, 2, 16), (table, q, kv, 3, 12, 2, 20),
+                (table, [9, 9], kv, 3, 12, 2, 16), (table, ints(q).float(), ints(kv), 3, 12, 2, 16),
+                (table, torch.tensor(q), ints(kv), 3, 12, 2, 16)):
+        with pytest.raises(ValueError):
+            paged_plan(*bad)
+    with pytest.raises(RuntimeError, match="Hq"):
+        paged_plan(table, q, kv, 3, 12, 5, 16)
+    for bad in ((query[:2], k, v, plan, SCALE), (query.float(), k, v, plan, SCALE),
+                (query.bfloat16(), k, v, plan, SCALE), (query, k[:, :1], v[:, :1], plan, SCALE),
+                (query, k, v[:-1], plan, SCALE), (query, k, v.bfloat16(), plan, SCALE),
+                (query.cpu(), k, v, plan, SCALE), (query, k.transpose(2, 3), v, plan, SCALE),
+                (query, k.transpose(1, 2).contiguous().transpose(1, 2), v, plan, SCALE)):
+        with pytest.raises(ValueError):
+            paged_attention(*bad)
+    for scale in (0.0, -1.0, math.inf, math.nan):
+        with pytest.raises(RuntimeError, match="scale"):
+            paged_attention(query, k, v, plan, scale)
+    with pytest.raises(RuntimeError, match="page strides"):
+        paged_attention(query, k[:1].expand(k.shape), v, plan, SCALE)
+    with pytest.raises(RuntimeError, match="no backward"):
+        paged_attention(query.clone().requires_grad_(), k, v, plan, SCALE)
+    rows = [torch.zeros(3, h * DIM, dtype=FP16, device="cuda") for h in (12, 2, 2)]
+    cos = torch.ones(1, 50, DIM, device="cuda")
+    for bad in ((rows[0], rows[1], rows[2][:2], cos, cos), (rows[0].float(), *rows[1:], cos, cos),
+                (*rows, cos[:, :, :64], cos), (*rows, cos[0, :2], cos[0, :2]),
+                (*rows, cos.expand(3, 50, DIM), cos.expand(3, 50, DIM)), (*rows, cos[:, :0], cos[:, :0])):
+        with pytest.raises(ValueError):
+            paged_append(*bad, k, v, plan)
+    pages = torch.zeros(2, 2, 8, 2, 16, DIM, dtype=FP16, device="cuda")
+    state = [torch.full((3, 2), -1, dtype=torch.int32, device="cuda"), ints([0] * 3), ints([0] * 8)]
+    for bad in ((pages[0], *state), (pages[:, :, ::2], *state[:2], state[2][:4]),
+                (pages.float(), *state), (pages, state[0], state[1][:2], state[2]),
+                (pages, *state[:2], state[2][:7]), (pages, *state, ints([0, 0])),
+                (pages, *state, None, ints([1, 1, 1]).long())):
+        with pytest.raises(ValueError):
+            remap_pages(*bad)
+    with pytest.raises(ValueError):
+        PagedCache(1, 4, 17, 1, 1, 16)
+
+
+# ------------------------------------------------------------------------------------------------
+# together
+# ------------------------------------------------------------------------------------------------
+class Mirror:
+    """The same sequences as plain lists of rows, per layer."""
+
+    def __init__(self, layers, slots):
+        self.rows = [[[] for _ in range(slots)] for _ in range(layers)]  # (k, v) of every token
+
+    def fork(self, source, target):
+        for layer in self.rows:
+            layer[target] = list(layer[source])
+
+
+def answer(cache, mirror, q_lengths, heads, kv_heads, cos, sin, gen, n_rows=None):
+    """One step through every layer, checked against attention over the mirror's rows."""
+    n = n_rows or sum(q_lengths)
+    plan = cache.step(ints(q_lengths), n, heads)
+    for layer, rows in enumerate(mirror.rows):
+        proj = [torch.randn(n, h * DIM, generator=gen).to(cache.pages.dtype) for h in
+                (heads, kv_heads, kv_heads)]
+        keys, values = cache.keys(layer), cache.values(layer)
+        query = paged_append(*(x.cuda() for x in proj), cos, sin, keys, values, plan)
+        out = paged_attention(query, keys, values, plan, SCALE).cpu().double().view(n, heads, DIM)
+        seq, pos = plan.sequences.tolist(), plan.positions.tolist()
+        for i in range(n):
+            if seq[i] < 0:
+                assert not out[i].any()
+                continue
+            c, s = (x[0, pos[i]][None].cpu() for x in (cos, sin))
+            k = orc.rotate(proj[1][i].double().view(1, kv_heads, DIM), c, s)[0]
+            k = k.float().to(cache.pages.dtype).double()
+            assert pos[i] == len(rows[seq[i]])
+            rows[seq[i]].append((k, proj[2][i].double().view(kv_heads, DIM)))
+        got_q = query.cpu()
+        for i in range(n):
+            if seq[i] < 0:
+                continue
+            # (rotated keys round once in fp32 first: half a step of fp32 may move a 16-bit rounding
+            # by one step, 2^-10 (fp16) of a key of size 4, which moves a weight by less than 2^-8)
+            mine = rows[seq[i]][:pos[i] + 1]
+            k = torch.stack([r[0] for r in mine], 1)
+            v = torch.stack([r[1] for r in mine], 1)
+            for h in range(heads):
+                z = k[h // (heads // kv_heads)] @ got_q[i, h].double() * SCALE
+                w = torch.softmax(z, 0)
+                want = w @ v[h // (heads // kv_heads)]
+                size = w @ v[h // (heads // kv_heads)].abs()
+                bound = orc.attention_bound(want, size, cache.pages.dtype) + 2.0 ** -8 * size
+                assert ((out[i, h] - want).abs() <= bound).all()
+    return plan
+
+
+@pytest.mark.parametrize("dtype,page_size", [(FP16, 16), (BF16, 32)])
+def test_a_program_run(dtype, page_size):
+    """Prompts entered in chunks, decoding beside them, a fork into two more answers, drafted tokens
+    cut back, answers freed, the pool compacted in between; a step that lacks pages changes nothing."""
+    banner("a run", dtype, page_size)
+    layers, heads, kv_heads, slots = 2, 6, 2, 5
+    gen = torch.Generator().manual_seed(page_size)
+    cache = PagedCache(layers, 448 // page_size, page_size, kv_heads, slots, 256, dtype)
+    cache.pages.fill_(math.nan)
+    angle = torch.arange(256)[:, None] * (1e4 ** (-torch.arange(64) / 64.0))[None]
+    angle = torch.cat((angle, angle), -1)[None]
+    tables = (angle.cos().cuda(), angle.sin().cuda())
+    mirror = Mirror(layers, slots)
+
+    def go(q, **more):
+        return answer(cache, mirror, q, heads, kv_heads, *tables, gen, **more)
+
+    go([37, 0, 5, 0, 0])
+    go([30, 0, 1, 0, 0], n_rows=40)
+    go([1, 20, 1, 0, 0])
+    cache.fork(0, [3, 4])
+    for t in (3, 4):
+        mirror.fork(0, t)
+    assert cache.lengths.tolist() == [68, 20, 7, 68, 68]
+    go([1, 1, 1, 1, 1])
+    go([4, 1, 0, 4, 1])  # drafted tokens ...
+    cache.remap(None, cache.lengths - ints([3, 0, 0, 1, 0]))  # ... of which some stay
+    for layer in mirror.rows:
+        del layer[0][-3:], layer[3][-1:]
+    go([1, 1, 1, 1, 1])
+    cache.free([1, 3])
+    for layer in mirror.rows:
+        layer[1], layer[3] = [], []
+    live = int(cache.compact())
+    assert live == int((cache.refs > 0).sum()) and int(cache.table.max()) < live
+    go([1, 9, 1, 0, 2])
+    cache.check()
+    kept = [x.clone() for x in (cache.table, cache.lengths, cache.refs, cache.pages)]
+    plan = cache.step([150, 100, 100, 0, 150], 500, heads)  # more than the pool holds
+    assert set(plan.sequences.tolist()) == {-1}
+    assert all(torch.equal(a, b) for a, b in zip(kept[:3], (cache.table, cache.lengths, cache.refs)))
+    with pytest.raises(RuntimeError, match="lacked"):
+        cache.check()
+    go([1, 1, 1, 0, 1])
+    cache.check()
+    refs = torch.bincount(cache.table[cache.table >= 0].long(), minlength=cache.refs.numel())
+    assert torch.equal(refs.int(), cache.refs)
+
+
+def test_a_captured_decode_step_runs_on():
+    """step, append and attention captured once, replayed until the answers are long; the same steps
+    run eagerly give the same cache and outputs."""
+    banner("captured decode")
+    heads, kv_heads, slots, ps = 12, 2, 3, 16
+    gen = torch.Generator().manual_seed(0)
+    angle = torch.rand(1, 256, DIM, generator=gen) * 6
+    cos, sin = angle.cos().cuda(), angle.sin().cuda()
+    caches = [PagedCache(1, 40, ps, kv_heads, slots, 200, BF16) for _ in range(2)]
+    rows = [torch.zeros(slots, h * DIM, dtype=BF16, device="cuda") for h in (heads, kv_heads, kv_heads)]
+    one = ints([1, 0, 1])
+
+    def step(cache):
+        plan = cache.step(one, slots, heads)
+        query = paged_append(*rows, cos, sin, cache.keys(0), cache.values(0), plan)
+        return paged_attention(query, cache.keys(0), cache.values(0), plan, SCALE)
+
+    for cache in caches:
+        cache.pages.zero_()
+        cache.remap(None, ints([20, 0, 0]))
+    step(caches[0])
+    caches[0].remap(None, ints([20, 0, 0]))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(caches[0])
+    caches[0].pages.copy_(caches[1].pages)
+    for i in range(40):
+        for x in rows:
+            x.copy_(torch.randn(x.shape, generator=gen).to(BF16))
+        graph.replay()
+        want = step(caches[1])
+        torch.cuda.synchronize()
+        assert torch.equal(got, want), i
+        assert caches[0].lengths.tolist() == [21 + i, 0, 1 + i]
+        assert torch.equal(caches[0].table, caches[1].table)
+    assert torch.equal(caches[0].pages, caches[1].pages)

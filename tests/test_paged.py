@@ -1,0 +1,172 @@
+"""The paged cache's entry points without a GPU: sizes, refusals before any launch, and the
+references that the GPU tests compare with."""
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import hackaton_amd
+from hackaton_amd import _lib, paged
+from tests import paged_oracle as orc
+
+OK = (2, 8, 12, 2, 16, 4)  # n_seqs, n_tokens, hq, hkv, page_size, table_width
+
+
+def words(*sizes):
+    out = ctypes.c_int64()
+    return _lib.lib().va_paged_plan_words(*sizes, ctypes.byref(out)), out.value
+
+
+def test_the_entry_points_are_public():
+    for name in ("paged_plan", "paged_append", "paged_attention", "remap_pages", "compact_pages",
+                 "PagedCache"):
+        assert name in hackaton_amd.__all__ and getattr(hackaton_amd, name) is getattr(paged, name)
+
+
+@pytest.mark.parametrize("at,value,code", [
+    (0, -1, _lib.VA_ESHAPE), (0, 8193, _lib.VA_ESHAPE), (1, -1, _lib.VA_ESHAPE),
+    (1, 1 << 40, _lib.VA_ESHAPE), (2, 0, _lib.VA_ESHAPE), (2, 13, _lib.VA_ESHAPE),
+    (3, 0, _lib.VA_ESHAPE), (4, 0, _lib.VA_ESHAPE), (4, 8, _lib.VA_ESHAPE), (4, 24, _lib.VA_ESHAPE),
+    (4, 512, _lib.VA_ESHAPE), (5, -1, _lib.VA_ESHAPE), (5, 1 << 30, _lib.VA_ESHAPE)])
+def test_plan_sizes_are_checked(at, value, code):
+    sizes = list(OK)
+    assert words(*sizes)[0] == 0 and words(*sizes)[1] >= sizes[0] + 1 + 2 * sizes[1]
+    sizes[at] = value
+    assert words(*sizes)[0] == code
+    assert _lib.lib().va_last_error()
+
+
+def buffers():
+    """A 16-byte aligned host buffer: the calls below are refused before anything would read it."""
+    raw = np.zeros(4096, dtype=np.uint8)
+    return raw, raw.ctypes.data + (-raw.ctypes.data) % 16
+
+
+def attention_args(p):
+    stride = 2 * 16 * 128
+    return [p, p, p, stride, stride, 4, 16, p, 4, p, 2, 8, 12, 2, 128, 0.1, 0, p, p, 1 << 40, None]
+
+
+@pytest.mark.parametrize("at,value,code", [
+    (0, None, _lib.VA_EINVAL), (1, None, _lib.VA_EINVAL), (3, 8, _lib.VA_EINVAL),
+    (4, 2 * 16 * 128 + 4, _lib.VA_EINVAL), (5, -1, _lib.VA_ESHAPE), (7, None, _lib.VA_EINVAL),
+    (9, None, _lib.VA_EINVAL), (14, 64, _lib.VA_ESHAPE), (15, 0.0, _lib.VA_EINVAL),
+    (15, float("nan"), _lib.VA_EINVAL), (16, 2, _lib.VA_EDTYPE), (17, None, _lib.VA_EINVAL)])
+def test_attention_arguments_are_checked(at, value, code):
+    raw, p = buffers()
+    args = attention_args(p)
+    args[at] = value
+    assert _lib.lib().va_paged_attention(*args) == code
+    args = attention_args(p)
+    args[0] = p + 2
+    assert _lib.lib().va_paged_attention(*args) == _lib.VA_EINVAL
+
+
+def test_attention_workspace_is_checked():
+    need = ctypes.c_int64()
+    sizes = (64, 64, 12, 2, 16, 512)
+    assert _lib.lib().va_paged_attention_workspace(*sizes, ctypes.byref(need)) == 0
+    if need.value:
+        raw, p = buffers()
+        args = attention_args(p)
+        args[10:14] = [64, 64, 12, 2]
+        args[8], args[19] = 512, need.value - 1
+        assert _lib.lib().va_paged_attention(*args) == _lib.VA_ECAPACITY
+
+
+def append_args(p):
+    stride = 2 * 16 * 128
+    return [p, p, p, p, p, 0, 128, 0, 64, p, p, 2, 4, p, p, p, stride, stride, 4, 16, 8, 12, 2, 128,
+            0, 0, None]
+
+
+@pytest.mark.parametrize("at,value,code", [
+    (0, None, _lib.VA_EINVAL), (5, 2, _lib.VA_EINVAL), (6, -4, _lib.VA_EINVAL),
+    (7, 3, _lib.VA_EINVAL), (8, -1, _lib.VA_EINVAL), (10, None, _lib.VA_EINVAL),
+    (13, None, _lib.VA_EINVAL), (14, None, _lib.VA_EINVAL), (16, 128, _lib.VA_EINVAL),
+    (19, 17, _lib.VA_ESHAPE), (21, 11, _lib.VA_ESHAPE), (23, 96, _lib.VA_ESHAPE),
+    (24, 3, _lib.VA_EDTYPE), (25, 2, _lib.VA_EDTYPE)])
+def test_append_arguments_are_checked(at, value, code):
+    raw, p = buffers()
+    args = append_args(p)
+    args[at] = value
+    assert _lib.lib().va_paged_append(*args) == code
+
+
+@pytest.mark.parametrize("at,value,code", [
+    (0, None, _lib.VA_EINVAL), (1, -1, _lib.VA_ESHAPE), (2, -1, _lib.VA_ESHAPE),
+    (3, 0, _lib.VA_ESHAPE), (4, 20, _lib.VA_ESHAPE), (5, 64, _lib.VA_ESHAPE),
+    (6, None, _lib.VA_EINVAL), (7, None, _lib.VA_EINVAL), (8, None, _lib.VA_EINVAL),
+    (11, -1, _lib.VA_ESHAPE), (12, -1, _lib.VA_ESHAPE), (13, None, _lib.VA_EINVAL),
+    (16, None, _lib.VA_EINVAL), (17, None, _lib.VA_EINVAL), (18, 8, _lib.VA_ECAPACITY)])
+def test_remap_arguments_are_checked(at, value, code):
+    raw, p = buffers()
+    args = [p, 4, 8, 2, 16, 128, p, p, p, None, None, 4, 4, p + 256, p + 512, p + 768, p + 1024,
+            p + 1280, 1 << 20, None]
+    args[at] = value
+    assert _lib.lib().va_pages_remap(*args) == code
+
+
+def test_bookkeeping_outputs_may_not_be_the_inputs():
+    raw, p = buffers()
+    for at, same in ((13, 6), (14, 7), (15, 8)):
+        args = [p, 4, 8, 2, 16, 128, p, p + 64, p + 128, None, None, 4, 4, p + 256, p + 512, p + 768,
+                p + 1024, p + 1280, 1 << 20, None]
+        args[at] = args[same]
+        assert _lib.lib().va_pages_remap(*args) == _lib.VA_EINVAL
+    for at, same in ((11, 6), (12, 8)):
+        args = [p, 4, 8, 2, 16, 128, p, p + 64, p + 128, 4, 4, p + 256, p + 512, p + 768, p + 1024,
+                1 << 20, None]
+        args[at] = args[same]
+        assert _lib.lib().va_pages_compact(*args) == _lib.VA_EINVAL
+
+
+def test_nothing_to_do_returns_at_once():
+    lib = _lib.lib()
+    args = attention_args(None)
+    args[11] = 0
+    args[1] = args[2] = args[7] = buffers()[1]
+    assert lib.va_paged_attention(*args) == 0
+    assert lib.va_paged_plan(None, None, 2, 0, 12, 2, 16, 4, None, 0, None) == 0
+
+
+def test_host_tensors_are_refused():
+    table = torch.zeros(2, 4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="GPU"):
+        hackaton_amd.paged_plan(table, [1, 1], [1, 1], 2, 12, 2, 16)
+    pages = torch.zeros(1, 2, 4, 2, 16, 128, dtype=torch.float16)
+    ints = torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="GPU"):
+        hackaton_amd.remap_pages(pages, table, ints[:2], ints)
+    with pytest.raises(ValueError, match="GPU"):
+        hackaton_amd.compact_pages(pages, table, ints[:2], ints)
+
+
+@pytest.mark.parametrize("q,kv,n,words", [
+    ([-1, 1], [1, 1], 2, "negative"), ([2, 1], [4, 4], 2, "sum"), ([1, 1], [1, 65], 2, "kv_lengths"),
+    ([1, 1], [-1, 4], 2, "kv_lengths"), ([2, 1], [1, 4], 3, "exceed")])
+def test_host_lengths_are_checked(q, kv, n, words):
+    with pytest.raises(ValueError, match=words):
+        paged._check_host_lengths(q, kv, n, 64)
+
+
+def test_reference_remap_covers_its_rules():
+    """Page size 4. Slots 0 and 1 share page 5; slot 0 ends in page 2 (two rows)."""
+    table, lengths, refs = [[5, 2, -1], [5, -1, -1], [-1, -1, -1]], [6, 4, 0], [0, 0, 1, 0, 0, 2, 0, 0]
+    out = orc.remap(table, lengths, refs, [0, 1, 0], [7, 4, 6], 4)
+    assert out == ([[5, 2, -1], [5, -1, -1], [5, 0, -1]], [7, 4, 6], [1, 0, 1, 0, 0, 3, 0, 0], 0,
+                   [(2, 0, 2)])
+    # cut inside a page that another slot holds whole: a copy of the rows that stay
+    out = orc.remap(table, lengths, refs, None, [6, 3, 0], 4)
+    assert out[0] == [[5, 2, -1], [0, -1, -1], [-1, -1, -1]] and out[4] == [(5, 0, 3)]
+    # too long for the table: nothing changes
+    assert orc.remap(table, lengths, refs, None, [6, 4, 13], 4)[:4] == (table, lengths, refs, 1)
+
+
+def test_reference_compact_moves_to_the_front():
+    table, refs = [[5, 2], [5, -1]], [0, 0, 1, 0, 0, 2]
+    out, counts, live, moves = orc.compact(table, [6, 4], refs, 4)
+    assert live == 2 and moves == [(2, 0), (5, 1)]
+    assert out == [[1, 0], [1, -1]] and counts == [1, 2, 0, 0, 0, 0]

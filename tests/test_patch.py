@@ -121,3 +121,51 @@ def test_patched_attention_matches_original_forward(left, patched):
     for name in ref_grads:
         assert cosine(grads[name], ref_grads[name]) > 0.995, name
     assert cosine(xg, ref_xg) > 0.995
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", ["rows", "batch of one"])
+def test_paged_branch_answers_like_the_dense_cache(patched, shape):
+    """Two prompts of different lengths, then single tokens, through the patched layers with a
+    PagedCache, against transformers' own forward over the whole sequences (causal mask, fp32): hidden
+    states in fp16 with fp32 accumulation differ by the same 3e-2 as the packed branch's."""
+    from hackaton_amd import PagedCache
+
+    torch.manual_seed(1)
+    model = tiny_model("cuda").eval().half()
+    layers = [layer.self_attn for layer in model.model.layers]
+    lengths, extra = [23, 70], 3
+    hidden = [torch.randn(n + extra, HIDDEN, device="cuda").half() for n in lengths]
+    cache = PagedCache(len(layers), 16, 16, KV_HEADS, 2, 128)
+    got = [[[] for _ in hidden] for _ in layers]
+    with torch.no_grad():
+        done = [0, 0]
+        for step in [lengths] + [[1, 1]] * extra:
+            plan = cache.step(torch.tensor(step, dtype=torch.int32, device="cuda"), sum(step), HEADS)
+            rows = torch.cat([h[d:d + n] for h, d, n in zip(hidden, done, step)])
+            tables = model.model.rotary_emb(rows[None].float(), plan.positions.long()[None])
+            for i, layer in enumerate(layers):
+                given = rows if shape == "rows" else rows[None]
+                out, weights = layer(given, tables, None, paged=(cache, plan))
+                assert weights is None and out.shape == given.shape
+                for s, part in enumerate(out.reshape(-1, HIDDEN).split(step)):
+                    got[i][s].append(part)
+            done = [d + n for d, n in zip(done, step)]
+        cache.check()
+        reference = tiny_model("cuda").eval()
+        reference.load_state_dict({k: v.float() for k, v in model.state_dict().items()})
+        for s, h in enumerate(hidden):
+            n = h.shape[0]
+            pos = torch.arange(n, device="cuda")[None]
+            tables = reference.model.rotary_emb(h[None].float(), pos)
+            mask = torch.ones(n, n, dtype=torch.bool, device="cuda").tril()[None, None]
+            for i in range(len(layers)):
+                ref, _ = reference.model.layers[i].self_attn(h[None].float(), tables, mask)
+                out = torch.cat(got[i][s]).float()
+                assert float((out - ref[0]).abs().max()) <= 3e-2
+
+
+def test_a_call_is_either_packed_or_paged(patched):
+    layer = tiny_model("cpu").model.layers[0].self_attn
+    with pytest.raises(ValueError, match="packed or paged"):
+        layer(torch.zeros(1, HIDDEN), (None, None), None, packed=(0,) * 5, paged=(None, None))
