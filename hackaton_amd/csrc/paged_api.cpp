@@ -60,6 +60,11 @@ int check_step(int32_t n_seqs, int64_t n_tokens, int32_t hq, int32_t hkv, int32_
   return VA_OK;
 }
 
+va::PagedLayout layout_of(int32_t n_seqs, int64_t n_tokens, int32_t hq, int32_t hkv,
+                          int32_t page_size, int32_t table_width) {
+  return va::paged_layout(n_seqs, n_tokens, hq, hkv, (int64_t)table_width * page_size);
+}
+
 // Pages of one layer, keys and values.
 int check_pool(const void* k_pages, const void* v_pages, int64_t k_stride, int64_t v_stride,
                int32_t n_pages, int32_t hkv, int32_t page_size, const int32_t* table,
@@ -81,7 +86,7 @@ extern "C" int va_paged_plan_words(int32_t n_seqs, int64_t n_tokens, int32_t hq,
   const int rc = check_step(n_seqs, n_tokens, hq, hkv, page_size, table_width, "va_paged_plan_words");
   if (rc) return rc;
   if (words == nullptr) return va::fail(VA_EINVAL, "va_paged_plan_words: NULL output");
-  *words = va::paged_layout(n_seqs, n_tokens).words;
+  *words = layout_of(n_seqs, n_tokens, hq, hkv, page_size, table_width).words;
   return VA_OK;
 }
 
@@ -92,7 +97,7 @@ extern "C" int va_paged_plan(const int32_t* q_lengths, const int32_t* kv_lengths
   int rc = check_step(n_seqs, n_tokens, hq, hkv, page_size, table_width, "va_paged_plan");
   if (rc) return rc;
   if (n_tokens == 0) return VA_OK;
-  const va::PagedLayout layout = va::paged_layout(n_seqs, n_tokens);
+  const va::PagedLayout layout = layout_of(n_seqs, n_tokens, hq, hkv, page_size, table_width);
   if (plan_words < layout.words)
     return va::fail(VA_ECAPACITY, "va_paged_plan: %lld words, need %lld", (long long)plan_words,
                     (long long)layout.words);
@@ -127,7 +132,7 @@ extern "C" int va_paged_append(const void* q, const void* k, const void* v, cons
     return rc;
   if (n_tokens == 0) return VA_OK;
   if ((rc = check_buffers({q, k, v, cos, sin, plan, q_out}, what))) return rc;
-  const va::PagedLayout layout = va::paged_layout(n_seqs, n_tokens);
+  const va::PagedLayout layout = layout_of(n_seqs, n_tokens, hq, hkv, page_size, table_width);
   va::PagedAppendArgs a{q, k, v, cos, sin, cos_batch_stride, cos_seq_stride, cos_token_stride,
                         cos_rows, plan + layout.seq, plan + layout.pos,
                         va::PagedPool{page_table, table_width, n_pages, shift_of(page_size),
@@ -144,7 +149,7 @@ extern "C" int va_paged_attention_workspace(int32_t n_seqs, int64_t n_tokens, in
                             "va_paged_attention_workspace");
   if (rc) return rc;
   if (bytes == nullptr) return va::fail(VA_EINVAL, "va_paged_attention_workspace: NULL output");
-  *bytes = 0;
+  *bytes = va::paged_workspace(layout_of(n_seqs, n_tokens, hq, hkv, page_size, table_width));
   return VA_OK;
 }
 
@@ -168,8 +173,8 @@ extern "C" int va_paged_attention(const void* q, const void* k_pages, const void
                        n_seqs, table_width, what)))
     return rc;
   if (n_tokens == 0) return VA_OK;
-  int64_t need = 0;
-  va_paged_attention_workspace(n_seqs, n_tokens, hq, hkv, page_size, table_width, &need);
+  const va::PagedLayout layout = layout_of(n_seqs, n_tokens, hq, hkv, page_size, table_width);
+  const int64_t need = va::paged_workspace(layout);
   if (workspace_bytes < need)
     return va::fail(VA_ECAPACITY, "%s: workspace %lld bytes, need %lld", what,
                     (long long)workspace_bytes, (long long)need);
@@ -178,8 +183,8 @@ extern "C" int va_paged_attention(const void* q, const void* k_pages, const void
   va::PagedAttnArgs a{q, k_pages, v_pages,
                       va::PagedPool{page_table, table_width, n_pages, shift_of(page_size),
                                     k_stride, v_stride},
-                      plan, va::paged_layout(n_seqs, n_tokens), n_seqs, (int)n_tokens, hq, hkv,
-                      scale, dtype, out, workspace, (hipStream_t)stream};
+                      plan, layout, n_seqs, (int)n_tokens, hq, hkv, scale, dtype, out,
+                      (float*)workspace, (hipStream_t)stream};
   return launched(va::launch_paged_attention(a), what);
 }
 

@@ -1,5 +1,22 @@
 // Attention of a step's new tokens over a paged key/value cache: the plan kernel that places every
-// row, and the attention.
+// row and splits the work, the attention, and the merge of split key ranges.
+//
+// An item is a tile of rows x a range of keys of one sequence and key/value head. Rows are (token, query
+// head of the group) pairs, so all query heads of a group read a key once. Scores and the running
+// maximum, sum and output of every row stay in fp32; weights are rounded to 16 bits for the product
+// with the values on v_mfma_f32_32x32x16, and their sum is taken over the rounded ones.
+//
+//   few rows (up to 32: single and drafted tokens)   four waves share the keys out, each with a K and
+//       a V tile of 32 keys of its own in LDS, no barrier until the waves meet at the end;
+//   many rows (prompt chunks)   128 rows, a strip of 32 per wave, 64-key tiles in two LDS stages that
+//       all waves read.
+//
+// Both copy pages straight from memory into LDS (16 rows of a page per wave and step, so a page border
+// never falls into a copy), rows past the end of the range as zeros: what earlier sequences left in a
+// page is never read. S^T = K Q^T has one row's scores in a lane and its half-wave partner; O^T += V^T
+// P^T reads V^T from the row-major tile with transposed LDS reads. A tile's rows are stored in groups of
+// 4 (1 KB, one copy instruction) 1088 bytes apart, chunk c of row r at c ^ (r & 3), so that both reads
+// touch all banks.
 #include "../../include/varlen_attn.h"
 #include "va_common.h"
 #include "va_kernels.h"
@@ -10,16 +27,60 @@ namespace va {
 
 namespace {
 
+// ------------------------------------------------------------------------------------------------
+// plan
+// ------------------------------------------------------------------------------------------------
 constexpr int PT = 1024;                    // threads of a planning work-group
 constexpr int SPT = kPagedMaxSeqs / PT;     // sequences per thread
 constexpr int kPlanRowsPerGroup = 4 * PT;   // rows that a planning work-group places
 
-// Every work-group sums the lengths by itself (at most 64 KB of them) and places its own rows: one
-// launch, nothing handed from one work-group to another.
+enum { kFew = 0, kMany = 1, kPad = 2 };     // kinds of items
+
+struct Item {
+  int token0, seq, pos0, head;        // the sequence's first row and its position; key/value head | kind << 16
+  int row, row_end, key, key_end;     // flattened rows of the sequence and keys
+  int part_row;                       // first workspace row of a split range's part, -1: whole
+  int pad[3];
+};
+static_assert(sizeof(Item) == 4 * kPagedItemWords, "item words");
+
+struct Merge {
+  int token0, head, row, rows;        // 1 to 8 flattened rows
+  int part_row, stride, parts, pad;   // workspace row of the first one in the first part; rows per part
+};
+static_assert(sizeof(Merge) == 4 * kPagedMergeWords, "merge words");
+
+// Tiles of a sequence and the keys that tile i sees.
+struct Rows {
+  int rows, tiles, pos0, kv;
+};
+__device__ inline Rows rows_of(int q, int rows_left, int kv, int max_keys, int group) {
+  Rows r;
+  r.kv = min(max(kv, 0), max_keys);
+  r.pos0 = r.kv - q;
+  r.rows = rows_left * group;
+  r.tiles = r.rows <= kPagedFewRows ? (r.rows > 0) : (r.rows + kPagedTileRows - 1) / kPagedTileRows;
+  return r;
+}
+__device__ inline int tile_keys(const Rows& r, int i, int group) {
+  const int end = min((i + 1) * kPagedTileRows, r.rows);
+  return max(r.pos0 + (end - 1) / group + 1, 0);
+}
+
+// Work-group 0 writes the work list, the others place the rows. Each sums the lengths by itself (at most
+// 64 KB of them): one launch, nothing handed from one work-group to another.
+//
+// A tile's keys are split into parts of at most `chunk` keys, equal but for the last: chunk is the
+// step's total over all tiles and heads divided by kPagedParts, so a step of few long tiles fills the
+// card with about that many parts, and one of many tiles splits only what is longer than its share.
+// Tiles of prompt chunks come first, the last (longest) ones of a sequence before its first.
 __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a) {
   __shared__ int s_cu[kPagedMaxSeqs + 1];
+  __shared__ int s_many[kPagedMaxSeqs], s_few[kPagedMaxSeqs];  // tiles before a sequence's, per kind
   __shared__ long long s_scan[PT / 64];
-  const int tid = threadIdx.x;
+  // of the tiles in hand: first item, first workspace row, first merge record; parts, their keys, all keys
+  __shared__ int s_first[PT], s_row[PT], s_merge[PT], s_parts[PT], s_chunk[PT], s_keys[PT];
+  const int tid = threadIdx.x, group = a.hq / a.hkv;
   int q[SPT];
   long long sum = 0;
 #pragma unroll
@@ -39,100 +100,745 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a) {
   if (tid == PT - 1 && a.n_seqs == kPagedMaxSeqs)
     s_cu[kPagedMaxSeqs] = (int)min(total, (long long)a.n_tokens);
   __syncthreads();
-  if (blockIdx.x == 0)
-    for (int s = tid; s <= a.n_seqs; s += PT) a.plan[s] = s_cu[s];
   const int rows = s_cu[a.n_seqs];
-  const int end = min((int)(blockIdx.x + 1) * kPlanRowsPerGroup, a.n_tokens);
-  for (int n = blockIdx.x * kPlanRowsPerGroup + tid; n < end; n += PT) {
-    int seq = -1, pos = -1;
-    if (n < rows) {
-      int lo = 0, hi = a.n_seqs - 1;  // last sequence that starts at or before row n
+  if (blockIdx.x > 0) {
+    const int first = (blockIdx.x - 1) * kPlanRowsPerGroup;
+    const int end = min(first + kPlanRowsPerGroup, a.n_tokens);
+    for (int n = first + tid; n < end; n += PT) {
+      int seq = -1, pos = -1;
+      if (n < rows) {
+        int lo = 0, hi = a.n_seqs - 1;  // last sequence that starts at or before row n
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (s_cu[mid] <= n) lo = mid;
+          else hi = mid - 1;
+        }
+        seq = lo;
+        pos = min(max(a.kv_lengths[lo], 0), a.max_keys) - max(a.q_lengths[lo], 0) + (n - s_cu[lo]);
+      }
+      a.plan[a.layout.seq + n] = seq;
+      a.plan[a.layout.pos + n] = pos;
+    }
+    return;
+  }
+  for (int s = tid; s <= a.n_seqs; s += PT) a.plan[s] = s_cu[s];
+
+  // Tiles of every sequence and the step's keys: the keys of a sequence's tiles grow evenly, so half the
+  // sum of the first and the last (each rounded up) times their number bounds their sum.
+  auto rows_at = [&](int s) {
+    return rows_of(max(a.q_lengths[s], 0), s_cu[s + 1] - s_cu[s], a.kv_lengths[s], a.max_keys, group);
+  };
+  long long many = 0, few = 0, keys = 0;
+#pragma unroll
+  for (int i = 0; i < SPT; ++i) {
+    const int s = tid * SPT + i;
+    if (s >= a.n_seqs || s_cu[s + 1] == s_cu[s]) continue;
+    const Rows r = rows_at(s);
+    if (r.rows > kPagedFewRows) many += r.tiles;
+    else few += r.tiles;
+    const int step = kPagedTileRows / group + 2;
+    keys += (tile_keys(r, 0, group) + (long long)tile_keys(r, r.tiles - 1, group) + step + 1) *
+            r.tiles / 2 + 1;
+  }
+  long long n_many, n_few, all_keys;
+  long long first_many = block_exclusive_sum<PT / 64>(many, s_scan, n_many);
+  long long first_few = block_exclusive_sum<PT / 64>(few, s_scan, n_few);
+  block_exclusive_sum<PT / 64>(keys, s_scan, all_keys);
+#pragma unroll
+  for (int i = 0; i < SPT; ++i) {
+    const int s = tid * SPT + i;
+    if (s >= a.n_seqs) continue;
+    s_many[s] = (int)first_many;
+    s_few[s] = (int)first_few;
+    const Rows r = rows_at(s);
+    if (r.rows > kPagedFewRows) first_many += r.tiles;
+    else first_few += r.tiles;
+  }
+  __syncthreads();
+  const long long per_part = (all_keys * a.hkv + kPagedParts - 1) / kPagedParts;
+  const int chunk =
+      (int)((max(per_part, (long long)kPagedMinKeys) + kPagedChunkKeys - 1) / kPagedChunkKeys) *
+      kPagedChunkKeys;
+  Item* items = reinterpret_cast<Item*>(a.plan + a.layout.items);
+  Merge* merges = reinterpret_cast<Merge*>(a.plan + a.layout.merges);
+  const int n_tiles = (int)(n_many + n_few);
+  int item0 = 0, part0 = 0, merge0 = 0;  // so far
+  // A tile's place: its sequence (the last one whose tiles start at or before it) and first row.
+  struct Place {
+    int seq, row;
+  };
+  auto place_of = [&](int j) {
+    const bool is_many = j < n_many;
+    const int number = is_many ? (int)n_many - 1 - j : j - (int)n_many;
+    const int* first = is_many ? s_many : s_few;
+    int lo = 0, hi = a.n_seqs - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (first[mid] <= number) lo = mid;
+      else hi = mid - 1;
+    }
+    return Place{lo, (number - first[lo]) * kPagedTileRows};
+  };
+  for (int base = 0; base < n_tiles; base += PT) {
+    const int j = base + tid;
+    int parts = 0, n_keys = 0, c = 0, n_rows = 0;
+    if (j < n_tiles) {
+      const Place pl = place_of(j);
+      const Rows r = rows_at(pl.seq);
+      n_keys = tile_keys(r, pl.row / kPagedTileRows, group);
+      n_rows = min(kPagedTileRows, r.rows - pl.row);
+      parts = max(1, (n_keys + chunk - 1) / chunk);
+      c = ((n_keys + parts - 1) / parts + kPagedChunkKeys - 1) / kPagedChunkKeys * kPagedChunkKeys;
+      if (parts > 1) parts = (n_keys + c - 1) / c;
+    }
+    long long n_items, n_parts, n_merges;
+    const int records = parts < 2 ? 0 : parts <= 8 ? (n_rows + 7) / 8 : n_rows;
+    s_first[tid] = (int)block_exclusive_sum<PT / 64>((long long)parts * a.hkv, s_scan, n_items);
+    s_row[tid] = (int)block_exclusive_sum<PT / 64>((long long)(parts < 2 ? 0 : parts * n_rows) * a.hkv,
+                                                   s_scan, n_parts);
+    s_merge[tid] = (int)block_exclusive_sum<PT / 64>((long long)records * a.hkv, s_scan, n_merges);
+    s_parts[tid] = parts;
+    s_chunk[tid] = c;
+    s_keys[tid] = n_keys;
+    __syncthreads();
+    const int here = min(PT, n_tiles - base);
+    for (int i = tid; i < (int)n_items; i += PT) {
+      int lo = 0, hi = here - 1;
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (s_cu[mid] <= n) lo = mid;
+        if (s_first[mid] <= i) lo = mid;
         else hi = mid - 1;
       }
-      seq = lo;
-      const int kv = min(max(a.kv_lengths[lo], 0), a.max_keys);
-      pos = kv - max(a.q_lengths[lo], 0) + (n - s_cu[lo]);
+      const Place pl = place_of(base + lo);
+      const Rows r = rows_at(pl.seq);
+      const int in = i - s_first[lo], head = in % a.hkv, part = in / a.hkv;
+      const int p = s_parts[lo], count = min(kPagedTileRows, r.rows - pl.row);
+      Item it;
+      it.token0 = s_cu[pl.seq];
+      it.seq = pl.seq;
+      it.pos0 = r.pos0;
+      it.head = head | (base + lo < n_many ? kMany : kFew) << 16;
+      it.row = pl.row;
+      it.row_end = pl.row + count;
+      it.key = part * s_chunk[lo];
+      it.key_end = min(it.key + s_chunk[lo], s_keys[lo]);
+      it.part_row = p < 2 ? -1 : part0 + s_row[lo] + (head * p + part) * count;
+      if (item0 + i < a.layout.max_items) items[item0 + i] = it;
     }
-    a.plan[a.layout.seq + n] = seq;
-    a.plan[a.layout.pos + n] = pos;
+    for (int i = tid; i < (int)n_merges; i += PT) {
+      int lo = 0, hi = here - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (s_merge[mid] <= i) lo = mid;
+        else hi = mid - 1;
+      }
+      const Place pl = place_of(base + lo);
+      const Rows r = rows_at(pl.seq);
+      const int p = s_parts[lo], count = min(kPagedTileRows, r.rows - pl.row);
+      const int each = p <= 8 ? 8 : 1, per_head = (count + each - 1) / each;
+      const int in = i - s_merge[lo], head = in / per_head, first = in % per_head * each;
+      Merge m;
+      m.token0 = s_cu[pl.seq];
+      m.head = head;
+      m.row = pl.row + first;
+      m.rows = min(each, count - first);
+      m.part_row = part0 + s_row[lo] + head * p * count + first;
+      m.stride = count;
+      m.parts = p;
+      m.pad = 0;
+      if (merge0 + i < a.layout.max_merges) merges[merge0 + i] = m;
+    }
+    item0 += (int)n_items;
+    part0 += (int)n_parts;
+    merge0 += (int)n_merges;
+    __syncthreads();
+  }
+  const int n_pad = (a.n_tokens - rows + kPagedPadRows - 1) / kPagedPadRows;
+  for (int i = tid; i < n_pad; i += PT) {
+    Item it{};
+    it.head = kPad << 16;
+    it.row = rows + i * kPagedPadRows;
+    it.row_end = min(it.row + kPagedPadRows, a.n_tokens);
+    if (item0 + i < a.layout.max_items) items[item0 + i] = it;
+  }
+  if (tid == 0) {
+    a.plan[a.layout.counts] = (int)min((long)(item0 + n_pad), (long)a.layout.max_items);
+    a.plan[a.layout.counts + 1] = (int)min((long)merge0, (long)a.layout.max_merges);
   }
 }
 
-// One wave per row and query head, 16 lanes per key, four keys at a time: each 16-lane group keeps
-// the running maximum and sum of its keys, the groups meet at the end.
-template <class E>
-__global__ __launch_bounds__(256) void paged_row_kernel(PagedAttnArgs a) {
-  constexpr int D = kHeadDim;
-  const long item = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (item >= (long)a.n_tokens * a.hq) return;
-  const int row = (int)(item / a.hq), h = (int)(item % a.hq), lane = threadIdx.x & 63;
-  const int kvh = h / (a.hq / a.hkv), grp = lane >> 4, d0 = 8 * (lane & 15);
-  const int seq = a.plan[a.layout.seq + row];
-  const int keys = seq < 0 ? 0 : a.plan[a.layout.pos + row] + 1;
-  const int ps = 1 << a.pool.page_shift;
-  const uint16_t* k = (const uint16_t*)a.k;
-  const uint16_t* v = (const uint16_t*)a.v;
-  float q[8], o[8];
-  const u32x4 qv = gload16((const uint16_t*)a.q + item * D + d0);
+// ------------------------------------------------------------------------------------------------
+// attention
+// ------------------------------------------------------------------------------------------------
+constexpr int NW = 4, NT = 64 * NW;
+constexpr int D = kHeadDim;
+constexpr int GRP = 4 * D + 32;  // halfs from one group of 4 rows to the next
+constexpr int TILE = 16 * GRP;   // a 64-key K or V tile
+constexpr int LDS_HALFS = 4 * TILE;
+constexpr float kRescaleLog2 = 8.f;  // many rows: the maximum moves when a tile exceeds it by 2^8
+
+// Read offsets (halfs) inside a tile. K (A operand of S^T): row perm32(l32), chunk 2 kk + hi. V^T: row
+// 8 hi + 2 (src >> 2) + e (+ 16 c), chunk 8 (grp & 1) + 2 db + (sg >> 1): registers [8 c, 8 c + 8) of
+// accumulator db then hold d = 16 db + 64 c + 8 hi + 0..7 of the lane's row.
+struct Offsets {
+  int k[2], v[2][2];
+};
+__device__ inline Offsets offsets_of(int lane) {
+  Offsets o;
+  const int l32 = lane & 31, hi = lane >> 5, src = lane & 15, grp = lane >> 4;
+  const int r = perm32(l32);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    q[e] = E::to_f32(half_of(qv, e)) * a.scale * kLog2e;
-    o[e] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  for (int t = grp; t < keys; t += 4) {
-    const int page = a.pool.table[(long)seq * a.pool.table_width + (t >> a.pool.page_shift)];
-    u32x4 kv = u32x4{0u, 0u, 0u, 0u}, vv = kv;
-    if (page >= 0 && page < a.pool.n_pages) {
-      const long in = ((long)kvh * ps + (t & (ps - 1))) * D + d0;
-      kv = gload16(k + page * a.pool.k_stride + in);
-      vv = gload16(v + page * a.pool.v_stride + in);
+  for (int p = 0; p < 2; ++p) o.k[p] = (r >> 2) * GRP + (r & 3) * D + 8 * ((2 * p + hi) ^ (r & 3));
+  const int sg = (((src & 3) & 1) << 1) | ((src & 3) >> 1);
+#pragma unroll
+  for (int p = 0; p < 2; ++p)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int rr = 8 * hi + 2 * (src >> 2) + e;
+      o.v[p][e] = (rr >> 2) * GRP + (rr & 3) * D +
+                  8 * (8 * (grp & 1) + ((2 * p + (sg >> 1)) ^ (rr & 3))) + 4 * (sg & 1);
     }
-    float s = 0.f;
+  return o;
+}
+__device__ inline u32x4 read_k(const lds_u16* kb, const Offsets& o, int kk, int b) {
+  return ld128(kb + o.k[kk & 1] + 32 * (kk >> 1) + 8 * b * GRP);
+}
+__device__ inline u32x4 read_v(const lds_u16* vb, const Offsets& o, int i) {  // i = (b, c, db)
+  const lds_u16* p = vb + (8 * (i >> 3) + 4 * ((i >> 2) & 1)) * GRP + 32 * ((i & 3) >> 1);
+  const u32x2 x = ldtr(p + o.v[i & 1][0]), y = ldtr(p + o.v[i & 1][1]);
+  return u32x4{x[0], x[1], y[0], y[1]};
+}
+
+// Buffer descriptors and items in scalar registers (the loads that they come from are not always).
+__device__ inline int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ inline u32x4 scalar_rsrc(const void* base, long bytes) {
+  u32x4 r = make_rsrc4(base, bytes);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s = fmaf(q[e], E::to_f32(half_of(kv, e)), s);
-    s = sum_rows16(s);
-    const float m_new = fmaxf(m, s);
-    const float m_use = m_new == -INFINITY ? 0.f : m_new;
-    const float alpha = fast_exp2(m - m_use), p = fast_exp2(s - m_use);
-    m = m_new;
-    l = l * alpha + p;
+  for (int i = 0; i < 4; ++i) r[i] = (uint32_t)scalar((int)r[i]);
+  return r;
+}
+
+struct State {
+  f32x16 o[4];
+  float m, l;  // the row's running maximum (log2 units) and this half-wave's share of its sum
+};
+__device__ inline void start(State& st) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = fmaf(o[e], alpha, p * E::to_f32(half_of(vv, e)));
+  for (int db = 0; db < 4; ++db) st.o[db] = f32x16{};
+  st.m = -INFINITY;
+  st.l = 0.f;
+}
+
+// S^T of one tile of 32 BLOCKS keys, each K operand read 4 ahead.
+template <class E, int BLOCKS>
+__device__ inline void scores(const lds_u16* kb, const Offsets& o, const u32x4 (&qf)[8], f32x16 (&s)[BLOCKS]) {
+  constexpr int N = 8 * BLOCKS;
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b) s[b] = f32x16{};
+  u32x4 ka[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) ka[i] = read_k(kb, o, i / BLOCKS, i % BLOCKS);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    s[i % BLOCKS] = E::mfma(ka[i & 3], qf[i / BLOCKS], s[i % BLOCKS]);
+    if (i + 4 < N) ka[i & 3] = read_k(kb, o, (i + 4) / BLOCKS, (i + 4) % BLOCKS);
+  }
+  if constexpr (BLOCKS == 2) {
+    VA_SCHED(kSchedDsRead, 4);
+#pragma unroll
+    for (int i = 0; i < N - 4; ++i) {
+      VA_SCHED(kSchedMfma, 1);
+      VA_SCHED(kSchedDsRead, 1);
+    }
+    VA_SCHED(kSchedMfma, 4);
+  }
+}
+
+// Mask (keys past `lim` of the tile), running maximum and sum, weights of one tile. The maximum moves
+// when some row's tile maximum exceeds its own by more than 2^margin.
+template <class E, int BLOCKS>
+__device__ inline void soften(f32x16 (&s)[BLOCKS], bool mask, int lim, int hi, float scale_log2,
+                              float margin, State& st, u32x4 (&pf)[BLOCKS][2]) {
+  if (mask) {
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (32 * b + reg_row(j, hi) > lim) s[b][j] = -INFINITY;
+  }
+  float mt = -INFINITY;
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) mt = fmaxf(mt, s[b][j]);
+  mt = max_with_other_half(mt) * scale_log2;
+  if (__builtin_amdgcn_ballot_w64(mt > st.m + margin) != 0) {
+    const float m_new = fmaxf(st.m, mt);
+    const float alpha = fast_exp2(st.m - (m_new == -INFINITY ? 0.f : m_new));
+    st.m = m_new;
+    st.l *= alpha;
+#pragma unroll
+    for (int db = 0; db < 4; ++db) st.o[db] *= alpha;
+  }
+  const float m_use = st.m == -INFINITY ? 0.f : st.m;
+  float rs = 0.f;
+#pragma unroll
+  for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float p[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p[e] = fast_exp2(fmaf(s[b][8 * c + e], scale_log2, -m_use));
+      pf[b][c] = pack8_tr<E>(p);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) rs = E::sum2(pf[b][c][w], rs);
+    }
+  st.l += rs;
+}
+
+// O^T += V^T P^T; the first four V operands are in `va`, the others are read 4 ahead.
+template <class E, int BLOCKS>
+__device__ inline void weigh(const lds_u16* vb, const Offsets& o, const u32x4 (&pf)[BLOCKS][2],
+                             u32x4 (&va)[4], State& st) {
+  constexpr int N = 8 * BLOCKS;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    st.o[i & 3] = E::mfma(va[i & 3], pf[i >> 3][(i >> 2) & 1], st.o[i & 3]);
+    if (i + 4 < N) va[i & 3] = read_v(vb, o, i + 4);
+  }
+}
+
+// 16 rows of a page: where they lie in the pools, and how many of them the range holds.
+struct PageRows {
+  const uint16_t* k;
+  const uint16_t* v;
+  long bytes;
+};
+__device__ inline PageRows page_rows(const PagedAttnArgs& a, int page, int head, int pos, int end) {
+  PageRows r;
+  const int shift = a.pool.page_shift;
+  const bool there = page >= 0 && page < a.pool.n_pages;
+  const long in = ((long)(head << shift) + (pos & ((1 << shift) - 1))) * D;
+  const long p = there ? page : 0;
+  r.k = (const uint16_t*)a.k + p * a.pool.k_stride + in;
+  r.v = (const uint16_t*)a.v + p * a.pool.v_stride + in;
+  r.bytes = there ? (long)max(0, min(end - pos, 16)) * (D * 2) : 0;
+  return r;
+}
+
+// An item's rows: row r of the sequence is token r / group, query head r % group of the group.
+// Divisions of small numbers by the group: exact in fp32 (rows below 2^13, half a unit to spare).
+struct RowMap {
+  int token, rest, group;  // of the item's first row
+  float inv;
+  __device__ RowMap(int row, int g) : token(row / g), rest(row % g), group(g), inv(1.f / (float)g) {}
+  __device__ inline void at(int r, int& tok, int& h) const {
+    const int x = r + rest, t = (int)(((float)x + 0.5f) * inv);
+    tok = token + t;
+    h = x - t * group;
+  }
+};
+
+template <class E>
+__device__ inline void few_rows(const PagedAttnArgs& a, const Item& it, lds_u16* smem, char* smem_raw) {
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int head = it.head & 0xffff, group = a.hq / a.hkv, n_rows = it.row_end - it.row;
+  const float scale_log2 = a.scale * kLog2e;
+  const RowMap map(it.row, group);
+  const Offsets off = offsets_of(lane);
+  const int32_t* table = a.pool.table + (long)it.seq * a.pool.table_width;
+  const int n_tiles = (it.key_end - it.key + 31) >> 5;
+
+  // This wave's rows: all waves hold the same queries.
+  u32x4 qf[8];
+  int my_lim = -1;
+  {
+    int tok, h;
+    map.at(l32, tok, h);
+    if (l32 < n_rows) my_lim = it.pos0 + tok;
+    const uint16_t* q = (const uint16_t*)a.q + ((long)(it.token0 + tok) * a.hq + head * group + h) * D;
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) {
+      qf[kk] = u32x4{0u, 0u, 0u, 0u};
+      if (l32 < n_rows) qf[kk] = gload16(q + 16 * kk + 8 * hi);
+    }
+  }
+  // Page numbers of this wave's next 32 tiles, two per tile (16 rows each): lane 2 i + h holds half h.
+  auto load_pages = [&](int t) {
+    const int pos = it.key + 32 * (t + NW * (lane >> 1)) + 16 * (lane & 1);
+    return pos < it.key_end ? table[pos >> a.pool.page_shift] : -1;
+  };
+  const uint32_t kl = lds_addr(smem + wave * (TILE)), vl = lds_addr(smem + wave * TILE + TILE / 2);
+  const lds_u16* kb = smem + wave * TILE;
+  const lds_u16* vb = kb + TILE / 2;
+  const int c_row = lane >> 4, coff = (c_row * D + 8 * ((lane & 15) ^ c_row)) * 2;
+  auto copy = [&](const uint16_t* const (&base)[2], const long (&bytes)[2], uint32_t dst) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const u32x4 r = scalar_rsrc(base[h], bytes[h]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) dma16_opaque(r, dst + (4 * h + j) * GRP * 2, coff + j * 4 * D * 2);
+    }
+  };
+  State st;
+  start(st);
+  int pages = 0, i = 0;  // i: this wave's tiles so far
+  const uint16_t *kp[2], *vp[2];
+  long bytes[2];
+  auto locate = [&](int t, int n) {  // this wave's n-th tile, tile t of the item
+    if ((n & 31) == 0) pages = load_pages(t);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int page = __builtin_amdgcn_readlane(pages, 2 * (n & 31) + h);
+      const PageRows r = page_rows(a, page, head, it.key + 32 * t + 16 * h, it.key_end);
+      kp[h] = r.k;
+      vp[h] = r.v;
+      bytes[h] = r.bytes;
+    }
+  };
+  if (wave < n_tiles) {
+    locate(wave, 0);
+    copy(kp, bytes, kl);
+    copy(vp, bytes, vl);
   }
 #pragma unroll
-  for (int off = 16; off < 64; off <<= 1) {
-    const float m_b = __shfl_xor(m, off), m_tot = fmaxf(m, m_b);
-    const float m_use = m_tot == -INFINITY ? 0.f : m_tot;
-    const float ca = fast_exp2(m - m_use), cb = fast_exp2(m_b - m_use);
-    m = m_tot;
-    l = l * ca + __shfl_xor(l, off) * cb;
+  for (int kk = 0; kk < 8; ++kk) settle(qf[kk]);
+  const int first_lim = it.pos0 + map.token;  // the first row's last key: keys past it need the mask
+  for (int t = wave; t < n_tiles; t += NW, ++i) {
+    const bool more = t + NW < n_tiles;
+    asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // this tile's K; its V (8 copies) may be in flight
+    f32x16 s[1];
+    scores<E, 1>(kb, off, qf, s);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K read: its place is free
+    if (more) {
+      locate(t + NW, i + 1);
+      copy(kp, bytes, kl);
+    }
+    const int kv0 = it.key + 32 * t;
+    u32x4 pf[1][2];
+    soften<E, 1>(s, kv0 + 31 > first_lim, my_lim - kv0, hi, scale_log2, 0.f, st, pf);
+    if (more) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // V; the next K in flight
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    u32x4 va[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = o[e] * ca + __shfl_xor(o[e], off) * cb;
+    for (int j = 0; j < 4; ++j) va[j] = read_v(vb, off, j);
+    weigh<E, 1>(vb, off, pf, va, st);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V read
+    if (more) copy(vp, bytes, vl);
+  }
+
+  // The waves meet: fp32 rows of 132 words per wave, then their maxima and sums.
+  constexpr int LT = D + 4;
+  float* xo = reinterpret_cast<float*>(smem_raw);
+  float* xs = xo + NW * 32 * LT;
+  static_assert((NW * 32 * LT + NW * 32 * 2) * 4 <= LDS_HALFS * 2, "the waves' rows fit in LDS");
+  __syncthreads();  // every wave has read its tiles
+  const float l_row = sum_with_other_half(st.l);
+  if (l32 < n_rows) {
+    float* row = xo + (wave * 32 + l32) * LT;
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float* p = row + 16 * db + 64 * c + 8 * hi;
+        *reinterpret_cast<f32x4*>(p) = f32x4{st.o[db][8 * c], st.o[db][8 * c + 1],
+                                             st.o[db][8 * c + 2], st.o[db][8 * c + 3]};
+        *reinterpret_cast<f32x4*>(p + 4) = f32x4{st.o[db][8 * c + 4], st.o[db][8 * c + 5],
+                                                 st.o[db][8 * c + 6], st.o[db][8 * c + 7]};
+      }
+    if (hi == 0) {
+      xs[2 * (wave * 32 + l32)] = st.m;
+      xs[2 * (wave * 32 + l32) + 1] = l_row;
+    }
+  }
+  __syncthreads();
+  const int r = tid >> 3, d0 = 16 * (tid & 7);
+  if (r >= n_rows) return;
+  float m[NW], l = 0.f, m_all = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) m_all = fmaxf(m_all, m[w] = xs[2 * (w * 32 + r)]);
+  const float m_use = m_all == -INFINITY ? 0.f : m_all;
+  f32x4 o[4] = {};
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    const float c = fast_exp2(m[w] - m_use);
+    l += c * xs[2 * (w * 32 + r) + 1];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      o[e] += c * *reinterpret_cast<const f32x4*>(xo + (w * 32 + r) * LT + d0 + 4 * e);
+  }
+  if (it.part_row >= 0) {
+    const long row = it.part_row + r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      *reinterpret_cast<f32x4*>(a.workspace + row * D + d0 + 4 * e) = o[e];
+    if (d0 == 0)
+      *reinterpret_cast<f32x2*>(a.workspace + a.layout.max_part_rows * D + 2 * row) = f32x2{m_all, l};
+    return;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  if (grp == 0)
-    gstore16((uint16_t*)a.out + item * D + d0,
-             pack8<E>(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv, o[4] * inv, o[5] * inv,
-                      o[6] * inv, o[7] * inv));
+  int tok, h;
+  map.at(r, tok, h);
+  uint16_t* out = (uint16_t*)a.out + ((long)(it.token0 + tok) * a.hq + head * group + h) * D + d0;
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    gstore16(out + 8 * e, pack8<E>(o[2 * e][0] * inv, o[2 * e][1] * inv, o[2 * e][2] * inv,
+                                   o[2 * e][3] * inv, o[2 * e + 1][0] * inv, o[2 * e + 1][1] * inv,
+                                   o[2 * e + 1][2] * inv, o[2 * e + 1][3] * inv));
+}
+
+template <class E>
+__device__ inline void many_rows(const PagedAttnArgs& a, const Item& it, lds_u16* smem) {
+  constexpr int KEYS = 64, STAGE = 2 * TILE;
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int head = it.head & 0xffff, group = a.hq / a.hkv, n_rows = it.row_end - it.row;
+  const float scale_log2 = a.scale * kLog2e;
+  const RowMap map(it.row, group);
+  const Offsets off = offsets_of(lane);
+  const int32_t* table = a.pool.table + (long)it.seq * a.pool.table_width;
+  const int n_tiles = (it.key_end - it.key + KEYS - 1) / KEYS;
+  const int c_row = lane >> 4;
+
+  // Copies, in tile order: wave w moves rows [16 w, 16 w + 16) of K and of V, which lie in one page; the
+  // page numbers of its next 64 tiles are in its lanes.
+  int pages = 0, tc = 0;
+  const int coff = (c_row * D + 8 * ((lane & 15) ^ c_row)) * 2;
+  auto copy_next = [&](uint32_t dst) {
+    if ((tc & 63) == 0) {
+      const int pos = it.key + KEYS * (tc + lane) + 16 * wave;
+      pages = pos < it.key_end ? table[pos >> a.pool.page_shift] : -1;
+    }
+    const int page = __builtin_amdgcn_readlane(pages, tc & 63);
+    const PageRows r = page_rows(a, page, head, it.key + KEYS * tc + 16 * wave, it.key_end);
+    const u32x4 rk = scalar_rsrc(r.k, r.bytes), rv = scalar_rsrc(r.v, r.bytes);
+    dst += 4 * wave * GRP * 2;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) dma16_opaque(rk, dst + j * GRP * 2, coff + j * 4 * D * 2);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) dma16_opaque(rv, dst + (TILE + j * GRP) * 2, coff + j * 4 * D * 2);
+    ++tc;
+  };
+
+  // Q from stage 1 on (32 row groups), tile 0 into stage 0; every lane reads its row.
+  const long q0 = ((long)(it.token0 + map.token) * a.hq + head * group) * D;  // the first row's token
+  {
+    const long span = (long)((map.rest + n_rows - 1) / group * a.hq + group) * D * 2;
+    const u32x4 rq = scalar_rsrc((const uint16_t*)a.q + q0, span);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int r = 32 * wave + 4 * j + c_row;
+      int tok, h;
+      map.at(r, tok, h);
+      const int o = (((tok - map.token) * a.hq + h) * D + 8 * ((lane & 15) ^ c_row)) * 2;
+      dma16_opaque(rq, lds_addr(smem + STAGE + (8 * wave + j) * GRP), r < n_rows ? o : 0x7fffff00);
+    }
+  }
+  if (n_tiles > 0) copy_next(lds_addr(smem));
+  wait_vmcnt<0>();
+  __syncthreads();
+  u32x4 qf[8];
+  {
+    const lds_u16* qt = smem + STAGE + (8 * wave + (l32 >> 2)) * GRP + (l32 & 3) * D;
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk)
+      qf[kk] = ld128(qt + 8 * ((2 * (kk & 1) + hi) ^ (l32 & 3)) + 32 * (kk >> 1));
+  }
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) settle(qf[kk]);
+  __syncthreads();  // every wave holds its rows before the second stage is written
+
+  int my_tok, my_h;
+  map.at(32 * wave + l32, my_tok, my_h);
+  const int my_lim = it.pos0 + my_tok;
+  const int left = n_rows - 32 * wave;  // rows of this strip
+  const int first_lim = __builtin_amdgcn_readfirstlane(my_lim);
+  const int last_lim = __builtin_amdgcn_readlane(my_lim, max(0, min(31, left - 1)));
+  const int n_live = left <= 0 || last_lim < it.key
+                         ? 0
+                         : min((last_lim - it.key) / KEYS + 1, n_tiles);
+  State st;
+  start(st);
+  int t = 0;
+  for (; t < n_live; ++t) {
+    const lds_u16* kb = smem + (t & 1) * STAGE;
+    f32x16 s[2];
+    scores<E, 2>(kb, off, qf, s);
+    if (t + 1 < n_tiles) copy_next(lds_addr(smem + ((t + 1) & 1) * STAGE));
+    u32x4 va[4], pf[2][2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) va[j] = read_v(kb + TILE, off, j);
+    const int kv0 = it.key + KEYS * t;
+    soften<E, 2>(s, kv0 + KEYS - 1 > first_lim, my_lim - kv0, hi, scale_log2, kRescaleLog2, st, pf);
+    weigh<E, 2>(kb + TILE, off, pf, va, st);
+    wait_vmcnt<0>();
+    __syncthreads();
+  }
+  for (; t < n_tiles; ++t) {  // past this strip's keys the wave only copies
+    if (t + 1 < n_tiles) copy_next(lds_addr(smem + ((t + 1) & 1) * STAGE));
+    wait_vmcnt<0>();
+    __syncthreads();
+  }
+
+  const float l_row = sum_with_other_half(st.l);
+  if (it.part_row >= 0) {
+    if (l32 >= left) return;
+    const long row = it.part_row + 32 * wave + l32;
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float* p = a.workspace + row * D + 16 * db + 64 * c + 8 * hi;
+        *reinterpret_cast<f32x4*>(p) = f32x4{st.o[db][8 * c], st.o[db][8 * c + 1],
+                                             st.o[db][8 * c + 2], st.o[db][8 * c + 3]};
+        *reinterpret_cast<f32x4*>(p + 4) = f32x4{st.o[db][8 * c + 4], st.o[db][8 * c + 5],
+                                                 st.o[db][8 * c + 6], st.o[db][8 * c + 7]};
+      }
+    if (hi == 0)
+      *reinterpret_cast<f32x2*>(a.workspace + a.layout.max_part_rows * D + 2 * row) = f32x2{st.m, l_row};
+    return;
+  }
+  const float inv = l_row == 0.f ? 0.f : 1.f / l_row;
+  u32x4 w[8];  // chunk db + 4 c: d = 16 db + 64 c + 8 hi + 0..7 of the lane's row
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      w[db + 4 * c] = pack8<E>(st.o[db][8 * c] * inv, st.o[db][8 * c + 1] * inv,
+                               st.o[db][8 * c + 2] * inv, st.o[db][8 * c + 3] * inv,
+                               st.o[db][8 * c + 4] * inv, st.o[db][8 * c + 5] * inv,
+                               st.o[db][8 * c + 6] * inv, st.o[db][8 * c + 7] * inv);
+  static_assert(NW * 32 * (8 * 16 + 8) <= LDS_HALFS, "row tiles fit in LDS");
+  // (the last barrier has passed: no wave reads a tile any more)
+  store_rows32<16>(smem + wave * 32 * (8 * 16 + 8), w, lane,
+                   [&](int r) {
+                     int tok, h;
+                     map.at(32 * wave + r, tok, h);
+                     return (uint16_t*)a.out + ((long)(it.token0 + tok) * a.hq + head * group + h) * D;
+                   },
+                   left);
+}
+
+template <class E>
+__global__ __launch_bounds__(NT, 2) void paged_attn_kernel(PagedAttnArgs a) {
+  __shared__ __attribute__((aligned(16))) uint16_t smem_raw[LDS_HALFS];
+  lds_u16* smem = (lds_u16*)smem_raw;
+  if ((int)blockIdx.x >= a.plan[a.layout.counts]) return;
+  const Item* const p = reinterpret_cast<const Item*>(a.plan + a.layout.items) + blockIdx.x;
+  const Item it{scalar(p->token0), scalar(p->seq), scalar(p->pos0), scalar(p->head), scalar(p->row),
+                scalar(p->row_end), scalar(p->key), scalar(p->key_end), scalar(p->part_row), {}};
+  const int kind = it.head >> 16;
+  if (kind == kMany) {
+    many_rows<E>(a, it, smem);
+  } else if (kind == kFew) {
+    few_rows<E>(a, it, smem, (char*)smem_raw);
+  } else {
+    u32x4* out = (u32x4*)a.out + (long)it.row * a.hq * (D / 8);
+    const int chunks = (it.row_end - it.row) * a.hq * (D / 8);
+    for (int i = threadIdx.x; i < chunks; i += NT) out[i] = u32x4{0u, 0u, 0u, 0u};
+  }
+}
+
+// Parts of split key ranges: a record of 8 rows and up to 8 parts has 32 lanes (4 elements each) per row,
+// a record of one row and more parts shares the parts out to the 8 groups of 32 lanes.
+constexpr int kMergeGroups = 1024;
+template <class E>
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a) {
+  __shared__ f32x4 s_o[8][32];
+  __shared__ float s_m[8], s_l[8];
+  const int n = a.plan[a.layout.counts + 1];
+  const Merge* merges = reinterpret_cast<const Merge*>(a.plan + a.layout.merges);
+  const float* ml = a.workspace + a.layout.max_part_rows * D;
+  const int g = threadIdx.x >> 5, d0 = 4 * (threadIdx.x & 31), group = a.hq / a.hkv;
+  for (int i = blockIdx.x; i < n; i += gridDim.x) {
+    const Merge mg = merges[i];
+    const bool spread = mg.parts > 8;
+    const int r = spread ? 0 : g;
+    float m = -INFINITY, l = 0.f;
+    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (spread || g < mg.rows) {
+      const int from = spread ? g : 0, step = spread ? 8 : 1;
+      for (int p0 = from; p0 < mg.parts; p0 += 8 * step) {
+        f32x2 x[8];
+        f32x4 y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int p = p0 + e * step;
+          const long row = mg.part_row + r + (long)min(p, mg.parts - 1) * mg.stride;
+          x[e] = *reinterpret_cast<const f32x2*>(ml + 2 * row);
+          if (p >= mg.parts) x[e] = f32x2{-INFINITY, 0.f};
+          y[e] = *reinterpret_cast<const f32x4*>(a.workspace + row * D + d0);
+        }
+        float m_new = m;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m_new = fmaxf(m_new, x[e][0]);
+        const float m_use = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = fast_exp2(m - m_use);
+        m = m_new;
+        l *= alpha;
+        o *= alpha;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float c = p0 + e * step < mg.parts ? fast_exp2(x[e][0] - m_use) : 0.f;
+          l = fmaf(c, x[e][1], l);
+          if (c != 0.f) o += c * y[e];
+        }
+      }
+    }
+    if (spread) {
+      s_o[g][threadIdx.x & 31] = o;
+      if (d0 == 0) {
+        s_m[g] = m;
+        s_l[g] = l;
+      }
+      __syncthreads();
+      if (g == 0) {
+        float m_all = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) m_all = fmaxf(m_all, s_m[w]);
+        const float m_use = m_all == -INFINITY ? 0.f : m_all;
+        l = 0.f;
+        o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+          const float c = fast_exp2(s_m[w] - m_use);
+          l = fmaf(c, s_l[w], l);
+          o += c * s_o[w][threadIdx.x & 31];
+        }
+      }
+      __syncthreads();
+    }
+    if (spread ? g == 0 : g < mg.rows) {
+      const int row = mg.row + r, tok = row / group, h = row % group;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      uint16_t* out = (uint16_t*)a.out + ((long)(mg.token0 + tok) * a.hq + mg.head * group + h) * D + d0;
+      __builtin_nontemporal_store(u32x2{pack2<E>(o[0] * inv, o[1] * inv), pack2<E>(o[2] * inv, o[3] * inv)},
+                                  reinterpret_cast<u32x2*>(out));
+    }
+  }
+}
+
+template <class E>
+hipError_t launch_attention(const PagedAttnArgs& a) {
+  hipLaunchKernelGGL(paged_attn_kernel<E>, dim3((unsigned)a.layout.max_items), dim3(NT), 0, a.stream, a);
+  if (a.layout.max_merges > 0) {
+    const unsigned groups = (unsigned)(a.layout.max_merges < kMergeGroups ? a.layout.max_merges : kMergeGroups);
+    hipLaunchKernelGGL(paged_merge_kernel<E>, dim3(groups), dim3(256), 0, a.stream, a);
+  }
+  return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t launch_paged_plan(const PagedPlanArgs& a) {
-  const int groups = max(1, (a.n_tokens + kPlanRowsPerGroup - 1) / kPlanRowsPerGroup);
+  const int groups = 1 + (a.n_tokens + kPlanRowsPerGroup - 1) / kPlanRowsPerGroup;
   hipLaunchKernelGGL(paged_plan_kernel, dim3(groups), dim3(PT), 0, a.stream, a);
   return hipGetLastError();
 }
 
 hipError_t launch_paged_attention(const PagedAttnArgs& a) {
-  const unsigned groups = (unsigned)(((long)a.n_tokens * a.hq + 3) / 4);
-  if (a.dtype == 0) hipLaunchKernelGGL(paged_row_kernel<F16>, dim3(groups), dim3(256), 0, a.stream, a);
-  else hipLaunchKernelGGL(paged_row_kernel<BF16>, dim3(groups), dim3(256), 0, a.stream, a);
-  return hipGetLastError();
+  return a.dtype == 0 ? launch_attention<F16>(a) : launch_attention<BF16>(a);
 }
 
 }  // namespace va

@@ -5,23 +5,58 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "va_kernels.h"
+
 namespace va {
 
 constexpr int kPagedMaxSeqs = 8192;  // sequences of a step
 constexpr int kPageMin = 16, kPageMax = 256;
 
-// A step's plan, int32 words: cu (n_seqs + 1) row offsets of the sequences, then the sequence (-1:
-// padding) and the position of every row.
+// Work items of a step: rows (token, query head of the group) of one sequence and key/value head,
+// flattened token by token. Up to kPagedFewRows of them are one tile whose waves share the keys out;
+// more are tiles of kPagedTileRows, a strip of 32 per wave.
+constexpr int kPagedFewRows = 32;
+constexpr int kPagedTileRows = 128;
+constexpr int kPagedChunkKeys = 64;   // key ranges are split at multiples of this
+constexpr int kPagedMinKeys = 256;    // shortest part of a split key range (but the last)
+constexpr int kPagedParts = 1024;     // parts that a step's keys are split into, when they are
+constexpr int kPagedPadRows = 64;     // padding rows that one item zeroes
+
+// A step's plan, int32 words: cu (n_seqs + 1) row offsets of the sequences, the sequence (-1: padding)
+// and the position of every row, the counts of items and merge records, the items, the records.
+constexpr int kPagedItemWords = 12, kPagedMergeWords = 8;
 struct PagedLayout {
-  int64_t seq, pos, words;  // cu lies at 0
+  int64_t seq, pos, counts, items, merges, words;  // offsets; cu lies at 0
+  int64_t max_items, max_merges, max_part_rows;
 };
-inline PagedLayout paged_layout(int64_t n_seqs, int64_t n_tokens) {
+inline int64_t up4(int64_t x) { return (x + 3) & ~int64_t(3); }
+// Bounds: a sequence with rows makes one tile, and one more per full kPagedTileRows. Parts have at
+// least total / kPagedParts keys, so a tile of n > 1 parts stands for more than n - 1 >= n / 2 of the
+// kPagedParts, and the tiles that are split have at most 2 kPagedParts parts; each part holds at most
+// kPagedTileRows rows, and a row is in at most max_keys / kPagedMinKeys + 1 parts. A merge record
+// takes 8 rows of a tile of up to 8 parts, or one row of a tile of more.
+inline PagedLayout paged_layout(int64_t n_seqs, int64_t n_tokens, int64_t hq, int64_t hkv,
+                                int64_t max_keys) {
   PagedLayout l;
-  const int64_t rows = (n_tokens + 3) & ~int64_t(3);
-  l.seq = (n_seqs + 1 + 3) & ~int64_t(3);
-  l.pos = l.seq + rows;
-  l.words = l.pos + rows;
+  const int64_t tiles = (n_seqs < n_tokens ? n_seqs : n_tokens) + n_tokens * (hq / hkv) / kPagedTileRows;
+  const bool split = max_keys > kPagedMinKeys;
+  const int64_t rows = n_tokens * hq;
+  l.max_items = tiles * hkv + (split ? kPagedParts : 0) + (n_tokens + kPagedPadRows - 1) / kPagedPadRows;
+  l.max_merges = !split ? 0 : rows < 16 * kPagedParts ? rows : 16 * kPagedParts;
+  const int64_t by_row = rows * (max_keys / kPagedMinKeys + 1);
+  const int64_t by_part = 2 * kPagedParts * kPagedTileRows;
+  l.max_part_rows = !split ? 0 : by_row < by_part ? by_row : by_part;
+  l.seq = up4(n_seqs + 1);
+  l.pos = l.seq + up4(n_tokens);
+  l.counts = l.pos + up4(n_tokens);
+  l.items = l.counts + 4;
+  l.merges = l.items + l.max_items * kPagedItemWords;
+  l.words = l.merges + l.max_merges * kPagedMergeWords;
   return l;
+}
+// Partial results of split key ranges: O (rows, 128) fp32, then {maximum, sum} of every row.
+inline int64_t paged_workspace(const PagedLayout& l) {
+  return l.max_part_rows * (kHeadDim + 2) * 4;
 }
 
 struct PagedPlanArgs {
@@ -58,7 +93,7 @@ struct PagedAttnArgs {
   float scale;
   int dtype;
   void* out;
-  void* workspace;
+  float* workspace;
   hipStream_t stream;
 };
 
