@@ -30,12 +30,23 @@ _f32 = ctypes.c_float
 _pi32 = ctypes.POINTER(ctypes.c_int32)
 _pi64 = ctypes.POINTER(ctypes.c_int64)
 
+
 class RopeTables(ctypes.Structure):
     """va_rope_tables: the rotary tables of va_bwd_rotary_stage's epilogues."""
     _fields_ = [("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p),
                 ("cos_batch_stride", ctypes.c_int64), ("cos_seq_stride", ctypes.c_int64),
                 ("b_idx", ctypes.c_void_p), ("t_idx", ctypes.c_void_p)]
 
+
+class PagedStep(ctypes.Structure):
+    """va_paged_step: a step's page table, plan and sizes."""
+    _fields_ = [("page_table", ctypes.c_void_p), ("plan", ctypes.c_void_p),
+                ("n_tokens", ctypes.c_int64), ("n_seqs", ctypes.c_int32),
+                ("table_width", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("hq", ctypes.c_int32), ("hkv", ctypes.c_int32)]
+
+
+_pstep = ctypes.POINTER(PagedStep)
 
 # name -> (restype, argtypes); the same list the header declares.
 SIGNATURES = {
@@ -73,14 +84,13 @@ SIGNATURES = {
                                    _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p]),
     "va_pack_rows": (ctypes.c_int, [_p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _i32, _p]),
     "va_unpack_rows": (ctypes.c_int, [_p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _i32, _p]),
-    "va_paged_plan_words": (ctypes.c_int, [_i32, _i64, _i32, _i32, _i32, _i32, _pi64]),
-    "va_paged_plan": (ctypes.c_int, [_p, _p, _i32, _i64, _i32, _i32, _i32, _i32, _p, _i64, _p]),
-    "va_paged_append": (ctypes.c_int, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _p, _i32,
-                                       _i32, _p, _p, _p, _i64, _i64, _i32, _i32, _i64, _i32, _i32,
-                                       _i32, _i32, _i32, _p]),
-    "va_paged_attention_workspace": (ctypes.c_int, [_i32, _i64, _i32, _i32, _i32, _i32, _pi64]),
-    "va_paged_attention": (ctypes.c_int, [_p, _p, _p, _i64, _i64, _i32, _i32, _p, _i32, _p, _i32,
-                                          _i64, _i32, _i32, _i32, _f32, _i32, _p, _p, _i64, _p]),
+    "va_paged_plan_words": (ctypes.c_int, [_pstep, _pi64]),
+    "va_paged_plan": (ctypes.c_int, [_pstep, _p, _p, _i64, _p]),
+    "va_paged_append": (ctypes.c_int, [_pstep, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _p,
+                                       _p, _i64, _i64, _i32, _i32, _i32, _i32, _p]),
+    "va_paged_attention_workspace": (ctypes.c_int, [_pstep, _pi64]),
+    "va_paged_attention": (ctypes.c_int, [_pstep, _p, _p, _p, _i64, _i64, _i32, _i32, _f32, _i32,
+                                          _p, _p, _i64, _p]),
     "va_pages_scratch_words": (ctypes.c_int, [_i32, _i32, _pi64]),
     "va_pages_remap": (ctypes.c_int, [_p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _p, _p, _i32,
                                       _i32, _p, _p, _p, _p, _p, _i64, _p]),

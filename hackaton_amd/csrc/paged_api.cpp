@@ -43,148 +43,137 @@ int check_page_size(int32_t page_size, const char* what) {
 
 int shift_of(int32_t page_size) { return __builtin_ctz((unsigned)page_size); }
 
-int check_step(int32_t n_seqs, int64_t n_tokens, int32_t hq, int32_t hkv, int32_t page_size,
-               int32_t table_width, const char* what) {
-  if (n_seqs < 0 || n_seqs > va::kPagedMaxSeqs)
-    return va::fail(VA_ESHAPE, "%s: n_seqs=%d (at most %d)", what, n_seqs, va::kPagedMaxSeqs);
-  if (hq <= 0 || hkv <= 0 || hq % hkv != 0 || hq > 4096)
+int check_step(const va_paged_step* s, const char* what) {
+  if (s == nullptr) return va::fail(VA_EINVAL, "%s: step is NULL", what);
+  if (s->n_seqs < 0 || s->n_seqs > va::kPagedMaxSeqs)
+    return va::fail(VA_ESHAPE, "%s: n_seqs=%d (at most %d)", what, s->n_seqs, va::kPagedMaxSeqs);
+  if (s->hq <= 0 || s->hkv <= 0 || s->hq % s->hkv != 0 || s->hq > 4096)
     return va::fail(VA_ESHAPE, "%s: Hq=%d must be a positive multiple of Hkv=%d, at most 4096", what,
-                    hq, hkv);
-  if (n_tokens < 0 || n_tokens * (int64_t)hq > INT32_MAX / 2)
-    return va::fail(VA_ESHAPE, "%s: n_tokens=%lld out of range", what, (long long)n_tokens);
-  const int rc = check_page_size(page_size, what);
+                    s->hq, s->hkv);
+  if (s->n_tokens < 0 || s->n_tokens > INT32_MAX / 2 || s->n_tokens * s->hq > INT32_MAX / 2)
+    return va::fail(VA_ESHAPE, "%s: n_tokens=%lld out of range", what, (long long)s->n_tokens);
+  const int rc = check_page_size(s->page_size, what);
   if (rc) return rc;
-  if (table_width < 0 || (int64_t)table_width * page_size > INT32_MAX / 2)
-    return va::fail(VA_ESHAPE, "%s: table_width=%d x page_size=%d out of range", what, table_width,
-                    page_size);
+  if (s->table_width < 0 || (int64_t)s->table_width * s->page_size > INT32_MAX / 2)
+    return va::fail(VA_ESHAPE, "%s: table_width=%d x page_size=%d out of range", what,
+                    s->table_width, s->page_size);
   return VA_OK;
 }
 
-va::PagedLayout layout_of(int32_t n_seqs, int64_t n_tokens, int32_t hq, int32_t hkv,
-                          int32_t page_size, int32_t table_width) {
-  return va::paged_layout(n_seqs, n_tokens, hq, hkv, (int64_t)table_width * page_size);
+va::PagedLayout layout_of(const va_paged_step& s) {
+  return va::paged_layout(s.n_seqs, s.n_tokens, s.hq, s.hkv, (int64_t)s.table_width * s.page_size);
 }
 
-// Pages of one layer, keys and values.
-int check_pool(const void* k_pages, const void* v_pages, int64_t k_stride, int64_t v_stride,
-               int32_t n_pages, int32_t hkv, int32_t page_size, const int32_t* table,
-               int32_t n_seqs, int32_t table_width, const char* what) {
+// Pages of one layer, keys and values, and the step's table and plan.
+int check_pool(const va_paged_step& s, const void* k_pages, const void* v_pages, int64_t k_stride,
+               int64_t v_stride, int32_t n_pages, const char* what) {
   if (n_pages < 0) return va::fail(VA_ESHAPE, "%s: n_pages=%d", what, n_pages);
   for (int64_t stride : {k_stride, v_stride})
-    if (stride % 8 != 0 || stride < (int64_t)hkv * page_size * va::kHeadDim)
+    if (stride % 8 != 0 || stride < (int64_t)s.hkv * s.page_size * va::kHeadDim)
       return va::fail(VA_EINVAL, "%s: page strides must be multiples of 8 and cover a page", what);
   int rc = VA_OK;
   if (n_pages > 0 && (rc = check_buffers({k_pages, v_pages}, what))) return rc;
-  if (n_seqs > 0 && table_width > 0) rc = check_words({table}, what);
+  if (s.n_tokens > 0 && (rc = check_buffers({s.plan}, what))) return rc;
+  if (s.n_seqs > 0 && s.table_width > 0) rc = check_words({s.page_table}, what);
   return rc;
+}
+
+va::PagedPool pool_of(const va_paged_step& s, int64_t k_stride, int64_t v_stride, int32_t n_pages) {
+  return va::PagedPool{s.page_table, s.table_width, n_pages, shift_of(s.page_size), k_stride, v_stride};
 }
 
 }  // namespace
 
-extern "C" int va_paged_plan_words(int32_t n_seqs, int64_t n_tokens, int32_t hq, int32_t hkv,
-                                   int32_t page_size, int32_t table_width, int64_t* words) {
-  const int rc = check_step(n_seqs, n_tokens, hq, hkv, page_size, table_width, "va_paged_plan_words");
+extern "C" int va_paged_plan_words(const va_paged_step* step, int64_t* words) {
+  const int rc = check_step(step, "va_paged_plan_words");
   if (rc) return rc;
   if (words == nullptr) return va::fail(VA_EINVAL, "va_paged_plan_words: NULL output");
-  *words = layout_of(n_seqs, n_tokens, hq, hkv, page_size, table_width).words;
+  *words = layout_of(*step).words;
   return VA_OK;
 }
 
-extern "C" int va_paged_plan(const int32_t* q_lengths, const int32_t* kv_lengths, int32_t n_seqs,
-                             int64_t n_tokens, int32_t hq, int32_t hkv, int32_t page_size,
-                             int32_t table_width, int32_t* plan, int64_t plan_words,
-                             void* stream) {
-  int rc = check_step(n_seqs, n_tokens, hq, hkv, page_size, table_width, "va_paged_plan");
+extern "C" int va_paged_plan(const va_paged_step* step, const int32_t* q_lengths,
+                             const int32_t* kv_lengths, int64_t plan_words, void* stream) {
+  int rc = check_step(step, "va_paged_plan");
   if (rc) return rc;
-  if (n_tokens == 0) return VA_OK;
-  const va::PagedLayout layout = layout_of(n_seqs, n_tokens, hq, hkv, page_size, table_width);
+  const va_paged_step& s = *step;
+  if (s.n_tokens == 0) return VA_OK;
+  const va::PagedLayout layout = layout_of(s);
   if (plan_words < layout.words)
     return va::fail(VA_ECAPACITY, "va_paged_plan: %lld words, need %lld", (long long)plan_words,
                     (long long)layout.words);
-  if ((rc = check_buffers({plan}, "va_paged_plan"))) return rc;
-  if (n_seqs > 0 && (rc = check_words({q_lengths, kv_lengths}, "va_paged_plan"))) return rc;
-  va::PagedPlanArgs a{q_lengths, kv_lengths, n_seqs, (int)n_tokens, hq, hkv,
-                      table_width * page_size, plan, layout, (hipStream_t)stream};
+  if ((rc = check_buffers({s.plan}, "va_paged_plan"))) return rc;
+  if (s.n_seqs > 0 && (rc = check_words({q_lengths, kv_lengths}, "va_paged_plan"))) return rc;
+  va::PagedPlanArgs a{q_lengths, kv_lengths, s.n_seqs, (int)s.n_tokens, s.hq, s.hkv,
+                      s.table_width * s.page_size, s.plan, layout, (hipStream_t)stream};
   return launched(va::launch_paged_plan(a), "va_paged_plan");
 }
 
-extern "C" int va_paged_append(const void* q, const void* k, const void* v, const float* cos,
-                               const float* sin, int64_t cos_batch_stride, int64_t cos_seq_stride,
-                               int64_t cos_token_stride, int64_t cos_rows, const int32_t* plan,
-                               const int32_t* page_table, int32_t n_seqs, int32_t table_width,
-                               void* q_out, void* k_pages, void* v_pages, int64_t k_stride,
-                               int64_t v_stride, int32_t n_pages, int32_t page_size,
-                               int64_t n_tokens, int32_t hq, int32_t hkv, int32_t head_dim,
-                               int32_t in_dtype, int32_t out_dtype, void* stream) {
+extern "C" int va_paged_append(const va_paged_step* step, const void* q, const void* k,
+                               const void* v, const float* cos, const float* sin,
+                               int64_t cos_batch_stride, int64_t cos_seq_stride,
+                               int64_t cos_token_stride, int64_t cos_rows, void* q_out,
+                               void* k_pages, void* v_pages, int64_t k_stride, int64_t v_stride,
+                               int32_t n_pages, int32_t head_dim, int32_t in_dtype,
+                               int32_t out_dtype, void* stream) {
   const char* what = "va_paged_append";
   if (head_dim != va::kHeadDim)
     return va::fail(VA_ESHAPE, "%s: head_dim=%d, built for %d", what, head_dim, va::kHeadDim);
-  int rc = check_step(n_seqs, n_tokens, hq, hkv, page_size, table_width, what);
+  int rc = check_step(step, what);
   if (rc) return rc;
+  const va_paged_step& s = *step;
   if (in_dtype < VA_F16 || in_dtype > VA_F32 || (out_dtype != VA_F16 && out_dtype != VA_BF16))
     return va::fail(VA_EDTYPE, "%s: dtype", what);
   for (int64_t stride : {cos_batch_stride, cos_seq_stride, cos_token_stride})
     if (stride < 0 || stride % 4 != 0)
       return va::fail(VA_EINVAL, "%s: cos/sin strides must be non-negative multiples of 4", what);
   if (cos_rows < 0) return va::fail(VA_EINVAL, "%s: cos_rows", what);
-  if ((rc = check_pool(k_pages, v_pages, k_stride, v_stride, n_pages, hkv, page_size, page_table,
-                       n_seqs, table_width, what)))
-    return rc;
-  if (n_tokens == 0) return VA_OK;
-  if ((rc = check_buffers({q, k, v, cos, sin, plan, q_out}, what))) return rc;
-  const va::PagedLayout layout = layout_of(n_seqs, n_tokens, hq, hkv, page_size, table_width);
+  if ((rc = check_pool(s, k_pages, v_pages, k_stride, v_stride, n_pages, what))) return rc;
+  if (s.n_tokens == 0) return VA_OK;
+  if ((rc = check_buffers({q, k, v, cos, sin, q_out}, what))) return rc;
+  const va::PagedLayout layout = layout_of(s);
   va::PagedAppendArgs a{q, k, v, cos, sin, cos_batch_stride, cos_seq_stride, cos_token_stride,
-                        cos_rows, plan + layout.seq, plan + layout.pos,
-                        va::PagedPool{page_table, table_width, n_pages, shift_of(page_size),
-                                      k_stride, v_stride},
-                        q_out, k_pages, v_pages, (int)n_tokens, hq, hkv, in_dtype, out_dtype,
-                        (hipStream_t)stream};
+                        cos_rows, s.plan + layout.seq, s.plan + layout.pos,
+                        pool_of(s, k_stride, v_stride, n_pages), q_out, k_pages, v_pages,
+                        (int)s.n_tokens, s.hq, s.hkv, in_dtype, out_dtype, (hipStream_t)stream};
   return launched(va::launch_paged_append(a), what);
 }
 
-extern "C" int va_paged_attention_workspace(int32_t n_seqs, int64_t n_tokens, int32_t hq,
-                                            int32_t hkv, int32_t page_size, int32_t table_width,
-                                            int64_t* bytes) {
-  const int rc = check_step(n_seqs, n_tokens, hq, hkv, page_size, table_width,
-                            "va_paged_attention_workspace");
+extern "C" int va_paged_attention_workspace(const va_paged_step* step, int64_t* bytes) {
+  const int rc = check_step(step, "va_paged_attention_workspace");
   if (rc) return rc;
   if (bytes == nullptr) return va::fail(VA_EINVAL, "va_paged_attention_workspace: NULL output");
-  *bytes = va::paged_workspace(layout_of(n_seqs, n_tokens, hq, hkv, page_size, table_width));
+  *bytes = va::paged_workspace(layout_of(*step));
   return VA_OK;
 }
 
-extern "C" int va_paged_attention(const void* q, const void* k_pages, const void* v_pages,
-                                  int64_t k_stride, int64_t v_stride, int32_t n_pages,
-                                  int32_t page_size, const int32_t* page_table,
-                                  int32_t table_width, const int32_t* plan, int32_t n_seqs,
-                                  int64_t n_tokens, int32_t hq, int32_t hkv, int32_t head_dim,
-                                  float scale, int32_t dtype, void* out, void* workspace,
-                                  int64_t workspace_bytes, void* stream) {
+extern "C" int va_paged_attention(const va_paged_step* step, const void* q, const void* k_pages,
+                                  const void* v_pages, int64_t k_stride, int64_t v_stride,
+                                  int32_t n_pages, int32_t head_dim, float scale, int32_t dtype,
+                                  void* out, void* workspace, int64_t workspace_bytes,
+                                  void* stream) {
   const char* what = "va_paged_attention";
   if (head_dim != va::kHeadDim)
     return va::fail(VA_ESHAPE, "%s: head_dim=%d, built for %d", what, head_dim, va::kHeadDim);
-  int rc = check_step(n_seqs, n_tokens, hq, hkv, page_size, table_width, what);
+  int rc = check_step(step, what);
   if (rc) return rc;
+  const va_paged_step& s = *step;
   if (dtype != VA_F16 && dtype != VA_BF16)
     return va::fail(VA_EDTYPE, "%s: dtype %d: attention runs on VA_F16 or VA_BF16", what, dtype);
   if (!std::isfinite(scale) || scale <= 0.f)
     return va::fail(VA_EINVAL, "%s: scale must be finite and positive", what);
-  if ((rc = check_pool(k_pages, v_pages, k_stride, v_stride, n_pages, hkv, page_size, page_table,
-                       n_seqs, table_width, what)))
-    return rc;
-  if (n_tokens == 0) return VA_OK;
-  const va::PagedLayout layout = layout_of(n_seqs, n_tokens, hq, hkv, page_size, table_width);
+  if ((rc = check_pool(s, k_pages, v_pages, k_stride, v_stride, n_pages, what))) return rc;
+  if (s.n_tokens == 0) return VA_OK;
+  const va::PagedLayout layout = layout_of(s);
   const int64_t need = va::paged_workspace(layout);
   if (workspace_bytes < need)
     return va::fail(VA_ECAPACITY, "%s: workspace %lld bytes, need %lld", what,
                     (long long)workspace_bytes, (long long)need);
-  if ((rc = check_buffers({q, plan, out}, what))) return rc;
+  if ((rc = check_buffers({q, out}, what))) return rc;
   if (need > 0 && (rc = check_buffers({workspace}, what))) return rc;
-  va::PagedAttnArgs a{q, k_pages, v_pages,
-                      va::PagedPool{page_table, table_width, n_pages, shift_of(page_size),
-                                    k_stride, v_stride},
-                      plan, layout, n_seqs, (int)n_tokens, hq, hkv, scale, dtype, out,
-                      (float*)workspace, (hipStream_t)stream};
+  va::PagedAttnArgs a{q, k_pages, v_pages, pool_of(s, k_stride, v_stride, n_pages), s.plan, layout,
+                      s.n_seqs, (int)s.n_tokens, s.hq, s.hkv, scale, dtype, out, (float*)workspace,
+                      (hipStream_t)stream};
   return launched(va::launch_paged_attention(a), what);
 }
 

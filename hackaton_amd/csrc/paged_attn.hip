@@ -17,6 +17,8 @@
 // P^T reads V^T from the row-major tile with transposed LDS reads. A tile's rows are stored in groups of
 // 4 (1 KB, one copy instruction) 1088 bytes apart, chunk c of row r at c ^ (r & 3), so that both reads
 // touch all banks.
+#include <climits>
+
 #include "../../include/varlen_attn.h"
 #include "va_common.h"
 #include "va_kernels.h"
@@ -31,10 +33,9 @@ namespace {
 // plan
 // ------------------------------------------------------------------------------------------------
 constexpr int PT = 1024;                    // threads of a planning work-group
-constexpr int SPT = kPagedMaxSeqs / PT;     // sequences per thread
 constexpr int kPlanRowsPerGroup = 4 * PT;   // rows that a planning work-group places
 
-enum { kFew = 0, kMany = 1, kPad = 2 };     // kinds of items
+enum { kFew = 0, kMany = 1, kPad = 2, kNone = 3 };  // kinds of items
 
 struct Item {
   int token0, seq, pos0, head;        // the sequence's first row and its position; key/value head | kind << 16
@@ -46,224 +47,197 @@ static_assert(sizeof(Item) == 4 * kPagedItemWords, "item words");
 
 struct Merge {
   int token0, head, row, rows;        // 1 to 8 flattened rows
-  int part_row, stride, parts, pad;   // workspace row of the first one in the first part; rows per part
+  int part_row, stride, parts, pad;   // workspace row of the first one in the first part; rows per part;
+                                      // parts (0: the rows' only item has written them)
 };
 static_assert(sizeof(Merge) == 4 * kPagedMergeWords, "merge words");
 
-// Tiles of a sequence and the keys that tile i sees.
-struct Rows {
-  int rows, tiles, pos0, kv;
-};
-__device__ inline Rows rows_of(int q, int rows_left, int kv, int max_keys, int group) {
-  Rows r;
-  r.kv = min(max(kv, 0), max_keys);
-  r.pos0 = r.kv - q;
-  r.rows = rows_left * group;
-  r.tiles = r.rows <= kPagedFewRows ? (r.rows > 0) : (r.rows + kPagedTileRows - 1) / kPagedTileRows;
-  return r;
+// Tiles of a sequence with `rows` rows, and the keys that the row before `end` sees (pos0: the position
+// of the first one).
+__device__ inline int tiles_of(int rows) {
+  return rows <= kPagedFewRows ? (rows > 0) : (rows + kPagedTileRows - 1) / kPagedTileRows;
 }
-__device__ inline int tile_keys(const Rows& r, int i, int group) {
-  const int end = min((i + 1) * kPagedTileRows, r.rows);
-  return max(r.pos0 + (end - 1) / group + 1, 0);
+__device__ inline int keys_of(int pos0, int end, int group) { return max(pos0 + (end - 1) / group + 1, 0); }
+// The last of n ascending numbers at or below x (the first one is).
+__device__ inline int last_at_most(const int* v, int n, int x) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (v[mid] <= x) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
 }
 
-// Work-group 0 writes the work list, the others place the rows. Each sums the lengths by itself (at most
-// 64 KB of them): one launch, nothing handed from one work-group to another.
+// The first `writers` work-groups write the work list, the others place the rows. Each sums the lengths
+// by itself (at most 32 KB of them): one launch, nothing handed from one work-group to another.
 //
-// A tile's keys are split into parts of at most `chunk` keys, equal but for the last: chunk is the
-// step's total over all tiles and heads divided by kPagedParts, so a step of few long tiles fills the
-// card with about that many parts, and one of many tiles splits only what is longer than its share.
-// Tiles of prompt chunks come first, the last (longest) ones of a sequence before its first.
-__global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a) {
-  __shared__ int s_cu[kPagedMaxSeqs + 1];
-  __shared__ int s_many[kPagedMaxSeqs], s_few[kPagedMaxSeqs];  // tiles before a sequence's, per kind
-  __shared__ long long s_scan[PT / 64];
-  // of the tiles in hand: first item, first workspace row, first merge record; parts, their keys, all keys
-  __shared__ int s_first[PT], s_row[PT], s_merge[PT], s_parts[PT], s_chunk[PT], s_keys[PT];
+// The keys of all tiles of a sequence are split at the same places, into parts of at most `chunk` keys,
+// equal but for the last: chunk is the total over the tiles of a kind and all heads (each tile with its
+// sequence's longest) divided by the kind's number of parts, so a step of few long tiles fills the card
+// with about that many parts, and one of many tiles splits only what is longer than its share.
+// Prompt tiles come first, the last (longest) ones of a sequence before its first. Work-group i runs on
+// XCD i mod 8: with a multiple of 8 items per tile, the tiles that read the same keys run on one XCD
+// and find them in its L2, so the parts are rounded down to that where there are enough of them
+// (128 new tokens on 32,768, 28/4 heads: 9 parts per tile and head 113 us, 8 parts 89 us).
+template <int SPT>  // sequences per thread
+__global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int writers) {
+  constexpr int S = PT * SPT;
+  // of every sequence: first row, its position, items before it (per kind), workspace rows and merge
+  // records before it, parts, keys of a part
+  __shared__ int s_cu[S + 1], s_pos0[S], s_many[S], s_few[S], s_part[S], s_merge[S], s_parts[S], s_chunk[S];
+  __shared__ int s_scan[4 * PT / 64];
+  __shared__ long long s_sum[PT / 64];
   const int tid = threadIdx.x, group = a.hq / a.hkv;
   int q[SPT];
-  long long sum = 0;
+  int sum[2] = {0, 0}, sums[2];  // low 15 bits and the rest, so that no sum passes 32 bits
 #pragma unroll
   for (int i = 0; i < SPT; ++i) {
     const int s = tid * SPT + i;
-    q[i] = s < a.n_seqs ? max(a.q_lengths[s], 0) : 0;
-    sum += q[i];
+    const bool in = s < a.n_seqs;
+    const int len = in ? max(a.q_lengths[s], 0) : 0;
+    const int kv = in ? min(max(a.kv_lengths[s], 0), a.max_keys) : 0;
+    s_pos0[s] = kv - len;
+    q[i] = min(len, a.n_tokens);
+    sum[0] += q[i] & 0x7fff;
+    sum[1] += q[i] >> 15;
   }
-  long long total;
-  long long at = block_exclusive_sum<PT / 64>(sum, s_scan, total);
+  block_exclusive_sums<PT / 64>(sum, sums, s_scan);
+  long long at = ((long long)sum[1] << 15) + sum[0];
+  int n_rows[SPT];  // flattened rows of a sequence
 #pragma unroll
   for (int i = 0; i < SPT; ++i) {
-    const int s = tid * SPT + i;
-    if (s <= a.n_seqs) s_cu[s] = (int)min(at, (long long)a.n_tokens);
+    const int first = (int)min(at, (long long)a.n_tokens);
     at += q[i];
+    s_cu[tid * SPT + i] = first;
+    n_rows[i] = ((int)min(at, (long long)a.n_tokens) - first) * group;
   }
-  if (tid == PT - 1 && a.n_seqs == kPagedMaxSeqs)
-    s_cu[kPagedMaxSeqs] = (int)min(total, (long long)a.n_tokens);
-  __syncthreads();
-  const int rows = s_cu[a.n_seqs];
-  if (blockIdx.x > 0) {
-    const int first = (blockIdx.x - 1) * kPlanRowsPerGroup;
+  if (tid == PT - 1) s_cu[S] = (int)min(at, (long long)a.n_tokens);
+  if ((int)blockIdx.x >= writers) {
+    __syncthreads();
+    const int rows = s_cu[a.n_seqs], first = (blockIdx.x - writers) * kPlanRowsPerGroup;
     const int end = min(first + kPlanRowsPerGroup, a.n_tokens);
     for (int n = first + tid; n < end; n += PT) {
       int seq = -1, pos = -1;
       if (n < rows) {
-        int lo = 0, hi = a.n_seqs - 1;  // last sequence that starts at or before row n
-        while (lo < hi) {
-          const int mid = (lo + hi + 1) >> 1;
-          if (s_cu[mid] <= n) lo = mid;
-          else hi = mid - 1;
-        }
-        seq = lo;
-        pos = min(max(a.kv_lengths[lo], 0), a.max_keys) - max(a.q_lengths[lo], 0) + (n - s_cu[lo]);
+        seq = last_at_most(s_cu, a.n_seqs, n);
+        pos = s_pos0[seq] + (n - s_cu[seq]);
       }
       a.plan[a.layout.seq + n] = seq;
       a.plan[a.layout.pos + n] = pos;
     }
     return;
   }
-  for (int s = tid; s <= a.n_seqs; s += PT) a.plan[s] = s_cu[s];
 
-  // Tiles of every sequence and the step's keys: the keys of a sequence's tiles grow evenly, so half the
-  // sum of the first and the last (each rounded up) times their number bounds their sum.
-  auto rows_at = [&](int s) {
-    return rows_of(max(a.q_lengths[s], 0), s_cu[s + 1] - s_cu[s], a.kv_lengths[s], a.max_keys, group);
-  };
-  long long many = 0, few = 0, keys = 0;
+  long long keys[2] = {0, 0}, tiles[2] = {0, 0};  // many rows, few rows
 #pragma unroll
-  for (int i = 0; i < SPT; ++i) {
-    const int s = tid * SPT + i;
-    if (s >= a.n_seqs || s_cu[s + 1] == s_cu[s]) continue;
-    const Rows r = rows_at(s);
-    if (r.rows > kPagedFewRows) many += r.tiles;
-    else few += r.tiles;
-    const int step = kPagedTileRows / group + 2;
-    keys += (tile_keys(r, 0, group) + (long long)tile_keys(r, r.tiles - 1, group) + step + 1) *
-            r.tiles / 2 + 1;
+  for (int i = 0; i < SPT; ++i)
+    if (n_rows[i] > 0) {
+      const int kind = n_rows[i] <= kPagedFewRows, t = tiles_of(n_rows[i]);
+      keys[kind] += (long long)t * keys_of(s_pos0[tid * SPT + i], n_rows[i], group);
+      tiles[kind] += t;
+    }
+  int chunks[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const long long all = k == 0 ? kPagedManyParts : kPagedFewParts;
+    const long long parts = max(all - block_sum<PT / 64>(tiles[k], s_sum) * a.hkv, all / 4);
+    const long long share = max((block_sum<PT / 64>(keys[k], s_sum) * a.hkv + parts - 1) / parts,
+                                (long long)(k == 0 ? kPagedManyKeys : kPagedFewKeys));
+    chunks[k] = a.max_keys <= kPagedWholeKeys
+                    ? INT_MAX / 2
+                    : (int)((share + kPagedChunkKeys - 1) / kPagedChunkKeys) * kPagedChunkKeys;
   }
-  long long n_many, n_few, all_keys;
-  long long first_many = block_exclusive_sum<PT / 64>(many, s_scan, n_many);
-  long long first_few = block_exclusive_sum<PT / 64>(few, s_scan, n_few);
-  block_exclusive_sum<PT / 64>(keys, s_scan, all_keys);
+  const int aligned = 8 / (a.hkv % 8 == 0 ? 8 : a.hkv % 4 == 0 ? 4 : a.hkv % 2 == 0 ? 2 : 1);
+  int x[4] = {0, 0, 0, 0}, n[4];  // items of both kinds, workspace rows, merge records
+  int own[SPT][4];
+#pragma unroll
+  for (int i = 0; i < SPT; ++i) {
+    const int s = tid * SPT + i, rows = n_rows[i], kind = rows <= kPagedFewRows;
+    const int longest = rows > 0 ? keys_of(s_pos0[s], rows, group) : 0;
+    int parts = max(1, (longest + chunks[kind] - 1) / chunks[kind]);
+    if (kind == 0 && parts > aligned) parts -= parts % aligned;
+    const int c =
+        ((longest + parts - 1) / parts + kPagedChunkKeys - 1) / kPagedChunkKeys * kPagedChunkKeys;
+    if (parts > 1) parts = (longest + c - 1) / c;
+    s_parts[s] = parts;
+    s_chunk[s] = max(c, 1);
+    const int items = tiles_of(rows) * parts * a.hkv;
+    own[i][0] = kind == 0 ? items : 0;
+    own[i][1] = kind == 0 ? 0 : items;
+    own[i][2] = parts > 1 ? rows * parts * a.hkv : 0;
+    own[i][3] = parts > 1 ? (parts <= 8 ? (rows + 7) / 8 : rows) * a.hkv : 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] += own[i][k];
+  }
+  block_exclusive_sums<PT / 64>(x, n, s_scan);
 #pragma unroll
   for (int i = 0; i < SPT; ++i) {
     const int s = tid * SPT + i;
-    if (s >= a.n_seqs) continue;
-    s_many[s] = (int)first_many;
-    s_few[s] = (int)first_few;
-    const Rows r = rows_at(s);
-    if (r.rows > kPagedFewRows) first_many += r.tiles;
-    else first_few += r.tiles;
+    s_many[s] = x[0];
+    s_few[s] = x[1];
+    s_part[s] = x[2];
+    s_merge[s] = x[3];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] += own[i][k];
   }
   __syncthreads();
-  const long long per_part = (all_keys * a.hkv + kPagedParts - 1) / kPagedParts;
-  const int chunk =
-      (int)((max(per_part, (long long)kPagedMinKeys) + kPagedChunkKeys - 1) / kPagedChunkKeys) *
-      kPagedChunkKeys;
   Item* items = reinterpret_cast<Item*>(a.plan + a.layout.items);
   Merge* merges = reinterpret_cast<Merge*>(a.plan + a.layout.merges);
-  const int n_tiles = (int)(n_many + n_few);
-  int item0 = 0, part0 = 0, merge0 = 0;  // so far
-  // A tile's place: its sequence (the last one whose tiles start at or before it) and first row.
-  struct Place {
-    int seq, row;
-  };
-  auto place_of = [&](int j) {
-    const bool is_many = j < n_many;
-    const int number = is_many ? (int)n_many - 1 - j : j - (int)n_many;
-    const int* first = is_many ? s_many : s_few;
-    int lo = 0, hi = a.n_seqs - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (first[mid] <= number) lo = mid;
-      else hi = mid - 1;
-    }
-    return Place{lo, (number - first[lo]) * kPagedTileRows};
-  };
-  for (int base = 0; base < n_tiles; base += PT) {
-    const int j = base + tid;
-    int parts = 0, n_keys = 0, c = 0, n_rows = 0;
-    if (j < n_tiles) {
-      const Place pl = place_of(j);
-      const Rows r = rows_at(pl.seq);
-      n_keys = tile_keys(r, pl.row / kPagedTileRows, group);
-      n_rows = min(kPagedTileRows, r.rows - pl.row);
-      parts = max(1, (n_keys + chunk - 1) / chunk);
-      c = ((n_keys + parts - 1) / parts + kPagedChunkKeys - 1) / kPagedChunkKeys * kPagedChunkKeys;
-      if (parts > 1) parts = (n_keys + c - 1) / c;
-    }
-    long long n_items, n_parts, n_merges;
-    const int records = parts < 2 ? 0 : parts <= 8 ? (n_rows + 7) / 8 : n_rows;
-    s_first[tid] = (int)block_exclusive_sum<PT / 64>((long long)parts * a.hkv, s_scan, n_items);
-    s_row[tid] = (int)block_exclusive_sum<PT / 64>((long long)(parts < 2 ? 0 : parts * n_rows) * a.hkv,
-                                                   s_scan, n_parts);
-    s_merge[tid] = (int)block_exclusive_sum<PT / 64>((long long)records * a.hkv, s_scan, n_merges);
-    s_parts[tid] = parts;
-    s_chunk[tid] = c;
-    s_keys[tid] = n_keys;
-    __syncthreads();
-    const int here = min(PT, n_tiles - base);
-    for (int i = tid; i < (int)n_items; i += PT) {
-      int lo = 0, hi = here - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (s_first[mid] <= i) lo = mid;
-        else hi = mid - 1;
-      }
-      const Place pl = place_of(base + lo);
-      const Rows r = rows_at(pl.seq);
-      const int in = i - s_first[lo], head = in % a.hkv, part = in / a.hkv;
-      const int p = s_parts[lo], count = min(kPagedTileRows, r.rows - pl.row);
-      Item it;
-      it.token0 = s_cu[pl.seq];
-      it.seq = pl.seq;
-      it.pos0 = r.pos0;
-      it.head = head | (base + lo < n_many ? kMany : kFew) << 16;
-      it.row = pl.row;
-      it.row_end = pl.row + count;
-      it.key = part * s_chunk[lo];
-      it.key_end = min(it.key + s_chunk[lo], s_keys[lo]);
-      it.part_row = p < 2 ? -1 : part0 + s_row[lo] + (head * p + part) * count;
-      if (item0 + i < a.layout.max_items) items[item0 + i] = it;
-    }
-    for (int i = tid; i < (int)n_merges; i += PT) {
-      int lo = 0, hi = here - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (s_merge[mid] <= i) lo = mid;
-        else hi = mid - 1;
-      }
-      const Place pl = place_of(base + lo);
-      const Rows r = rows_at(pl.seq);
-      const int p = s_parts[lo], count = min(kPagedTileRows, r.rows - pl.row);
-      const int each = p <= 8 ? 8 : 1, per_head = (count + each - 1) / each;
-      const int in = i - s_merge[lo], head = in / per_head, first = in % per_head * each;
-      Merge m;
-      m.token0 = s_cu[pl.seq];
-      m.head = head;
-      m.row = pl.row + first;
-      m.rows = min(each, count - first);
-      m.part_row = part0 + s_row[lo] + head * p * count + first;
-      m.stride = count;
-      m.parts = p;
-      m.pad = 0;
-      if (merge0 + i < a.layout.max_merges) merges[merge0 + i] = m;
-    }
-    item0 += (int)n_items;
-    part0 += (int)n_parts;
-    merge0 += (int)n_merges;
-    __syncthreads();
+  const int first = blockIdx.x * PT + tid, step = writers * PT;
+  const int n_items = (int)min((long)n[0] + n[1], (long)a.layout.max_items);
+  for (int i = first; i < n_items; i += step) {
+    const bool many = i < n[0];
+    const int* before = many ? s_many : s_few;
+    const int j = many ? i : i - n[0], s = last_at_most(before, a.n_seqs, j);
+    const int rows = (s_cu[s + 1] - s_cu[s]) * group, parts = s_parts[s], chunk = s_chunk[s];
+    const int in = j - before[s], per_tile = parts * a.hkv, tile = tiles_of(rows) - 1 - in / per_tile;
+    const int head = in % a.hkv, part = in % per_tile / a.hkv;
+    Item it;
+    it.token0 = s_cu[s];
+    it.seq = s;
+    it.pos0 = s_pos0[s];
+    it.row = tile * kPagedTileRows;
+    it.row_end = min(it.row + kPagedTileRows, rows);
+    const int all = keys_of(it.pos0, it.row_end, group);
+    it.key = part * chunk;
+    it.key_end = parts == 1 ? all : min(it.key + chunk, all);
+    it.head = head | (it.key >= all && part > 0 ? kNone : many ? kMany : kFew) << 16;
+    it.part_row = parts == 1 || all <= chunk ? -1 : s_part[s] + (head * parts + part) * rows + it.row;
+    it.pad[0] = it.pad[1] = it.pad[2] = 0;
+    items[i] = it;
   }
-  const int n_pad = (a.n_tokens - rows + kPagedPadRows - 1) / kPagedPadRows;
+  const int n_merges = (int)min((long)n[3], (long)a.layout.max_merges);
+  for (int i = first; i < n_merges; i += step) {
+    const int s = last_at_most(s_merge, a.n_seqs, i), in = i - s_merge[s];
+    const int rows = (s_cu[s + 1] - s_cu[s]) * group, parts = s_parts[s], chunk = s_chunk[s];
+    const int each = parts <= 8 ? 8 : 1, per_head = (rows + each - 1) / each;
+    const int head = in / per_head, row = in % per_head * each;
+    const int all = keys_of(s_pos0[s], min((row / kPagedTileRows + 1) * kPagedTileRows, rows), group);
+    Merge m;
+    m.token0 = s_cu[s];
+    m.head = head;
+    m.row = row;
+    m.rows = min(each, rows - row);
+    m.part_row = s_part[s] + head * parts * rows + row;
+    m.stride = rows;
+    m.parts = all <= chunk ? 0 : (all + chunk - 1) / chunk;
+    m.pad = 0;
+    merges[i] = m;
+  }
+  if (blockIdx.x > 0) return;
+  for (int s = tid; s <= a.n_seqs; s += PT) a.plan[s] = s_cu[s];
+  const int rows = s_cu[a.n_seqs], n_pad = (a.n_tokens - rows + kPagedPadRows - 1) / kPagedPadRows;
   for (int i = tid; i < n_pad; i += PT) {
     Item it{};
     it.head = kPad << 16;
     it.row = rows + i * kPagedPadRows;
     it.row_end = min(it.row + kPagedPadRows, a.n_tokens);
-    if (item0 + i < a.layout.max_items) items[item0 + i] = it;
+    if (n_items + i < a.layout.max_items) items[n_items + i] = it;
   }
   if (tid == 0) {
-    a.plan[a.layout.counts] = (int)min((long)(item0 + n_pad), (long)a.layout.max_items);
-    a.plan[a.layout.counts + 1] = (int)min((long)merge0, (long)a.layout.max_merges);
+    a.plan[a.layout.counts] = (int)min((long)(n_items + n_pad), (long)a.layout.max_items);
+    a.plan[a.layout.counts + 1] = n_merges;
   }
 }
 
@@ -724,16 +698,18 @@ template <class E>
 __global__ __launch_bounds__(NT, 2) void paged_attn_kernel(PagedAttnArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t smem_raw[LDS_HALFS];
   lds_u16* smem = (lds_u16*)smem_raw;
-  if ((int)blockIdx.x >= a.plan[a.layout.counts]) return;
+  const int n_items = a.plan[a.layout.counts];
   const Item* const p = reinterpret_cast<const Item*>(a.plan + a.layout.items) + blockIdx.x;
   const Item it{scalar(p->token0), scalar(p->seq), scalar(p->pos0), scalar(p->head), scalar(p->row),
                 scalar(p->row_end), scalar(p->key), scalar(p->key_end), scalar(p->part_row), {}};
+  // (the list has room for max_items: the item's words are in flight beside the count)
+  if ((int)blockIdx.x >= scalar(n_items)) return;
   const int kind = it.head >> 16;
   if (kind == kMany) {
     many_rows<E>(a, it, smem);
   } else if (kind == kFew) {
     few_rows<E>(a, it, smem, (char*)smem_raw);
-  } else {
+  } else if (kind == kPad) {
     u32x4* out = (u32x4*)a.out + (long)it.row * a.hq * (D / 8);
     const int chunks = (it.row_end - it.row) * a.hq * (D / 8);
     for (int i = threadIdx.x; i < chunks; i += NT) out[i] = u32x4{0u, 0u, 0u, 0u};
@@ -742,55 +718,68 @@ __global__ __launch_bounds__(NT, 2) void paged_attn_kernel(PagedAttnArgs a) {
 
 // Parts of split key ranges: a record of 8 rows and up to 8 parts has 32 lanes (4 elements each) per row,
 // a record of one row and more parts shares the parts out to the 8 groups of 32 lanes.
-constexpr int kMergeGroups = 1024;
+struct Sum {
+  float m, l;
+  f32x4 o;
+};
+// Adds N parts of one row, `step` parts apart (the first `count` of them exist), all loads at once.
+template <int N>
+__device__ inline void add_parts(const float* o, const float* ml, long row, long step, int count, int d0,
+                                 Sum& sum) {
+  f32x2 x[N];
+  f32x4 y[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const long r = row + min(e, count - 1) * step;
+    x[e] = *reinterpret_cast<const f32x2*>(ml + 2 * r);
+    y[e] = *reinterpret_cast<const f32x4*>(o + r * D + d0);
+  }
+  float m = sum.m;
+#pragma unroll
+  for (int e = 0; e < N; ++e) m = fmaxf(m, x[e][0]);
+  const float m_use = m == -INFINITY ? 0.f : m, alpha = fast_exp2(sum.m - m_use);
+  sum.m = m;
+  sum.l *= alpha;
+  sum.o *= alpha;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const float c = e < count ? fast_exp2(x[e][0] - m_use) : 0.f;
+    sum.l = fmaf(c, x[e][1], sum.l);
+    if (c != 0.f) sum.o += c * y[e];
+  }
+}
+
+constexpr int kMergeGroups = 2048;
 template <class E>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a) {
   __shared__ f32x4 s_o[8][32];
   __shared__ float s_m[8], s_l[8];
   const int n = a.plan[a.layout.counts + 1];
   const Merge* merges = reinterpret_cast<const Merge*>(a.plan + a.layout.merges);
+  const float* o = a.workspace;
   const float* ml = a.workspace + a.layout.max_part_rows * D;
   const int g = threadIdx.x >> 5, d0 = 4 * (threadIdx.x & 31), group = a.hq / a.hkv;
   for (int i = blockIdx.x; i < n; i += gridDim.x) {
     const Merge mg = merges[i];
+    if (mg.parts < 2) continue;  // (the same in all threads)
     const bool spread = mg.parts > 8;
     const int r = spread ? 0 : g;
-    float m = -INFINITY, l = 0.f;
-    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (spread || g < mg.rows) {
-      const int from = spread ? g : 0, step = spread ? 8 : 1;
-      for (int p0 = from; p0 < mg.parts; p0 += 8 * step) {
-        f32x2 x[8];
-        f32x4 y[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int p = p0 + e * step;
-          const long row = mg.part_row + r + (long)min(p, mg.parts - 1) * mg.stride;
-          x[e] = *reinterpret_cast<const f32x2*>(ml + 2 * row);
-          if (p >= mg.parts) x[e] = f32x2{-INFINITY, 0.f};
-          y[e] = *reinterpret_cast<const f32x4*>(a.workspace + row * D + d0);
-        }
-        float m_new = m;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) m_new = fmaxf(m_new, x[e][0]);
-        const float m_use = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = fast_exp2(m - m_use);
-        m = m_new;
-        l *= alpha;
-        o *= alpha;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float c = p0 + e * step < mg.parts ? fast_exp2(x[e][0] - m_use) : 0.f;
-          l = fmaf(c, x[e][1], l);
-          if (c != 0.f) o += c * y[e];
-        }
-      }
+    const long row = mg.part_row + r;
+    Sum sum{-INFINITY, 0.f, f32x4{0.f, 0.f, 0.f, 0.f}};
+    if (spread) {
+      for (int p = g; p < mg.parts; p += 64)
+        add_parts<8>(o, ml, row + (long)p * mg.stride, 8L * mg.stride,
+                     min(8, (mg.parts - p + 7) / 8), d0, sum);
+    } else if (g < mg.rows) {
+      if (mg.parts <= 2) add_parts<2>(o, ml, row, mg.stride, mg.parts, d0, sum);
+      else if (mg.parts <= 4) add_parts<4>(o, ml, row, mg.stride, mg.parts, d0, sum);
+      else add_parts<8>(o, ml, row, mg.stride, mg.parts, d0, sum);
     }
     if (spread) {
-      s_o[g][threadIdx.x & 31] = o;
+      s_o[g][threadIdx.x & 31] = sum.o;
       if (d0 == 0) {
-        s_m[g] = m;
-        s_l[g] = l;
+        s_m[g] = sum.m;
+        s_l[g] = sum.l;
       }
       __syncthreads();
       if (g == 0) {
@@ -798,23 +787,23 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a) {
 #pragma unroll
         for (int w = 0; w < 8; ++w) m_all = fmaxf(m_all, s_m[w]);
         const float m_use = m_all == -INFINITY ? 0.f : m_all;
-        l = 0.f;
-        o = f32x4{0.f, 0.f, 0.f, 0.f};
+        sum = Sum{m_all, 0.f, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
         for (int w = 0; w < 8; ++w) {
           const float c = fast_exp2(s_m[w] - m_use);
-          l = fmaf(c, s_l[w], l);
-          o += c * s_o[w][threadIdx.x & 31];
+          sum.l = fmaf(c, s_l[w], sum.l);
+          sum.o += c * s_o[w][threadIdx.x & 31];
         }
       }
       __syncthreads();
     }
     if (spread ? g == 0 : g < mg.rows) {
-      const int row = mg.row + r, tok = row / group, h = row % group;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int row_in = mg.row + r, tok = row_in / group, h = row_in % group;
+      const float inv = sum.l == 0.f ? 0.f : 1.f / sum.l;
       uint16_t* out = (uint16_t*)a.out + ((long)(mg.token0 + tok) * a.hq + mg.head * group + h) * D + d0;
-      __builtin_nontemporal_store(u32x2{pack2<E>(o[0] * inv, o[1] * inv), pack2<E>(o[2] * inv, o[3] * inv)},
-                                  reinterpret_cast<u32x2*>(out));
+      __builtin_nontemporal_store(
+          u32x2{pack2<E>(sum.o[0] * inv, sum.o[1] * inv), pack2<E>(sum.o[2] * inv, sum.o[3] * inv)},
+          reinterpret_cast<u32x2*>(out));
     }
   }
 }
@@ -832,8 +821,10 @@ hipError_t launch_attention(const PagedAttnArgs& a) {
 }  // namespace
 
 hipError_t launch_paged_plan(const PagedPlanArgs& a) {
-  const int groups = 1 + (a.n_tokens + kPlanRowsPerGroup - 1) / kPlanRowsPerGroup;
-  hipLaunchKernelGGL(paged_plan_kernel, dim3(groups), dim3(PT), 0, a.stream, a);
+  const int placers = (a.n_tokens + kPlanRowsPerGroup - 1) / kPlanRowsPerGroup;
+  const int writers = (int)((a.layout.max_items + 4 * PT - 1) / (4 * PT));
+  const auto kernel = a.n_seqs <= PT ? paged_plan_kernel<1> : paged_plan_kernel<kPagedMaxSeqs / PT>;
+  hipLaunchKernelGGL(kernel, dim3(writers + placers), dim3(PT), 0, a.stream, a, writers);
   return hipGetLastError();
 }
 

@@ -14,21 +14,26 @@ namespace va {
 namespace {
 
 constexpr int T = 256;        // threads of the wide kernels
-constexpr int ST = 1024;      // threads of the one work-group that hands out pages
+constexpr int ST = 1024;      // threads of the one work-group that counts and hands out pages
+constexpr int SW = ST / 64;
+constexpr int PER = 4;        // pages per thread and step
 constexpr int kCopyGroups = 2048;  // work-groups that copy rows (eight per CU)
+constexpr int kLdsPages = 16384;   // pages whose counts fit in LDS (128 KB)
 
 // scratch words: per page the count without part-filled last pages, the lowest row that ends in the
 // page (INT_MAX: none; kTaken: handed out in this call) and the pages handed out, in order; per row
-// its first entry in that list and the rows that copy their last page; then the totals.
-constexpr int kTaken = -1;
-enum { kNeed = 0, kCopies = 1, kFailed = 2 };
+// its first entry in that list (kCopied: the row copies its last kept page into it) and the rows that
+// copy; then the totals.
+constexpr int kTaken = -1, kCopied = 1 << 30;
+enum { kCopies = 0, kFailed = 1 };
 struct Scratch {
   int32_t *count, *keeper, *list, *start, *copies, *totals;
 };
 __device__ inline Scratch scratch_of(const PagesArgs& a) {
   int32_t* p = a.scratch;
-  return Scratch{p, p + a.n_pages, p + 2 * (long)a.n_pages, p + 3 * (long)a.n_pages,
-                 p + 3 * (long)a.n_pages + a.n_slots, p + 3 * (long)a.n_pages + 2 * (long)a.n_slots};
+  const long pages = a.n_pages, slots = a.n_slots;
+  return Scratch{p, p + pages, p + 2 * pages, p + 3 * pages, p + 3 * pages + slots,
+                 p + 3 * pages + 2 * slots};
 }
 
 __device__ inline int pages_of(const PagesArgs& a, int tokens) {
@@ -56,6 +61,106 @@ __device__ inline Slot slot_of(const PagesArgs& a, int slot) {
   r.part = (r.kept & ((1 << a.page_shift) - 1)) != 0;
   return r;
 }
+// The part-filled last page that row `slot` keeps, or a number that is no page.
+__device__ inline int last_page(const PagesArgs& a, const Slot& s) {
+  return s.part ? a.table[(long)s.parent * a.width + s.kept_pages - 1] : -1;
+}
+
+// Row `slot` gives back its old pages and holds the ones it keeps, entries first, first + step, ...:
+// whole adds and a minimum, so their order does not matter.
+__device__ inline void count_row(const PagesArgs& a, int slot, int first, int step, int32_t* count,
+                                 int32_t* keeper) {
+  const Slot s = slot_of(a, slot);
+  const int old_pages = pages_of(a, clamp_length(a, a.lengths[slot]));
+  const int32_t* mine = a.table + (long)slot * a.width;
+  const int32_t* from = a.table + (long)max(s.parent, 0) * a.width;
+  const int whole = s.kept_pages - s.part;
+  // (its own whole pages are held before and after)
+  for (int j = first + (s.parent == slot ? whole : 0); j < max(old_pages, s.kept_pages); j += step) {
+    if (j < old_pages && is_page(a, mine[j])) atomicAdd(&count[mine[j]], -1);
+    if (j >= s.kept_pages || !is_page(a, from[j])) continue;
+    if (j >= whole) atomicMin(&keeper[from[j]], slot);
+    else atomicAdd(&count[from[j]], 1);
+  }
+}
+
+// One work-group hands out the free pages: how many every row needs, then the free pages in ascending
+// order until all are served.
+__device__ inline void hand_out(const PagesArgs& a, const Scratch& sc, int32_t* count, int32_t* keeper,
+                                int* s_scan, long long* s_sum) {
+  const int tid = threadIdx.x;
+  long long need = 0, beyond = 0;
+  int first = 0, copies = 0;  // so far (these wrap only where the total passes the pages)
+  for (int base = 0; base < a.n_slots; base += ST) {
+    const int slot = base + tid;
+    int x[2] = {0, 0}, total[2];
+    if (slot < a.n_slots) {
+      const Slot s = slot_of(a, slot);
+      const int last = last_page(a, s);
+      x[1] = is_page(a, last) && !(count[last] <= 0 && keeper[last] == slot);
+      x[0] = x[1] + s.wanted_pages - s.kept_pages;
+      need += x[0];
+      beyond += max(0, s.wanted_pages - a.width);
+    }
+    const int copy = x[1];
+    block_exclusive_sums<SW>(x, total, s_scan);
+    if (slot < a.n_slots) sc.start[slot] = ((first + x[0]) & (kCopied - 1)) | (copy ? kCopied : 0);
+    if (copy) sc.copies[copies + x[1]] = slot;
+    first += total[0];
+    copies += total[1];
+  }
+  need = block_sum<SW>(need, s_sum);
+  beyond = block_sum<SW>(beyond, s_sum);
+  long long found = 0;
+  for (int base = 0; base < a.n_pages && found < need; base += PER * ST) {
+    bool is_free[PER];
+    int at[PER], total;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int page = base + i * ST + tid;
+      is_free[i] = page < a.n_pages && count[page] <= 0 && keeper[page] == INT_MAX;
+    }
+    block_places<SW>(is_free, at, total, s_scan);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (is_free[i] && found + at[i] < need) {
+        sc.list[found + at[i]] = base + i * ST + tid;
+        keeper[base + i * ST + tid] = kTaken;
+      }
+    found += total;
+  }
+  const long long lacking = max(0LL, need - found) + beyond;
+  if (tid == 0) {
+    sc.totals[kCopies] = copies;
+    sc.totals[kFailed] = lacking != 0;
+    a.result[0] = (int)min(lacking, (long long)INT_MAX);
+  }
+  // the counts of the next step, or of this one again
+  __syncthreads();
+#pragma unroll 4
+  for (int p = tid; p < a.n_pages; p += ST) {
+    const int k = keeper[p], c = count[p];
+    a.refs_out[p] = lacking != 0 ? a.refs[p] : k == kTaken || (k != INT_MAX && c <= 0) ? 1 : max(c, 0);
+  }
+}
+
+// Pools of up to kLdsPages pages: one work-group counts in LDS and hands out.
+__global__ __launch_bounds__(ST) void remap_small_kernel(PagesArgs a) {
+  __shared__ int32_t s_count[kLdsPages], s_keeper[kLdsPages];
+  __shared__ int s_scan[PER * SW];
+  __shared__ long long s_sum[SW];
+#pragma unroll 4
+  for (int p = threadIdx.x; p < a.n_pages; p += ST) {
+    s_count[p] = a.refs[p];
+    s_keeper[p] = INT_MAX;
+  }
+  __syncthreads();
+  // 16 lanes per row: rows that go on as themselves only have their last page to look at
+  for (int slot = threadIdx.x >> 4; slot < a.n_slots; slot += ST / 16)
+    count_row(a, slot, threadIdx.x & 15, 16, s_count, s_keeper);
+  __syncthreads();
+  hand_out(a, scratch_of(a), s_count, s_keeper, s_scan, s_sum);
+}
 
 __global__ __launch_bounds__(T) void remap_clear_kernel(PagesArgs a) {
   const Scratch sc = scratch_of(a);
@@ -64,110 +169,37 @@ __global__ __launch_bounds__(T) void remap_clear_kernel(PagesArgs a) {
   sc.count[p] = a.refs[p];
   sc.keeper[p] = INT_MAX;
 }
-
-// One work-group per row: its old pages are given back, the pages it keeps counted (whole adds and a
-// minimum, so their order does not matter) and written to its new table row.
 __global__ __launch_bounds__(T) void remap_rows_kernel(PagesArgs a) {
   const Scratch sc = scratch_of(a);
-  const int slot = blockIdx.x;
-  const Slot s = slot_of(a, slot);
-  const int old_pages = pages_of(a, clamp_length(a, a.lengths[slot]));
-  const int32_t* mine = a.table + (long)slot * a.width;
-  const int32_t* from = a.table + (long)max(s.parent, 0) * a.width;
-  for (int j = threadIdx.x; j < a.width; j += T) {
-    const bool keep = j < s.kept_pages, tail = keep && s.part && j == s.kept_pages - 1;
-    const int page = keep ? from[j] : -1;
-    a.table_out[(long)slot * a.width + j] = page;
-    if (s.parent == slot && keep && !tail) continue;  // held before and after
-    if (j < old_pages && is_page(a, mine[j])) atomicAdd(&sc.count[mine[j]], -1);
-    if (!keep || !is_page(a, page)) continue;
-    if (tail) atomicMin(&sc.keeper[page], slot);
-    else atomicAdd(&sc.count[page], 1);
-  }
+  count_row(a, blockIdx.x, threadIdx.x, T, sc.count, sc.keeper);
 }
-
-// Whether row `slot` gets a copy of its last kept page: another row or the program holds it too.
-__device__ inline int has_copy(const PagesArgs& a, const Scratch& sc, int slot, const Slot& s) {
-  if (!s.part) return 0;
-  const int last = a.table_out[(long)slot * a.width + s.kept_pages - 1];
-  return is_page(a, last) && !(sc.count[last] <= 0 && sc.keeper[last] == slot);
-}
-
-// One work-group hands out the free pages: how many every row needs, then the free pages in
-// ascending order until all are served.
 __global__ __launch_bounds__(ST) void remap_hand_out_kernel(PagesArgs a) {
-  __shared__ long long s_scan[ST / 64];
+  __shared__ int s_scan[PER * SW];
+  __shared__ long long s_sum[SW];
   const Scratch sc = scratch_of(a);
-  const int tid = threadIdx.x;
-  long long need = 0, copies = 0, beyond = 0;  // totals so far
-  for (int base = 0; base < a.n_slots; base += ST) {
-    const int slot = base + tid;
-    long long mine = 0, copy = 0, over = 0;
-    if (slot < a.n_slots) {
-      const Slot s = slot_of(a, slot);
-      copy = has_copy(a, sc, slot, s);
-      mine = copy + s.wanted_pages - s.kept_pages;
-      over = max(0, s.wanted_pages - a.width);
-    }
-    long long all;
-    const long long before = block_exclusive_sum<ST / 64>(mine, s_scan, all);
-    if (slot < a.n_slots) sc.start[slot] = (int)min(need + before, (long long)INT_MAX);
-    need += all;
-    const long long place = block_exclusive_sum<ST / 64>(copy, s_scan, all);
-    if (copy) sc.copies[copies + place] = slot;
-    copies += all;
-    block_exclusive_sum<ST / 64>(over, s_scan, all);
-    beyond += all;
-  }
-  long long found = 0;
-  for (int base = 0; base < a.n_pages && found < need; base += ST) {
-    const int page = base + tid;
-    const bool is_free = page < a.n_pages && sc.count[page] <= 0 && sc.keeper[page] == INT_MAX;
-    long long all;
-    const long long at = found + block_exclusive_sum<ST / 64>((long long)is_free, s_scan, all);
-    if (is_free && at < need) {
-      sc.list[at] = page;
-      sc.keeper[page] = kTaken;
-    }
-    found += all;
-  }
-  if (tid == 0) {
-    const long long lacking = max(0LL, need - found) + beyond;
-    sc.totals[kNeed] = (int)min(need, (long long)INT_MAX);
-    sc.totals[kCopies] = (int)copies;
-    sc.totals[kFailed] = lacking != 0;
-    a.result[0] = (int)min(lacking, (long long)INT_MAX);
-  }
+  hand_out(a, sc, sc.count, sc.keeper, s_scan, s_sum);
 }
 
-// The last step: work-groups below n_slots write the rows' new pages, the next ones the counts, the
-// others copy the part-filled pages. Where the pages did not suffice everything stays as it was.
-__global__ __launch_bounds__(T) void remap_finish_kernel(PagesArgs a, int count_groups) {
+// The last step: work-groups below n_slots write the rows, the others copy the part-filled pages. Where
+// the pages did not suffice everything stays as it was.
+__global__ __launch_bounds__(T) void remap_finish_kernel(PagesArgs a) {
   const Scratch sc = scratch_of(a);
   const bool failed = sc.totals[kFailed] != 0;
   const int tid = threadIdx.x;
   if ((int)blockIdx.x < a.n_slots) {
     const int slot = blockIdx.x;
-    int32_t* out = a.table_out + (long)slot * a.width;
-    if (failed) {
-      for (int j = tid; j < a.width; j += T) out[j] = a.table[(long)slot * a.width + j];
-      if (tid == 0) a.lengths_out[slot] = a.lengths[slot];
-      return;
-    }
     const Slot s = slot_of(a, slot);
-    const int copy = has_copy(a, sc, slot, s);
-    const int32_t* list = sc.list + sc.start[slot];
-    for (int j = s.kept_pages + tid; j < s.wanted_pages; j += T) out[j] = list[copy + j - s.kept_pages];
-    if (tid == 0) a.lengths_out[slot] = s.wanted;
-    __syncthreads();  // every thread has read the row's last kept page
-    if (tid == 0 && copy) out[s.kept_pages - 1] = list[0];
-    return;
-  }
-  if ((int)blockIdx.x < a.n_slots + count_groups) {
-    const int p = (blockIdx.x - a.n_slots) * T + tid;
-    if (p >= a.n_pages) return;
-    const int held = sc.keeper[p] == kTaken || (sc.keeper[p] != INT_MAX && sc.count[p] <= 0);
-    a.refs_out[p] = failed ? a.refs[p] : held ? 1 : max(sc.count[p], 0);
+    const int32_t* from = a.table + (long)(failed ? slot : max(s.parent, 0)) * a.width;
+    const int given = sc.start[slot], copy = (given & kCopied) != 0;
+    // page j of the row is list[j] for the copied last page and the ones that it grows by
+    const int32_t* list = sc.list + (long)(given & (kCopied - 1)) - (s.kept_pages - copy);
+    for (int j = tid; j < a.width; j += T) {
+      int page = -1;
+      if (failed || j < s.kept_pages - copy) page = from[j];
+      else if (j < s.wanted_pages) page = list[j];
+      a.table_out[(long)slot * a.width + j] = page;
+    }
+    if (tid == 0) a.lengths_out[slot] = failed ? a.lengths[slot] : s.wanted;
     return;
   }
   if (failed) return;
@@ -175,12 +207,11 @@ __global__ __launch_bounds__(T) void remap_finish_kernel(PagesArgs a, int count_
   const int ps = 1 << a.page_shift, row_chunks = kHeadDim / 8;
   const long page_chunks = (long)a.kv_heads * ps * row_chunks;
   u32x4* pages = (u32x4*)a.pages;
-  for (long u = blockIdx.x - a.n_slots - count_groups; u < units; u += kCopyGroups) {
+  for (long u = blockIdx.x - a.n_slots; u < units; u += kCopyGroups) {
     const int slot = sc.copies[u / a.outer];
     const long o = u % a.outer;
     const Slot s = slot_of(a, slot);
-    const int src = a.table[(long)s.parent * a.width + s.kept_pages - 1];
-    const int dst = sc.list[sc.start[slot]];
+    const int src = last_page(a, s), dst = sc.list[sc.start[slot] & (kCopied - 1)];
     const int run = (s.kept & (ps - 1)) * row_chunks;  // 16-byte chunks of a head
     const u32x4* from = pages + (o * a.n_pages + src) * page_chunks;
     u32x4* to = pages + (o * a.n_pages + dst) * page_chunks;
@@ -192,76 +223,88 @@ __global__ __launch_bounds__(T) void remap_finish_kernel(PagesArgs a, int count_
 }
 
 // ------------------------------------------------------------------------------------------------
-// compaction: scratch words are place (where every page goes), from (where it comes from) and the
-// movers' list; totals hold their number and the live pages.
+// compaction: scratch words are the pages that move, the free pages that take them (in the same order),
+// for a page that moves its new place and for a page that is taken where its rows come from.
 // ------------------------------------------------------------------------------------------------
-__global__ __launch_bounds__(ST) void compact_plan_kernel(PagesArgs a) {
-  __shared__ int s_scan[ST / 64];
+struct Moves {
+  int32_t *movers, *holes, *other, *totals;
+};
+__device__ inline Moves moves_of(const PagesArgs& a) {
   const Scratch sc = scratch_of(a);
-  int32_t *place = sc.count, *from = sc.keeper, *movers = sc.list;
+  return Moves{sc.count, sc.keeper, sc.list, sc.totals};
+}
+
+__global__ __launch_bounds__(ST) void compact_plan_kernel(PagesArgs a) {
+  __shared__ int s_scan[PER * SW];
+  __shared__ long long s_sum[SW];
+  const Moves mv = moves_of(a);
   const int tid = threadIdx.x;
-  int n_live = 0, all;
-  for (int base = 0; base < a.n_pages; base += ST) {
-    const int p = base + tid;
-    block_exclusive_sum<ST / 64>((int)(p < a.n_pages && a.refs[p] > 0), s_scan, all);
-    n_live += all;
-  }
-  // live pages past n_live, in order; then the free pages below it take them in the same order
+  long long live = 0;
+#pragma unroll 4
+  for (int p = tid; p < a.n_pages; p += ST) live += a.refs[p] > 0;
+  const int n_live = (int)block_sum<SW>(live, s_sum);
   int moves = 0, holes = 0;
-  for (int base = 0; base < a.n_pages; base += ST) {
-    const int p = base + tid;
-    const bool moves_out = p < a.n_pages && p >= n_live && a.refs[p] > 0;
-    const int at = block_exclusive_sum<ST / 64>((int)moves_out, s_scan, all);
-    if (moves_out) movers[moves + at] = p;
-    moves += all;
-  }
-  __syncthreads();
-  for (int base = 0; base < a.n_pages; base += ST) {
-    const int p = base + tid;
-    const bool hole = p < n_live && a.refs[p] <= 0;
-    const int at = block_exclusive_sum<ST / 64>((int)hole, s_scan, all);
-    if (hole) {
-      const int src = movers[holes + at];
-      place[src] = p;
-      from[p] = src;
-    } else if (p < a.n_pages) {
-      from[p] = p;
-      if (p < n_live) place[p] = p;
+  for (int base = 0; base < a.n_pages; base += PER * ST) {
+    bool wanted[PER];
+    int at[PER], total;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int p = base + i * ST + tid;
+      wanted[i] = p < a.n_pages && (a.refs[p] > 0) != (p < n_live);
     }
-    holes += all;
+    // (free pages below n_live, then live pages from n_live on: a step that has both has them in this
+    // order, and the holes' total is known when the movers begin)
+    block_places<SW>(wanted, at, total, s_scan);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (wanted[i]) {
+        const int p = base + i * ST + tid;
+        if (p < n_live) mv.holes[holes + at[i]] = p;
+        else mv.movers[holes + at[i]] = p;  // shifted by all holes, taken back below
+      }
+    holes += total;
+  }
+  moves = holes / 2;  // as many pages move as are taken
+  __syncthreads();
+  for (int k = tid; k < moves; k += ST) {
+    const int src = mv.movers[moves + k], dst = mv.holes[k];
+    mv.other[src] = dst;
+    mv.other[dst] = src;
   }
   if (tid == 0) {
-    sc.totals[0] = moves;
+    mv.totals[0] = moves;
     a.result[0] = n_live;
   }
 }
 
 __global__ __launch_bounds__(T) void compact_move_kernel(PagesArgs a, int count_groups) {
-  const Scratch sc = scratch_of(a);
-  const int32_t *place = sc.count, *from = sc.keeper, *movers = sc.list;
-  const int n_live = a.result[0], tid = threadIdx.x;
+  const Moves mv = moves_of(a);
+  const int n_live = a.result[0], moves = mv.totals[0], tid = threadIdx.x;
   if ((int)blockIdx.x < a.n_slots) {
     const long row = (long)blockIdx.x * a.width;
     const int used = pages_of(a, clamp_length(a, a.lengths[blockIdx.x]));
     for (int j = tid; j < a.width; j += T) {
       const int page = j < used ? a.table[row + j] : -1;
-      a.table_out[row + j] = is_page(a, page) && a.refs[page] > 0 ? place[page] : -1;
+      const bool held = is_page(a, page) && a.refs[page] > 0;
+      a.table_out[row + j] = !held ? -1 : page < n_live ? page : mv.other[page];
     }
     return;
   }
   if ((int)blockIdx.x < a.n_slots + count_groups) {
     const int p = (blockIdx.x - a.n_slots) * T + tid;
-    if (p < a.n_pages) a.refs_out[p] = p < n_live ? a.refs[from[p]] : 0;
+    if (p >= a.n_pages) return;
+    const int own = a.refs[p];
+    a.refs_out[p] = p >= n_live ? 0 : own > 0 ? own : a.refs[mv.other[p]];
     return;
   }
   const long page_chunks = (long)a.kv_heads * (kHeadDim / 8) << a.page_shift;
   u32x4* pages = (u32x4*)a.pages;
-  const long units = (long)sc.totals[0] * a.outer;
+  const long units = (long)moves * a.outer;
   for (long u = blockIdx.x - a.n_slots - count_groups; u < units; u += kCopyGroups) {
-    const int src = movers[u / a.outer];
+    const int src = mv.movers[moves + u / a.outer];
     const long layer = u % a.outer * a.n_pages;
     const u32x4* x = pages + (layer + src) * page_chunks;
-    u32x4* y = pages + (layer + place[src]) * page_chunks;
+    u32x4* y = pages + (layer + mv.other[src]) * page_chunks;
     for (long i = tid; i < page_chunks; i += T) y[i] = x[i];
   }
 }
@@ -269,14 +312,15 @@ __global__ __launch_bounds__(T) void compact_move_kernel(PagesArgs a, int count_
 }  // namespace
 
 hipError_t launch_pages_remap(const PagesArgs& a) {
-  const int count_groups = (a.n_pages + T - 1) / T;
-  if (count_groups > 0)
-    hipLaunchKernelGGL(remap_clear_kernel, dim3(count_groups), dim3(T), 0, a.stream, a);
-  if (a.n_slots > 0)
-    hipLaunchKernelGGL(remap_rows_kernel, dim3(a.n_slots), dim3(T), 0, a.stream, a);
-  hipLaunchKernelGGL(remap_hand_out_kernel, dim3(1), dim3(ST), 0, a.stream, a);
-  hipLaunchKernelGGL(remap_finish_kernel, dim3(a.n_slots + count_groups + kCopyGroups), dim3(T), 0,
-                     a.stream, a, count_groups);
+  if (a.n_pages <= kLdsPages) {
+    hipLaunchKernelGGL(remap_small_kernel, dim3(1), dim3(ST), 0, a.stream, a);
+  } else {
+    hipLaunchKernelGGL(remap_clear_kernel, dim3((a.n_pages + T - 1) / T), dim3(T), 0, a.stream, a);
+    if (a.n_slots > 0)
+      hipLaunchKernelGGL(remap_rows_kernel, dim3(a.n_slots), dim3(T), 0, a.stream, a);
+    hipLaunchKernelGGL(remap_hand_out_kernel, dim3(1), dim3(ST), 0, a.stream, a);
+  }
+  hipLaunchKernelGGL(remap_finish_kernel, dim3(a.n_slots + kCopyGroups), dim3(T), 0, a.stream, a);
   return hipGetLastError();
 }
 

@@ -9,7 +9,7 @@
 
 namespace va {
 
-constexpr int kPagedMaxSeqs = 8192;  // sequences of a step
+constexpr int kPagedMaxSeqs = 4096;  // sequences of a step
 constexpr int kPageMin = 16, kPageMax = 256;
 
 // Work items of a step: rows (token, query head of the group) of one sequence and key/value head,
@@ -17,9 +17,12 @@ constexpr int kPageMin = 16, kPageMax = 256;
 // more are tiles of kPagedTileRows, a strip of 32 per wave.
 constexpr int kPagedFewRows = 32;
 constexpr int kPagedTileRows = 128;
-constexpr int kPagedChunkKeys = 64;   // key ranges are split at multiples of this
-constexpr int kPagedMinKeys = 256;    // shortest part of a split key range (but the last)
-constexpr int kPagedParts = 1024;     // parts that a step's keys are split into, when they are
+constexpr int kPagedChunkKeys = 64;  // key ranges are split at multiples of this
+// Parts that a step's keys are split into, by kind of tile, the shortest part (but a range's last) and
+// the longest table row that is never split.
+constexpr int kPagedFewParts = 512, kPagedManyParts = 256;
+constexpr int kPagedFewKeys = 256, kPagedManyKeys = 512;
+constexpr int kPagedWholeKeys = 1024;
 constexpr int kPagedPadRows = 64;     // padding rows that one item zeroes
 
 // A step's plan, int32 words: cu (n_seqs + 1) row offsets of the sequences, the sequence (-1: padding)
@@ -30,21 +33,24 @@ struct PagedLayout {
   int64_t max_items, max_merges, max_part_rows;
 };
 inline int64_t up4(int64_t x) { return (x + 3) & ~int64_t(3); }
-// Bounds: a sequence with rows makes one tile, and one more per full kPagedTileRows. Parts have at
-// least total / kPagedParts keys, so a tile of n > 1 parts stands for more than n - 1 >= n / 2 of the
-// kPagedParts, and the tiles that are split have at most 2 kPagedParts parts; each part holds at most
-// kPagedTileRows rows, and a row is in at most max_keys / kPagedMinKeys + 1 parts. A merge record
-// takes 8 rows of a tile of up to 8 parts, or one row of a tile of more.
+// Bounds: a sequence with rows makes one tile, and one more per full kPagedTileRows. A kind's parts have
+// at least its total (tiles times the longest of the sequence) / its number of parts keys, so the
+// tiles of a sequence of n > 1 parts stand for more than n - 1 >= n / 2 of them each, and all split
+// tiles have at most twice as many parts; each part holds at most the kind's rows, and a row is in at
+// most max_keys / kPagedFewKeys + 1 parts. A merge record takes 8 rows of a sequence of up to 8 parts,
+// or one row of one of more.
 inline PagedLayout paged_layout(int64_t n_seqs, int64_t n_tokens, int64_t hq, int64_t hkv,
                                 int64_t max_keys) {
   PagedLayout l;
   const int64_t tiles = (n_seqs < n_tokens ? n_seqs : n_tokens) + n_tokens * (hq / hkv) / kPagedTileRows;
-  const bool split = max_keys > kPagedMinKeys;
+  const bool split = max_keys > kPagedWholeKeys;
   const int64_t rows = n_tokens * hq;
-  l.max_items = tiles * hkv + (split ? kPagedParts : 0) + (n_tokens + kPagedPadRows - 1) / kPagedPadRows;
-  l.max_merges = !split ? 0 : rows < 16 * kPagedParts ? rows : 16 * kPagedParts;
-  const int64_t by_row = rows * (max_keys / kPagedMinKeys + 1);
-  const int64_t by_part = 2 * kPagedParts * kPagedTileRows;
+  l.max_items = tiles * hkv + (split ? kPagedFewParts + kPagedManyParts : 0) +
+                (n_tokens + kPagedPadRows - 1) / kPagedPadRows;
+  const int64_t merges = kPagedFewParts * (kPagedFewRows / 8) + kPagedManyParts * (kPagedTileRows / 8);
+  l.max_merges = !split ? 0 : rows < merges ? rows : merges;
+  const int64_t by_row = rows * (max_keys / kPagedFewKeys + 1);
+  const int64_t by_part = 2 * (kPagedFewParts * kPagedFewRows + kPagedManyParts * kPagedTileRows);
   l.max_part_rows = !split ? 0 : by_row < by_part ? by_row : by_part;
   l.seq = up4(n_seqs + 1);
   l.pos = l.seq + up4(n_tokens);

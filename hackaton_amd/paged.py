@@ -27,37 +27,35 @@ from ._lib import check, lib
 from .attention import _DTYPES, HEAD_DIM, _attn_dtype, _rope_strides, _stream, _tables
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
-MAX_SEQUENCES = 8192  # of one step
 
 
 def _no_grad(*tensors):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError("the paged cache has no backward: call it under torch.no_grad() or "
-                           "torch.inference_mode()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise RuntimeError("the paged cache has no backward: call it under torch.no_grad() "
+                                   "or torch.inference_mode()")
 
 
-def _one_device(*tensors):
-    device = tensors[0].device
+def _one_device(first, *tensors):
+    device = first.device
+    if device.type != "cuda":
+        raise ValueError(f"the paged cache lives on the GPU only: got a tensor on {device}")
     for t in tensors:
-        if not t.is_cuda:
-            raise ValueError(f"the paged cache lives on the GPU only: got a tensor on {t.device}")
         if t.device != device:
             raise ValueError(f"tensors on {device} and {t.device}")
     return device
 
 
 def _on_device(fn):
-    """Run `fn` with the device of its tensors current (launches and allocations go there)."""
+    """Run `fn` with the device of its first tensor current (launches and allocations go there)."""
 
     @functools.wraps(fn)
-    def call(*args, **kwargs):
-        for t in args:
-            if isinstance(t, torch.Tensor):
-                if t.is_cuda and t.device.index != torch._C._cuda_getDevice():
-                    with torch.cuda.device(t.device):
-                        return fn(*args, **kwargs)
-                break
-        return fn(*args, **kwargs)
+    def call(first, *args, **kwargs):
+        if first.is_cuda and first.device.index != torch._C._cuda_getDevice():
+            with torch.cuda.device(first.device):
+                return fn(first, *args, **kwargs)
+        return fn(first, *args, **kwargs)
 
     return call
 
@@ -110,9 +108,9 @@ def _check_host_lengths(q_lengths, kv_lengths, n_tokens, most):
 def _plan_sizes(n_seqs, n_tokens, heads, kv_heads, page_size, width):
     """(int32 words of a plan, workspace bytes of an attention over it)."""
     words, nbytes = ctypes.c_int64(), ctypes.c_int64()
-    sizes = (n_seqs, n_tokens, heads, kv_heads, page_size, width)
-    check(lib().va_paged_plan_words(*sizes, ctypes.byref(words)), "va_paged_plan_words")
-    check(lib().va_paged_attention_workspace(*sizes, ctypes.byref(nbytes)),
+    step = _lib.PagedStep(None, None, n_tokens, n_seqs, width, page_size, heads, kv_heads)
+    check(lib().va_paged_plan_words(step, ctypes.byref(words)), "va_paged_plan_words")
+    check(lib().va_paged_attention_workspace(step, ctypes.byref(nbytes)),
           "va_paged_attention_workspace")
     return words.value, nbytes.value
 
@@ -122,8 +120,8 @@ class PagedPlan:
     page table and follows its entries as they are when a call runs; the lengths were read when the
     plan was made (a captured plan reads them again in every replay)."""
 
-    __slots__ = ("page_table", "words", "n_tokens", "n_seqs", "width", "heads", "kv_heads",
-                 "page_size", "workspace_bytes", "_stream")
+    __slots__ = ("page_table", "words", "n_tokens", "n_seqs", "heads", "kv_heads", "page_size",
+                 "workspace_bytes", "_step", "_page", "_stream")
 
     def _rows(self, which):
         rows = -(-self.n_tokens // 4) * 4
@@ -167,12 +165,14 @@ def paged_plan(page_table, q_lengths, kv_lengths, n_tokens, heads, kv_heads, pag
     n_words, plan.workspace_bytes = _plan_sizes(n_seqs, n_tokens, heads, kv_heads, page_size, width)
     q_lengths = _lengths("q_lengths", q_lengths, n_seqs, device)
     kv_lengths = _lengths("kv_lengths", kv_lengths, n_seqs, device)
-    plan.page_table, plan.n_tokens, plan.n_seqs, plan.width = page_table, n_tokens, n_seqs, width
+    plan.page_table, plan.n_tokens, plan.n_seqs = page_table, n_tokens, n_seqs
     plan.heads, plan.kv_heads, plan.page_size = heads, kv_heads, page_size
+    plan._page = (kv_heads, page_size, HEAD_DIM)
     plan.words = torch.empty(n_words, dtype=torch.int32, device=device)
     plan._stream = _stream()
-    check(lib().va_paged_plan(q_lengths.data_ptr(), kv_lengths.data_ptr(), n_seqs, n_tokens, heads,
-                              kv_heads, page_size, width, plan.words.data_ptr(), n_words,
+    plan._step = _lib.PagedStep(page_table.data_ptr(), plan.words.data_ptr(), n_tokens, n_seqs, width,
+                                page_size, heads, kv_heads)
+    check(lib().va_paged_plan(plan._step, q_lengths.data_ptr(), kv_lengths.data_ptr(), n_words,
                               plan._stream), "va_paged_plan")
     return plan
 
@@ -180,20 +180,19 @@ def paged_plan(page_table, q_lengths, kv_lengths, n_tokens, heads, kv_heads, pag
 def _pages_of(k_pages, v_pages, plan):
     """(elements from one key page to the next, value page, number of pages) of one layer."""
     shape = k_pages.shape
-    if v_pages.shape != shape or len(shape) != 4 or tuple(shape[1:]) != (
-            plan.kv_heads, plan.page_size, HEAD_DIM):
-        raise ValueError(f"pages must be (n_pages, {plan.kv_heads}, {plan.page_size}, {HEAD_DIM}), "
-                         f"got {tuple(shape)} and {tuple(v_pages.shape)}")
+    if v_pages.shape != shape or shape[1:] != plan._page:
+        raise ValueError("pages must be (n_pages, %d, %d, %d), got " % plan._page +
+                         f"{tuple(shape)} and {tuple(v_pages.shape)}")
     if k_pages.dtype != v_pages.dtype:
         raise ValueError(f"keys in {k_pages.dtype}, values in {v_pages.dtype}")
-    row = (plan.page_size * HEAD_DIM, HEAD_DIM, 1)
     strides = []
     for pages in (k_pages, v_pages):
-        stride = pages.stride()
-        if stride[1:] != row and not (plan.kv_heads == 1 and stride[2:] == row[1:]):
-            raise ValueError(f"every page must be contiguous, got strides {stride}")
+        stride, head, row, element = pages.stride()
+        if element != 1 or row != HEAD_DIM or (head != row * plan.page_size and plan.kv_heads != 1):
+            raise ValueError(f"every page must be contiguous, got strides {pages.stride()}")
         # (a pool of one page: its stride is free)
-        strides.append(max(stride[0], plan.kv_heads * row[0]) if shape[0] <= 1 else stride[0])
+        least = plan.kv_heads * plan.page_size * HEAD_DIM
+        strides.append(max(stride, least) if shape[0] <= 1 else stride)
     return strides[0], strides[1], shape[0]
 
 
@@ -232,11 +231,10 @@ def paged_append(q, k, v, cos, sin, k_pages, v_pages, plan):
     batch, row = (0, 0) if by_row else _rope_strides(cos)
     q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
     check(lib().va_paged_append(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), cos.data_ptr(), sin.data_ptr(), batch, row,
-        HEAD_DIM if by_row else 0, 0 if by_row else cos.shape[1], plan.words.data_ptr(),
-        plan.page_table.data_ptr(), plan.n_seqs, plan.width, query.data_ptr(), k_pages.data_ptr(),
-        v_pages.data_ptr(), k_stride, v_stride, n_pages, plan.page_size, n, heads, kv_heads,
-        HEAD_DIM, _DTYPES[q.dtype], out_dtype, plan._use()), "va_paged_append")
+        plan._step, q.data_ptr(), k.data_ptr(), v.data_ptr(), cos.data_ptr(), sin.data_ptr(), batch,
+        row, HEAD_DIM if by_row else 0, 0 if by_row else cos.shape[1], query.data_ptr(),
+        k_pages.data_ptr(), v_pages.data_ptr(), k_stride, v_stride, n_pages, HEAD_DIM,
+        _DTYPES[q.dtype], out_dtype, plan._use()), "va_paged_append")
     return query
 
 
@@ -245,26 +243,25 @@ def paged_attention(query, k_pages, v_pages, plan, scale):
     """Every new token attends to its sequence's keys at positions up to its own. query
     (n_tokens, heads, 128) in the pages' type; returns (n_tokens, heads * 128), zeros for padding and
     for rows that see no key. Key/value heads are shared by heads / kv_heads query heads each."""
-    _one_device(query, k_pages, v_pages, plan.words)
+    device = _one_device(query, k_pages, v_pages, plan.words)
     _no_grad(query, k_pages, v_pages)
     dtype = _attn_dtype(query)
     if k_pages.dtype != query.dtype:
         raise ValueError(f"query in {query.dtype}, pages in {k_pages.dtype}")
     n, heads = plan.n_tokens, plan.heads
-    if tuple(query.shape) != (n, heads, HEAD_DIM):
+    if query.shape != (n, heads, HEAD_DIM):
         raise ValueError(f"query must be ({n}, {heads}, {HEAD_DIM}), got {tuple(query.shape)}")
     k_stride, v_stride, n_pages = _pages_of(k_pages, v_pages, plan)
     query = query.contiguous()
-    out = torch.empty(n, heads * HEAD_DIM, dtype=query.dtype, device=query.device)
+    out = torch.empty((n, heads * HEAD_DIM), dtype=query.dtype, device=device)
     if n == 0:
         return out
     nbytes = plan.workspace_bytes
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=query.device) if nbytes else None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     check(lib().va_paged_attention(
-        query.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_stride, v_stride, n_pages,
-        plan.page_size, plan.page_table.data_ptr(), plan.width, plan.words.data_ptr(), plan.n_seqs,
-        n, heads, plan.kv_heads, HEAD_DIM, float(scale), dtype, out.data_ptr(),
-        ws.data_ptr() if nbytes else None, nbytes, plan._use()), "va_paged_attention")
+        plan._step, query.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_stride, v_stride,
+        n_pages, HEAD_DIM, scale, dtype, out.data_ptr(), ws.data_ptr() if nbytes else None, nbytes,
+        plan._use()), "va_paged_attention")
     return out
 
 

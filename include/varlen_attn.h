@@ -308,12 +308,16 @@ int va_unpack_rows(const void* src, void* dst, const int32_t* b_idx, const int32
  *
  * va_paged_plan writes the step's plan (va_paged_plan_words int32 of device memory, 16-byte aligned):
  * the sequence and the position of every row, and the attention's work list. It depends on the
- * lengths and sizes alone, so all layers of a step share it. n_seqs <= 8192. */
-int va_paged_plan_words(int32_t n_seqs, int64_t n_tokens, int32_t hq, int32_t hkv,
-                        int32_t page_size, int32_t table_width, int64_t* words);
-int va_paged_plan(const int32_t* q_lengths, const int32_t* kv_lengths, int32_t n_seqs,
-                  int64_t n_tokens, int32_t hq, int32_t hkv, int32_t page_size,
-                  int32_t table_width, int32_t* plan, int64_t plan_words, void* stream);
+ * lengths and sizes alone, so all layers of a step share it. n_seqs <= 4096. */
+typedef struct va_paged_step {
+  const int32_t* page_table;
+  int32_t* plan;
+  int64_t n_tokens;
+  int32_t n_seqs, table_width, page_size, hq, hkv;
+} va_paged_step;
+int va_paged_plan_words(const va_paged_step* step, int64_t* words);
+int va_paged_plan(const va_paged_step* step, const int32_t* q_lengths, const int32_t* kv_lengths,
+                  int64_t plan_words, void* stream);
 
 /* The new rows of a step: q (N, Hq*D) rotated into q_out (N, Hq, D), k (N, Hkv*D) rotated and v cast
  * into their pages, in fp32 and rounded once to out_dtype (VA_F16 / VA_BF16), from in_dtype
@@ -321,25 +325,20 @@ int va_paged_plan(const int32_t* q_lengths, const int32_t* kv_lengths, int32_t n
  * t * cos_seq_stride + n * cos_token_stride of the fp32 tables (strides in elements, non-negative
  * multiples of 4). cos_rows bounds t (0: no bound, for tables read by token): rows past it, padding
  * rows and rows at negative positions get zero q_out and write nothing. */
-int va_paged_append(const void* q, const void* k, const void* v, const float* cos,
-                    const float* sin, int64_t cos_batch_stride, int64_t cos_seq_stride,
-                    int64_t cos_token_stride, int64_t cos_rows, const int32_t* plan,
-                    const int32_t* page_table, int32_t n_seqs, int32_t table_width, void* q_out,
+int va_paged_append(const va_paged_step* step, const void* q, const void* k, const void* v,
+                    const float* cos, const float* sin, int64_t cos_batch_stride,
+                    int64_t cos_seq_stride, int64_t cos_token_stride, int64_t cos_rows, void* q_out,
                     void* k_pages, void* v_pages, int64_t k_stride, int64_t v_stride,
-                    int32_t n_pages, int32_t page_size, int64_t n_tokens, int32_t hq,
-                    int32_t hkv, int32_t head_dim, int32_t in_dtype, int32_t out_dtype,
+                    int32_t n_pages, int32_t head_dim, int32_t in_dtype, int32_t out_dtype,
                     void* stream);
 
 /* out (N, Hq, 128) = softmax(scale q k^T) v of every new token over its sequence's keys at positions
  * up to its own; zeros for padding rows and for rows that see no key. The workspace
  * (va_paged_attention_workspace bytes, possibly 0) holds partial results of split key ranges; calls
  * that may overlap need one each. scale must be finite and > 0. Deterministic. */
-int va_paged_attention_workspace(int32_t n_seqs, int64_t n_tokens, int32_t hq, int32_t hkv,
-                                 int32_t page_size, int32_t table_width, int64_t* bytes);
-int va_paged_attention(const void* q, const void* k_pages, const void* v_pages, int64_t k_stride,
-                       int64_t v_stride, int32_t n_pages, int32_t page_size,
-                       const int32_t* page_table, int32_t table_width, const int32_t* plan,
-                       int32_t n_seqs, int64_t n_tokens, int32_t hq, int32_t hkv,
+int va_paged_attention_workspace(const va_paged_step* step, int64_t* bytes);
+int va_paged_attention(const va_paged_step* step, const void* q, const void* k_pages,
+                       const void* v_pages, int64_t k_stride, int64_t v_stride, int32_t n_pages,
                        int32_t head_dim, float scale, int32_t dtype, void* out, void* workspace,
                        int64_t workspace_bytes, void* stream);
 

@@ -88,8 +88,10 @@ def test_long_contexts_split_over_the_card(dtype):
 
 
 @pytest.mark.parametrize("q,kv,heads,kv_heads", [([300], [300], 12, 2), ([257, 129], [700, 129], 14, 2),
-                                                 ([200], [2300], 2, 2)])
+                                                 ([200], [2300], 2, 2), ([1500], [1500], 4, 1)])
 def test_prompt_chunks(q, kv, heads, kv_heads):
+    """Whole prompts and chunks on top of others; a prompt whose first tiles see less keys than a part
+    of its last ones' range has."""
     for dtype in (FP16, BF16):
         check_attention(q, kv, heads, kv_heads, dtype, 32)
 

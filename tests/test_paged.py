@@ -11,12 +11,16 @@ import hackaton_amd
 from hackaton_amd import _lib, paged
 from tests import paged_oracle as orc
 
-OK = (2, 8, 12, 2, 16, 4)  # n_seqs, n_tokens, hq, hkv, page_size, table_width
+OK = dict(n_tokens=8, n_seqs=2, table_width=4, page_size=16, hq=12, hkv=2)
 
 
-def words(*sizes):
+def step(p=None, **sizes):
+    return _lib.PagedStep(p, p, *(dict(OK, **sizes)[k] for k in OK))
+
+
+def words(**sizes):
     out = ctypes.c_int64()
-    return _lib.lib().va_paged_plan_words(*sizes, ctypes.byref(out)), out.value
+    return _lib.lib().va_paged_plan_words(step(**sizes), ctypes.byref(out)), out.value
 
 
 def test_the_entry_points_are_public():
@@ -25,17 +29,15 @@ def test_the_entry_points_are_public():
         assert name in hackaton_amd.__all__ and getattr(hackaton_amd, name) is getattr(paged, name)
 
 
-@pytest.mark.parametrize("at,value,code", [
-    (0, -1, _lib.VA_ESHAPE), (0, 8193, _lib.VA_ESHAPE), (1, -1, _lib.VA_ESHAPE),
-    (1, 1 << 40, _lib.VA_ESHAPE), (2, 0, _lib.VA_ESHAPE), (2, 13, _lib.VA_ESHAPE),
-    (3, 0, _lib.VA_ESHAPE), (4, 0, _lib.VA_ESHAPE), (4, 8, _lib.VA_ESHAPE), (4, 24, _lib.VA_ESHAPE),
-    (4, 512, _lib.VA_ESHAPE), (5, -1, _lib.VA_ESHAPE), (5, 1 << 30, _lib.VA_ESHAPE)])
-def test_plan_sizes_are_checked(at, value, code):
-    sizes = list(OK)
-    assert words(*sizes)[0] == 0 and words(*sizes)[1] >= sizes[0] + 1 + 2 * sizes[1]
-    sizes[at] = value
-    assert words(*sizes)[0] == code
+@pytest.mark.parametrize("name,value", [
+    ("n_seqs", -1), ("n_seqs", 4097), ("n_tokens", -1), ("n_tokens", 1 << 40), ("hq", 0), ("hq", 13),
+    ("hkv", 0), ("page_size", 0), ("page_size", 8), ("page_size", 24), ("page_size", 512),
+    ("table_width", -1), ("table_width", 1 << 30)])
+def test_plan_sizes_are_checked(name, value):
+    assert words()[0] == 0 and words()[1] >= 3 + 2 * 8
+    assert words(**{name: value})[0] == _lib.VA_ESHAPE
     assert _lib.lib().va_last_error()
+    assert _lib.lib().va_paged_plan_words(None, ctypes.byref(ctypes.c_int64())) == _lib.VA_EINVAL
 
 
 def buffers():
@@ -44,55 +46,61 @@ def buffers():
     return raw, raw.ctypes.data + (-raw.ctypes.data) % 16
 
 
-def attention_args(p):
+def attention_args(p, **sizes):
     stride = 2 * 16 * 128
-    return [p, p, p, stride, stride, 4, 16, p, 4, p, 2, 8, 12, 2, 128, 0.1, 0, p, p, 1 << 40, None]
+    return [step(p, **sizes), p, p, p, stride, stride, 4, 128, 0.1, 0, p, p, 1 << 40, None]
 
 
 @pytest.mark.parametrize("at,value,code", [
-    (0, None, _lib.VA_EINVAL), (1, None, _lib.VA_EINVAL), (3, 8, _lib.VA_EINVAL),
-    (4, 2 * 16 * 128 + 4, _lib.VA_EINVAL), (5, -1, _lib.VA_ESHAPE), (7, None, _lib.VA_EINVAL),
-    (9, None, _lib.VA_EINVAL), (14, 64, _lib.VA_ESHAPE), (15, 0.0, _lib.VA_EINVAL),
-    (15, float("nan"), _lib.VA_EINVAL), (16, 2, _lib.VA_EDTYPE), (17, None, _lib.VA_EINVAL)])
+    (0, None, _lib.VA_EINVAL), (1, None, _lib.VA_EINVAL), (2, None, _lib.VA_EINVAL),
+    (4, 8, _lib.VA_EINVAL), (5, 2 * 16 * 128 + 4, _lib.VA_EINVAL), (6, -1, _lib.VA_ESHAPE),
+    (7, 64, _lib.VA_ESHAPE), (8, 0.0, _lib.VA_EINVAL), (8, float("nan"), _lib.VA_EINVAL),
+    (9, 2, _lib.VA_EDTYPE), (10, None, _lib.VA_EINVAL)])
 def test_attention_arguments_are_checked(at, value, code):
     raw, p = buffers()
     args = attention_args(p)
     args[at] = value
     assert _lib.lib().va_paged_attention(*args) == code
     args = attention_args(p)
-    args[0] = p + 2
+    args[1] = p + 2
+    assert _lib.lib().va_paged_attention(*args) == _lib.VA_EINVAL
+    args = attention_args(p)
+    args[0].page_table = None
+    assert _lib.lib().va_paged_attention(*args) == _lib.VA_EINVAL
+    args[0] = step(p)
+    args[0].plan = None
     assert _lib.lib().va_paged_attention(*args) == _lib.VA_EINVAL
 
 
 def test_attention_workspace_is_checked():
     need = ctypes.c_int64()
-    sizes = (64, 64, 12, 2, 16, 512)
-    assert _lib.lib().va_paged_attention_workspace(*sizes, ctypes.byref(need)) == 0
-    if need.value:
-        raw, p = buffers()
-        args = attention_args(p)
-        args[10:14] = [64, 64, 12, 2]
-        args[8], args[19] = 512, need.value - 1
-        assert _lib.lib().va_paged_attention(*args) == _lib.VA_ECAPACITY
+    sizes = dict(n_tokens=64, n_seqs=64, table_width=512)
+    assert _lib.lib().va_paged_attention_workspace(step(**sizes), ctypes.byref(need)) == 0
+    assert need.value > 0
+    raw, p = buffers()
+    args = attention_args(p, **sizes)
+    args[12] = need.value - 1
+    assert _lib.lib().va_paged_attention(*args) == _lib.VA_ECAPACITY
 
 
 def append_args(p):
     stride = 2 * 16 * 128
-    return [p, p, p, p, p, 0, 128, 0, 64, p, p, 2, 4, p, p, p, stride, stride, 4, 16, 8, 12, 2, 128,
-            0, 0, None]
+    return [step(p), p, p, p, p, p, 0, 128, 0, 64, p, p, p, stride, stride, 4, 128, 0, 0, None]
 
 
 @pytest.mark.parametrize("at,value,code", [
-    (0, None, _lib.VA_EINVAL), (5, 2, _lib.VA_EINVAL), (6, -4, _lib.VA_EINVAL),
-    (7, 3, _lib.VA_EINVAL), (8, -1, _lib.VA_EINVAL), (10, None, _lib.VA_EINVAL),
-    (13, None, _lib.VA_EINVAL), (14, None, _lib.VA_EINVAL), (16, 128, _lib.VA_EINVAL),
-    (19, 17, _lib.VA_ESHAPE), (21, 11, _lib.VA_ESHAPE), (23, 96, _lib.VA_ESHAPE),
-    (24, 3, _lib.VA_EDTYPE), (25, 2, _lib.VA_EDTYPE)])
+    (0, None, _lib.VA_EINVAL), (1, None, _lib.VA_EINVAL), (6, 2, _lib.VA_EINVAL),
+    (7, -4, _lib.VA_EINVAL), (8, 3, _lib.VA_EINVAL), (9, -1, _lib.VA_EINVAL),
+    (10, None, _lib.VA_EINVAL), (11, None, _lib.VA_EINVAL), (13, 128, _lib.VA_EINVAL),
+    (16, 96, _lib.VA_ESHAPE), (17, 3, _lib.VA_EDTYPE), (18, 2, _lib.VA_EDTYPE)])
 def test_append_arguments_are_checked(at, value, code):
     raw, p = buffers()
     args = append_args(p)
     args[at] = value
     assert _lib.lib().va_paged_append(*args) == code
+    args = append_args(p)
+    args[0] = step(p, page_size=17)
+    assert _lib.lib().va_paged_append(*args) == _lib.VA_ESHAPE
 
 
 @pytest.mark.parametrize("at,value,code", [
@@ -125,11 +133,11 @@ def test_bookkeeping_outputs_may_not_be_the_inputs():
 
 def test_nothing_to_do_returns_at_once():
     lib = _lib.lib()
-    args = attention_args(None)
-    args[11] = 0
-    args[1] = args[2] = args[7] = buffers()[1]
+    raw, p = buffers()
+    args = attention_args(p, n_tokens=0)
+    args[1] = args[10] = args[11] = None
     assert lib.va_paged_attention(*args) == 0
-    assert lib.va_paged_plan(None, None, 2, 0, 12, 2, 16, 4, None, 0, None) == 0
+    assert lib.va_paged_plan(step(n_tokens=0), None, None, 0, None) == 0
 
 
 def test_host_tensors_are_refused():
