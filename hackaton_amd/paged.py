@@ -70,7 +70,7 @@ def _int32(name, t, *shape):
     if t.dtype != torch.int32 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor, got {t.dtype}, "
                          f"strides {t.stride()}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
 
 
@@ -78,18 +78,20 @@ def _lengths(name, lengths, n_seqs, device):
     """Lengths of every sequence as an int32 device tensor, from one or from a host list."""
     if not isinstance(lengths, torch.Tensor):
         lengths = torch.tensor([int(x) for x in lengths], dtype=torch.int32, device=device)
-    lengths = lengths.reshape(-1)
     if lengths.dtype.is_floating_point or lengths.dtype == torch.bool:
         raise ValueError(f"{name} must be whole numbers, got {lengths.dtype}")
     if lengths.device != device:
         raise ValueError(f"{name} on {lengths.device}, page_table on {device}")
     if lengths.numel() != n_seqs:
         raise ValueError(f"{lengths.numel()} {name} for {n_seqs} page table rows")
-    return lengths.to(torch.int32).contiguous()
+    return lengths if lengths.dtype == torch.int32 and lengths.is_contiguous() else \
+        lengths.to(torch.int32).contiguous()
 
 
 def _check_host_lengths(q_lengths, kv_lengths, n_tokens, most):
     """Host lists are checked before anything runs; device lengths cannot be without a read."""
+    if isinstance(q_lengths, torch.Tensor) and isinstance(kv_lengths, torch.Tensor):
+        return
     q_host = None if isinstance(q_lengths, torch.Tensor) else [int(x) for x in q_lengths]
     kv_host = None if isinstance(kv_lengths, torch.Tensor) else [int(x) for x in kv_lengths]
     if q_host is not None:
@@ -121,7 +123,7 @@ class PagedPlan:
     plan was made (a captured plan reads them again in every replay)."""
 
     __slots__ = ("page_table", "words", "n_tokens", "n_seqs", "heads", "kv_heads", "page_size",
-                 "workspace_bytes", "_step", "_page", "_stream")
+                 "workspace_bytes", "_step", "_page", "_strides", "_stream")
 
     def _rows(self, which):
         rows = -(-self.n_tokens // 4) * 4
@@ -140,7 +142,7 @@ class PagedPlan:
 
     def _use(self):
         """The plan's memory is used on the current stream: not handed out again before that is done."""
-        stream = _stream()
+        stream = torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
         if stream != self._stream and not torch._C._cuda_isCurrentStreamCapturing():
             current = torch.cuda.current_stream()
             self.words.record_stream(current)
@@ -168,6 +170,7 @@ def paged_plan(page_table, q_lengths, kv_lengths, n_tokens, heads, kv_heads, pag
     plan.page_table, plan.n_tokens, plan.n_seqs = page_table, n_tokens, n_seqs
     plan.heads, plan.kv_heads, plan.page_size = heads, kv_heads, page_size
     plan._page = (kv_heads, page_size, HEAD_DIM)
+    plan._strides = (page_size * HEAD_DIM, HEAD_DIM, 1)
     plan.words = torch.empty(n_words, dtype=torch.int32, device=device)
     plan._stream = _stream()
     plan._step = _lib.PagedStep(page_table.data_ptr(), plan.words.data_ptr(), n_tokens, n_seqs, width,
@@ -185,15 +188,15 @@ def _pages_of(k_pages, v_pages, plan):
                          f"{tuple(shape)} and {tuple(v_pages.shape)}")
     if k_pages.dtype != v_pages.dtype:
         raise ValueError(f"keys in {k_pages.dtype}, values in {v_pages.dtype}")
-    strides = []
-    for pages in (k_pages, v_pages):
-        stride, head, row, element = pages.stride()
-        if element != 1 or row != HEAD_DIM or (head != row * plan.page_size and plan.kv_heads != 1):
-            raise ValueError(f"every page must be contiguous, got strides {pages.stride()}")
-        # (a pool of one page: its stride is free)
+    k_stride, v_stride = k_pages.stride(), v_pages.stride()
+    if k_stride[1:] != plan._strides or v_stride[1:] != plan._strides:
+        for stride in (k_stride, v_stride):
+            if stride[2:] != plan._strides[1:] or plan.kv_heads != 1:  # (one head: its stride is free)
+                raise ValueError(f"every page must be contiguous, got strides {stride}")
+    if shape[0] <= 1:  # a pool of one page: its stride is free
         least = plan.kv_heads * plan.page_size * HEAD_DIM
-        strides.append(max(stride, least) if shape[0] <= 1 else stride)
-    return strides[0], strides[1], shape[0]
+        return max(k_stride[0], least), max(v_stride[0], least), shape[0]
+    return k_stride[0], v_stride[0], shape[0]
 
 
 @_on_device
@@ -207,7 +210,7 @@ def paged_append(q, k, v, cos, sin, k_pages, v_pages, plan):
     device = _one_device(q, k, v, cos, sin, k_pages, v_pages, plan.words)
     _no_grad(q, k, v, k_pages, v_pages)
     n, heads, kv_heads = plan.n_tokens, plan.heads, plan.kv_heads
-    if (tuple(q.shape) != (n, heads * HEAD_DIM) or tuple(k.shape) != (n, kv_heads * HEAD_DIM)
+    if (q.shape != (n, heads * HEAD_DIM) or k.shape != (n, kv_heads * HEAD_DIM)
             or v.shape != k.shape):
         raise ValueError(f"projections must be ({n}, {heads} and {kv_heads} * {HEAD_DIM}), got "
                          f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
@@ -223,7 +226,7 @@ def paged_append(q, k, v, cos, sin, k_pages, v_pages, plan):
     cos, sin = _tables(cos[None] if by_row else cos, sin[None] if by_row else sin)
     if not by_row and cos.shape[0] not in (1, plan.n_seqs):
         raise ValueError(f"cos/sin for {cos.shape[0]} sequences, the plan has {plan.n_seqs}")
-    query = torch.empty(n, heads, HEAD_DIM, dtype=k_pages.dtype, device=device)
+    query = torch.empty((n, heads, HEAD_DIM), dtype=k_pages.dtype, device=device)
     if n == 0:
         return query
     if cos.shape[1] == 0:
