@@ -18,22 +18,23 @@ constexpr int ST = 1024;      // threads of the one work-group that counts and h
 constexpr int SW = ST / 64;
 constexpr int PER = 4;        // pages per thread and step
 constexpr int kCopyGroups = 2048;  // work-groups that copy rows (eight per CU)
-constexpr int kLdsPages = 16384;   // pages whose counts fit in LDS (128 KB)
+constexpr int kLdsPages = 16384;   // pages whose counts fit in LDS (128 KB) beside 1024 rows
 
 // scratch words: per page the count without part-filled last pages, the lowest row that ends in the
 // page (INT_MAX: none; kTaken: handed out in this call) and the pages handed out, in order; per row
-// its first entry in that list (kCopied: the row copies its last kept page into it) and the rows that
-// copy; then the totals.
+// its parent, what it keeps and becomes, its first entry in that list (kCopied: the row copies its last
+// kept page into it) and the rows that copy; then the totals.
 constexpr int kTaken = -1, kCopied = 1 << 30;
 enum { kCopies = 0, kFailed = 1 };
 struct Scratch {
-  int32_t *count, *keeper, *list, *start, *copies, *totals;
+  int32_t *count, *keeper, *list, *parent, *kept, *wanted, *start, *copies, *totals;
 };
 __device__ inline Scratch scratch_of(const PagesArgs& a) {
   int32_t* p = a.scratch;
   const long pages = a.n_pages, slots = a.n_slots;
-  return Scratch{p, p + pages, p + 2 * pages, p + 3 * pages, p + 3 * pages + slots,
-                 p + 3 * pages + 2 * slots};
+  int32_t* rows = p + 3 * pages;
+  return Scratch{p, p + pages, p + 2 * pages, rows, rows + slots, rows + 2 * slots, rows + 3 * slots,
+                 rows + 4 * slots, rows + 5 * slots};
 }
 
 __device__ inline int pages_of(const PagesArgs& a, int tokens) {
@@ -44,34 +45,31 @@ __device__ inline int clamp_length(const PagesArgs& a, int tokens) {
 }
 __device__ inline bool is_page(const PagesArgs& a, int page) { return page >= 0 && page < a.n_pages; }
 
-// What row `slot` keeps of its parent, and what it becomes.
+// What a row keeps of its parent, and what it becomes.
 struct Slot {
   int parent, kept, wanted, kept_pages, wanted_pages;
   bool part;  // the last kept page is part-filled
 };
-__device__ inline Slot slot_of(const PagesArgs& a, int slot) {
-  Slot r;
-  const int p = a.parents == nullptr ? slot : a.parents[slot];
-  r.parent = p >= 0 && p < a.n_slots ? p : -1;
-  const int had = r.parent < 0 ? 0 : clamp_length(a, a.lengths[r.parent]);
-  r.wanted = a.new_lengths == nullptr ? had : max(a.new_lengths[slot], 0);
-  r.kept = min(had, r.wanted);
-  r.kept_pages = pages_of(a, r.kept);
-  r.wanted_pages = pages_of(a, r.wanted);
-  r.part = (r.kept & ((1 << a.page_shift) - 1)) != 0;
-  return r;
+__device__ inline Slot slot_from(const PagesArgs& a, int parent, int kept, int wanted) {
+  return Slot{parent, kept, wanted, pages_of(a, kept), pages_of(a, wanted),
+              (kept & ((1 << a.page_shift) - 1)) != 0};
 }
-// The part-filled last page that row `slot` keeps, or a number that is no page.
+__device__ inline Slot slot_of(const PagesArgs& a, int slot) {
+  const int p = a.parents == nullptr ? slot : a.parents[slot];
+  const int parent = p >= 0 && p < a.n_slots ? p : -1;
+  const int had = parent < 0 ? 0 : clamp_length(a, a.lengths[parent]);
+  const int wanted = a.new_lengths == nullptr ? had : max(a.new_lengths[slot], 0);
+  return slot_from(a, parent, min(had, wanted), wanted);
+}
+// The part-filled last page that a row keeps, or a number that is no page.
 __device__ inline int last_page(const PagesArgs& a, const Slot& s) {
   return s.part ? a.table[(long)s.parent * a.width + s.kept_pages - 1] : -1;
 }
 
 // Row `slot` gives back its old pages and holds the ones it keeps, entries first, first + step, ...:
 // whole adds and a minimum, so their order does not matter.
-__device__ inline void count_row(const PagesArgs& a, int slot, int first, int step, int32_t* count,
-                                 int32_t* keeper) {
-  const Slot s = slot_of(a, slot);
-  const int old_pages = pages_of(a, clamp_length(a, a.lengths[slot]));
+__device__ inline void count_row(const PagesArgs& a, int slot, const Slot& s, int old_pages, int first,
+                                 int step, int32_t* count, int32_t* keeper) {
   const int32_t* mine = a.table + (long)slot * a.width;
   const int32_t* from = a.table + (long)max(s.parent, 0) * a.width;
   const int whole = s.kept_pages - s.part;
@@ -84,23 +82,44 @@ __device__ inline void count_row(const PagesArgs& a, int slot, int first, int st
   }
 }
 
+// out[p] = value(p) for all pages, by one work-group: four at a time where `out` is 16-byte aligned.
+template <class Value>
+__device__ inline void for_pages(const PagesArgs& a, int32_t* out, Value value) {
+  const bool wide = ((uintptr_t)out & 15) == 0;
+  for (int p = 4 * threadIdx.x; p < a.n_pages; p += 4 * ST) {
+    if (wide && p + 4 <= a.n_pages) {
+      *reinterpret_cast<int4*>(out + p) = int4{value(p), value(p + 1), value(p + 2), value(p + 3)};
+    } else {
+      for (int i = p; i < min(p + 4, a.n_pages); ++i) out[i] = value(i);
+    }
+  }
+}
+
 // One work-group hands out the free pages: how many every row needs, then the free pages in ascending
-// order until all are served.
+// order until all are served. info(slot, last) gives a row and its part-filled last page.
+template <class Info>
 __device__ inline void hand_out(const PagesArgs& a, const Scratch& sc, int32_t* count, int32_t* keeper,
-                                int* s_scan, long long* s_sum) {
+                                int* s_scan, Info info) {
   const int tid = threadIdx.x;
   long long need = 0, beyond = 0;
-  int first = 0, copies = 0;  // so far (these wrap only where the total passes the pages)
+  int first = 0, copies = 0;  // so far (`first` wraps only where the total passes the pages)
   for (int base = 0; base < a.n_slots; base += ST) {
     const int slot = base + tid;
-    int x[2] = {0, 0}, total[2];
+    // pages, copies; pages and pages beyond the table row in pieces whose sums stay in 32 bits
+    int x[6] = {}, total[6];
     if (slot < a.n_slots) {
-      const Slot s = slot_of(a, slot);
-      const int last = last_page(a, s);
+      int last;
+      const Slot s = info(slot, last);
       x[1] = is_page(a, last) && !(count[last] <= 0 && keeper[last] == slot);
       x[0] = x[1] + s.wanted_pages - s.kept_pages;
-      need += x[0];
-      beyond += max(0, s.wanted_pages - a.width);
+      const int over = max(0, s.wanted_pages - a.width);
+      x[2] = x[0] & 0x7fff;
+      x[3] = x[0] >> 15;
+      x[4] = over & 0x7fff;
+      x[5] = over >> 15;
+      sc.parent[slot] = s.parent;
+      sc.kept[slot] = s.kept;
+      sc.wanted[slot] = s.wanted;
     }
     const int copy = x[1];
     block_exclusive_sums<SW>(x, total, s_scan);
@@ -108,9 +127,9 @@ __device__ inline void hand_out(const PagesArgs& a, const Scratch& sc, int32_t* 
     if (copy) sc.copies[copies + x[1]] = slot;
     first += total[0];
     copies += total[1];
+    need += ((long long)total[3] << 15) + total[2];
+    beyond += ((long long)total[5] << 15) + total[4];
   }
-  need = block_sum<SW>(need, s_sum);
-  beyond = block_sum<SW>(beyond, s_sum);
   long long found = 0;
   for (int base = 0; base < a.n_pages && found < need; base += PER * ST) {
     bool is_free[PER];
@@ -137,29 +156,51 @@ __device__ inline void hand_out(const PagesArgs& a, const Scratch& sc, int32_t* 
   }
   // the counts of the next step, or of this one again
   __syncthreads();
-#pragma unroll 4
-  for (int p = tid; p < a.n_pages; p += ST) {
+  for_pages(a, a.refs_out, [&](int p) {
     const int k = keeper[p], c = count[p];
-    a.refs_out[p] = lacking != 0 ? a.refs[p] : k == kTaken || (k != INT_MAX && c <= 0) ? 1 : max(c, 0);
-  }
+    return lacking != 0 ? a.refs[p] : k == kTaken || (k != INT_MAX && c <= 0) ? 1 : max(c, 0);
+  });
 }
 
-// Pools of up to kLdsPages pages: one work-group counts in LDS and hands out.
+// Pools of up to kLdsPages pages and up to 1024 rows: one work-group counts in LDS and hands out. What
+// the rows are is read once, beside the counts.
 __global__ __launch_bounds__(ST) void remap_small_kernel(PagesArgs a) {
-  __shared__ int32_t s_count[kLdsPages], s_keeper[kLdsPages];
-  __shared__ int s_scan[PER * SW];
-  __shared__ long long s_sum[SW];
+  __shared__ __attribute__((aligned(16))) int32_t s_count[kLdsPages], s_keeper[kLdsPages];
+  __shared__ int s_parent[ST], s_kept[ST], s_wanted[ST], s_last[ST], s_old[ST];
+  __shared__ int s_scan[6 * SW];
+  const int tid = threadIdx.x;
+  if (tid < a.n_slots) {
+    const Slot s = slot_of(a, tid);
+    s_parent[tid] = s.parent;
+    s_kept[tid] = s.kept;
+    s_wanted[tid] = s.wanted;
+    s_last[tid] = last_page(a, s);
+    s_old[tid] = pages_of(a, clamp_length(a, a.lengths[tid]));
+  }
+  const bool wide = ((uintptr_t)a.refs & 15) == 0;
 #pragma unroll 4
-  for (int p = threadIdx.x; p < a.n_pages; p += ST) {
-    s_count[p] = a.refs[p];
-    s_keeper[p] = INT_MAX;
+  for (int p = 4 * tid; p < a.n_pages; p += 4 * ST) {
+    int4 r;
+    if (wide && p + 4 <= a.n_pages) {
+      r = *reinterpret_cast<const int4*>(a.refs + p);
+    } else {
+      int* const one[4] = {&r.x, &r.y, &r.z, &r.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *one[i] = p + i < a.n_pages ? a.refs[p + i] : 0;
+    }
+    *reinterpret_cast<int4*>(s_count + p) = r;  // (kLdsPages is a multiple of 4)
+    *reinterpret_cast<int4*>(s_keeper + p) = int4{INT_MAX, INT_MAX, INT_MAX, INT_MAX};
   }
   __syncthreads();
   // 16 lanes per row: rows that go on as themselves only have their last page to look at
-  for (int slot = threadIdx.x >> 4; slot < a.n_slots; slot += ST / 16)
-    count_row(a, slot, threadIdx.x & 15, 16, s_count, s_keeper);
+  for (int slot = tid >> 4; slot < a.n_slots; slot += ST / 16)
+    count_row(a, slot, slot_from(a, s_parent[slot], s_kept[slot], s_wanted[slot]), s_old[slot], tid & 15,
+              16, s_count, s_keeper);
   __syncthreads();
-  hand_out(a, scratch_of(a), s_count, s_keeper, s_scan, s_sum);
+  hand_out(a, scratch_of(a), s_count, s_keeper, s_scan, [&](int slot, int& last) {
+    last = s_last[slot];
+    return slot_from(a, s_parent[slot], s_kept[slot], s_wanted[slot]);
+  });
 }
 
 __global__ __launch_bounds__(T) void remap_clear_kernel(PagesArgs a) {
@@ -171,13 +212,18 @@ __global__ __launch_bounds__(T) void remap_clear_kernel(PagesArgs a) {
 }
 __global__ __launch_bounds__(T) void remap_rows_kernel(PagesArgs a) {
   const Scratch sc = scratch_of(a);
-  count_row(a, blockIdx.x, threadIdx.x, T, sc.count, sc.keeper);
+  const int slot = blockIdx.x;
+  count_row(a, slot, slot_of(a, slot), pages_of(a, clamp_length(a, a.lengths[slot])), threadIdx.x, T,
+            sc.count, sc.keeper);
 }
 __global__ __launch_bounds__(ST) void remap_hand_out_kernel(PagesArgs a) {
-  __shared__ int s_scan[PER * SW];
-  __shared__ long long s_sum[SW];
+  __shared__ int s_scan[6 * SW];
   const Scratch sc = scratch_of(a);
-  hand_out(a, sc, sc.count, sc.keeper, s_scan, s_sum);
+  hand_out(a, sc, sc.count, sc.keeper, s_scan, [&](int slot, int& last) {
+    const Slot s = slot_of(a, slot);
+    last = last_page(a, s);
+    return s;
+  });
 }
 
 // The last step: work-groups below n_slots write the rows, the others copy the part-filled pages. Where
@@ -188,7 +234,7 @@ __global__ __launch_bounds__(T) void remap_finish_kernel(PagesArgs a) {
   const int tid = threadIdx.x;
   if ((int)blockIdx.x < a.n_slots) {
     const int slot = blockIdx.x;
-    const Slot s = slot_of(a, slot);
+    const Slot s = slot_from(a, sc.parent[slot], sc.kept[slot], sc.wanted[slot]);
     const int32_t* from = a.table + (long)(failed ? slot : max(s.parent, 0)) * a.width;
     const int given = sc.start[slot], copy = (given & kCopied) != 0;
     // page j of the row is list[j] for the copied last page and the ones that it grows by
@@ -210,7 +256,7 @@ __global__ __launch_bounds__(T) void remap_finish_kernel(PagesArgs a) {
   for (long u = blockIdx.x - a.n_slots; u < units; u += kCopyGroups) {
     const int slot = sc.copies[u / a.outer];
     const long o = u % a.outer;
-    const Slot s = slot_of(a, slot);
+    const Slot s = slot_from(a, sc.parent[slot], sc.kept[slot], sc.wanted[slot]);
     const int src = last_page(a, s), dst = sc.list[sc.start[slot] & (kCopied - 1)];
     const int run = (s.kept & (ps - 1)) * row_chunks;  // 16-byte chunks of a head
     const u32x4* from = pages + (o * a.n_pages + src) * page_chunks;
@@ -236,14 +282,14 @@ __device__ inline Moves moves_of(const PagesArgs& a) {
 
 __global__ __launch_bounds__(ST) void compact_plan_kernel(PagesArgs a) {
   __shared__ int s_scan[PER * SW];
-  __shared__ long long s_sum[SW];
   const Moves mv = moves_of(a);
   const int tid = threadIdx.x;
-  long long live = 0;
+  int live[1] = {0}, all[1];
 #pragma unroll 4
-  for (int p = tid; p < a.n_pages; p += ST) live += a.refs[p] > 0;
-  const int n_live = (int)block_sum<SW>(live, s_sum);
-  int moves = 0, holes = 0;
+  for (int p = tid; p < a.n_pages; p += ST) live[0] += a.refs[p] > 0;
+  block_exclusive_sums<SW>(live, all, s_scan);
+  const int n_live = all[0];
+  int holes = 0;
   for (int base = 0; base < a.n_pages; base += PER * ST) {
     bool wanted[PER];
     int at[PER], total;
@@ -264,7 +310,7 @@ __global__ __launch_bounds__(ST) void compact_plan_kernel(PagesArgs a) {
       }
     holes += total;
   }
-  moves = holes / 2;  // as many pages move as are taken
+  const int moves = holes / 2;  // as many pages move as are taken
   __syncthreads();
   for (int k = tid; k < moves; k += ST) {
     const int src = mv.movers[moves + k], dst = mv.holes[k];
@@ -312,7 +358,7 @@ __global__ __launch_bounds__(T) void compact_move_kernel(PagesArgs a, int count_
 }  // namespace
 
 hipError_t launch_pages_remap(const PagesArgs& a) {
-  if (a.n_pages <= kLdsPages) {
+  if (a.n_pages <= kLdsPages && a.n_slots <= ST) {
     hipLaunchKernelGGL(remap_small_kernel, dim3(1), dim3(ST), 0, a.stream, a);
   } else {
     hipLaunchKernelGGL(remap_clear_kernel, dim3((a.n_pages + T - 1) / T), dim3(T), 0, a.stream, a);

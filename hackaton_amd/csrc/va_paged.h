@@ -143,7 +143,7 @@ struct PagesArgs {
   hipStream_t stream;
 };
 inline int64_t pages_scratch_words(int64_t n_slots, int64_t n_pages) {
-  return 3 * n_pages + 2 * n_slots + 16;
+  return 3 * n_pages + 5 * n_slots + 16;
 }
 
 hipError_t launch_paged_plan(const PagedPlanArgs& a);

@@ -68,18 +68,4 @@ __device__ inline void block_places(const bool (&flag)[K], int (&place)[K], int&
   __syncthreads();
 }
 
-// Sum over the threads of a work-group, the same in all of them. `buf` is LDS of WAVES words.
-template <int WAVES>
-__device__ inline long long block_sum(long long x, long long* buf) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off);
-  if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = x;
-  __syncthreads();
-  x = 0;
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) x += buf[w];
-  __syncthreads();
-  return x;
-}
-
 }  // namespace va
