@@ -32,8 +32,9 @@ namespace {
 // ------------------------------------------------------------------------------------------------
 // plan
 // ------------------------------------------------------------------------------------------------
-constexpr int PT = 1024;                    // threads of a planning work-group
+constexpr int PT = 256;                     // threads of a planning work-group
 constexpr int kPlanRowsPerGroup = 4 * PT;   // rows that a planning work-group places
+constexpr int kPlanWriters = 64;            // work-groups that write items (and as many for the merges)
 
 enum { kFew = 0, kMany = 1, kPad = 2, kNone = 3 };  // kinds of items
 
@@ -830,8 +831,11 @@ hipError_t launch_attention(const PagedAttnArgs& a) {
 
 hipError_t launch_paged_plan(const PagedPlanArgs& a) {
   const int placers = (a.n_tokens + kPlanRowsPerGroup - 1) / kPlanRowsPerGroup;
-  const int writers = (int)((a.layout.max_items + 4 * PT - 1) / (4 * PT));
-  const auto kernel = a.n_seqs <= PT ? paged_plan_kernel<1> : paged_plan_kernel<kPagedMaxSeqs / PT>;
+  const int64_t wanted = (a.layout.max_items + PT - 1) / PT;
+  const int writers = (int)(wanted < kPlanWriters ? wanted : kPlanWriters);
+  const auto kernel = a.n_seqs <= PT       ? paged_plan_kernel<1>
+                      : a.n_seqs <= 4 * PT ? paged_plan_kernel<4>
+                                           : paged_plan_kernel<kPagedMaxSeqs / PT>;
   hipLaunchKernelGGL(kernel, dim3(2 * writers + placers), dim3(PT), 0, a.stream, a, writers);
   return hipGetLastError();
 }
