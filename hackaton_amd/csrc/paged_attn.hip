@@ -6,10 +6,11 @@
 // maximum, sum and output of every row stay in fp32; weights are rounded to 16 bits for the product
 // with the values on v_mfma_f32_32x32x16, and their sum is taken over the rounded ones.
 //
-//   few rows (up to 32: single and drafted tokens)   four waves share the keys out, each with a K and
-//       a V tile of 32 keys of its own in LDS, no barrier until the waves meet at the end;
-//   many rows (prompt chunks)   128 rows, a strip of 32 per wave, 64-key tiles in two LDS stages that
-//       all waves read.
+//   few rows (up to 32: single and drafted tokens)   the waves share the keys out, each with a K and a V
+//       tile of 32 keys of its own in LDS, no barrier until the waves meet at the end;
+//   many rows (prompt chunks)   128 rows, a strip of 32 per wave or pair of waves, 64-key tiles in LDS
+//       stages that all waves read: two stages and four waves, or four stages and eight waves, where the
+//       two waves of a strip take half of a tile's keys each and meet at the end.
 //
 // Both copy pages straight from memory into LDS (16 rows of a page per wave and step, so a page border
 // never falls into a copy), rows past the end of the range as zeros: what earlier sequences left in a
@@ -250,11 +251,18 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
 // ------------------------------------------------------------------------------------------------
 // attention
 // ------------------------------------------------------------------------------------------------
-constexpr int NW = 4, NT = 64 * NW;
 constexpr int D = kHeadDim;
 constexpr int GRP = 4 * D + 32;  // halfs from one group of 4 rows to the next
-constexpr int TILE = 16 * GRP;   // a 64-key K or V tile
-constexpr int LDS_HALFS = 4 * TILE;
+constexpr int TILE = 16 * GRP;   // a 64-key K or V tile, or a 32-key tile of each
+template <int W>  // waves of a work-group: 4 (two work-groups per CU) or 8 (one)
+struct Shape {
+  static constexpr int THREADS = 64 * W;
+  static constexpr int STAGES = W / 2;        // prompt tiles: 64-key stages of K and V
+  static constexpr int LDS = STAGES * 2 * TILE;  // halfs: one 32-key K and V tile per wave, as much
+  static constexpr int HALVES = W / 4;        // prompt tiles: waves per strip, which share a tile's keys out
+  static constexpr int BLOCKS = 2 / HALVES;   // 32-key blocks per wave and tile
+  static constexpr int GROUPS = 16 / W;       // row groups that a wave copies per K or V tile
+};
 constexpr float kRescaleLog2 = 8.f;  // many rows: the maximum moves when a tile exceeds it by 2^8
 
 // Read offsets (halfs) inside a tile. K (A operand of S^T): row perm32(l32), chunk 2 kk + hi. V^T: row
@@ -419,8 +427,9 @@ struct RowMap {
   }
 };
 
-template <class E>
+template <class E, int W>
 __device__ inline void few_rows(const PagedAttnArgs& a, const Item& it, lds_u16* smem, char* smem_raw) {
+  constexpr int NW = W;
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int head = it.head & 0xffff, group = a.hq / a.hkv, n_rows = it.row_end - it.row;
@@ -512,7 +521,7 @@ __device__ inline void few_rows(const PagedAttnArgs& a, const Item& it, lds_u16*
   constexpr int LT = D + 4;
   float* xo = reinterpret_cast<float*>(smem_raw);
   float* xs = xo + NW * 32 * LT;
-  static_assert((NW * 32 * LT + NW * 32 * 2) * 4 <= LDS_HALFS * 2, "the waves' rows fit in LDS");
+  static_assert((NW * 32 * LT + NW * 32 * 2) * 4 <= Shape<W>::LDS * 2, "the waves' rows fit in LDS");
   __syncthreads();  // every wave has read its tiles
   const float l_row = sum_with_other_half(st.l);
   if (l32 < n_rows) {
@@ -533,25 +542,26 @@ __device__ inline void few_rows(const PagedAttnArgs& a, const Item& it, lds_u16*
     }
   }
   __syncthreads();
-  const int r = tid >> 3, d0 = 16 * (tid & 7);
+  constexpr int PER = 32 * D / Shape<W>::THREADS;  // elements of a row per thread
+  const int r = tid / (D / PER), d0 = PER * (tid % (D / PER));
   if (r >= n_rows) return;
   float m[NW], l = 0.f, m_all = -INFINITY;
 #pragma unroll
   for (int w = 0; w < NW; ++w) m_all = fmaxf(m_all, m[w] = xs[2 * (w * 32 + r)]);
   const float m_use = m_all == -INFINITY ? 0.f : m_all;
-  f32x4 o[4] = {};
+  f32x4 o[PER / 4] = {};
 #pragma unroll
   for (int w = 0; w < NW; ++w) {
     const float c = fast_exp2(m[w] - m_use);
     l += c * xs[2 * (w * 32 + r) + 1];
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < PER / 4; ++e)
       o[e] += c * *reinterpret_cast<const f32x4*>(xo + (w * 32 + r) * LT + d0 + 4 * e);
   }
   if (it.part_row >= 0) {
     const long row = it.part_row + r;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < PER / 4; ++e)
       *reinterpret_cast<f32x4*>(a.workspace + row * D + d0 + 4 * e) = o[e];
     if (d0 == 0)
       *reinterpret_cast<f32x2*>(a.workspace + a.layout.max_part_rows * D + 2 * row) = f32x2{m_all, l};
@@ -562,17 +572,18 @@ __device__ inline void few_rows(const PagedAttnArgs& a, const Item& it, lds_u16*
   map.at(r, tok, h);
   uint16_t* out = (uint16_t*)a.out + ((long)(it.token0 + tok) * a.hq + head * group + h) * D + d0;
 #pragma unroll
-  for (int e = 0; e < 2; ++e)
+  for (int e = 0; e < PER / 8; ++e)
     gstore16(out + 8 * e, pack8<E>(o[2 * e][0] * inv, o[2 * e][1] * inv, o[2 * e][2] * inv,
                                    o[2 * e][3] * inv, o[2 * e + 1][0] * inv, o[2 * e + 1][1] * inv,
                                    o[2 * e + 1][2] * inv, o[2 * e + 1][3] * inv));
 }
 
-template <class E>
+template <class E, int W>
 __device__ inline void many_rows(const PagedAttnArgs& a, const Item& it, lds_u16* smem) {
-  constexpr int KEYS = 64, STAGE = 2 * TILE;
+  using S = Shape<W>;
+  constexpr int KEYS = 64, STAGE = 2 * TILE, STAGES = S::STAGES, BLOCKS = S::BLOCKS, GROUPS = S::GROUPS;
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), strip = wave & 3, half = wave >> 2;
   const int head = it.head & 0xffff, group = a.hq / a.hkv, n_rows = it.row_end - it.row;
   const float scale_log2 = a.scale * kLog2e;
   const RowMap map(it.row, group);
@@ -581,23 +592,24 @@ __device__ inline void many_rows(const PagedAttnArgs& a, const Item& it, lds_u16
   const int n_tiles = (it.key_end - it.key + KEYS - 1) / KEYS;
   const int c_row = lane >> 4;
 
-  // Copies, in tile order: wave w moves rows [16 w, 16 w + 16) of K and of V, which lie in one page; the
-  // page numbers of its next 64 tiles are in its lanes.
+  // Copies, in tile order: wave w moves 4 GROUPS rows of K and of V, which lie in one page; the page
+  // numbers of its next 64 tiles are in its lanes.
   int pages = 0, tc = 0;
   const int coff = (c_row * D + 8 * ((lane & 15) ^ c_row)) * 2;
-  auto copy_next = [&](uint32_t dst) {
+  auto copy_next = [&]() {
+    const int row = 4 * GROUPS * wave;
     if ((tc & 63) == 0) {
-      const int pos = it.key + KEYS * (tc + lane) + 16 * wave;
+      const int pos = it.key + KEYS * (tc + lane) + row;
       pages = pos < it.key_end ? table[pos >> a.pool.page_shift] : -1;
     }
     const int page = __builtin_amdgcn_readlane(pages, tc & 63);
-    const PageRows r = page_rows(a, page, head, it.key + KEYS * tc + 16 * wave, it.key_end);
+    const PageRows r = page_rows(a, page, head, it.key + KEYS * tc + row, it.key_end);
     const u32x4 rk = scalar_rsrc(r.k, r.bytes), rv = scalar_rsrc(r.v, r.bytes);
-    dst += 4 * wave * GRP * 2;
+    const uint32_t dst = lds_addr(smem + (tc & (STAGES - 1)) * STAGE + GROUPS * wave * GRP);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) dma16_opaque(rk, dst + j * GRP * 2, coff + j * 4 * D * 2);
+    for (int j = 0; j < GROUPS; ++j) dma16_opaque(rk, dst + j * GRP * 2, coff + j * 4 * D * 2);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) dma16_opaque(rv, dst + (TILE + j * GRP) * 2, coff + j * 4 * D * 2);
+    for (int j = 0; j < GROUPS; ++j) dma16_opaque(rv, dst + (TILE + j * GRP) * 2, coff + j * 4 * D * 2);
     ++tc;
   };
 
@@ -607,20 +619,20 @@ __device__ inline void many_rows(const PagedAttnArgs& a, const Item& it, lds_u16
     const long span = (long)((map.rest + n_rows - 1) / group * a.hq + group) * D * 2;
     const u32x4 rq = scalar_rsrc((const uint16_t*)a.q + q0, span);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int r = 32 * wave + 4 * j + c_row;
+    for (int j = 0; j < 32 / W; ++j) {
+      const int g = 32 / W * wave + j, r = 4 * g + c_row;
       int tok, h;
       map.at(r, tok, h);
       const int o = (((tok - map.token) * a.hq + h) * D + 8 * ((lane & 15) ^ c_row)) * 2;
-      dma16_opaque(rq, lds_addr(smem + STAGE + (8 * wave + j) * GRP), r < n_rows ? o : 0x7fffff00);
+      dma16_opaque(rq, lds_addr(smem + STAGE + g * GRP), r < n_rows ? o : 0x7fffff00);
     }
   }
-  if (n_tiles > 0) copy_next(lds_addr(smem));
+  if (n_tiles > 0) copy_next();
   wait_vmcnt<0>();
   __syncthreads();
   u32x4 qf[8];
   {
-    const lds_u16* qt = smem + STAGE + (8 * wave + (l32 >> 2)) * GRP + (l32 & 3) * D;
+    const lds_u16* qt = smem + STAGE + (8 * strip + (l32 >> 2)) * GRP + (l32 & 3) * D;
 #pragma unroll
     for (int kk = 0; kk < 8; ++kk)
       qf[kk] = ld128(qt + 8 * ((2 * (kk & 1) + hi) ^ (l32 & 3)) + 32 * (kk >> 1));
@@ -628,43 +640,82 @@ __device__ inline void many_rows(const PagedAttnArgs& a, const Item& it, lds_u16
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk) settle(qf[kk]);
   __syncthreads();  // every wave holds its rows before the second stage is written
+#pragma unroll
+  for (int t = 1; t < STAGES - 1; ++t)
+    if (t < n_tiles) copy_next();
 
   int my_tok, my_h;
-  map.at(32 * wave + l32, my_tok, my_h);
+  map.at(32 * strip + l32, my_tok, my_h);
   const int my_lim = it.pos0 + my_tok;
-  const int left = n_rows - 32 * wave;  // rows of this strip
+  const int left = n_rows - 32 * strip;  // rows of this strip
   const int first_lim = __builtin_amdgcn_readfirstlane(my_lim);
   const int last_lim = __builtin_amdgcn_readlane(my_lim, max(0, min(31, left - 1)));
-  const int n_live = left <= 0 || last_lim < it.key
-                         ? 0
-                         : min((last_lim - it.key) / KEYS + 1, n_tiles);
+  const int key0 = it.key + 32 * BLOCKS * half;  // this wave's keys of the first tile
+  const int n_live = left <= 0 || last_lim < key0 ? 0 : min((last_lim - key0) / KEYS + 1, n_tiles);
   State st;
   start(st);
+  // This wave's copies of tile t + 1 have landed; those of the tiles behind it stay in flight.
+  auto next = [&](int t) {
+    if (t + STAGES - 1 < n_tiles) wait_vmcnt<(STAGES - 2) * 2 * GROUPS>();
+    else wait_vmcnt<0>();
+    __syncthreads();
+  };
   int t = 0;
   for (; t < n_live; ++t) {
-    const lds_u16* kb = smem + (t & 1) * STAGE;
-    f32x16 s[2];
-    scores<E, 2>(kb, off, qf, s);
-    if (t + 1 < n_tiles) copy_next(lds_addr(smem + ((t + 1) & 1) * STAGE));
-    u32x4 va[4], pf[2][2];
+    const lds_u16* kb = smem + (t & (STAGES - 1)) * STAGE + 8 * BLOCKS * half * GRP;
+    f32x16 s[BLOCKS];
+    scores<E, BLOCKS>(kb, off, qf, s);
+    if (t + STAGES - 1 < n_tiles) copy_next();
+    u32x4 va[4], pf[BLOCKS][2];
 #pragma unroll
     for (int j = 0; j < 4; ++j) va[j] = read_v(kb + TILE, off, j);
-    const int kv0 = it.key + KEYS * t;
-    soften<E, 2>(s, kv0 + KEYS - 1 > first_lim, my_lim - kv0, hi, scale_log2, kRescaleLog2, st, pf);
-    weigh<E, 2>(kb + TILE, off, pf, va, st);
-    wait_vmcnt<0>();
-    __syncthreads();
+    const int kv0 = key0 + KEYS * t;
+    soften<E, BLOCKS>(s, kv0 + 32 * BLOCKS - 1 > first_lim, my_lim - kv0, hi, scale_log2,
+                      kRescaleLog2, st, pf);
+    weigh<E, BLOCKS>(kb + TILE, off, pf, va, st);
+    next(t);
   }
   for (; t < n_tiles; ++t) {  // past this strip's keys the wave only copies
-    if (t + 1 < n_tiles) copy_next(lds_addr(smem + ((t + 1) & 1) * STAGE));
-    wait_vmcnt<0>();
-    __syncthreads();
+    if (t + STAGES - 1 < n_tiles) copy_next();
+    next(t);
   }
 
+  // (The last barrier has passed and every copy has landed: the LDS is free.) Two waves of a strip meet:
+  // the second hands its rows over, in the accumulators' order.
+  if constexpr (S::HALVES == 2) {
+    lds_f32x4* xo = (lds_f32x4*)smem;
+    lds_f32x4* xs = xo + 4 * 16 * 64;
+    static_assert((4 * 16 + 4) * 64 * 16 + 4 * 32 * (8 * 16 + 8) * 2 <= S::LDS * 2,
+                  "the rows and the row tiles fit in LDS");
+    if (half == 1) {
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        xo[(16 * strip + k) * 64 + lane] =
+            f32x4{st.o[k >> 2][4 * (k & 3)], st.o[k >> 2][4 * (k & 3) + 1],
+                  st.o[k >> 2][4 * (k & 3) + 2], st.o[k >> 2][4 * (k & 3) + 3]};
+      xs[64 * strip + lane] = f32x4{st.m, st.l, 0.f, 0.f};
+    }
+    __syncthreads();
+    if (half == 1) return;
+    const f32x4 ml = xs[64 * strip + lane];
+    const float m = fmaxf(st.m, ml[0]), m_use = m == -INFINITY ? 0.f : m;
+    const float ca = fast_exp2(st.m - m_use), cb = fast_exp2(ml[0] - m_use);
+    st.m = m;
+    st.l = st.l * ca + ml[1] * cb;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const f32x4 y = xo[(16 * strip + k) * 64 + lane];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float& x = reinterpret_cast<float(&)[16]>(st.o[k >> 2])[4 * (k & 3) + e];
+        x = x * ca + y[e] * cb;
+      }
+    }
+  }
   const float l_row = sum_with_other_half(st.l);
   if (it.part_row >= 0) {
     if (l32 >= left) return;
-    const long row = it.part_row + 32 * wave + l32;
+    const long row = it.part_row + 32 * strip + l32;
 #pragma unroll
     for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -691,20 +742,20 @@ __device__ inline void many_rows(const PagedAttnArgs& a, const Item& it, lds_u16
                                st.o[db][8 * c + 2] * inv, st.o[db][8 * c + 3] * inv,
                                st.o[db][8 * c + 4] * inv, st.o[db][8 * c + 5] * inv,
                                st.o[db][8 * c + 6] * inv, st.o[db][8 * c + 7] * inv);
-  static_assert(NW * 32 * (8 * 16 + 8) <= LDS_HALFS, "row tiles fit in LDS");
-  // (the last barrier has passed: no wave reads a tile any more)
-  store_rows32<16>(smem + wave * 32 * (8 * 16 + 8), w, lane,
+  constexpr int ROWS = 32 * (8 * 16 + 8);  // a strip's row tile, behind what the halves hand over
+  static_assert(4 * ROWS <= S::LDS, "row tiles fit in LDS");
+  store_rows32<16>(smem + (S::HALVES == 2 ? (4 * 16 + 4) * 64 * 8 : 0) + strip * ROWS, w, lane,
                    [&](int r) {
                      int tok, h;
-                     map.at(32 * wave + r, tok, h);
+                     map.at(32 * strip + r, tok, h);
                      return (uint16_t*)a.out + ((long)(it.token0 + tok) * a.hq + head * group + h) * D;
                    },
                    left);
 }
 
-template <class E>
-__global__ __launch_bounds__(NT, 2) void paged_attn_kernel(PagedAttnArgs a) {
-  __shared__ __attribute__((aligned(16))) uint16_t smem_raw[LDS_HALFS];
+template <class E, int W>
+__global__ __launch_bounds__(Shape<W>::THREADS, 2) void paged_attn_kernel(PagedAttnArgs a) {
+  __shared__ __attribute__((aligned(16))) uint16_t smem_raw[Shape<W>::LDS];
   lds_u16* smem = (lds_u16*)smem_raw;
   const int n_items = a.plan[a.layout.counts];
   const Item* const p = reinterpret_cast<const Item*>(a.plan + a.layout.items) + blockIdx.x;
@@ -714,13 +765,13 @@ __global__ __launch_bounds__(NT, 2) void paged_attn_kernel(PagedAttnArgs a) {
   if ((int)blockIdx.x >= scalar(n_items)) return;
   const int kind = it.head >> 16;
   if (kind == kMany) {
-    many_rows<E>(a, it, smem);
+    many_rows<E, W>(a, it, smem);
   } else if (kind == kFew) {
-    few_rows<E>(a, it, smem, (char*)smem_raw);
+    few_rows<E, W>(a, it, smem, (char*)smem_raw);
   } else if (kind == kPad) {
     u32x4* out = (u32x4*)a.out + (long)it.row * a.hq * (D / 8);
     const int chunks = (it.row_end - it.row) * a.hq * (D / 8);
-    for (int i = threadIdx.x; i < chunks; i += NT) out[i] = u32x4{0u, 0u, 0u, 0u};
+    for (int i = threadIdx.x; i < chunks; i += Shape<W>::THREADS) out[i] = u32x4{0u, 0u, 0u, 0u};
   }
 }
 
@@ -819,7 +870,9 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a) {
 
 template <class E>
 hipError_t launch_attention(const PagedAttnArgs& a) {
-  hipLaunchKernelGGL(paged_attn_kernel<E>, dim3((unsigned)a.layout.max_items), dim3(NT), 0, a.stream, a);
+  const auto kernel = a.layout.wide ? paged_attn_kernel<E, 8> : paged_attn_kernel<E, 4>;
+  const int threads = a.layout.wide ? Shape<8>::THREADS : Shape<4>::THREADS;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)a.layout.max_items), dim3(threads), 0, a.stream, a);
   if (a.layout.max_merges > 0) {
     const unsigned groups = (unsigned)(a.layout.max_merges < kMergeGroups ? a.layout.max_merges : kMergeGroups);
     hipLaunchKernelGGL(paged_merge_kernel<E>, dim3(groups), dim3(256), 0, a.stream, a);

@@ -18,8 +18,20 @@ constexpr int kPageMin = 16, kPageMax = 256;
 constexpr int kPagedFewRows = 32;
 constexpr int kPagedTileRows = 128;
 constexpr int kPagedChunkKeys = 64;  // key ranges are split at multiples of this
+// The attention's work-groups: 8 waves, one work-group per CU, for steps with prompts (more rows than
+// sequences) of up to this many tiles x heads, by the sizes that the host knows; 4 waves, two per CU,
+// for the others. us with 4 / 8 waves: 2 x 2048 tokens, 12/2 heads (388 tiles) 50 / 42; 4096 tokens
+// (386) 86 / 76; 8 x 300 on 700 (240) 30 / 27; two chunks of 512 beside 62 answers, 28/4 heads (492) 67 /
+// 64; 2 x 1024 on 500 (456) 48 / 47; 3 x 1024 (684) 63 / 69; 4 x 1024 (912) 79 / 85; four chunks of 2048
+// 636 / 703; 64 answers of 64 to 8192 tokens 30 / 32, 16 of 1500 12.0 / 12.5.
+constexpr int kPagedWideTiles = 512;
 // Parts that a step's keys are split into, by kind of tile, the shortest part (but a range's last) and
-// the longest table row that is never split.
+// the longest table row that is never split. us at 384 / 512 / 1024 few-row parts: 64 answers of 64 to
+// 8192 tokens, 12/2 heads 33 / 30 / 32, four of 65,536, 28/4 heads 109 / 102 / 103; shortest few-row part
+// 128 / 256 / 512: one answer of 8192 9.1 / 10.0 / 12.0, 16 of 1500 13.4 / 12.3 / 13.3. At 256 / 512
+// prompt parts: two chunks of 512 beside 62 answers 61 / 69, 128 new tokens on 32,768 94 / 80; shortest
+// prompt part 256 / 512 / 704: 512 new tokens on 1536 28 / 26 / 27. Four answers of 512, table rows of 576:
+// split 8.8, whole 8.0 and a launch less.
 constexpr int kPagedFewParts = 512, kPagedManyParts = 256;
 constexpr int kPagedFewKeys = 256, kPagedManyKeys = 512;
 constexpr int kPagedWholeKeys = 1024;
@@ -31,6 +43,7 @@ constexpr int kPagedItemWords = 12, kPagedMergeWords = 8;
 struct PagedLayout {
   int64_t seq, pos, counts, items, merges, words;  // offsets; cu lies at 0
   int64_t max_items, max_merges, max_part_rows;
+  bool wide;
 };
 inline int64_t up4(int64_t x) { return (x + 3) & ~int64_t(3); }
 // Bounds: a sequence with rows makes one tile, and one more per full kPagedTileRows. A kind's parts have
@@ -45,6 +58,7 @@ inline PagedLayout paged_layout(int64_t n_seqs, int64_t n_tokens, int64_t hq, in
   const int64_t tiles = (n_seqs < n_tokens ? n_seqs : n_tokens) + n_tokens * (hq / hkv) / kPagedTileRows;
   const bool split = max_keys > kPagedWholeKeys;
   const int64_t rows = n_tokens * hq;
+  l.wide = n_tokens > n_seqs && tiles * hkv <= kPagedWideTiles;
   l.max_items = tiles * hkv + (split ? kPagedFewParts + kPagedManyParts : 0) +
                 (n_tokens + kPagedPadRows - 1) / kPagedPadRows;
   const int64_t merges = kPagedFewParts * (kPagedFewRows / 8) + kPagedManyParts * (kPagedTileRows / 8);

@@ -335,7 +335,9 @@ int va_paged_append(const va_paged_step* step, const void* q, const void* k, con
 /* out (N, Hq, 128) = softmax(scale q k^T) v of every new token over its sequence's keys at positions
  * up to its own; zeros for padding rows and for rows that see no key. The workspace
  * (va_paged_attention_workspace bytes, possibly 0) holds partial results of split key ranges; calls
- * that may overlap need one each. scale must be finite and > 0. Deterministic. */
+ * that may overlap need one each. scale must be finite and > 0. Deterministic: the same step gives the
+ * same bits; where a row's keys are split depends on the whole step, so the same sequence in another
+ * step agrees to rounding. */
 int va_paged_attention_workspace(const va_paged_step* step, int64_t* bytes);
 int va_paged_attention(const va_paged_step* step, const void* q, const void* k_pages,
                        const void* v_pages, int64_t k_stride, int64_t v_stride, int32_t n_pages,

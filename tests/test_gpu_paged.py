@@ -96,6 +96,26 @@ def test_prompt_chunks(q, kv, heads, kv_heads):
         check_attention(q, kv, heads, kv_heads, dtype, 32)
 
 
+@pytest.mark.parametrize("q,kv,heads,kv_heads,dtype", [
+    ([300, 140, 1, 9], [1300, 140, 700, 2000], 8, 8, FP16),    # 8 waves, parts
+    ([700, 40], [1800, 2100], 8, 4, BF16),                     # 8 waves, parts of prompts
+    ([260] * 10 + [1] * 5, [260] * 10 + [900] * 5, 8, 8, BF16),  # 8 waves, whole ranges
+    ([320] * 9, [330] * 9, 24, 24, FP16)])                      # 4 waves
+def test_prompt_tiles_of_both_shapes(q, kv, heads, kv_heads, dtype):
+    """Steps on both sides of the rule that picks 4 or 8 waves for a tile."""
+    check_attention(q, kv, heads, kv_heads, dtype, 16)
+
+
+@pytest.mark.parametrize("n_seqs", [257, 1025, 4096])
+def test_many_sequences(n_seqs):
+    """More sequences than a planning work-group has threads, some without new tokens or cached ones."""
+    rng = np.random.default_rng(n_seqs)
+    kv = rng.integers(0, 20, n_seqs)
+    q = np.minimum(rng.integers(0, 3, n_seqs), kv)
+    kv[n_seqs // 2], q[n_seqs // 2] = 600, 70
+    check_attention(q.tolist(), kv.tolist(), 2, 1, FP16, 16)
+
+
 @pytest.mark.parametrize("dtype", [FP16, BF16])
 def test_peaky_scores(dtype):
     """Queries and keys three times as large: the running maximum moves over the whole range."""
@@ -192,7 +212,11 @@ def test_a_pool_past_32_bits():
     plan = paged_plan(grown, [1, 1], lengths, 2, heads, kv_heads, page_size)
     rows = query[:1].cuda().expand(2, heads, DIM)
     both = paged_attention(rows, pages[0, 0], pages[0, 1], plan, SCALE)
-    assert torch.equal(both[0], both[1]) and torch.equal(both[0], out[0])
+    assert torch.equal(both[0], both[1])
+    # (another step than the one above, so its sums may be split elsewhere: equal to rounding, not by bits)
+    ref, size = orc.attention(query[:1], k, v, table[:1], [1], [700])
+    bound = orc.attention_bound(ref, size, BF16)
+    assert ((both[:1].cpu().double().view_as(ref) - ref).abs() <= bound).all()
     proj = torch.randn(2, (heads + 2 * kv_heads) * DIM, device="cuda").to(BF16)
     parts = proj.split([heads * DIM, kv_heads * DIM, kv_heads * DIM], 1)
     cos, sin = torch.ones(2, DIM, device="cuda"), torch.zeros(2, DIM, device="cuda")
@@ -404,6 +428,23 @@ def test_remap_of_many_slots_and_pages():
     refs += [0] * 6000
     run_remap(table, lengths, refs, parents, None, 16, layers=1, kv_heads=1)
     run_remap(table, lengths, refs, None, [min(48, x + 1) for x in lengths], 16, layers=1, kv_heads=1)
+
+
+def test_counts_at_any_word():
+    """refs that start at any word of a buffer."""
+    rng = np.random.default_rng(9)
+    table, lengths, refs = orc.random_state(rng, 20, 6, 150, 16)
+    pages = torch.randn(1, 2, 150, 1, 16, DIM, device="cuda").to(FP16)
+    parents = ints(rng.integers(-1, 20, 20).tolist())
+    want = remap_pages(pages.clone(), ints(table), ints(lengths), ints(refs), parents)
+    packed = compact_pages(pages.clone(), ints(table), ints(lengths), ints(refs))
+    for shift in (1, 2, 3):
+        held = torch.zeros(160, dtype=torch.int32, device="cuda")[shift:shift + 150]
+        held.copy_(ints(refs))
+        got = remap_pages(pages.clone(), ints(table), ints(lengths), held, parents)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        got = compact_pages(pages.clone(), ints(table), ints(lengths), held)
+        assert all(torch.equal(a, b) for a, b in zip(got, packed))
 
 
 def test_remap_of_nothing():
