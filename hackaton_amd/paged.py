@@ -22,9 +22,9 @@ import functools
 
 import torch
 
-from . import _lib
+from . import _lib, attention
 from ._lib import check, lib
-from .attention import _DTYPES, HEAD_DIM, _attn_dtype, _rope_strides, _stream, _tables
+from .attention import _DTYPES, HEAD_DIM, _attn_dtype, _rope_strides, _tables
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 
@@ -39,7 +39,7 @@ def _no_grad(*tensors):
 
 def _one_device(first, *tensors):
     device = first.device
-    if device.type != "cuda":
+    if not first.is_cuda:
         raise ValueError(f"the paged cache lives on the GPU only: got a tensor on {device}")
     for t in tensors:
         if t.device != device:
@@ -47,17 +47,8 @@ def _one_device(first, *tensors):
     return device
 
 
-def _on_device(fn):
-    """Run `fn` with the device of its first tensor current (launches and allocations go there)."""
-
-    @functools.wraps(fn)
-    def call(first, *args, **kwargs):
-        if first.is_cuda and first.device.index != torch._C._cuda_getDevice():
-            with torch.cuda.device(first.device):
-                return fn(first, *args, **kwargs)
-        return fn(first, *args, **kwargs)
-
-    return call
+_current_device = torch._C._cuda_getDevice
+_current_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _page_size(page_size):
@@ -123,7 +114,8 @@ class PagedPlan:
     plan was made (a captured plan reads them again in every replay)."""
 
     __slots__ = ("page_table", "words", "n_tokens", "n_seqs", "heads", "kv_heads", "page_size",
-                 "workspace_bytes", "_step", "_page", "_strides", "_stream")
+                 "workspace_bytes", "_step", "_page", "_strides", "_stream",
+                 "_captured")
 
     def _rows(self, which):
         rows = -(-self.n_tokens // 4) * 4
@@ -141,22 +133,33 @@ class PagedPlan:
         return self._rows(1)
 
     def _use(self):
-        """The plan's memory is used on the current stream: not handed out again before that is done."""
-        stream = torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
-        if stream != self._stream and not torch._C._cuda_isCurrentStreamCapturing():
+        """The current stream, with the plan's memory kept for it: a graph that captures a call over a
+        plan made before reads it in every replay, whatever becomes of the plan object (kept until
+        `release_captured_plans()`, as the work lists of `varlen_attention`); another stream than the
+        plan's own reads it before it is handed out again."""
+        stream = _current_stream(_current_device())
+        if torch._C._cuda_isCurrentStreamCapturing():
+            if not self._captured:
+                attention._CAPTURED_PLANS.add(self)
+        elif stream != self._stream:
             current = torch.cuda.current_stream()
             self.words.record_stream(current)
             self.page_table.record_stream(current)
         return stream
 
 
-@_on_device
 def paged_plan(page_table, q_lengths, kv_lengths, n_tokens, heads, kv_heads, page_size):
     """The plan of a step: `q_lengths[s]` new tokens of every sequence (packed rows, one sequence
     after the other, `n_tokens` rows in all; rows behind the last sequence are padding) and
-    `kv_lengths[s]` cached tokens with the new ones included. Both are host lists or device tensors;
-    `page_table` is (sequences, pages per sequence) int32 on the GPU. One launch."""
+    `kv_lengths[s]` cached tokens with the new ones included. Both are host lists or device tensors
+    (for a captured step: device tensors); `page_table` is (sequences, pages per sequence) int32 on
+    the GPU, at most 4096 sequences. Device lengths are not read back: negative ones count as 0, kv
+    lengths end with the table row, new tokens with the rows. One launch."""
     device = _one_device(page_table)
+    if device.index != _current_device():  # launches and allocations go to the tensors' device
+        with torch.cuda.device(device):
+            return paged_plan(page_table, q_lengths, kv_lengths, n_tokens, heads, kv_heads,
+                              page_size)
     if page_table.dim() != 2:
         raise ValueError(f"page_table must be (sequences, pages), got {tuple(page_table.shape)}")
     n_seqs, width = page_table.shape
@@ -172,7 +175,8 @@ def paged_plan(page_table, q_lengths, kv_lengths, n_tokens, heads, kv_heads, pag
     plan._page = (kv_heads, page_size, HEAD_DIM)
     plan._strides = (page_size * HEAD_DIM, HEAD_DIM, 1)
     plan.words = torch.empty(n_words, dtype=torch.int32, device=device)
-    plan._stream = _stream()
+    plan._stream = _current_stream(device.index)
+    plan._captured = torch._C._cuda_isCurrentStreamCapturing()
     plan._step = _lib.PagedStep(page_table.data_ptr(), plan.words.data_ptr(), n_tokens, n_seqs, width,
                                 page_size, heads, kv_heads)
     check(lib().va_paged_plan(plan._step, q_lengths.data_ptr(), kv_lengths.data_ptr(), n_words,
@@ -199,7 +203,6 @@ def _pages_of(k_pages, v_pages, plan):
     return k_stride[0], v_stride[0], shape[0]
 
 
-@_on_device
 def paged_append(q, k, v, cos, sin, k_pages, v_pages, plan):
     """The step's new rows: q (n_tokens, heads * 128), k and v (n_tokens, kv_heads * 128) projections
     in fp16, bf16 or fp32. Returns q rotated, (n_tokens, heads, 128) in the pages' type; k rotated and
@@ -208,6 +211,9 @@ def paged_append(q, k, v, cos, sin, k_pages, v_pages, plan):
     read by row. Rows without a place (padding, positions past the tables or in no page) write
     nothing; padding and positions outside the cos / sin table give zeros in q."""
     device = _one_device(q, k, v, cos, sin, k_pages, v_pages, plan.words)
+    if device.index != _current_device():  # launches and allocations go to the tensors' device
+        with torch.cuda.device(device):
+            return paged_append(q, k, v, cos, sin, k_pages, v_pages, plan)
     _no_grad(q, k, v, k_pages, v_pages)
     n, heads, kv_heads = plan.n_tokens, plan.heads, plan.kv_heads
     if (q.shape != (n, heads * HEAD_DIM) or k.shape != (n, kv_heads * HEAD_DIM)
@@ -241,12 +247,18 @@ def paged_append(q, k, v, cos, sin, k_pages, v_pages, plan):
     return query
 
 
-@_on_device
 def paged_attention(query, k_pages, v_pages, plan, scale):
     """Every new token attends to its sequence's keys at positions up to its own. query
     (n_tokens, heads, 128) in the pages' type; returns (n_tokens, heads * 128), zeros for padding and
-    for rows that see no key. Key/value heads are shared by heads / kv_heads query heads each."""
+    for rows that see no key. Key/value heads are shared by heads / kv_heads query heads each. What a
+    page holds behind its sequence's end is never read. (A sequence's own values that are infinite or
+    not a number also reach the rows of their 64-key tile that come before them, as in
+    `varlen_attention`.) The same step gives the same bits; the same sequence in another step agrees to
+    rounding."""
     device = _one_device(query, k_pages, v_pages, plan.words)
+    if device.index != _current_device():  # launches and allocations go to the tensors' device
+        with torch.cuda.device(device):
+            return paged_attention(query, k_pages, v_pages, plan, scale)
     _no_grad(query, k_pages, v_pages)
     dtype = _attn_dtype(query)
     if k_pages.dtype != query.dtype:
@@ -272,23 +284,28 @@ def paged_attention(query, k_pages, v_pages, plan, scale):
 # page bookkeeping
 # ------------------------------------------------------------------------------------------------
 def _pool_of(pages):
-    if pages.dim() != 6 or pages.shape[1] != 2 or pages.shape[5] != HEAD_DIM:
+    shape = pages.shape
+    if len(shape) != 6 or shape[1] != 2 or shape[5] != HEAD_DIM:
         raise ValueError(f"pages must be (layers, 2, n_pages, kv_heads, page_size, {HEAD_DIM}), got "
-                         f"{tuple(pages.shape)}")
+                         f"{tuple(shape)}")
     if not pages.is_contiguous():
         raise ValueError(f"pages must be contiguous, got strides {pages.stride()}")
     _attn_dtype(pages)
-    layers, _, n_pages, kv_heads, page_size, _ = pages.shape
-    return 2 * layers, n_pages, kv_heads, _page_size(page_size)
+    return 2 * shape[0], shape[2], shape[3], _page_size(shape[4])
 
 
-def _state_of(table, lengths, refs, n_pages):
+def _state_of(n_pages, table, lengths, refs, **more):
+    """(slots, pages per slot) of a cache's state, every tensor of which is checked; `more` holds one
+    number per slot each (or None)."""
     if table.dim() != 2:
         raise ValueError(f"table must be (slots, pages), got {tuple(table.shape)}")
     slots, width = table.shape
     _int32("table", table, slots, width)
     _int32("lengths", lengths, slots)
     _int32("refs", refs, n_pages)
+    for name, t in more.items():
+        if t is not None:
+            _int32(name, t, slots)
     return slots, width
 
 
@@ -300,7 +317,6 @@ def _scratch_words(slots, n_pages):
     return words.value
 
 
-@_on_device
 def remap_pages(pages, table, lengths, refs, parents=None, new_lengths=None):
     """The page tables of the next step. Slot i goes on as slot `parents[i]` (None: every slot as
     itself; outside the table: as nobody), cut to `new_lengths[i]` tokens or grown to them with free
@@ -318,42 +334,48 @@ def remap_pages(pages, table, lengths, refs, parents=None, new_lengths=None):
     slot that ends in it if nobody else holds it, and the others get a copy of its filled rows, in
     every layer. Free pages are handed out in ascending order, slot after slot. shortfall (1): 0, or
     how many pages the pool or the table rows lack, in which case nothing changes."""
-    given = [t for t in (parents, new_lengths) if t is not None]
-    device = _one_device(pages, table, lengths, refs, *given)
+    device = _one_device(pages, table, lengths, refs,
+                         *(t for t in (parents, new_lengths) if t is not None))
+    if device.index != _current_device():  # launches and allocations go to the tensors' device
+        with torch.cuda.device(device):
+            return remap_pages(pages, table, lengths, refs, parents, new_lengths)
     outer, n_pages, kv_heads, page_size = _pool_of(pages)
-    slots, width = _state_of(table, lengths, refs, n_pages)
-    for name, t in (("parents", parents), ("new_lengths", new_lengths)):
-        if t is not None:
-            _int32(name, t, slots)
-    out = [torch.empty_like(table), torch.empty_like(lengths), torch.empty_like(refs),
-           torch.empty(1, dtype=torch.int32, device=device)]
+    slots, width = _state_of(n_pages, table, lengths, refs, parents=parents, new_lengths=new_lengths)
+    table_out, lengths_out, refs_out = (torch.empty_like(table), torch.empty_like(lengths),
+                                        torch.empty_like(refs))
+    shortfall = torch.empty(1, dtype=torch.int32, device=device)
     words = _scratch_words(slots, n_pages)
     scratch = torch.empty(words, dtype=torch.int32, device=device)
     check(lib().va_pages_remap(
         pages.data_ptr(), outer, n_pages, kv_heads, page_size, HEAD_DIM, table.data_ptr(),
         lengths.data_ptr(), refs.data_ptr(), None if parents is None else parents.data_ptr(),
-        None if new_lengths is None else new_lengths.data_ptr(), slots, width,
-        *(t.data_ptr() for t in out), scratch.data_ptr(), words, _stream()), "va_pages_remap")
-    return tuple(out)
+        None if new_lengths is None else new_lengths.data_ptr(), slots, width, table_out.data_ptr(),
+        lengths_out.data_ptr(), refs_out.data_ptr(), shortfall.data_ptr(), scratch.data_ptr(), words,
+        _current_stream(device.index)), "va_pages_remap")
+    return table_out, lengths_out, refs_out, shortfall
 
 
-@_on_device
 def compact_pages(pages, table, lengths, refs):
     """The live pages (refs > 0) to the front of the pool: the k-th live page at or past their number
     moves to the k-th free page below it, in every layer. Arguments as for `remap_pages`. Returns
-    new (table, refs, live); live (1): how many pages are in use, all of them below that number."""
+    new (table, refs, live); live (1): how many pages are in use, all of them below that number. Pages
+    that the program holds without a table row move too: a row of their own keeps track of them."""
     device = _one_device(pages, table, lengths, refs)
+    if device.index != _current_device():  # launches and allocations go to the tensors' device
+        with torch.cuda.device(device):
+            return compact_pages(pages, table, lengths, refs)
     outer, n_pages, kv_heads, page_size = _pool_of(pages)
-    slots, width = _state_of(table, lengths, refs, n_pages)
-    out = [torch.empty_like(table), torch.empty_like(refs),
-           torch.empty(1, dtype=torch.int32, device=device)]
+    slots, width = _state_of(n_pages, table, lengths, refs)
+    table_out, refs_out = torch.empty_like(table), torch.empty_like(refs)
+    live = torch.empty(1, dtype=torch.int32, device=device)
     words = _scratch_words(slots, n_pages)
     scratch = torch.empty(words, dtype=torch.int32, device=device)
     check(lib().va_pages_compact(
         pages.data_ptr(), outer, n_pages, kv_heads, page_size, HEAD_DIM, table.data_ptr(),
-        lengths.data_ptr(), refs.data_ptr(), slots, width, *(t.data_ptr() for t in out),
-        scratch.data_ptr(), words, _stream()), "va_pages_compact")
-    return tuple(out)
+        lengths.data_ptr(), refs.data_ptr(), slots, width, table_out.data_ptr(), refs_out.data_ptr(),
+        live.data_ptr(), scratch.data_ptr(), words, _current_stream(device.index)),
+        "va_pages_compact")
+    return table_out, refs_out, live
 
 
 class PagedCache:
@@ -420,7 +442,9 @@ class PagedCache:
 
     def step(self, q_lengths, n_tokens, heads):
         """Room for `q_lengths[s]` new tokens of every slot, and the step's plan: `n_tokens` rows in
-        all. Where pages are lacking no slot grows and every row of the plan is padding."""
+        all, no fewer than their sum (host lists are checked). Where pages are lacking no slot grows
+        and every row of the plan is padding."""
+        _check_host_lengths(q_lengths, self.lengths, int(n_tokens), 0)
         q = _lengths("q_lengths", q_lengths, self.slots, self.table.device).clamp(min=0)
         before = self.lengths.clone()
         self.remap(None, before + q)

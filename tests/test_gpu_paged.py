@@ -263,6 +263,57 @@ def test_captured_steps_follow_the_lengths():
                 x.mul_(1.0)  # eager work between the replays
 
 
+def test_a_graph_keeps_the_plan_that_it_reads():
+    """Calls captured over a plan that was made before: the program drops the plan and fills the memory
+    that it gave back; the replays read the plan all the same, until release_captured_plans()."""
+    from hackaton_amd import attention as att
+
+    banner("captured calls over an eager plan")
+    q, kv = [1, 50, 3], [1400, 90, 65]
+    query, k, v, table = (x.cuda() for x in orc.paged_case(12, q, kv, 12, 2, FP16, 16))
+    want, _ = attend(query, k, v, table, q, kv, 16)
+    plan = paged_plan(table, q, kv, sum(q), 12, 2, 16)
+    size = plan.words.numel()
+    paged_attention(query, k, v, plan, SCALE)
+    torch.cuda.synchronize()
+    kept = len(att._CAPTURED_PLANS)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = paged_attention(query, k, v, plan, SCALE)
+    assert len(att._CAPTURED_PLANS) == kept + 1
+    del plan
+    fill = [torch.full((size,), 1 << 20, dtype=torch.int32, device="cuda") for _ in range(8)]
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.view_as(want), want)
+    del fill, graph
+    att.release_captured_plans()
+    assert not att._CAPTURED_PLANS
+
+
+def test_steps_without_sequences_pages_or_rows():
+    banner("empty steps")
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    query = torch.randn(70, 4, DIM, device="cuda").to(FP16)
+    pages = torch.randn(3, 2, 16, DIM, device="cuda").to(FP16)
+    for table, q, kv, pool in ((none.view(0, 3), [], [], pages), (none.view(2, 0), [70, 0], [0, 0], pages),
+                               (ints([[0, 1]] * 2), [0, 0], [20, 3], pages),
+                               (ints([[0, 1]] * 2), [40, 30], [32, 30], pages[:0])):
+        plan = paged_plan(table, ints(q), ints(kv), 70, 4, 2, 16)
+        out = paged_attention(query, pool, pool, plan, SCALE)
+        assert torch.equal(out, torch.zeros_like(out))
+        rows = torch.randn(70, 8 * DIM, device="cuda").to(FP16)
+        before = pool.clone()
+        cos = torch.ones(70, DIM, device="cuda")
+        paged_append(*rows.split([4 * DIM, 2 * DIM, 2 * DIM], 1), cos, cos, pool, pool.clone(), plan)
+        assert torch.equal(pool, before)
+    plan = paged_plan(ints([[0, 1]]), [0], [20], 0, 4, 2, 16)
+    assert paged_attention(query[:0], pages, pages, plan, SCALE).shape == (0, 4 * DIM)
+    assert plan.sequences.numel() == plan.positions.numel() == 0
+
+
 def test_another_stream_and_calls_at_once():
     banner("streams")
     q, kv = [1, 30, 1], [800, 90, 65]
@@ -528,6 +579,13 @@ def test_refusals():
             remap_pages(*bad)
     with pytest.raises(ValueError):
         PagedCache(1, 4, 17, 1, 1, 16)
+    cache = PagedCache(1, 8, 16, 1, 2, 64)
+    for bad in ([3, 1], [-1, 1], [1, 1, 1]):
+        with pytest.raises(ValueError):
+            cache.step(bad, 3, 2)
+    for call in (lambda: cache.fork(2, [0]), lambda: cache.fork(0, [5]), lambda: cache.free([-1])):
+        with pytest.raises(ValueError):
+            call()
 
 
 # ------------------------------------------------------------------------------------------------
