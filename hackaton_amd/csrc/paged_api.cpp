@@ -71,6 +71,8 @@ int check_pool(const va_paged_step& s, const void* k_pages, const void* v_pages,
   for (int64_t stride : {k_stride, v_stride})
     if (stride % 8 != 0 || stride < (int64_t)s.hkv * s.page_size * va::kHeadDim)
       return va::fail(VA_EINVAL, "%s: page strides must be multiples of 8 and cover a page", what);
+    else if (stride > (int64_t)(UINT32_MAX / 2))
+      return va::fail(VA_ESHAPE, "%s: page strides of 4 GiB or more", what);
   int rc = VA_OK;
   if (n_pages > 0 && (rc = check_buffers({k_pages, v_pages}, what))) return rc;
   if (s.n_tokens > 0 && (rc = check_buffers({s.plan}, what))) return rc;
@@ -79,7 +81,8 @@ int check_pool(const va_paged_step& s, const void* k_pages, const void* v_pages,
 }
 
 va::PagedPool pool_of(const va_paged_step& s, int64_t k_stride, int64_t v_stride, int32_t n_pages) {
-  return va::PagedPool{s.page_table, s.table_width, n_pages, shift_of(s.page_size), k_stride, v_stride};
+  return va::PagedPool{s.page_table, s.table_width, n_pages, shift_of(s.page_size),
+                       (uint32_t)(2 * k_stride), (uint32_t)(2 * v_stride)};
 }
 
 }  // namespace

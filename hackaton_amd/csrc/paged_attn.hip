@@ -396,23 +396,33 @@ __device__ inline void weigh(const lds_u16* vb, const Offsets& o, const u32x4 (&
   }
 }
 
-// 16 rows of a page: where they lie in the pools, and how many of them the range holds.
-struct PageRows {
-  const uint16_t* k;
-  const uint16_t* v;
-  long bytes;
+// Where the rows of one key/value head lie, and buffer descriptors of up to 16 rows of a page: built by
+// scalar instructions, of which each costs the wave as much as a vector one.
+struct Head {
+  uint64_t k, v;  // addresses of the head's rows in page 0
+  uint32_t k_stride, v_stride, mask;
+  int n_pages, end;  // the range's end
+  __device__ Head(const PagedAttnArgs& a, const Item& it, int head)
+      : k((uint64_t)a.k + ((uint64_t)(head << a.pool.page_shift) * (D * 2))),
+        v((uint64_t)a.v + ((uint64_t)(head << a.pool.page_shift) * (D * 2))),
+        k_stride(a.pool.k_stride), v_stride(a.pool.v_stride), mask((1u << a.pool.page_shift) - 1),
+        n_pages(a.pool.n_pages), end(it.key_end) {}
+  // The page of the row at `pos`; -1 where there is none, or the range has ended.
+  __device__ inline int page(const int32_t* table, int shift, int pos) const {
+    const int p = pos < end ? table[pos >> shift] : -1;
+    return (uint32_t)p < (uint32_t)n_pages ? p : -1;
+  }
+  // The rows from `pos` on: the page's, up to 16 and up to the range's end; the others read as zeros.
+  __device__ inline void rows(int page, int pos, u32x4& rk, u32x4& rv) const {
+    const uint32_t in = ((uint32_t)pos & mask) * (D * 2), p = (uint32_t)max(page, 0);
+    const uint32_t bytes = page < 0 ? 0 : (uint32_t)min(end - pos, 16) * (D * 2);
+    const uint64_t ak = k + (uint64_t)p * k_stride + in, av = v + (uint64_t)p * v_stride + in;
+    rk = u32x4{(uint32_t)scalar((int)ak), (uint32_t)scalar((int)(ak >> 32)) & 0xffffu,
+               (uint32_t)scalar((int)bytes), 0x00020000u};
+    rv = u32x4{(uint32_t)scalar((int)av), (uint32_t)scalar((int)(av >> 32)) & 0xffffu,
+               (uint32_t)scalar((int)bytes), 0x00020000u};
+  }
 };
-__device__ inline PageRows page_rows(const PagedAttnArgs& a, int page, int head, int pos, int end) {
-  PageRows r;
-  const int shift = a.pool.page_shift;
-  const bool there = page >= 0 && page < a.pool.n_pages;
-  const long in = ((long)(head << shift) + (pos & ((1 << shift) - 1))) * D;
-  const long p = there ? page : 0;
-  r.k = (const uint16_t*)a.k + p * a.pool.k_stride + in;
-  r.v = (const uint16_t*)a.v + p * a.pool.v_stride + in;
-  r.bytes = there ? (long)max(0, min(end - pos, 16)) * (D * 2) : 0;
-  return r;
-}
 
 // An item's rows: row r of the sequence is token r / group, query head r % group of the group.
 // Divisions of small numbers by the group: exact in fp32 (rows below 2^13, half a unit to spare).
@@ -454,42 +464,35 @@ __device__ inline void few_rows(const PagedAttnArgs& a, const Item& it, lds_u16*
     }
   }
   // Page numbers of this wave's next 32 tiles, two per tile (16 rows each): lane 2 i + h holds half h.
+  const Head rows(a, it, head);
   auto load_pages = [&](int t) {
-    const int pos = it.key + 32 * (t + NW * (lane >> 1)) + 16 * (lane & 1);
-    return pos < it.key_end ? table[pos >> a.pool.page_shift] : -1;
+    return rows.page(table, a.pool.page_shift, it.key + 32 * (t + NW * (lane >> 1)) + 16 * (lane & 1));
   };
   const uint32_t kl = lds_addr(smem + wave * (TILE)), vl = lds_addr(smem + wave * TILE + TILE / 2);
   const lds_u16* kb = smem + wave * TILE;
   const lds_u16* vb = kb + TILE / 2;
   const int c_row = lane >> 4, coff = (c_row * D + 8 * ((lane & 15) ^ c_row)) * 2;
-  auto copy = [&](const uint16_t* const (&base)[2], const long (&bytes)[2], uint32_t dst) {
+  auto copy = [&](const u32x4 (&from)[2], uint32_t dst) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const u32x4 r = scalar_rsrc(base[h], bytes[h]);
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) dma16_opaque(r, dst + (4 * h + j) * GRP * 2, coff + j * 4 * D * 2);
-    }
+      for (int j = 0; j < 4; ++j)
+        dma16_opaque(from[h], dst + (4 * h + j) * GRP * 2, coff + j * 4 * D * 2);
   };
   State st;
   start(st);
   int pages = 0, i = 0;  // i: this wave's tiles so far
-  const uint16_t *kp[2], *vp[2];
-  long bytes[2];
+  u32x4 rk[2], rv[2];
   auto locate = [&](int t, int n) {  // this wave's n-th tile, tile t of the item
     if ((n & 31) == 0) pages = load_pages(t);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int page = __builtin_amdgcn_readlane(pages, 2 * (n & 31) + h);
-      const PageRows r = page_rows(a, page, head, it.key + 32 * t + 16 * h, it.key_end);
-      kp[h] = r.k;
-      vp[h] = r.v;
-      bytes[h] = r.bytes;
-    }
+    for (int h = 0; h < 2; ++h)
+      rows.rows(__builtin_amdgcn_readlane(pages, 2 * (n & 31) + h), it.key + 32 * t + 16 * h, rk[h], rv[h]);
   };
   if (wave < n_tiles) {
     locate(wave, 0);
-    copy(kp, bytes, kl);
-    copy(vp, bytes, vl);
+    copy(rk, kl);
+    copy(rv, vl);
   }
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk) settle(qf[kk]);
@@ -502,7 +505,7 @@ __device__ inline void few_rows(const PagedAttnArgs& a, const Item& it, lds_u16*
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K read: its place is free
     if (more) {
       locate(t + NW, i + 1);
-      copy(kp, bytes, kl);
+      copy(rk, kl);
     }
     const int kv0 = it.key + 32 * t;
     u32x4 pf[1][2];
@@ -514,7 +517,7 @@ __device__ inline void few_rows(const PagedAttnArgs& a, const Item& it, lds_u16*
     for (int j = 0; j < 4; ++j) va[j] = read_v(vb, off, j);
     weigh<E, 1>(vb, off, pf, va, st);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V read
-    if (more) copy(vp, bytes, vl);
+    if (more) copy(rv, vl);
   }
 
   // The waves meet: fp32 rows of 132 words per wave, then their maxima and sums.
@@ -594,17 +597,14 @@ __device__ inline void many_rows(const PagedAttnArgs& a, const Item& it, lds_u16
 
   // Copies, in tile order: wave w moves 4 GROUPS rows of K and of V, which lie in one page; the page
   // numbers of its next 64 tiles are in its lanes.
+  const Head rows(a, it, head);
   int pages = 0, tc = 0;
   const int coff = (c_row * D + 8 * ((lane & 15) ^ c_row)) * 2;
   auto copy_next = [&]() {
-    const int row = 4 * GROUPS * wave;
-    if ((tc & 63) == 0) {
-      const int pos = it.key + KEYS * (tc + lane) + row;
-      pages = pos < it.key_end ? table[pos >> a.pool.page_shift] : -1;
-    }
-    const int page = __builtin_amdgcn_readlane(pages, tc & 63);
-    const PageRows r = page_rows(a, page, head, it.key + KEYS * tc + row, it.key_end);
-    const u32x4 rk = scalar_rsrc(r.k, r.bytes), rv = scalar_rsrc(r.v, r.bytes);
+    const int pos = it.key + 4 * GROUPS * wave + KEYS * tc;
+    if ((tc & 63) == 0) pages = rows.page(table, a.pool.page_shift, pos + KEYS * lane);
+    u32x4 rk, rv;
+    rows.rows(__builtin_amdgcn_readlane(pages, tc & 63), pos, rk, rv);
     const uint32_t dst = lds_addr(smem + (tc & (STAGES - 1)) * STAGE + GROUPS * wave * GRP);
 #pragma unroll
     for (int j = 0; j < GROUPS; ++j) dma16_opaque(rk, dst + j * GRP * 2, coff + j * 4 * D * 2);

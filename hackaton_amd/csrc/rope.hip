@@ -326,7 +326,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_paged_kernel(PagedAppendArg
       y2[e] = r2;
     }
     const gvoid y = pick3(is_q, is_v, a.q_out, a.k_pages, a.v_pages);
-    const long stride = is_v ? uniform(a.pool.v_stride) : uniform(a.pool.k_stride);
+    const long stride = (is_v ? uniform(a.pool.v_stride) : uniform(a.pool.k_stride)) / 2;  // elements
     const long row = is_q ? (tl.pid * a.heads + head) * D
                           : page * stride + ((long)head * ps + (pos & (ps - 1))) * D;
     store8<OUT>(y, row + c0, y1);

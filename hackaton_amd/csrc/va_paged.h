@@ -97,7 +97,7 @@ struct PagedPool {
   int table_width;
   int n_pages;
   int page_shift;               // log2 of page_size
-  int64_t k_stride, v_stride;  // elements from page to page
+  uint32_t k_stride, v_stride;  // bytes from page to page
 };
 
 struct PagedAttnArgs {
