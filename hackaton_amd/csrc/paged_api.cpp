@@ -137,7 +137,7 @@ extern "C" int va_paged_append(const va_paged_step* step, const void* q, const v
   const va::PagedLayout layout = layout_of(s);
   va::PagedAppendArgs a{q, k, v, cos, sin, cos_batch_stride, cos_seq_stride, cos_token_stride,
                         cos_rows, s.plan + layout.seq, s.plan + layout.pos,
-                        pool_of(s, k_stride, v_stride, n_pages), q_out, k_pages, v_pages,
+                        pool_of(s, k_stride, v_stride, n_pages), q_out, k_pages, v_pages, s.n_seqs,
                         (int)s.n_tokens, s.hq, s.hkv, in_dtype, out_dtype, (hipStream_t)stream};
   return launched(va::launch_paged_append(a), what);
 }

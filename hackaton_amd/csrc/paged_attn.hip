@@ -759,6 +759,28 @@ __device__ inline void many_rows(const PagedAttnArgs& a, const Item& it, lds_u16
                    left);
 }
 
+// Whether an entry of the list lies inside the call's rows, sequences, keys and workspace: a list that was
+// made for other sizes computes nothing useful, but reads and writes nothing out of bounds. (Where a row
+// stands, pos0, only moves its mask.)
+__device__ inline bool inside(const PagedAttnArgs& a, const Item& it, int kind) {
+  const int rows = it.row_end - it.row;
+  if (it.row < 0 || it.row_end < 0 || rows <= 0) return false;
+  if (kind == kPad) return rows <= kPagedPadRows && it.row_end <= a.n_tokens;
+  const int group = a.hq / a.hkv;
+  return rows <= (kind == kMany ? kPagedTileRows : kPagedFewRows) && it.token0 >= 0 &&
+         (long)it.token0 * group + it.row_end <= (long)a.n_tokens * group && it.seq >= 0 &&
+         it.seq < a.n_seqs && (it.head & 0xffff) < a.hkv && it.key >= 0 && it.key % kPagedChunkKeys == 0 &&
+         it.key_end >= 0 && it.key_end <= a.pool.table_width << a.pool.page_shift &&
+         (it.part_row < 0 || (long)it.part_row + rows <= a.layout.max_part_rows);
+}
+__device__ inline bool inside(const PagedAttnArgs& a, const Merge& m) {
+  const int group = a.hq / a.hkv;
+  return m.rows > 0 && m.rows <= 8 && m.row >= 0 && m.token0 >= 0 && m.head >= 0 && m.head < a.hkv &&
+         (long)m.token0 * group + m.row + m.rows <= (long)a.n_tokens * group && m.parts > 1 &&
+         m.stride >= 0 && m.part_row >= 0 &&
+         m.part_row + (m.parts - 1) * (long)m.stride + m.rows <= a.layout.max_part_rows;
+}
+
 template <class E, int W>
 __global__ __launch_bounds__(Shape<W>::THREADS, 2) void paged_attn_kernel(PagedAttnArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t smem_raw[Shape<W>::LDS];
@@ -770,6 +792,7 @@ __global__ __launch_bounds__(Shape<W>::THREADS, 2) void paged_attn_kernel(PagedA
   // (the list has room for max_items: the item's words are in flight beside the count)
   if ((int)blockIdx.x >= scalar(n_items)) return;
   const int kind = it.head >> 16;
+  if (!inside(a, it, kind)) return;  // (the same in all threads)
   if (kind == kMany) {
     many_rows<E, W>(a, it, smem);
   } else if (kind == kFew) {
@@ -819,7 +842,7 @@ template <class E>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a) {
   __shared__ f32x4 s_o[8][32];
   __shared__ float s_m[8], s_l[8];
-  const int n = a.plan[a.layout.counts + 1];
+  const int n = min(a.plan[a.layout.counts + 1], (int)a.layout.max_merges);
   const Merge* merges = reinterpret_cast<const Merge*>(a.plan + a.layout.merges);
   const float* o = a.workspace;
   const float* ml = a.workspace + a.layout.max_part_rows * D;
@@ -827,7 +850,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a) {
   Merge mg = merges[blockIdx.x];  // (there is room for every work-group's first record)
   for (int i = blockIdx.x; i < n; i += gridDim.x) {
     if (i != (int)blockIdx.x) mg = merges[i];
-    if (mg.parts < 2) continue;  // (the same in all threads)
+    if (!inside(a, mg)) continue;  // (the same in all threads)
     const bool spread = mg.parts > 8;
     const int r = spread ? 0 : g;
     const long row = mg.part_row + r;

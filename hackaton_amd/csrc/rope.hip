@@ -289,7 +289,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_paged_kernel(PagedAppendArg
   const TokenLanes tl = token_lanes(a.n_tokens);
   if (!tl.valid) return;
   const int c0 = 8 * tl.j, seq = a.seq[tl.pid], pos = a.pos[tl.pid];
-  const bool placed = seq >= 0 && pos >= 0 && (a.cos_rows == 0 || pos < a.cos_rows);
+  const bool placed = seq >= 0 && seq < a.n_seqs && pos >= 0 && (a.cos_rows == 0 || pos < a.cos_rows);
   int page = -1;
   const int at = pos >> a.pool.page_shift, ps = 1 << a.pool.page_shift;
   if (placed && at < a.pool.table_width)

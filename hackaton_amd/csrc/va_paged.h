@@ -131,7 +131,7 @@ struct PagedAppendArgs {
   void* q_out;
   void* k_pages;
   void* v_pages;
-  int n_tokens;
+  int n_seqs, n_tokens;
   int heads, kv_heads;
   int in_dtype, out_dtype;
   hipStream_t stream;

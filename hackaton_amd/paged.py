@@ -445,7 +445,8 @@ class PagedCache:
         all, no fewer than their sum (host lists are checked). Where pages are lacking no slot grows
         and every row of the plan is padding."""
         _check_host_lengths(q_lengths, self.lengths, int(n_tokens), 0)
-        q = _lengths("q_lengths", q_lengths, self.slots, self.table.device).clamp(min=0)
+        # (no table row names 2^30 tokens: what passes it lacks pages, and the sums stay in 32 bits)
+        q = _lengths("q_lengths", q_lengths, self.slots, self.table.device).clamp(0, 2 ** 30)
         before = self.lengths.clone()
         self.remap(None, before + q)
         return paged_plan(self.table, self.lengths - before, self.lengths, n_tokens, heads,

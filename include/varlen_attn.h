@@ -294,7 +294,8 @@ int va_unpack_rows(const void* src, void* dst, const int32_t* b_idx, const int32
  * only (its generation goes through transformers' dense cache); the entry points follow the
  * attention's conventions above. Layouts:
  *   k_pages, v_pages  n_pages pages of (Hkv, page_size, 128) contiguous 16-bit elements, the pages
- *                     k_stride / v_stride elements apart (multiples of 8, at least Hkv page_size 128)
+ *                     k_stride / v_stride elements apart (multiples of 8, at least
+ *                     Hkv page_size 128, under 2^31)
  *   page_table        (n_seqs, table_width) int32: row t of sequence s lies in page
  *                     page_table[s][t / page_size], row t % page_size. Entries outside [0, n_pages)
  *                     name no page: their rows are neither read (zero keys and values) nor written.
@@ -308,7 +309,9 @@ int va_unpack_rows(const void* src, void* dst, const int32_t* b_idx, const int32
  *
  * va_paged_plan writes the step's plan (va_paged_plan_words int32 of device memory, 16-byte aligned):
  * the sequence and the position of every row, and the attention's work list. It depends on the
- * lengths and sizes alone, so all layers of a step share it. n_seqs <= 4096. */
+ * lengths and sizes alone, so all layers of a step share it. n_seqs <= 4096. The calls that read a
+ * plan skip entries that do not lie inside their own sizes: one made for other sizes computes nothing
+ * useful, but reads and writes nothing out of bounds. */
 typedef struct va_paged_step {
   const int32_t* page_table;
   int32_t* plan;

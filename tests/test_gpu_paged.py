@@ -9,6 +9,7 @@ import torch
 
 from hackaton_amd import (PagedCache, compact_pages, paged_append, paged_attention, paged_plan,
                           remap_pages)
+from hackaton_amd._lib import check, lib
 from tests import paged_oracle as orc
 from tests.paged_oracle import DIM, HALF_STEP, SCALE
 
@@ -261,6 +262,122 @@ def test_captured_steps_follow_the_lengths():
                 torch.cuda.synchronize()
                 assert all(torch.equal(a, b) for a, b in zip(got, want)), (new, total)
                 x.mul_(1.0)  # eager work between the replays
+
+
+ITEM = ("token0", "seq", "pos0", "head", "row", "row_end", "key", "key_end", "part_row")
+MERGE = ("token0", "head", "row", "rows", "part_row", "stride", "parts")
+
+
+@pytest.mark.parametrize("q,kv", [([1], [4000]), ([70], [4000])], ids=["one token", "a chunk"])
+def test_plan_entries_outside_the_step_are_skipped(q, kv):
+    """One entry of a plan at a time is set to what its step does not hold: what it names is left out, the
+    other rows come out as before, and what lies around the output and the workspace stays."""
+    banner("entries outside", q, kv)
+    heads, kv_heads, ps = 4, 2, 16
+    n, width = sum(q) + 70, 256  # (70 rows of padding: two items)
+    query, k, v, table = orc.paged_case(13, q, kv, heads, kv_heads, FP16, ps, padding=70, width=width)
+    query, k, v, table = query.cuda(), k.cuda(), v.cuda(), table.cuda()
+    plan = paged_plan(table, q, kv, n, heads, kv_heads, ps)
+    good = plan.words.cpu()
+    counts = -(-(len(q) + 1) // 4) * 4 + 2 * (-(-n // 4) * 4)
+    n_items, n_merges = good[counts].item(), good[counts + 1].item()
+    assert n_items > 4 and n_merges > 1
+    max_items = kv_heads * (len(q) + n * (heads // kv_heads) // 128) + 768 + (n + 63) // 64
+    merges = counts + 4 + 12 * max_items
+    room, pool_stride = plan.workspace_bytes // 4, kv_heads * ps * DIM
+    part_rows = room // (DIM + 2)
+
+    def run():
+        out = torch.full((n + 128, heads, DIM), 7.0, dtype=FP16, device="cuda")
+        ws = torch.full((room + 8192,), 5.0, device="cuda")
+        check(lib().va_paged_attention(
+            plan._step, query.data_ptr(), k.data_ptr(), v.data_ptr(), pool_stride, pool_stride,
+            k.shape[0], DIM, SCALE, 0, out[64:].data_ptr(), ws[4096:].data_ptr(), 4 * room,
+            torch.cuda.current_stream().cuda_stream), "va_paged_attention")
+        torch.cuda.synchronize()
+        assert (out[:64] == 7).all() and (out[-64:] == 7).all()
+        assert (ws[:4096] == 5).all() and (ws[-4096:] == 5).all()
+        return out[64:-64]
+
+    whole = run()
+    assert (whole[:sum(q)] != 7).all() and (whole[sum(q):] == 0).all()
+    big, low, group = (1 << 31) - 1, -(1 << 31), heads // kv_heads
+    first, last = counts + 4, counts + 4 + 12 * (n_items - 1)  # a part of the rows, the last padding rows
+    bad = []
+    for name, values in {"token0": (-1, n, big), "seq": (-1, 1, big, low), "head": (kv_heads, big, low),
+                         "row": (-1, big, low), "row_end": (0, 2 * n + 1, big, low),
+                         "key": (-64, 8, big, low), "key_end": (-1, width * ps + 1, big, low),
+                         "part_row": (part_rows - 1, part_rows, big)}.items():
+        bad += [(first + ITEM.index(name), x) for x in values]
+    bad += [(last + ITEM.index("row_end"), x) for x in (0, n + 1, big)]
+    bad += [(last + ITEM.index("row"), x) for x in (-1, 0, n, big, low)]
+    for name, values in {"token0": (-1, n, big), "head": (-1, kv_heads, big), "row": (-1, 2 * n, big),
+                         "rows": (0, 9, big, low), "part_row": (-1, part_rows, big),
+                         "stride": (-1, part_rows, big), "parts": (1, part_rows + 1, big, low)}.items():
+        bad += [(merges + MERGE.index(name), x) for x in values]
+    for at, x in bad:
+        words = good.clone()
+        words[at] = x
+        plan.words.copy_(words)
+        out = run()
+        others = torch.ones_like(out, dtype=torch.bool)  # what the entry has no part in
+        if at >= merges:
+            token0, head, row, rows = good[merges:merges + 4].tolist()
+        elif at < last:
+            token0, head, row = (good[first + i].item() for i in (0, 3, 4))
+            rows, head = good[first + 5].item() - row, head & 0xffff
+        if first <= at < last or at >= merges:
+            others[token0 + row // group:token0 + (row + rows - 1) // group + 1,
+                   head * group:(head + 1) * group] = False
+        else:
+            others[good[last + 4].item():] = False
+            assert (out[~others] == 7).all()
+        assert torch.equal(out[others], whole[others]), (at, x)
+    for at, x in ((counts, big), (counts + 1, big), (counts + 1, low)):  # (entries past the list are skipped)
+        words = good.clone()
+        words[first + 12 * n_items:merges] = -1
+        words[merges + 8 * n_merges:] = -1
+        words[at] = x
+        plan.words.copy_(words)
+        out = run()
+        assert x == low or torch.equal(out, whole)
+    plan.words.copy_(good)
+    assert torch.equal(run(), whole)
+
+
+def test_append_over_a_plan_of_other_sizes():
+    """Sequences and positions that the step does not hold: nothing is written, zeros in q or, where a
+    position exceeds the table row only, the rotated row."""
+    banner("append over other rows")
+    heads, kv_heads, ps, n = 4, 2, 16, 6
+    table = ints([[0, 1], [2, 3]])
+    plan = paged_plan(table, [3, 3], [20, 20], n, heads, kv_heads, ps)
+    at = 4  # behind the row offsets: sequences, then positions, of 8 words each
+    assert plan.words[at:at + n].tolist() == [0, 0, 0, 1, 1, 1]
+    plan.words[at:at + n].copy_(ints([-1, 2, (1 << 31) - 1, 0, 1, 1]))
+    plan.words[at + 8:at + 8 + n].copy_(ints([0, 0, 0, -1, 32, (1 << 31) - 1]))
+    k = torch.full((6, kv_heads, ps, DIM), 3.0, dtype=FP16, device="cuda")
+    v = k.clone()
+    rows = torch.randn(n, (heads + 2 * kv_heads) * DIM, device="cuda").to(FP16)
+    q = paged_append(*rows.split([heads * DIM, kv_heads * DIM, kv_heads * DIM], 1),
+                     torch.ones(2, 40, DIM, device="cuda"), torch.zeros(2, 40, DIM, device="cuda"), k[1:5],
+                     v[1:5], plan)
+    assert (k == 3).all() and (v == 3).all()
+    assert torch.equal(q[4].flatten(), rows[4, :heads * DIM])
+    assert (q[[0, 1, 2, 3, 5]] == 0).all()
+
+
+def test_counts_that_pass_32_bits_lack_pages():
+    """Device counts are not read: a slot that would pass every table row lacks pages, and nothing changes."""
+    banner("counts past 32 bits")
+    cache = PagedCache(1, 8, 16, 2, 2, 64)
+    cache.step([5, 20], 25, 4)
+    before = cache.lengths.clone(), cache.table.clone(), cache.refs.clone()
+    plan = cache.step(ints([(1 << 31) - 1, 1]), 2, 4)
+    assert plan.positions.tolist() == [-1, -1]
+    assert all(torch.equal(x, y) for x, y in zip(before, (cache.lengths, cache.table, cache.refs)))
+    with pytest.raises(RuntimeError, match="lacked"):
+        cache.check()
 
 
 def test_a_graph_keeps_the_plan_that_it_reads():

@@ -72,6 +72,14 @@ def test_attention_arguments_are_checked(at, value, code):
     assert _lib.lib().va_paged_attention(*args) == _lib.VA_EINVAL
 
 
+def test_pages_of_4_gib_are_refused():
+    raw, p = buffers()
+    for at in (4, 5):
+        args = attention_args(p)
+        args[at] = 1 << 31
+        assert _lib.lib().va_paged_attention(*args) == _lib.VA_ESHAPE
+
+
 def test_attention_workspace_is_checked():
     need = ctypes.c_int64()
     sizes = dict(n_tokens=64, n_seqs=64, table_width=512)
