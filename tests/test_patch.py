@@ -165,6 +165,36 @@ def test_paged_branch_answers_like_the_dense_cache(patched, shape):
                 assert float((out - ref[0]).abs().max()) <= 3e-2
 
 
+@pytest.mark.gpu
+def test_the_whole_model_answers_from_pages(patched):
+    """Two prompts in one call of the model, one of them in two chunks, then single tokens, against the
+    dense forward of each sequence. fp32 model, fp16 pages: a layer's branch is off by at most six half
+    steps of fp16 of its size (q and k in scores of size about 1, weights, values, output), 3e-3; two
+    layers, logits up to 2: 1.2e-2."""
+    from hackaton_amd import PagedCache
+
+    model = tiny_model("cuda").eval()
+    gen = torch.Generator().manual_seed(2)
+    tokens = [torch.randint(0, 1000, (n,), generator=gen).cuda() for n in (41, 90)]
+    cache = PagedCache(2, 16, 16, KV_HEADS, 2, 128)
+    got, done = [[], []], [0, 0]
+    with torch.inference_mode():
+        for step in ([39, 50], [1, 38], [1, 1], [0, 1]):
+            plan = cache.step(step, sum(step) + 2, HEADS)  # (two rows of padding)
+            rows = torch.cat([t[d:d + n] for t, d, n in zip(tokens, done, step)])
+            rows = torch.nn.functional.pad(rows, (0, 2))
+            out = model(input_ids=rows[None], position_ids=plan.positions.clamp(min=0).long()[None],
+                        paged=(cache, plan), use_cache=False).logits[0]
+            for s, part in enumerate(out[:sum(step)].split(step)):
+                got[s].append(part)
+            done = [d + n for d, n in zip(done, step)]
+        cache.check()
+        assert done == [41, 90] and cache.lengths.tolist() == done
+        for t, parts in zip(tokens, got):
+            ref = model(input_ids=t[None], use_cache=False).logits[0]
+            assert float((torch.cat(parts) - ref).abs().max()) <= 1.2e-2
+
+
 def test_a_call_is_either_packed_or_paged(patched):
     layer = tiny_model("cpu").model.layers[0].self_attn
     with pytest.raises(ValueError, match="packed or paged"):
