@@ -93,7 +93,8 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
   const int tid = threadIdx.x, group = a.hq / a.hkv;
   // Row offsets need sums of q; the split shares need, per kind (many rows, few rows), the tiles and
   // their keys, here from the lengths as they are given (cut to n_tokens one by one), which is no less
-  // than what the rows make. Sums that could pass 32 bits go in pieces of 15 and 20 bits.
+  // than what the rows make. Sums that could pass 32 bits go in pieces of 15 and 19 bits: 4096 sequences
+  // times 2^19 - 1 stay below 2^31, three pieces hold 2^57 (a sequence has up to 2^23 tiles of 2^30 keys).
   int q[SPT], sum[10] = {}, sums[10];
 #pragma unroll
   for (int i = 0; i < SPT; ++i) {
@@ -111,7 +112,7 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
-      for (int b = 0; b < 3; ++b) sum[4 + 3 * k + b] += k == kind ? (int)(keys >> 20 * b) & 0xfffff : 0;
+      for (int b = 0; b < 3; ++b) sum[4 + 3 * k + b] += k == kind ? (int)(keys >> 19 * b) & 0x7ffff : 0;
   }
   block_exclusive_sums<PT / 64>(sum, sums, s_scan);
   long long at = ((long long)sum[1] << 15) + sum[0];
@@ -148,7 +149,7 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
     const long long all = k == 0 ? kPagedManyParts : kPagedFewParts;
     const long long parts = max(all - (long long)sums[2 + k] * a.hkv, all / 4);
     const long long keys =
-        ((long long)sums[6 + 3 * k] << 40) + ((long long)sums[5 + 3 * k] << 20) + sums[4 + 3 * k];
+        ((long long)sums[6 + 3 * k] << 38) + ((long long)sums[5 + 3 * k] << 19) + sums[4 + 3 * k];
     const long long share =
         max((keys * a.hkv + parts - 1) / parts, (long long)(k == 0 ? kPagedManyKeys : kPagedFewKeys));
     chunks[k] = split ? (int)((share + kPagedChunkKeys - 1) / kPagedChunkKeys) * kPagedChunkKeys

@@ -1,0 +1,138 @@
+"""The paged cache at the edges of its sizes: work lists of many and of long sequences, calls that are
+refused or cut, and what they leave unchanged."""
+
+import numpy as np
+import pytest
+import torch
+
+from hackaton_amd import paged_attention, paged_plan
+from tests import paged_oracle as orc
+from tests.paged_oracle import DIM, SCALE
+from tests.test_gpu_paged import BF16, FP16, banner, check_attention, ints
+
+pytestmark = pytest.mark.gpu
+
+FEW, MANY, PAD, NONE = range(4)  # kinds of items
+
+
+def lists_of(plan):
+    """(items (n, 12), merge records (n, 8), their room) of a plan whose table rows pass 1024 keys."""
+    words, n = plan.words.cpu().numpy(), plan.n_tokens
+    counts = -(-(plan.n_seqs + 1) // 4) * 4 + 2 * (-(-n // 4) * 4)
+    tiles = min(plan.n_seqs, n) + n * (plan.heads // plan.kv_heads) // 128
+    max_items = tiles * plan.kv_heads + 512 + 256 + -(-n // 64)
+    merges = counts + 4 + 12 * max_items
+    n_items, n_merges = words[counts], words[counts + 1]
+    assert 0 <= n_items <= max_items and 0 <= n_merges <= (words.size - merges) // 8
+    return (words[counts + 4:counts + 4 + 12 * n_items].reshape(-1, 12),
+            words[merges:merges + 8 * n_merges].reshape(-1, 8))
+
+
+def check_lists(plan, q, kv):
+    """Every row of every key/value head: its keys in parts that join without a gap, each part with
+    workspace rows of its own, and a merge record wherever there is more than one. Returns how many
+    parts the split tiles of both kinds have, by kind."""
+    q, kv = np.asarray(q, dtype=np.int64), np.asarray(kv, dtype=np.int64)
+    group, hkv = plan.heads // plan.kv_heads, plan.kv_heads
+    rows_of, cu = q * group, np.concatenate(([0], np.cumsum(q)))
+    items, merges = lists_of(plan)
+    items = items.astype(np.int64)
+    kind = items[:, 3] >> 16
+    pads = items[kind == PAD]
+    assert (pads[:, 5] - pads[:, 4]).sum() == plan.n_tokens - cu[-1]
+    items = items[(kind == FEW) | (kind == MANY)]
+    token0, seq, pos0, head, row, end, key, key_end, part_row = items[:, :9].T
+    kind, head = head >> 16, head & 0xffff
+    rows = rows_of[seq]
+    assert (token0 == cu[seq]).all() and (pos0 == (kv - q)[seq]).all() and (head < hkv).all()
+    assert ((kind == FEW) == (rows <= 32)).all()
+    assert (row % 128 == 0).all() and (end == np.minimum(row + 128, rows)).all()
+    keys = np.maximum(pos0 + (end - 1) // group + 1, 0)
+    # parts in order of their keys, tile after tile
+    order = np.lexsort((key, row, head, seq))
+    tile = np.stack((seq, head, row), 1)[order]
+    first = np.concatenate(([True], (tile[1:] != tile[:-1]).any(1)))
+    last = np.concatenate((first[1:], [True]))
+    tiles = np.where(rows_of == 0, 0, np.where(rows_of <= 32, 1, -(-rows_of // 128)))
+    assert first.sum() == tiles.sum() * hkv
+    key, key_end, part_row, count = key[order], key_end[order], part_row[order], (end - row)[order]
+    assert (key[first] == 0).all() and (key_end[last] == keys[order][last]).all()
+    assert (key[1:] == key_end[:-1])[~first[1:]].all() and (key % 64 == 0).all()
+    parts = np.diff(np.append(np.flatnonzero(first), first.size))
+    split = np.repeat(parts > 1, parts)
+    assert ((part_row >= 0) == split).all()
+    places = np.sort(np.concatenate([part_row[split][:, None], (part_row + count)[split][:, None]], 1), 0)
+    assert (places[1:, 0] >= places[:-1, 1]).all()
+    assert not split.any() or places[-1, 1] <= plan.workspace_bytes // (4 * (DIM + 2))
+    # the merge records' rows are the split tiles' rows, and read the parts of theirs
+    want = {}
+    for t in np.flatnonzero(first & split):
+        n = int(parts[np.searchsorted(np.flatnonzero(first), t)])
+        stride = int(part_row[t + 1] - part_row[t])
+        assert (np.diff(part_row[t:t + n]) == stride).all()
+        for i in range(int(count[t])):
+            s, h, r = (int(x) for x in tile[t])
+            want[int(cu[s]), h, r + i] = (int(part_row[t]) + i, stride, n)
+    got = {}
+    for token, h, r, n, place, stride, n_parts, _ in merges.tolist():
+        for i in range(n if n_parts > 1 else 0):
+            assert (token, h, r + i) not in got
+            got[token, h, r + i] = (place + i, stride, n_parts)
+    assert got == want
+    of = kind[order][first]
+    return parts[of == FEW], parts[of == MANY]
+
+
+def long_plan(q, kv, heads, kv_heads, page_size=256):
+    """The plan of a step whose pages nothing reads."""
+    table = torch.zeros(len(q), -(-max(kv) // page_size), dtype=torch.int32, device="cuda")
+    plan = paged_plan(table, ints(q), ints(kv), sum(q), heads, kv_heads, page_size)
+    torch.cuda.synchronize()
+    return plan
+
+
+@pytest.mark.parametrize("n_seqs,q,kv,heads,kv_heads", [
+    (4096, 1, 600064, 12, 2), (4096, 1, 600064, 1, 1), (2049, 1, 1048575, 12, 2),
+    (4096, 512, 32768, 12, 2), (4096, 183, 65336, 28, 4)])
+def test_lists_of_many_long_sequences(n_seqs, q, kv, heads, kv_heads):
+    """Steps whose keys sum to more than 2^31: the shares follow the sum, so the lists have room."""
+    banner("many long sequences", n_seqs, q, kv, heads, kv_heads)
+    plan = long_plan([q] * n_seqs, [kv] * n_seqs, heads, kv_heads)
+    few, many = check_lists(plan, [q] * n_seqs, [kv] * n_seqs)
+    assert (few == 1).all() and (many == 1).all()  # (more tiles than parts: nothing to split)
+
+
+def test_many_forks_of_a_long_prompt():
+    """4096 single tokens over 600,064 keys each, all of which are the 256 rows of one page: the weights
+    repeat, so every row equals the attention over the page. The bound adds the worst case of the fp32
+    sums, a quarter of the keys (one wave's) times half a step of 2^-23, in the sum and the output."""
+    banner("many forks of a long prompt")
+    n, ps, kv = 4096, 256, 600064
+    gen = torch.Generator().manual_seed(0)
+    query = torch.randn(n, 1, DIM, generator=gen).to(FP16)
+    k, v = (torch.randn(1, 1, ps, DIM, generator=gen).to(FP16) for _ in range(2))
+    table = torch.zeros(n, kv // ps, dtype=torch.int32, device="cuda")
+    plan = paged_plan(table, ints([1] * n), ints([kv] * n), n, 1, 1, ps)
+    out = paged_attention(query.cuda(), k.cuda(), v.cuda(), plan, SCALE).cpu().double()
+    weights = torch.softmax(query[:, 0].double() @ k[0, 0].double().T * SCALE, 1)
+    want, size = weights @ v[0, 0].double(), weights @ v[0, 0].double().abs()
+    bound = orc.attention_bound(want, size, FP16) + 2 * kv / 4 * 2.0 ** -24 * size
+    assert float(want.abs().max(1).values.min()) > float(bound.max())  # (an unwritten row would show)
+    assert ((out - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("n_seqs", [256, 257, 1024, 1025, 4096])
+def test_split_ranges_among_many_sequences(n_seqs):
+    """A few long answers and prompts between many short sequences, at the borders of the planning
+    threads' shares: both kinds of tiles are split, whatever the number of sequences per thread."""
+    rng = np.random.default_rng(n_seqs)
+    kv = rng.integers(0, 12, n_seqs)
+    q = np.minimum(rng.integers(0, 3, n_seqs), kv)
+    for at, new, total in ((0, 1, 9000), (3, 40, 1500), (4, 2, 700), (15, 90, 2500), (16, 1, 1200),
+                           (63, 1, 3000), (64, 33, 1030), (255, 5, 4000), (n_seqs - 1, 70, 2000)):
+        q[at], kv[at] = new, total
+    q, kv = q.tolist(), kv.tolist()
+    for heads, kv_heads, dtype in ((2, 1, FP16), (2, 2, BF16)):
+        _, plan = check_attention(q, kv, heads, kv_heads, dtype, 16, padding=3)
+        few, many = check_lists(plan, q, kv)
+        assert (few > 1).any() and (many > 1).any() and (few > 8).any()
