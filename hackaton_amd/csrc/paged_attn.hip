@@ -150,10 +150,14 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
     const long long parts = max(all - (long long)sums[2 + k] * a.hkv, all / 4);
     const long long keys =
         ((long long)sums[6 + 3 * k] << 38) + ((long long)sums[5 + 3 * k] << 19) + sums[4 + 3 * k];
+    // (at most INT_MAX / 2, which no range is longer than: such a share splits nothing; a prompt of 2^20
+    // tokens, 32/8 heads, makes 2^32. Rounded up and added to a range it stays below 2^31.)
     const long long share =
-        max((keys * a.hkv + parts - 1) / parts, (long long)(k == 0 ? kPagedManyKeys : kPagedFewKeys));
-    chunks[k] = split ? (int)((share + kPagedChunkKeys - 1) / kPagedChunkKeys) * kPagedChunkKeys
-                      : INT_MAX / 2;
+        split ? min(max((keys * a.hkv + parts - 1) / parts,
+                        (long long)(k == 0 ? kPagedManyKeys : kPagedFewKeys)),
+                    (long long)(INT_MAX / 2))
+              : INT_MAX / 2;
+    chunks[k] = (int)((share + kPagedChunkKeys - 1) / kPagedChunkKeys * kPagedChunkKeys);
   }
   const int aligned = 8 / (a.hkv % 8 == 0 ? 8 : a.hkv % 4 == 0 ? 4 : a.hkv % 2 == 0 ? 2 : 1);
   int x[4] = {0, 0, 0, 0}, n[4];  // items of both kinds, workspace rows, merge records

@@ -102,6 +102,16 @@ def test_lists_of_many_long_sequences(n_seqs, q, kv, heads, kv_heads):
     assert (few == 1).all() and (many == 1).all()  # (more tiles than parts: nothing to split)
 
 
+@pytest.mark.parametrize("q,kv,heads,kv_heads", [
+    (1 << 20, 1 << 20, 32, 8), (1 << 20, (1 << 20) + 2, 32, 8), (1 << 20, (1 << 20) + 256, 32, 8),
+    (1 << 20, 1 << 20, 28, 4), (1 << 19, 1 << 22, 32, 8), (1 << 20, (1 << 30) - 256, 12, 2)])
+def test_lists_of_long_prompts(q, kv, heads, kv_heads):
+    """Prompts whose share of keys passes 2^31, 2^32 and further: none of their ranges is split."""
+    banner("long prompts", q, kv, heads, kv_heads)
+    few, many = check_lists(long_plan([q, 1], [kv, 700000], heads, kv_heads), [q, 1], [kv, 700000])
+    assert (many == 1).all() and (few > 8).all()
+
+
 def test_many_forks_of_a_long_prompt():
     """4096 single tokens over 600,064 keys each, all of which are the 256 rows of one page: the weights
     repeat, so every row equals the attention over the page. The bound adds the worst case of the fp32
