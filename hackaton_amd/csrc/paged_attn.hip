@@ -778,11 +778,12 @@ __device__ inline bool inside(const PagedAttnArgs& a, const Item& it, int kind) 
          it.key_end >= 0 && it.key_end <= a.pool.table_width << a.pool.page_shift &&
          (it.part_row < 0 || (long)it.part_row + rows <= a.layout.max_part_rows);
 }
+// (A sequence's parts lie at least the record's rows apart, which with the workspace bounds their number.)
 __device__ inline bool inside(const PagedAttnArgs& a, const Merge& m) {
   const int group = a.hq / a.hkv;
   return m.rows > 0 && m.rows <= 8 && m.row >= 0 && m.token0 >= 0 && m.head >= 0 && m.head < a.hkv &&
          (long)m.token0 * group + m.row + m.rows <= (long)a.n_tokens * group && m.parts > 1 &&
-         m.stride >= 0 && m.part_row >= 0 &&
+         m.stride >= m.rows && m.part_row >= 0 &&
          m.part_row + (m.parts - 1) * (long)m.stride + m.rows <= a.layout.max_part_rows;
 }
 

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from hackaton_amd import paged_attention, paged_plan
+from hackaton_amd._lib import check, lib
 from tests import paged_oracle as orc
 from tests.paged_oracle import DIM, SCALE
 from tests.test_gpu_paged import BF16, FP16, banner, check_attention, ints
@@ -15,16 +16,21 @@ pytestmark = pytest.mark.gpu
 FEW, MANY, PAD, NONE = range(4)  # kinds of items
 
 
-def lists_of(plan):
-    """(items (n, 12), merge records (n, 8), their room) of a plan whose table rows pass 1024 keys."""
-    words, n = plan.words.cpu().numpy(), plan.n_tokens
+def places_of(plan):
+    """Where the counts, the items and the merge records of a plan whose table rows pass 1024 keys lie."""
+    n = plan.n_tokens
     counts = -(-(plan.n_seqs + 1) // 4) * 4 + 2 * (-(-n // 4) * 4)
     tiles = min(plan.n_seqs, n) + n * (plan.heads // plan.kv_heads) // 128
     max_items = tiles * plan.kv_heads + 512 + 256 + -(-n // 64)
-    merges = counts + 4 + 12 * max_items
+    return counts, counts + 4, counts + 4 + 12 * max_items
+
+
+def lists_of(plan):
+    """(items (n, 12), merge records (n, 8)) of such a plan."""
+    words, (counts, items, merges) = plan.words.cpu().numpy(), places_of(plan)
     n_items, n_merges = words[counts], words[counts + 1]
-    assert 0 <= n_items <= max_items and 0 <= n_merges <= (words.size - merges) // 8
-    return (words[counts + 4:counts + 4 + 12 * n_items].reshape(-1, 12),
+    assert 0 <= n_items <= (merges - items) // 12 and 0 <= n_merges <= (words.size - merges) // 8
+    return (words[items:items + 12 * n_items].reshape(-1, 12),
             words[merges:merges + 8 * n_merges].reshape(-1, 8))
 
 
@@ -146,3 +152,43 @@ def test_split_ranges_among_many_sequences(n_seqs):
         _, plan = check_attention(q, kv, heads, kv_heads, dtype, 16, padding=3)
         few, many = check_lists(plan, q, kv)
         assert (few > 1).any() and (many > 1).any() and (few > 8).any()
+
+
+def test_merge_records_of_parts_in_one_place_are_skipped():
+    """Records whose parts do not lie apart, of any number: they name no parts of a sequence, so their
+    rows are left out; the others come out as before."""
+    banner("merge records of parts in one place")
+    heads, kv_heads, ps, q, kv = 4, 2, 16, [20, 1], [3000, 4000]
+    query, k, v, table = (x.cuda() for x in orc.paged_case(14, q, kv, heads, kv_heads, FP16, ps))
+    n, group, stride = sum(q), heads // kv_heads, kv_heads * ps * DIM
+    plan = paged_plan(table, q, kv, n, heads, kv_heads, ps)
+    good = plan.words.cpu()
+    records = lists_of(plan)[1]
+    ws = torch.zeros(plan.workspace_bytes, dtype=torch.uint8, device="cuda")
+
+    def run():
+        out = torch.full((n, heads, DIM), 7.0, dtype=FP16, device="cuda")
+        check(lib().va_paged_attention(
+            plan._step, query.data_ptr(), k.data_ptr(), v.data_ptr(), stride, stride, k.shape[0], DIM,
+            SCALE, 0, out.data_ptr(), ws.data_ptr(), ws.numel(),
+            torch.cuda.current_stream().cuda_stream), "va_paged_attention")
+        torch.cuda.synchronize()
+        return out
+
+    whole = run()
+    assert (whole != 7).all()
+    for i in (0, len(records) - 1):  # a record of eight rows, one of the single token
+        token0, head, row, rows, _, step, parts = records[i, :7].tolist()
+        at = places_of(plan)[2] + 8 * i
+        assert good[at:at + 7].tolist() == records[i, :7].tolist() and parts > 1 and step >= rows
+        skipped = torch.zeros_like(whole, dtype=torch.bool)
+        for r in range(row, row + rows):
+            skipped[token0 + r // group, head * group + r % group] = True
+        for bad, many in ((0, parts), (0, 9), (0, (1 << 31) - 1), (0, (1 << 31) - 64), (rows - 1, parts)):
+            words = good.clone()
+            words[at + 5], words[at + 6] = bad, many
+            plan.words.copy_(words)
+            out = run()
+            assert torch.equal(out[~skipped], whole[~skipped]) and (out[skipped] == 7).all(), (i, bad, many)
+    plan.words.copy_(good)
+    assert torch.equal(run(), whole)
