@@ -442,15 +442,18 @@ class PagedCache:
 
     def step(self, q_lengths, n_tokens, heads):
         """Room for `q_lengths[s]` new tokens of every slot, and the step's plan: `n_tokens` rows in
-        all, no fewer than their sum (host lists are checked). Where pages are lacking no slot grows
-        and every row of the plan is padding."""
-        _check_host_lengths(q_lengths, self.lengths, int(n_tokens), 0)
+        all, no fewer than their sum (host lists are checked). At most 4096 slots. Where pages are
+        lacking no slot grows and every row of the plan is padding."""
+        n_tokens, kv_heads = int(n_tokens), self.pages.shape[3]
+        _check_host_lengths(q_lengths, self.lengths, n_tokens, 0)
+        # (a step that the plan would refuse is refused before a slot has grown)
+        _plan_sizes(self.slots, n_tokens, heads, kv_heads, self.page_size, self.table.shape[1])
         # (no table row names 2^30 tokens: what passes it lacks pages, and the sums stay in 32 bits)
         q = _lengths("q_lengths", q_lengths, self.slots, self.table.device).clamp(0, 2 ** 30)
         before = self.lengths.clone()
         self.remap(None, before + q)
-        return paged_plan(self.table, self.lengths - before, self.lengths, n_tokens, heads,
-                          self.pages.shape[3], self.page_size)
+        return paged_plan(self.table, self.lengths - before, self.lengths, n_tokens, heads, kv_heads,
+                          self.page_size)
 
     def compact(self):
         """The live pages to the front of the pool; returns their number as a (1) int32 tensor."""

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from hackaton_amd import paged_attention, paged_plan
+from hackaton_amd import PagedCache, paged_attention, paged_plan
 from hackaton_amd._lib import check, lib
 from tests import paged_oracle as orc
 from tests.paged_oracle import DIM, SCALE
@@ -192,3 +192,30 @@ def test_merge_records_of_parts_in_one_place_are_skipped():
             assert torch.equal(out[~skipped], whole[~skipped]) and (out[skipped] == 7).all(), (i, bad, many)
     plan.words.copy_(good)
     assert torch.equal(run(), whole)
+
+
+def state_of(cache):
+    return [x.clone() for x in (cache.table, cache.lengths, cache.refs)]
+
+
+def same_state(cache, kept):
+    return all(torch.equal(a, b) for a, b in zip(kept, (cache.table, cache.lengths, cache.refs)))
+
+
+def test_a_refused_step_changes_nothing():
+    banner("refused steps")
+    cache = PagedCache(1, 8, 16, 2, 2, 64)
+    cache.step([5, 20], 25, 4)
+    kept = state_of(cache)
+    for q, n, heads in (([1, 1], 2, 5), (ints([1, 1]), 2, 0), (ints([1, 1]), -1, 4), ([1, 1], 1 << 30, 4),
+                        (ints([1, 1]), 1 << 40, 4)):
+        with pytest.raises(RuntimeError):
+            cache.step(q, n, heads)
+        assert same_state(cache, kept)
+    wide = PagedCache(1, 8, 16, 2, 5000, 64)
+    kept = state_of(wide)
+    with pytest.raises(RuntimeError, match="4096"):
+        wide.step(ints([1] * 5000), 5000, 4)
+    assert same_state(wide, kept)
+    assert cache.step([1, 1], 2, 4).positions.tolist() == [5, 20]
+    cache.check()
