@@ -92,6 +92,7 @@ SIGNATURES = {
     "va_paged_attention": (ctypes.c_int, [_pstep, _p, _p, _p, _i64, _i64, _i32, _i32, _f32, _i32,
                                           _p, _p, _i64, _p]),
     "va_pages_scratch_words": (ctypes.c_int, [_i32, _i32, _pi64]),
+    "va_pages_growth": (ctypes.c_int, [_p, _p, _i32, _i64, _p, _p, _p]),
     "va_pages_remap": (ctypes.c_int, [_p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _p, _p, _i32,
                                       _i32, _p, _p, _p, _p, _p, _i64, _p]),
     "va_pages_compact": (ctypes.c_int, [_p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _i32, _i32,

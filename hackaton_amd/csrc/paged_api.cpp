@@ -209,6 +209,20 @@ extern "C" int va_pages_scratch_words(int32_t n_slots, int32_t n_pages, int64_t*
   return VA_OK;
 }
 
+extern "C" int va_pages_growth(const int32_t* lengths, const int32_t* q_lengths, int32_t n_slots,
+                               int64_t n_tokens, int32_t* new_lengths, int32_t* excess,
+                               void* stream) {
+  const char* what = "va_pages_growth";
+  if (n_slots < 0 || n_slots > (1 << 20) || n_tokens < 0)
+    return va::fail(VA_ESHAPE, "%s: n_slots=%d n_tokens=%lld", what, n_slots, (long long)n_tokens);
+  if (n_slots == 0) return VA_OK;
+  const int rc = check_words({lengths, q_lengths, new_lengths, excess}, what);
+  if (rc) return rc;
+  va::PagesGrowthArgs a{lengths, q_lengths, n_slots, n_tokens, new_lengths, excess,
+                        (hipStream_t)stream};
+  return launched(va::launch_pages_growth(a), what);
+}
+
 extern "C" int va_pages_remap(void* pages, int64_t outer, int32_t n_pages, int32_t kv_heads,
                               int32_t page_size, int32_t head_dim, const int32_t* table,
                               const int32_t* lengths, const int32_t* refs, const int32_t* parents,

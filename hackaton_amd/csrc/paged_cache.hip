@@ -226,6 +226,25 @@ __global__ __launch_bounds__(ST) void remap_hand_out_kernel(PagesArgs a) {
   });
 }
 
+// A step's lengths: every row's with its new tokens, unless those pass the step's rows all together. (A
+// few KB at most: bounded by its launch, 2 us, in place of a clamp, a sum and an addition.)
+__global__ __launch_bounds__(ST) void growth_kernel(PagesGrowthArgs a) {
+  __shared__ int s_scan[3 * SW];
+  long long sum = 0;
+  for (int i = threadIdx.x; i < a.n_slots; i += ST) sum += max(a.q_lengths[i], 0);
+  // (pieces of 20 bits: 1024 threads of them stay in 32)
+  int x[3] = {(int)(sum & 0xfffff), (int)(sum >> 20 & 0xfffff), (int)(sum >> 40)}, total[3];
+  block_exclusive_sums<SW>(x, total, s_scan);
+  const long long excess =
+      ((long long)total[2] << 40) + ((long long)total[1] << 20) + total[0] - a.n_tokens;
+  for (int i = threadIdx.x; i < a.n_slots; i += ST) {
+    const int q = excess > 0 ? 0 : max(a.q_lengths[i], 0);
+    a.new_lengths[i] = (int)min((long long)a.lengths[i] + q, (long long)INT_MAX);
+  }
+  if (threadIdx.x == 0 && excess > 0)
+    a.excess[0] = max(a.excess[0], (int)min(excess, (long long)INT_MAX));
+}
+
 // The last step: work-groups below n_slots write the rows, the others copy the part-filled pages. Where
 // the pages did not suffice everything stays as it was.
 __global__ __launch_bounds__(T) void remap_finish_kernel(PagesArgs a) {
@@ -356,6 +375,11 @@ __global__ __launch_bounds__(T) void compact_move_kernel(PagesArgs a, int count_
 }
 
 }  // namespace
+
+hipError_t launch_pages_growth(const PagesGrowthArgs& a) {
+  hipLaunchKernelGGL(growth_kernel, dim3(1), dim3(ST), 0, a.stream, a);
+  return hipGetLastError();
+}
 
 hipError_t launch_pages_remap(const PagesArgs& a) {
   if (a.n_pages <= kLdsPages && a.n_slots <= ST) {

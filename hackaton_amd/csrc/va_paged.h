@@ -160,9 +160,20 @@ inline int64_t pages_scratch_words(int64_t n_slots, int64_t n_pages) {
   return 3 * n_pages + 5 * n_slots + 16;
 }
 
+struct PagesGrowthArgs {
+  const int32_t* lengths;
+  const int32_t* q_lengths;
+  int n_slots;
+  int64_t n_tokens;
+  int32_t* new_lengths;
+  int32_t* excess;
+  hipStream_t stream;
+};
+
 hipError_t launch_paged_plan(const PagedPlanArgs& a);
 hipError_t launch_paged_attention(const PagedAttnArgs& a);
 hipError_t launch_paged_append(const PagedAppendArgs& a);
+hipError_t launch_pages_growth(const PagesGrowthArgs& a);
 hipError_t launch_pages_remap(const PagesArgs& a);
 hipError_t launch_pages_compact(const PagesArgs& a);
 

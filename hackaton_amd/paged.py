@@ -383,7 +383,7 @@ class PagedCache:
     of at most `max_length` tokens in it. State, all on the GPU: `pages`, `table`, `lengths`, `refs`.
     Every call updates it in place on the current stream, so the calls of one cache belong on one
     stream or in order across streams, and a captured step replays on the state it finds. A call
-    that lacks pages changes nothing; `check()` reports it."""
+    that lacks pages (or a step that lacks rows) changes nothing; `check()` reports it."""
 
     def __init__(self, layers, n_pages, page_size, kv_heads, slots, max_length,
                  dtype=torch.float16, device="cuda"):
@@ -396,7 +396,9 @@ class PagedCache:
         self.table = torch.full((slots, width), -1, **ints)
         self.lengths = torch.zeros(slots, **ints)
         self.refs = torch.zeros(n_pages, **ints)
-        self.shortfall = torch.zeros(1, **ints)
+        self._lacking = torch.zeros(2, **ints)
+        self.shortfall = self._lacking[:1]  # the most pages that a call has lacked since the last check
+        self.excess = self._lacking[1:]     # the most rows that a step has lacked
 
     @property
     def slots(self):
@@ -442,18 +444,30 @@ class PagedCache:
 
     def step(self, q_lengths, n_tokens, heads):
         """Room for `q_lengths[s]` new tokens of every slot, and the step's plan: `n_tokens` rows in
-        all, no fewer than their sum (host lists are checked). At most 4096 slots. Where pages are
-        lacking no slot grows and every row of the plan is padding."""
+        all, no fewer than their sum. At most 4096 slots. Where pages are lacking, or device lengths sum
+        to more than `n_tokens` (host lists are refused), no slot grows and every row of the plan is
+        padding."""
         n_tokens, kv_heads = int(n_tokens), self.pages.shape[3]
         _check_host_lengths(q_lengths, self.lengths, n_tokens, 0)
         # (a step that the plan would refuse is refused before a slot has grown)
         _plan_sizes(self.slots, n_tokens, heads, kv_heads, self.page_size, self.table.shape[1])
-        # (no table row names 2^30 tokens: what passes it lacks pages, and the sums stay in 32 bits)
-        q = _lengths("q_lengths", q_lengths, self.slots, self.table.device).clamp(0, 2 ** 30)
+        q = _lengths("q_lengths", q_lengths, self.slots, self.table.device)
         before = self.lengths.clone()
-        self.remap(None, before + q)
+        self.remap(None, self._grown(q, n_tokens))
         return paged_plan(self.table, self.lengths - before, self.lengths, n_tokens, heads, kv_heads,
                           self.page_size)
+
+    def _grown(self, q_lengths, n_tokens):
+        """The slots' lengths with their new tokens, or as they are where those pass the rows."""
+        device = self.table.device
+        if device.index != _current_device():  # launches and allocations go to the tensors' device
+            with torch.cuda.device(device):
+                return self._grown(q_lengths, n_tokens)
+        out = torch.empty_like(self.lengths)
+        check(lib().va_pages_growth(self.lengths.data_ptr(), q_lengths.data_ptr(), self.slots, n_tokens,
+                                    out.data_ptr(), self.excess.data_ptr(),
+                                    _current_stream(device.index)), "va_pages_growth")
+        return out
 
     def compact(self):
         """The live pages to the front of the pool; returns their number as a (1) int32 tensor."""
@@ -463,8 +477,9 @@ class PagedCache:
         return live
 
     def check(self):
-        """Raise if a call since the last check lacked pages (reads the GPU)."""
-        lacking = int(self.shortfall)
-        if lacking:
-            self.shortfall.zero_()
-            raise RuntimeError(f"the paged cache lacked {lacking} pages: that call changed nothing")
+        """Raise if a call since the last check lacked pages or rows (reads the GPU)."""
+        pages, rows = self._lacking.tolist()
+        if pages or rows:
+            self._lacking.zero_()
+            what = f"{pages} pages" if pages else f"{rows} rows for a step's new tokens"
+            raise RuntimeError(f"the paged cache lacked {what}: that call changed nothing")

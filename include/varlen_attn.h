@@ -360,10 +360,15 @@ int va_paged_attention(const va_paged_step* step, const void* q, const void* k_p
  * in it (all of them, where a row holds it whole or the program itself does) get a copy of its
  * kept % page_size rows in a free page. *shortfall = 0, or the number of pages that the pool or the
  * table rows lack: then nothing changes (the outputs repeat the inputs, no page is written).
+ * va_pages_growth: the new_lengths of a step of n_tokens rows, lengths + q_lengths (negative ones count
+ * as 0; at most INT32_MAX). Where the q_lengths sum to more than n_tokens no row grows (new_lengths =
+ * lengths), and *excess, which the caller clears, rises to what they pass it by.
  * va_pages_compact: with n_live = the number of pages with refs > 0, the k-th live page at or past
  * n_live moves to the k-th free page below it; *live = n_live. lengths do not change.
  * scratch: va_pages_scratch_words int32, contents do not matter. */
 int va_pages_scratch_words(int32_t n_slots, int32_t n_pages, int64_t* words);
+int va_pages_growth(const int32_t* lengths, const int32_t* q_lengths, int32_t n_slots, int64_t n_tokens,
+                    int32_t* new_lengths, int32_t* excess, void* stream);
 int va_pages_remap(void* pages, int64_t outer, int32_t n_pages, int32_t kv_heads,
                    int32_t page_size, int32_t head_dim, const int32_t* table,
                    const int32_t* lengths, const int32_t* refs, const int32_t* parents,

@@ -219,3 +219,45 @@ def test_a_refused_step_changes_nothing():
     assert same_state(wide, kept)
     assert cache.step([1, 1], 2, 4).positions.tolist() == [5, 20]
     cache.check()
+
+
+@pytest.mark.parametrize("slots,seed", [(1, 0), (3, 1), (1000, 2), (1025, 3), (4096, 4)])
+def test_a_step_of_more_tokens_than_rows_changes_nothing(slots, seed):
+    """Device lengths that sum to the rows, to one more and past 32 bits; eagerly and replayed."""
+    banner("more tokens than rows", slots)
+    rng = np.random.default_rng(seed)
+    n = 2 * slots
+    cache = PagedCache(1, 5 * slots, 16, 1, slots, 64)
+    fits = rng.multinomial(n, np.ones(slots) / slots).clip(max=30)
+    fits[int(rng.integers(slots))] += n - fits.sum()
+    cache.step(ints(fits.tolist()), n, 1)
+    assert cache.lengths.tolist() == fits.tolist()
+    cache.check()
+    q = ints(fits.tolist())
+    cache.remap(None, torch.zeros_like(q))
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        plan = cache.step(q, n, 1)
+    one_more = fits.copy()
+    one_more[-1] += 1
+    negative = np.where(np.arange(slots) % 2 == 0, fits, -fits - 1)
+    over = (one_more, np.full(slots, (1 << 31) - 1), np.full(slots, n + 1))
+    for given in (fits, *over, negative, *over, fits * 0):
+        kept, want = state_of(cache), np.maximum(given, 0)
+        q.copy_(ints(given.tolist()))
+        graph.replay()
+        torch.cuda.synchronize()
+        if want.sum() <= n:
+            assert cache.lengths.tolist() == (kept[1].cpu().numpy() + want).tolist()
+            assert plan.sequences.tolist() == np.repeat(np.arange(slots), want).tolist() + \
+                [-1] * (n - int(want.sum()))
+            cache.check()
+            continue
+        assert same_state(cache, kept) and set(plan.sequences.tolist()) == {-1}
+        eager = cache.step(q, n, 1)
+        assert same_state(cache, kept) and set(eager.sequences.tolist()) == {-1}
+        lacking = min(int(want.sum()) - n, (1 << 31) - 1)
+        with pytest.raises(RuntimeError, match=f"lacked {lacking} rows"):
+            cache.check()
+        cache.check()

@@ -1,8 +1,9 @@
 """The paged cache's refusals in an order that changes nothing, without a GPU."""
 
+import numpy as np
 import pytest
 
-from hackaton_amd import PagedCache
+from hackaton_amd import PagedCache, _lib
 from hackaton_amd._lib import VarlenAttnError
 
 
@@ -15,3 +16,19 @@ def test_a_step_is_checked_before_the_cache_grows(slots, q_lengths, n_tokens, he
     cache = PagedCache(1, 4, 16, 2, slots, 64, device="cpu")
     with pytest.raises(VarlenAttnError, match=words):
         cache.step(q_lengths, n_tokens, heads)
+
+
+@pytest.mark.parametrize("at,value,code", [
+    (0, None, _lib.VA_EINVAL), (1, None, _lib.VA_EINVAL), (2, -1, _lib.VA_ESHAPE),
+    (2, (1 << 20) + 1, _lib.VA_ESHAPE), (3, -1, _lib.VA_ESHAPE), (4, None, _lib.VA_EINVAL),
+    (5, None, _lib.VA_EINVAL)])
+def test_growth_arguments_are_checked(at, value, code):
+    raw = np.zeros(64, dtype=np.int32)
+    args = [raw.ctypes.data, raw.ctypes.data, 4, 8, raw.ctypes.data, raw.ctypes.data, None]
+    args[at] = value
+    assert _lib.lib().va_pages_growth(*args) == code
+    args = [raw.ctypes.data, raw.ctypes.data, 4, 8, raw.ctypes.data, raw.ctypes.data, None]
+    if at in (0, 1, 4, 5):
+        args[at] += 2  # not a word
+        assert _lib.lib().va_pages_growth(*args) == _lib.VA_EINVAL
+    assert _lib.lib().va_pages_growth(None, None, 0, 8, None, None, None) == 0
