@@ -385,7 +385,8 @@ hipError_t launch_pages_remap(const PagesArgs& a) {
   if (a.n_pages <= kLdsPages && a.n_slots <= ST) {
     hipLaunchKernelGGL(remap_small_kernel, dim3(1), dim3(ST), 0, a.stream, a);
   } else {
-    hipLaunchKernelGGL(remap_clear_kernel, dim3((a.n_pages + T - 1) / T), dim3(T), 0, a.stream, a);
+    if (a.n_pages > 0)
+      hipLaunchKernelGGL(remap_clear_kernel, dim3((a.n_pages + T - 1) / T), dim3(T), 0, a.stream, a);
     if (a.n_slots > 0)
       hipLaunchKernelGGL(remap_rows_kernel, dim3(a.n_slots), dim3(T), 0, a.stream, a);
     hipLaunchKernelGGL(remap_hand_out_kernel, dim3(1), dim3(ST), 0, a.stream, a);

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from hackaton_amd import PagedCache, paged_attention, paged_plan
+from hackaton_amd import PagedCache, compact_pages, paged_attention, paged_plan, remap_pages
 from hackaton_amd._lib import check, lib
 from tests import paged_oracle as orc
 from tests.paged_oracle import DIM, SCALE
@@ -261,3 +261,19 @@ def test_a_step_of_more_tokens_than_rows_changes_nothing(slots, seed):
         with pytest.raises(RuntimeError, match=f"lacked {lacking} rows"):
             cache.check()
         cache.check()
+
+
+@pytest.mark.parametrize("slots", [1, 1024, 1025, 3000])
+def test_a_pool_without_pages(slots):
+    """Nothing to hand out: a shortfall and the state as it was, on both sides of the one-work-group
+    path; no shortfall where nothing is asked for."""
+    banner("a pool without pages", slots)
+    pages = torch.zeros(1, 2, 0, 1, 16, DIM, dtype=FP16, device="cuda")
+    table = torch.full((slots, 3), -1, dtype=torch.int32, device="cuda")
+    lengths, none = torch.zeros_like(table[:, 0]), ints([])
+    out = remap_pages(pages, table, lengths, none, None, lengths + 20)
+    assert int(out[3]) == 2 * slots
+    assert torch.equal(out[0], table) and torch.equal(out[1], lengths) and out[2].numel() == 0
+    out = remap_pages(pages, table, lengths, none)
+    assert int(out[3]) == 0 and torch.equal(out[0], table) and torch.equal(out[1], lengths)
+    assert int(compact_pages(pages, table, lengths, none)[2]) == 0
