@@ -14,13 +14,14 @@ Pages hold `page_size` rows (a power of two, 16 to 256) of every key/value head:
 (n_pages, kv_heads, page_size, 128). Row t of a sequence lies in page `page_table[sequence, t //
 page_size]`, row `t % page_size`; entries outside the pool name no page. Lengths, tables and counts are
 int32 and stay on the GPU: no call reads them back, so a captured step follows them. None of the calls
-has a backward.
+has a backward or a forward-mode derivative; tensors that ask for one are refused.
 """
 
 import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, attention
 from ._lib import check, lib
@@ -35,6 +36,15 @@ def _no_grad(*tensors):
             if t.requires_grad:
                 raise RuntimeError("the paged cache has no backward: call it under torch.no_grad() "
                                    "or torch.inference_mode()")
+    _no_tangent(*tensors)
+
+
+def _no_tangent(*tensors):
+    if forward_ad._current_level >= 0:  # inside forward_ad.dual_level()
+        for t in tensors:
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("the paged cache has no forward-mode derivative: pass the primals "
+                                   "(torch.autograd.forward_ad.unpack_dual)")
 
 
 def _one_device(first, *tensors):
@@ -215,6 +225,7 @@ def paged_append(q, k, v, cos, sin, k_pages, v_pages, plan):
         with torch.cuda.device(device):
             return paged_append(q, k, v, cos, sin, k_pages, v_pages, plan)
     _no_grad(q, k, v, k_pages, v_pages)
+    _no_tangent(cos, sin)
     n, heads, kv_heads = plan.n_tokens, plan.heads, plan.kv_heads
     if (q.shape != (n, heads * HEAD_DIM) or k.shape != (n, kv_heads * HEAD_DIM)
             or v.shape != k.shape):
@@ -339,6 +350,7 @@ def remap_pages(pages, table, lengths, refs, parents=None, new_lengths=None):
     if device.index != _current_device():  # launches and allocations go to the tensors' device
         with torch.cuda.device(device):
             return remap_pages(pages, table, lengths, refs, parents, new_lengths)
+    _no_grad(pages)
     outer, n_pages, kv_heads, page_size = _pool_of(pages)
     slots, width = _state_of(n_pages, table, lengths, refs, parents=parents, new_lengths=new_lengths)
     table_out, lengths_out, refs_out = (torch.empty_like(table), torch.empty_like(lengths),
@@ -364,6 +376,7 @@ def compact_pages(pages, table, lengths, refs):
     if device.index != _current_device():  # launches and allocations go to the tensors' device
         with torch.cuda.device(device):
             return compact_pages(pages, table, lengths, refs)
+    _no_grad(pages)
     outer, n_pages, kv_heads, page_size = _pool_of(pages)
     slots, width = _state_of(n_pages, table, lengths, refs)
     table_out, refs_out = torch.empty_like(table), torch.empty_like(refs)

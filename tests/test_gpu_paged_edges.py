@@ -4,8 +4,10 @@ refused or cut, and what they leave unchanged."""
 import numpy as np
 import pytest
 import torch
+from torch.autograd import forward_ad
 
-from hackaton_amd import PagedCache, compact_pages, paged_attention, paged_plan, remap_pages
+from hackaton_amd import (PagedCache, compact_pages, paged_append, paged_attention, paged_plan,
+                          remap_pages)
 from hackaton_amd._lib import check, lib
 from tests import paged_oracle as orc
 from tests.paged_oracle import DIM, SCALE
@@ -277,3 +279,35 @@ def test_a_pool_without_pages(slots):
     out = remap_pages(pages, table, lengths, none)
     assert int(out[3]) == 0 and torch.equal(out[0], table) and torch.equal(out[1], lengths)
     assert int(compact_pages(pages, table, lengths, none)[2]) == 0
+
+
+def test_tensors_that_ask_for_derivatives_are_refused():
+    """Every floating tensor of every call: requires_grad while gradients are on, tangents always."""
+    banner("derivatives")
+    q, kv, heads, kv_heads, ps = [1, 2], [40, 33], 4, 2, 16
+    query, k, v, table = (x.cuda() for x in orc.paged_case(1, q, kv, heads, kv_heads, FP16, ps))
+    plan = paged_plan(table, q, kv, 3, heads, kv_heads, ps)
+    rows = [torch.zeros(3, h * DIM, dtype=FP16, device="cuda") for h in (heads, kv_heads, kv_heads)]
+    cos = torch.ones(1, 50, DIM, device="cuda")
+    pages = torch.zeros(1, 2, 4, kv_heads, ps, DIM, dtype=FP16, device="cuda")
+    state = [ints([[0, 1]]), ints([20]), ints([1, 1, 0, 0])]
+
+    def calls():
+        yield lambda *x: paged_attention(*x, plan, SCALE), [query, k, v]
+        yield lambda *x: paged_append(*x, plan), [*rows, cos, cos.clone(), k, v]
+        yield lambda x: remap_pages(x, *state), [pages]
+        yield lambda x: compact_pages(x, *state), [pages]
+
+    for call, tensors in calls():
+        for i, x in enumerate(tensors):
+            if not (x.dtype == torch.float32):  # (the rotary tables are constants, as in qkv_rotate)
+                bad = [t.clone().requires_grad_() if j == i else t for j, t in enumerate(tensors)]
+                with pytest.raises(RuntimeError, match="no backward"):
+                    call(*bad)
+                with torch.no_grad():
+                    call(*bad)
+            with torch.no_grad(), forward_ad.dual_level():
+                bad = [forward_ad.make_dual(t, t) if j == i else t for j, t in enumerate(tensors)]
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(*bad)
+                call(*tensors)

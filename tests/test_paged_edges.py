@@ -2,8 +2,10 @@
 
 import numpy as np
 import pytest
+import torch
+from torch.autograd import forward_ad
 
-from hackaton_amd import PagedCache, _lib
+from hackaton_amd import PagedCache, _lib, paged
 from hackaton_amd._lib import VarlenAttnError
 
 
@@ -32,3 +34,14 @@ def test_growth_arguments_are_checked(at, value, code):
         args[at] += 2  # not a word
         assert _lib.lib().va_pages_growth(*args) == _lib.VA_EINVAL
     assert _lib.lib().va_pages_growth(None, None, 0, 8, None, None, None) == 0
+
+
+def test_tangents_are_refused():
+    x = torch.randn(3)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, x)
+        for off in (torch.enable_grad, torch.no_grad):  # (no_grad leaves forward mode on)
+            with off(), pytest.raises(RuntimeError, match="forward-mode"):
+                paged._no_grad(x, dual)
+        paged._no_grad(x, forward_ad.unpack_dual(dual).primal)
+    paged._no_grad(x)
