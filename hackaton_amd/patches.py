@@ -6,8 +6,9 @@ built by solution/packed.py:153-176) take the packed path: the q/k/v projections
 `packed_attention` when the rows are right padded (`lengths` is a list), otherwise the padded
 layout with the caller's mask through `qkv_rotate(padded=True)`, SDPA and `pack_rows`. Calls that
 carry `paged=(cache, plan)` (a serving step over a `PagedCache`: hidden rows of the step's new
-tokens, rotary tables by row) append the rows to the layer's pages and attend to them. Every other
-call runs the original forward unchanged.
+tokens, rotary tables by row) append the rows to the layer's pages and attend to them; they read no
+mask, and a model called with `attention_mask={"full_attention": None}` builds none. Every other call
+runs the original forward unchanged.
 """
 
 import torch
