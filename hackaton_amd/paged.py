@@ -79,14 +79,15 @@ def _lengths(name, lengths, n_seqs, device):
     """Lengths of every sequence as an int32 device tensor, from one or from a host list."""
     if not isinstance(lengths, torch.Tensor):
         lengths = torch.tensor([int(x) for x in lengths], dtype=torch.int32, device=device)
-    if lengths.dtype.is_floating_point or lengths.dtype == torch.bool:
+    if lengths.dtype.is_floating_point or lengths.dtype.is_complex or lengths.dtype == torch.bool:
         raise ValueError(f"{name} must be whole numbers, got {lengths.dtype}")
     if lengths.device != device:
         raise ValueError(f"{name} on {lengths.device}, page_table on {device}")
     if lengths.numel() != n_seqs:
         raise ValueError(f"{lengths.numel()} {name} for {n_seqs} page table rows")
-    return lengths if lengths.dtype == torch.int32 and lengths.is_contiguous() else \
-        lengths.to(torch.int32).contiguous()
+    if lengths.dtype != torch.int32:  # (cut to their bounds, not to their low bits)
+        lengths = lengths.to(torch.int64).clamp(0, 2 ** 31 - 1).to(torch.int32)
+    return lengths.contiguous()
 
 
 def _check_host_lengths(q_lengths, kv_lengths, n_tokens, most):

@@ -311,3 +311,26 @@ def test_tensors_that_ask_for_derivatives_are_refused():
                 with pytest.raises(RuntimeError, match="forward-mode"):
                     call(*bad)
                 call(*tensors)
+
+
+def test_wide_lengths_past_their_bounds_are_cut():
+    """64-bit device lengths follow the rules of the 32-bit ones."""
+    banner("64-bit lengths")
+    q, kv = [2, 3], [50, 64]
+    query, k, v, table = (x.cuda() for x in orc.paged_case(6, q, kv, 12, 2, FP16, 16, width=4))
+
+    def run(q, kv):
+        plan = paged_plan(table, q, kv, 5, 12, 2, 16)
+        return paged_attention(query, k, v, plan, SCALE), plan.positions
+
+    for wide, narrow in (([2, (1 << 32) + 3], [2, (1 << 31) - 1]), ([2, -(1 << 32) + 3], [2, -5])):
+        got, want = (run(torch.tensor(x, device="cuda"), ints(kv)) for x in (wide, narrow))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    got, want = (run(ints(q), torch.tensor([50, x], device="cuda")) for x in ((1 << 32) + 1, 64))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    cache = PagedCache(1, 8, 16, 2, 2, 64)
+    kept = state_of(cache)
+    cache.step(torch.tensor([1, (1 << 32) + 1], device="cuda"), 2, 4)
+    assert same_state(cache, kept)
+    with pytest.raises(RuntimeError, match="rows"):
+        cache.check()

@@ -45,3 +45,24 @@ def test_tangents_are_refused():
                 paged._no_grad(x, dual)
         paged._no_grad(x, forward_ad.unpack_dual(dual).primal)
     paged._no_grad(x)
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32, torch.int16, torch.uint8])
+def test_lengths_of_any_whole_type(dtype):
+    """Those that pass 32 bits are cut to the largest; negative ones count as 0 either way."""
+    top = torch.iinfo(dtype).max
+    given = torch.tensor([0, 7, min(top, (1 << 32) + 5), min(top, 1 << 40), top], dtype=dtype)
+    got = paged._lengths("q_lengths", given, 5, given.device)
+    assert got.dtype == torch.int32 and got.is_contiguous()
+    assert got.tolist() == [min(x, (1 << 31) - 1) for x in given.tolist()]
+    strided = torch.stack((given, given), 1)[:, 0]
+    assert torch.equal(paged._lengths("q_lengths", strided, 5, given.device), got)
+    if dtype == torch.int64:
+        low = torch.tensor([-1, -(1 << 32) + 9, -(1 << 63)])
+        assert paged._lengths("q_lengths", low, 3, low.device).clamp(min=0).tolist() == [0, 0, 0]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float64, torch.complex64, torch.bool])
+def test_lengths_of_other_types_are_refused(dtype):
+    with pytest.raises(ValueError, match="whole numbers"):
+        paged._lengths("q_lengths", torch.zeros(2).to(dtype), 2, torch.device("cpu"))
