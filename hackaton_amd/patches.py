@@ -61,6 +61,10 @@ def patch_qwen2_attention():
 def _paged_forward(layer, hidden_states, position_embeddings, cache, plan):
     """The layer's rows of a serving step, (N, hidden) or (1, N, hidden): projections, append to the
     layer's pages, attention over them, output projection."""
+    window, reach = getattr(layer, "sliding_window", None), plan.page_table.shape[1] * plan.page_size
+    if window is not None and window < reach:  # a row past the window would see too many keys
+        raise ValueError(f"layer {layer.layer_idx} attends to a window of {window} tokens: the paged "
+                         f"attention has none, and a page table row holds {reach}")
     rows = hidden_states.reshape(-1, hidden_states.shape[-1])
     cos, sin = (x.reshape(-1, x.shape[-1]) for x in position_embeddings)
     keys, values = cache.keys(layer.layer_idx), cache.values(layer.layer_idx)

@@ -1,6 +1,8 @@
 """The patched layer's serving calls as a program makes them through the whole model: what the model
 does around them, and which ones are refused."""
 
+from types import SimpleNamespace
+
 import pytest
 import torch
 
@@ -34,6 +36,39 @@ def test_a_serving_call_builds_no_mask(patched, monkeypatch, n):  # noqa: F811
         out = model(input_ids=torch.zeros(1, n, dtype=torch.long), position_ids=positions,
                     attention_mask=NO_MASK, paged=(None, None), use_cache=False).logits
     assert out.shape == (1, n, 1000) and seen == [None, None]
+
+
+@pytest.mark.parametrize("window,width,fits", [(None, 1000, True), (64, 4, True), (64, 5, False),
+                                               (63, 4, False), (0, 1, False)])
+def test_a_window_shorter_than_the_tables_is_refused(patched, monkeypatch, window, width, fits):  # noqa: F811
+    """The paged attention sees every key up to a row's own: a layer with a sliding window that a page
+    table row passes would get other answers than transformers' forward."""
+    layer = tiny_model("cpu").model.layers[0].self_attn
+    layer.sliding_window = window
+    monkeypatch.setattr(patches, "paged_append", lambda q, *rest: q)
+    monkeypatch.setattr(patches, "paged_attention", lambda query, *rest: query)
+    cache = SimpleNamespace(keys=lambda i: None, values=lambda i: None)
+    plan = SimpleNamespace(page_table=torch.zeros(2, width, dtype=torch.int32), page_size=16)
+    x, tables = torch.zeros(3, HEADS * 128), (torch.ones(3, 128), torch.zeros(3, 128))
+    if fits:
+        assert layer(x, tables, None, paged=(cache, plan))[0].shape == x.shape
+    else:
+        with pytest.raises(ValueError, match="window"):
+            layer(x, tables, None, paged=(cache, plan))
+
+
+def test_layers_with_windows_of_a_model_are_refused(patched):  # noqa: F811
+    from transformers import Qwen2Config, Qwen2ForCausalLM
+
+    config = Qwen2Config(vocab_size=100, hidden_size=256, intermediate_size=64, num_hidden_layers=2,
+                         num_attention_heads=2, num_key_value_heads=1, use_sliding_window=True,
+                         sliding_window=32, max_window_layers=0)
+    model = Qwen2ForCausalLM(config).eval()
+    plan = SimpleNamespace(page_table=torch.zeros(1, 3, dtype=torch.int32), page_size=16)
+    masks = {"full_attention": None, "sliding_attention": None}
+    with torch.inference_mode(), pytest.raises(ValueError, match="window of 32"):
+        model(input_ids=torch.zeros(1, 4, dtype=torch.long), position_ids=torch.arange(4)[None],
+              attention_mask=masks, paged=(None, plan), use_cache=False)
 
 
 @pytest.mark.gpu
