@@ -263,10 +263,11 @@ def paged_attention(query, k_pages, v_pages, plan, scale):
     """Every new token attends to its sequence's keys at positions up to its own. query
     (n_tokens, heads, 128) in the pages' type; returns (n_tokens, heads * 128), zeros for padding and
     for rows that see no key. Key/value heads are shared by heads / kv_heads query heads each. What a
-    page holds behind its sequence's end is never read. (A sequence's own values that are infinite or
-    not a number also reach the rows of their 64-key tile that come before them, as in
-    `varlen_attention`.) The same step gives the same bits; the same sequence in another step agrees to
-    rounding."""
+    page holds behind its sequence's end is never read. (Keys that a row does not see never reach it,
+    whatever they hold. Values that are infinite or not a number do where they lie in a 64-key tile that
+    another of the 32 rows computed together sees, rows being pairs of a token and a query head of the
+    group: in rows of the same sequence up to 63 + ceil(31 kv_heads / heads) positions before their own.)
+    The same step gives the same bits; the same sequence in another step agrees to rounding."""
     device = _one_device(query, k_pages, v_pages, plan.words)
     if device.index != _current_device():  # launches and allocations go to the tensors' device
         with torch.cuda.device(device):

@@ -338,7 +338,9 @@ int va_paged_append(const va_paged_step* step, const void* q, const void* k, con
 /* out (N, Hq, 128) = softmax(scale q k^T) v of every new token over its sequence's keys at positions
  * up to its own; zeros for padding rows and for rows that see no key. The workspace
  * (va_paged_attention_workspace bytes, possibly 0) holds partial results of split key ranges; calls
- * that may overlap need one each. scale must be finite and > 0. Deterministic: the same step gives the
+ * that may overlap need one each. Values that are infinite or not a number (of the sequence's own new
+ * tokens) also reach rows up to 63 + ceil(31 Hkv / Hq) positions before them: tiles of 64 keys are
+ * multiplied whole for 32 (token, query head) rows at a time. scale must be finite and > 0. Deterministic: the same step gives the
  * same bits; where a row's keys are split depends on the whole step, so the same sequence in another
  * step agrees to rounding. */
 int va_paged_attention_workspace(const va_paged_step* step, int64_t* bytes);

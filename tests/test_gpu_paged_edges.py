@@ -11,7 +11,7 @@ from hackaton_amd import (PagedCache, compact_pages, paged_append, paged_attenti
 from hackaton_amd._lib import check, lib
 from tests import paged_oracle as orc
 from tests.paged_oracle import DIM, SCALE
-from tests.test_gpu_paged import BF16, FP16, banner, check_attention, ints
+from tests.test_gpu_paged import BF16, FP16, attend, banner, check_attention, ints
 
 pytestmark = pytest.mark.gpu
 
@@ -334,3 +334,33 @@ def test_wide_lengths_past_their_bounds_are_cut():
     assert same_state(cache, kept)
     with pytest.raises(RuntimeError, match="rows"):
         cache.check()
+
+
+@pytest.mark.parametrize("q,kv,heads,kv_heads", [
+    ([30], [70], 2, 2), ([5, 1], [300, 90], 6, 1),  # single tiles of few rows
+    ([300], [300], 2, 2), ([200, 1], [330, 40], 12, 2),  # prompts, whole ranges
+    ([200], [2300], 2, 2), ([20], [5000], 1, 1),  # split ranges
+    ([320] * 9, [330] * 9, 24, 24)])  # four waves a tile
+def test_how_far_values_that_are_not_finite_reach(q, kv, heads, kv_heads):
+    """A key of infinities, then a value of them, at one position of the last new rows: what comes before
+    a key keeps its bits, what comes more than 63 + ceil(31 / group) positions before a value does, and so
+    does every other sequence."""
+    banner("values that are not finite", q, kv, heads, kv_heads)
+    ps, group, dtype = 16, heads // kv_heads, FP16
+    query, k, v, table = orc.paged_case(21, q, kv, heads, kv_heads, dtype, ps)
+    want, plan = attend(query, k, v, table, q, kv, ps)
+    pos, own = plan.positions.cpu(), plan.sequences.cpu() == 0
+    assert torch.isfinite(want).all()
+    for back in (1, 2, 40, 64, 130):
+        at = kv[0] - back
+        if back > q[0]:
+            continue
+        page, row = int(table[0, at // ps]), at % ps
+        for x, reach in ((k.clone(), 0), (v.clone(), 63 + -(-31 // group))):
+            x[page, :, row] = float("inf")
+            pools = (k, x) if reach else (x, v)
+            got, _ = attend(query, *pools, table, q, kv, ps)
+            safe = (~own | (pos < at - reach)).cuda()
+            assert torch.equal(got[safe], want[safe]), (back, reach)
+            if reach:
+                assert not torch.isfinite(got[(own & (pos >= at)).cuda()]).any()
