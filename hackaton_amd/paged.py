@@ -36,15 +36,15 @@ def _no_grad(*tensors):
             if t.requires_grad:
                 raise RuntimeError("the paged cache has no backward: call it under torch.no_grad() "
                                    "or torch.inference_mode()")
-    _no_tangent(*tensors)
+    if forward_ad._current_level >= 0:  # inside forward_ad.dual_level()
+        _no_tangent(*tensors)
 
 
 def _no_tangent(*tensors):
-    if forward_ad._current_level >= 0:  # inside forward_ad.dual_level()
-        for t in tensors:
-            if forward_ad.unpack_dual(t).tangent is not None:
-                raise RuntimeError("the paged cache has no forward-mode derivative: pass the primals "
-                                   "(torch.autograd.forward_ad.unpack_dual)")
+    for t in tensors:
+        if forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("the paged cache has no forward-mode derivative: pass the primals "
+                               "(torch.autograd.forward_ad.unpack_dual)")
 
 
 def _one_device(first, *tensors):
@@ -79,15 +79,16 @@ def _lengths(name, lengths, n_seqs, device):
     """Lengths of every sequence as an int32 device tensor, from one or from a host list."""
     if not isinstance(lengths, torch.Tensor):
         lengths = torch.tensor([int(x) for x in lengths], dtype=torch.int32, device=device)
-    if lengths.dtype.is_floating_point or lengths.dtype.is_complex or lengths.dtype == torch.bool:
-        raise ValueError(f"{name} must be whole numbers, got {lengths.dtype}")
+    dtype = lengths.dtype
+    if dtype != torch.int32 and (dtype.is_floating_point or dtype.is_complex or dtype == torch.bool):
+        raise ValueError(f"{name} must be whole numbers, got {dtype}")
     if lengths.device != device:
         raise ValueError(f"{name} on {lengths.device}, page_table on {device}")
     if lengths.numel() != n_seqs:
         raise ValueError(f"{lengths.numel()} {name} for {n_seqs} page table rows")
-    if lengths.dtype != torch.int32:  # (cut to their bounds, not to their low bits)
+    if dtype != torch.int32:  # (cut to their bounds, not to their low bits)
         lengths = lengths.to(torch.int64).clamp(0, 2 ** 31 - 1).to(torch.int32)
-    return lengths.contiguous()
+    return lengths if lengths.is_contiguous() else lengths.contiguous()
 
 
 def _check_host_lengths(q_lengths, kv_lengths, n_tokens, most):
@@ -226,7 +227,8 @@ def paged_append(q, k, v, cos, sin, k_pages, v_pages, plan):
         with torch.cuda.device(device):
             return paged_append(q, k, v, cos, sin, k_pages, v_pages, plan)
     _no_grad(q, k, v, k_pages, v_pages)
-    _no_tangent(cos, sin)
+    if forward_ad._current_level >= 0:  # (the tables are constants, as in qkv_rotate)
+        _no_tangent(cos, sin)
     n, heads, kv_heads = plan.n_tokens, plan.heads, plan.kv_heads
     if (q.shape != (n, heads * HEAD_DIM) or k.shape != (n, kv_heads * HEAD_DIM)
             or v.shape != k.shape):

@@ -340,9 +340,9 @@ int va_paged_append(const va_paged_step* step, const void* q, const void* k, con
  * (va_paged_attention_workspace bytes, possibly 0) holds partial results of split key ranges; calls
  * that may overlap need one each. Values that are infinite or not a number (of the sequence's own new
  * tokens) also reach rows up to 63 + ceil(31 Hkv / Hq) positions before them: tiles of 64 keys are
- * multiplied whole for 32 (token, query head) rows at a time. scale must be finite and > 0. Deterministic: the same step gives the
- * same bits; where a row's keys are split depends on the whole step, so the same sequence in another
- * step agrees to rounding. */
+ * multiplied whole for 32 (token, query head) rows at a time. scale must be finite and > 0.
+ * Deterministic: the same step gives the same bits; where a row's keys are split depends on the whole
+ * step, so the same sequence in another step agrees to rounding. */
 int va_paged_attention_workspace(const va_paged_step* step, int64_t* bytes);
 int va_paged_attention(const va_paged_step* step, const void* q, const void* k_pages,
                        const void* v_pages, int64_t k_stride, int64_t v_stride, int32_t n_pages,
