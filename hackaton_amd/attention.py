@@ -257,7 +257,7 @@ def _capturing():
 
 def release_captured_plans():
     """Give back the work lists kept for captured graphs. Only for a program that will replay none of
-    the graphs that it has captured with host lengths so far."""
+    the graphs that it has captured so far with host lengths, or over a `paged_plan` made before."""
     _CAPTURED_PLANS.clear()
 
 

@@ -127,7 +127,7 @@ class PagedPlan:
 
     __slots__ = ("page_table", "words", "n_tokens", "n_seqs", "heads", "kv_heads", "page_size",
                  "workspace_bytes", "_step", "_page", "_strides", "_stream",
-                 "_captured")
+                 "_capture")
 
     def _rows(self, which):
         rows = -(-self.n_tokens // 4) * 4
@@ -146,12 +146,12 @@ class PagedPlan:
 
     def _use(self):
         """The current stream, with the plan's memory kept for it: a graph that captures a call over a
-        plan made before reads it in every replay, whatever becomes of the plan object (kept until
-        `release_captured_plans()`, as the work lists of `varlen_attention`); another stream than the
-        plan's own reads it before it is handed out again."""
+        plan made before (by another graph too) reads it in every replay, whatever becomes of the plan
+        object (kept until `release_captured_plans()`, as the work lists of `varlen_attention`); another
+        stream than the plan's own reads it before it is handed out again."""
         stream = _current_stream(_current_device())
         if torch._C._cuda_isCurrentStreamCapturing():
-            if not self._captured:
+            if self._capture != attention._capture_id():
                 attention._CAPTURED_PLANS.add(self)
         elif stream != self._stream:
             current = torch.cuda.current_stream()
@@ -188,7 +188,7 @@ def paged_plan(page_table, q_lengths, kv_lengths, n_tokens, heads, kv_heads, pag
     plan._strides = (page_size * HEAD_DIM, HEAD_DIM, 1)
     plan.words = torch.empty(n_words, dtype=torch.int32, device=device)
     plan._stream = _current_stream(device.index)
-    plan._captured = torch._C._cuda_isCurrentStreamCapturing()
+    plan._capture = attention._capture_id() if torch._C._cuda_isCurrentStreamCapturing() else None
     plan._step = _lib.PagedStep(page_table.data_ptr(), plan.words.data_ptr(), n_tokens, n_seqs, width,
                                 page_size, heads, kv_heads)
     check(lib().va_paged_plan(plan._step, q_lengths.data_ptr(), kv_lengths.data_ptr(), n_words,

@@ -364,3 +364,41 @@ def test_how_far_values_that_are_not_finite_reach(q, kv, heads, kv_heads):
             assert torch.equal(got[safe], want[safe]), (back, reach)
             if reach:
                 assert not torch.isfinite(got[(own & (pos >= at)).cuda()]).any()
+
+
+def test_a_graph_keeps_the_plan_of_another():
+    """A plan made in one capture and read by the calls of a second: the second graph keeps it when the
+    first one and the plan object are gone; the calls of the plan's own capture need not."""
+    from hackaton_amd import attention as att
+
+    banner("a plan of another graph")
+    q, kv = [1, 50, 3], [1400, 90, 65]
+    query, k, v, table = (x.cuda() for x in orc.paged_case(12, q, kv, 12, 2, FP16, 16))
+    want, plan = attend(query, k, v, table, q, kv, 16)
+    q_len, kv_len = ints(q), ints(kv)
+    paged_attention(query, k, v, plan, SCALE)
+    att.release_captured_plans()
+    torch.cuda.synchronize()
+    first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first):
+        plan = paged_plan(table, q_len, kv_len, sum(q), 12, 2, 16)
+        own = paged_attention(query, k, v, plan, SCALE)
+    assert not att._CAPTURED_PLANS
+    with torch.cuda.graph(second):
+        out = paged_attention(query, k, v, plan, SCALE)
+    assert att._CAPTURED_PLANS == {plan}
+    first.replay()
+    second.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(own.view_as(want), want) and torch.equal(out.view_as(want), want)
+    size = plan.words.numel()
+    del plan, own, first
+    torch.cuda.empty_cache()
+    fill = [torch.full((size,), 1 << 20, dtype=torch.int32, device="cuda") for _ in range(8)]
+    for _ in range(3):
+        out.zero_()
+        second.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.view_as(want), want)
+    del fill, second
+    att.release_captured_plans()
