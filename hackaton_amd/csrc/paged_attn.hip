@@ -82,7 +82,7 @@ __device__ inline int last_at_most(const int* v, int n, int x) {
 // Prompt tiles come first, the last (longest) ones of a sequence before its first. Work-group i runs on
 // XCD i mod 8: with a multiple of 8 items per tile, the tiles that read the same keys run on one XCD
 // and find them in its L2, so the parts are rounded down to that where there are enough of them
-// (128 new tokens on 32,768, 28/4 heads: 9 parts per tile and head 113 us, 8 parts 89 us).
+// (128 new tokens on 32,768, 28/4 heads: 9 parts per tile and head 85 us, 8 parts 80 us).
 template <int SPT>  // sequences per thread
 __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int writers) {
   constexpr int S = PT * SPT;

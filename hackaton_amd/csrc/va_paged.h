@@ -20,18 +20,19 @@ constexpr int kPagedTileRows = 128;
 constexpr int kPagedChunkKeys = 64;  // key ranges are split at multiples of this
 // The attention's work-groups: 8 waves, one work-group per CU, for steps with prompts (more rows than
 // sequences) of up to this many tiles x heads, by the sizes that the host knows; 4 waves, two per CU,
-// for the others. us with 4 / 8 waves: 2 x 2048 tokens, 12/2 heads (388 tiles) 50 / 42; 4096 tokens
-// (386) 86 / 76; 8 x 300 on 700 (240) 30 / 27; two chunks of 512 beside 62 answers, 28/4 heads (492) 67 /
-// 64; 2 x 1024 on 500 (456) 48 / 47; 3 x 1024 (684) 63 / 69; 4 x 1024 (912) 79 / 85; four chunks of 2048
-// 636 / 703; 64 answers of 64 to 8192 tokens 30 / 32, 16 of 1500 12.0 / 12.5.
+// for the others. us with 4 / 8 waves: 2 x 2048 tokens, 12/2 heads (388 tiles) 51 / 42; 4096 tokens
+// (386) 88 / 72; 8 x 300 on 700 (240) 27.5 / 26; two chunks of 512 beside 62 answers, 28/4 heads (492) 60 /
+// 59; 2 x 1024 on 500 (456) 46.5 / 47.5; 3 x 1024 (684) 62 / 67; 4 x 1024 (912) 78 / 82; four chunks of
+// 2048 623 / 680; 64 answers of 64 to 8192 tokens 30.4 / 32.0, 16 of 1500 12.1 / 12.8, four of 512 7.9 / 7.5.
 constexpr int kPagedWideTiles = 512;
 // Parts that a step's keys are split into, by kind of tile, the shortest part (but a range's last) and
 // the longest table row that is never split. us at 384 / 512 / 1024 few-row parts: 64 answers of 64 to
-// 8192 tokens, 12/2 heads 33 / 30 / 32, four of 65,536, 28/4 heads 109 / 102 / 103; shortest few-row part
-// 128 / 256 / 512: one answer of 8192 9.1 / 10.0 / 12.0, 16 of 1500 13.4 / 12.3 / 13.3. At 256 / 512
-// prompt parts: two chunks of 512 beside 62 answers 61 / 69, 128 new tokens on 32,768 94 / 80; shortest
-// prompt part 256 / 512 / 704: 512 new tokens on 1536 28 / 26 / 27. Four answers of 512, table rows of 576:
-// split 8.8, whole 8.0 and a launch less.
+// 8192 tokens, 12/2 heads 34 / 30 / 32, four of 65,536, 28/4 heads 103 / 97 / 100; shortest few-row part
+// 128 / 256 / 512: one answer of 8192 9.0 / 9.8 / 11.5, 16 of 1500 13.4 / 12.1 / 12.6. At 256 / 512
+// prompt parts: two chunks of 512 beside 62 answers 57 / 76, 128 new tokens on 32,768 80 / 94; shortest
+// prompt part 256 / 512 / 704: 300 new tokens on 1000 16.8 / 17.7 / 20.4, two of 64 on 8000 26.9 / 27.0 /
+// 27.8, where 256 would make twice the parts and room for the merge. Four answers of 512, table rows of
+// 576: split 8.5, whole 7.9 and a launch less.
 constexpr int kPagedFewParts = 512, kPagedManyParts = 256;
 constexpr int kPagedFewKeys = 256, kPagedManyKeys = 512;
 constexpr int kPagedWholeKeys = 1024;

@@ -397,10 +397,10 @@ def compact_pages(pages, table, lengths, refs):
 
 class PagedCache:
     """Keys and values of `layers` layers in one pool of `n_pages` pages, and up to `slots` sequences
-    of at most `max_length` tokens in it. State, all on the GPU: `pages`, `table`, `lengths`, `refs`.
-    Every call updates it in place on the current stream, so the calls of one cache belong on one
-    stream or in order across streams, and a captured step replays on the state it finds. A call
-    that lacks pages (or a step that lacks rows) changes nothing; `check()` reports it."""
+    of at most `max_length` tokens (rounded up to whole pages) in it. State, all on the GPU: `pages`,
+    `table`, `lengths`, `refs`. Every call updates it in place on the current stream, so the calls of one
+    cache belong on one stream or in order across streams, and a captured step replays on the state it
+    finds. A call that lacks pages (or a step that lacks rows) changes nothing; `check()` reports it."""
 
     def __init__(self, layers, n_pages, page_size, kv_heads, slots, max_length,
                  dtype=torch.float16, device="cuda"):
