@@ -7,14 +7,14 @@ of the reference (MLP, loss, norms, NF4, trainer) are outside this package's sco
 
 from .attention import (PackedAttention, PackRows, QKVRotate, VarlenAttention, pack_rows,
                         packed_attention, qkv_rotate, varlen_attention)
-from .paged import (PagedCache, PagedPlan, compact_pages, paged_append, paged_attention,
-                    paged_plan, remap_pages)
+from .paged import (PagedCache, PagedPlan, QuantizedPages, compact_pages, paged_accept, paged_append,
+                    paged_attention, paged_plan, remap_pages)
 from .patches import patch_qwen2_attention
 
 __all__ = ["apply", "patch_qwen2_attention", "packed_attention", "varlen_attention",
            "qkv_rotate", "pack_rows", "PackedAttention", "VarlenAttention", "QKVRotate",
            "PackRows", "paged_plan", "paged_append", "paged_attention", "remap_pages", "compact_pages",
-           "PagedCache", "PagedPlan"]
+           "PagedCache", "PagedPlan", "QuantizedPages", "paged_accept"]
 
 
 def apply():

@@ -13,7 +13,8 @@ LIB_PATH = os.environ.get("VA_LIB_PATH") or os.path.join(
     os.path.dirname(os.path.abspath(__file__)), "libvarlen_attn.so")
 
 VA_OK, VA_EINVAL, VA_ESHAPE, VA_EDTYPE, VA_ESEQ, VA_ECAPACITY = 0, -1, -2, -3, -4, -5
-VA_F16, VA_BF16, VA_F32 = 0, 1, 2
+VA_F16, VA_BF16, VA_F32, VA_E4M3 = 0, 1, 2, 3
+VA_TREE_TOKENS = 256
 VA_PLAN_FWD, VA_PLAN_BWD, VA_PLAN_BWD_HEADS, VA_PLAN_BWD_PAIRS = 0, 1, 2, 3
 VA_PLAN_BWD_GROUPS, VA_PLAN_BWD_GROUPS_ALL, VA_PLAN_FWD_NARROW = 4, 5, 6
 VA_BWD_PAIR_MIN_ITEMS = 1024
@@ -46,7 +47,17 @@ class PagedStep(ctypes.Structure):
                 ("hq", ctypes.c_int32), ("hkv", ctypes.c_int32)]
 
 
+class PagedPages(ctypes.Structure):
+    """va_paged_pages: one layer's pages, 16-bit or 8-bit with exponents."""
+    _fields_ = [("k_pages", ctypes.c_void_p), ("v_pages", ctypes.c_void_p),
+                ("k_exps", ctypes.c_void_p), ("v_exps", ctypes.c_void_p),
+                ("k_stride", ctypes.c_int64), ("v_stride", ctypes.c_int64),
+                ("k_exp_stride", ctypes.c_int64), ("v_exp_stride", ctypes.c_int64),
+                ("n_pages", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
 _pstep = ctypes.POINTER(PagedStep)
+_ppages = ctypes.POINTER(PagedPages)
 
 # name -> (restype, argtypes); the same list the header declares.
 SIGNATURES = {
@@ -97,6 +108,17 @@ SIGNATURES = {
                                       _i32, _p, _p, _p, _p, _p, _i64, _p]),
     "va_pages_compact": (ctypes.c_int, [_p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _i32, _i32,
                                         _p, _p, _p, _p, _i64, _p]),
+    "va_paged_tree_words": (ctypes.c_int, [_pstep, _pi64]),
+    "va_paged_tree": (ctypes.c_int, [_pstep, _p, _p, _i64, _p]),
+    "va_paged_append_pages": (ctypes.c_int, [_pstep, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64,
+                                             _p, _ppages, _i32, _i32, _i32, _p]),
+    "va_paged_attention_pages": (ctypes.c_int, [_pstep, _p, _p, _ppages, _i32, _f32, _i32, _p, _p,
+                                                _i64, _p]),
+    "va_paged_accept": (ctypes.c_int, [_pstep, _p, _p, _p, _i64, _i32, _i32, _i32, _p, _p, _p, _p]),
+    "va_pages_remap8": (ctypes.c_int, [_p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _p, _p,
+                                       _i32, _i32, _p, _p, _p, _p, _p, _i64, _p]),
+    "va_pages_compact8": (ctypes.c_int, [_p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _i32,
+                                         _i32, _p, _p, _p, _p, _i64, _p]),
     "va_probe_mfma": (ctypes.c_int, [_i32, _i32, _i32, _p, _p]),
     "va_probe_copy": (ctypes.c_int, [_p, _p, _i64, _i32, _p]),
 }

@@ -65,24 +65,103 @@ va::PagedLayout layout_of(const va_paged_step& s) {
 }
 
 // Pages of one layer, keys and values, and the step's table and plan.
-int check_pool(const va_paged_step& s, const void* k_pages, const void* v_pages, int64_t k_stride,
-               int64_t v_stride, int32_t n_pages, const char* what) {
-  if (n_pages < 0) return va::fail(VA_ESHAPE, "%s: n_pages=%d", what, n_pages);
-  for (int64_t stride : {k_stride, v_stride})
-    if (stride % 8 != 0 || stride < (int64_t)s.hkv * s.page_size * va::kHeadDim)
-      return va::fail(VA_EINVAL, "%s: page strides must be multiples of 8 and cover a page", what);
+int check_pool(const va_paged_step& s, const va_paged_pages& p, const char* what) {
+  const bool bytes = p.dtype == VA_E4M3;
+  if (p.n_pages < 0) return va::fail(VA_ESHAPE, "%s: n_pages=%d", what, p.n_pages);
+  for (int64_t stride : {p.k_stride, p.v_stride})
+    if (stride % (bytes ? 16 : 8) != 0 || stride < (int64_t)s.hkv * s.page_size * va::kHeadDim)
+      return va::fail(VA_EINVAL, "%s: page strides must be multiples of %d and cover a page", what,
+                      bytes ? 16 : 8);
     else if (stride > (int64_t)(UINT32_MAX / 2))
       return va::fail(VA_ESHAPE, "%s: page strides of 4 GiB or more", what);
   int rc = VA_OK;
-  if (n_pages > 0 && (rc = check_buffers({k_pages, v_pages}, what))) return rc;
+  if (p.n_pages > 0 && (rc = check_buffers({p.k_pages, p.v_pages}, what))) return rc;
+  if (bytes) {
+    for (int64_t stride : {p.k_exp_stride, p.v_exp_stride})
+      if (stride < (int64_t)s.hkv * s.page_size || stride > INT32_MAX)
+        return va::fail(VA_EINVAL, "%s: exponent strides must cover a page", what);
+    if (p.n_pages > 0 && (p.k_exps == nullptr || p.v_exps == nullptr))
+      return va::fail(VA_EINVAL, "%s: NULL exponents", what);
+  }
   if (s.n_tokens > 0 && (rc = check_buffers({s.plan}, what))) return rc;
   if (s.n_seqs > 0 && s.table_width > 0) rc = check_words({s.page_table}, what);
   return rc;
 }
 
-va::PagedPool pool_of(const va_paged_step& s, int64_t k_stride, int64_t v_stride, int32_t n_pages) {
-  return va::PagedPool{s.page_table, s.table_width, n_pages, shift_of(s.page_size),
-                       (uint32_t)(2 * k_stride), (uint32_t)(2 * v_stride)};
+va::PagedPool pool_of(const va_paged_step& s, const va_paged_pages& p) {
+  const bool bytes = p.dtype == VA_E4M3;
+  const int64_t size = bytes ? 1 : 2;
+  return va::PagedPool{s.page_table, s.table_width, p.n_pages, shift_of(s.page_size),
+                       (uint32_t)(size * p.k_stride), (uint32_t)(size * p.v_stride),
+                       bytes ? p.k_exps : nullptr, bytes ? p.v_exps : nullptr,
+                       bytes ? (uint32_t)p.k_exp_stride : 0, bytes ? (uint32_t)p.v_exp_stride : 0};
+}
+
+int append_checked(const va_paged_step* step, const int32_t* tree, const void* q, const void* k,
+                   const void* v, const float* cos, const float* sin, int64_t cos_batch_stride,
+                   int64_t cos_seq_stride, int64_t cos_token_stride, int64_t cos_rows, void* q_out,
+                   const va_paged_pages& pages, int32_t head_dim, int32_t in_dtype,
+                   int32_t out_dtype, void* stream, const char* what) {
+  if (head_dim != va::kHeadDim)
+    return va::fail(VA_ESHAPE, "%s: head_dim=%d, built for %d", what, head_dim, va::kHeadDim);
+  int rc = check_step(step, what);
+  if (rc) return rc;
+  const va_paged_step& s = *step;
+  if (in_dtype < VA_F16 || in_dtype > VA_F32 || (out_dtype != VA_F16 && out_dtype != VA_BF16) ||
+      (pages.dtype != out_dtype && pages.dtype != VA_E4M3))
+    return va::fail(VA_EDTYPE, "%s: dtype", what);
+  for (int64_t stride : {cos_batch_stride, cos_seq_stride, cos_token_stride})
+    if (stride < 0 || stride % 4 != 0)
+      return va::fail(VA_EINVAL, "%s: cos/sin strides must be non-negative multiples of 4", what);
+  if (cos_rows < 0) return va::fail(VA_EINVAL, "%s: cos_rows", what);
+  if ((rc = check_pool(s, pages, what))) return rc;
+  if (s.n_tokens == 0) return VA_OK;
+  if ((rc = check_buffers({q, k, v, cos, sin, q_out}, what))) return rc;
+  if (tree != nullptr && (rc = check_buffers({tree}, what))) return rc;
+  const va::PagedLayout layout = layout_of(s);
+  const int32_t* pos = s.plan + layout.pos;
+  va::PagedAppendArgs a{q, k, v, cos, sin, cos_batch_stride, cos_seq_stride, cos_token_stride,
+                        cos_rows, s.plan + layout.seq, pos,
+                        tree == nullptr ? pos : tree + va::tree_positions(s.n_tokens),
+                        pool_of(s, pages), q_out, pages.k_pages, pages.v_pages, s.n_seqs,
+                        (int)s.n_tokens, s.hq, s.hkv, in_dtype, out_dtype, (hipStream_t)stream};
+  return launched(va::launch_paged_append(a), what);
+}
+
+int attention_checked(const va_paged_step* step, const int32_t* tree, const void* q,
+                      const va_paged_pages& pages, int32_t head_dim, float scale, int32_t dtype,
+                      void* out, void* workspace, int64_t workspace_bytes, void* stream,
+                      const char* what) {
+  if (head_dim != va::kHeadDim)
+    return va::fail(VA_ESHAPE, "%s: head_dim=%d, built for %d", what, head_dim, va::kHeadDim);
+  int rc = check_step(step, what);
+  if (rc) return rc;
+  const va_paged_step& s = *step;
+  if ((dtype != VA_F16 && dtype != VA_BF16) || (pages.dtype != dtype && pages.dtype != VA_E4M3))
+    return va::fail(VA_EDTYPE, "%s: dtype %d: attention runs on VA_F16 or VA_BF16", what, dtype);
+  if (!std::isfinite(scale) || scale <= 0.f)
+    return va::fail(VA_EINVAL, "%s: scale must be finite and positive", what);
+  if ((rc = check_pool(s, pages, what))) return rc;
+  if (s.n_tokens == 0) return VA_OK;
+  const va::PagedLayout layout = layout_of(s);
+  const int64_t need = va::paged_workspace(layout);
+  if (workspace_bytes < need)
+    return va::fail(VA_ECAPACITY, "%s: workspace %lld bytes, need %lld", what,
+                    (long long)workspace_bytes, (long long)need);
+  if ((rc = check_buffers({q, out}, what))) return rc;
+  if (need > 0 && (rc = check_buffers({workspace}, what))) return rc;
+  if (tree != nullptr && (rc = check_buffers({tree}, what))) return rc;
+  va::PagedAttnArgs a{q, pages.k_pages, pages.v_pages, pool_of(s, pages), s.plan, layout,
+                      s.n_seqs, (int)s.n_tokens, s.hq, s.hkv, scale, dtype, out, (float*)workspace,
+                      (hipStream_t)stream, tree};
+  return launched(va::launch_paged_attention(a), what);
+}
+
+// (the 16-bit entry points' pages)
+va_paged_pages pages16(const void* k, const void* v, int64_t k_stride, int64_t v_stride,
+                       int32_t n_pages, int32_t dtype) {
+  return va_paged_pages{const_cast<void*>(k), const_cast<void*>(v), nullptr, nullptr, k_stride,
+                        v_stride, 0, 0, n_pages, dtype};
 }
 
 }  // namespace
@@ -119,27 +198,24 @@ extern "C" int va_paged_append(const va_paged_step* step, const void* q, const v
                                void* k_pages, void* v_pages, int64_t k_stride, int64_t v_stride,
                                int32_t n_pages, int32_t head_dim, int32_t in_dtype,
                                int32_t out_dtype, void* stream) {
-  const char* what = "va_paged_append";
-  if (head_dim != va::kHeadDim)
-    return va::fail(VA_ESHAPE, "%s: head_dim=%d, built for %d", what, head_dim, va::kHeadDim);
-  int rc = check_step(step, what);
-  if (rc) return rc;
-  const va_paged_step& s = *step;
-  if (in_dtype < VA_F16 || in_dtype > VA_F32 || (out_dtype != VA_F16 && out_dtype != VA_BF16))
-    return va::fail(VA_EDTYPE, "%s: dtype", what);
-  for (int64_t stride : {cos_batch_stride, cos_seq_stride, cos_token_stride})
-    if (stride < 0 || stride % 4 != 0)
-      return va::fail(VA_EINVAL, "%s: cos/sin strides must be non-negative multiples of 4", what);
-  if (cos_rows < 0) return va::fail(VA_EINVAL, "%s: cos_rows", what);
-  if ((rc = check_pool(s, k_pages, v_pages, k_stride, v_stride, n_pages, what))) return rc;
-  if (s.n_tokens == 0) return VA_OK;
-  if ((rc = check_buffers({q, k, v, cos, sin, q_out}, what))) return rc;
-  const va::PagedLayout layout = layout_of(s);
-  va::PagedAppendArgs a{q, k, v, cos, sin, cos_batch_stride, cos_seq_stride, cos_token_stride,
-                        cos_rows, s.plan + layout.seq, s.plan + layout.pos,
-                        pool_of(s, k_stride, v_stride, n_pages), q_out, k_pages, v_pages, s.n_seqs,
-                        (int)s.n_tokens, s.hq, s.hkv, in_dtype, out_dtype, (hipStream_t)stream};
-  return launched(va::launch_paged_append(a), what);
+  return append_checked(step, nullptr, q, k, v, cos, sin, cos_batch_stride, cos_seq_stride,
+                        cos_token_stride, cos_rows, q_out,
+                        pages16(k_pages, v_pages, k_stride, v_stride, n_pages, out_dtype), head_dim,
+                        in_dtype, out_dtype, stream, "va_paged_append");
+}
+
+extern "C" int va_paged_append_pages(const va_paged_step* step, const int32_t* tree, const void* q,
+                                     const void* k, const void* v, const float* cos,
+                                     const float* sin, int64_t cos_batch_stride,
+                                     int64_t cos_seq_stride, int64_t cos_token_stride,
+                                     int64_t cos_rows, void* q_out, const va_paged_pages* pages,
+                                     int32_t head_dim, int32_t in_dtype, int32_t out_dtype,
+                                     void* stream) {
+  const char* what = "va_paged_append_pages";
+  if (pages == nullptr) return va::fail(VA_EINVAL, "%s: pages is NULL", what);
+  return append_checked(step, tree, q, k, v, cos, sin, cos_batch_stride, cos_seq_stride,
+                        cos_token_stride, cos_rows, q_out, *pages, head_dim, in_dtype, out_dtype,
+                        stream, what);
 }
 
 extern "C" int va_paged_attention_workspace(const va_paged_step* step, int64_t* bytes) {
@@ -155,29 +231,45 @@ extern "C" int va_paged_attention(const va_paged_step* step, const void* q, cons
                                   int32_t n_pages, int32_t head_dim, float scale, int32_t dtype,
                                   void* out, void* workspace, int64_t workspace_bytes,
                                   void* stream) {
-  const char* what = "va_paged_attention";
-  if (head_dim != va::kHeadDim)
-    return va::fail(VA_ESHAPE, "%s: head_dim=%d, built for %d", what, head_dim, va::kHeadDim);
+  return attention_checked(step, nullptr, q,
+                           pages16(k_pages, v_pages, k_stride, v_stride, n_pages, dtype), head_dim,
+                           scale, dtype, out, workspace, workspace_bytes, stream,
+                           "va_paged_attention");
+}
+
+extern "C" int va_paged_attention_pages(const va_paged_step* step, const int32_t* tree,
+                                        const void* q, const va_paged_pages* pages,
+                                        int32_t head_dim, float scale, int32_t dtype, void* out,
+                                        void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* what = "va_paged_attention_pages";
+  if (pages == nullptr) return va::fail(VA_EINVAL, "%s: pages is NULL", what);
+  return attention_checked(step, tree, q, *pages, head_dim, scale, dtype, out, workspace,
+                           workspace_bytes, stream, what);
+}
+
+extern "C" int va_paged_tree_words(const va_paged_step* step, int64_t* words) {
+  const int rc = check_step(step, "va_paged_tree_words");
+  if (rc) return rc;
+  if (words == nullptr) return va::fail(VA_EINVAL, "va_paged_tree_words: NULL output");
+  *words = va::tree_words(step->n_tokens);
+  return VA_OK;
+}
+
+extern "C" int va_paged_tree(const va_paged_step* step, const int32_t* parents, int32_t* tree,
+                             int64_t tree_words, void* stream) {
+  const char* what = "va_paged_tree";
   int rc = check_step(step, what);
   if (rc) return rc;
   const va_paged_step& s = *step;
-  if (dtype != VA_F16 && dtype != VA_BF16)
-    return va::fail(VA_EDTYPE, "%s: dtype %d: attention runs on VA_F16 or VA_BF16", what, dtype);
-  if (!std::isfinite(scale) || scale <= 0.f)
-    return va::fail(VA_EINVAL, "%s: scale must be finite and positive", what);
-  if ((rc = check_pool(s, k_pages, v_pages, k_stride, v_stride, n_pages, what))) return rc;
   if (s.n_tokens == 0) return VA_OK;
-  const va::PagedLayout layout = layout_of(s);
-  const int64_t need = va::paged_workspace(layout);
-  if (workspace_bytes < need)
-    return va::fail(VA_ECAPACITY, "%s: workspace %lld bytes, need %lld", what,
-                    (long long)workspace_bytes, (long long)need);
-  if ((rc = check_buffers({q, out}, what))) return rc;
-  if (need > 0 && (rc = check_buffers({workspace}, what))) return rc;
-  va::PagedAttnArgs a{q, k_pages, v_pages, pool_of(s, k_stride, v_stride, n_pages), s.plan, layout,
-                      s.n_seqs, (int)s.n_tokens, s.hq, s.hkv, scale, dtype, out, (float*)workspace,
+  if (tree_words < va::tree_words(s.n_tokens))
+    return va::fail(VA_ECAPACITY, "%s: %lld words, need %lld", what, (long long)tree_words,
+                    (long long)va::tree_words(s.n_tokens));
+  if ((rc = check_buffers({s.plan, tree}, what))) return rc;
+  if ((rc = check_words({parents}, what))) return rc;
+  va::PagedTreeArgs a{s.plan, layout_of(s), parents, s.n_seqs, (int)s.n_tokens, tree,
                       (hipStream_t)stream};
-  return launched(va::launch_paged_attention(a), what);
+  return launched(va::launch_paged_tree(a), what);
 }
 
 namespace {
@@ -223,17 +315,18 @@ extern "C" int va_pages_growth(const int32_t* lengths, const int32_t* q_lengths,
   return launched(va::launch_pages_growth(a), what);
 }
 
-extern "C" int va_pages_remap(void* pages, int64_t outer, int32_t n_pages, int32_t kv_heads,
-                              int32_t page_size, int32_t head_dim, const int32_t* table,
-                              const int32_t* lengths, const int32_t* refs, const int32_t* parents,
-                              const int32_t* new_lengths, int32_t n_slots, int32_t table_width,
-                              int32_t* table_out, int32_t* lengths_out, int32_t* refs_out,
-                              int32_t* shortfall, int32_t* scratch, int64_t scratch_words,
-                              void* stream) {
-  const char* what = "va_pages_remap";
+namespace {
+
+int remap_checked(void* pages, uint8_t* exps, bool bytes, int64_t outer, int32_t n_pages,
+                  int32_t kv_heads, int32_t page_size, int32_t head_dim, const int32_t* table,
+                  const int32_t* lengths, const int32_t* refs, const int32_t* parents,
+                  const int32_t* new_lengths, int32_t n_slots, int32_t table_width,
+                  int32_t* table_out, int32_t* lengths_out, int32_t* refs_out, int32_t* shortfall,
+                  int32_t* scratch, int64_t scratch_words, void* stream, const char* what) {
   int rc = check_pages(pages, outer, n_pages, kv_heads, page_size, head_dim, n_slots, table_width,
                        scratch_words, what);
   if (rc) return rc;
+  if (bytes && n_pages > 0 && outer > 0 && (rc = check_buffers({exps}, what))) return rc;
   if ((rc = check_words({shortfall, scratch}, what))) return rc;
   if (n_slots > 0 && (rc = check_words({lengths, lengths_out}, what))) return rc;
   for (const int32_t* p : {parents, new_lengths})
@@ -243,10 +336,60 @@ extern "C" int va_pages_remap(void* pages, int64_t outer, int32_t n_pages, int32
   if ((table != nullptr && table == table_out) || (lengths != nullptr && lengths == lengths_out) ||
       (refs != nullptr && refs == refs_out))
     return va::fail(VA_EINVAL, "%s: outputs may not be the inputs", what);
-  va::PagesArgs a{pages, outer, n_pages, kv_heads, shift_of(page_size), table, lengths, refs,
-                  parents, new_lengths, n_slots, table_width, table_out, lengths_out, refs_out,
-                  shortfall, scratch, (hipStream_t)stream};
+  va::PagesArgs a{pages, bytes ? exps : nullptr, va::kHeadDim / (bytes ? 16 : 8), outer, n_pages,
+                  kv_heads, shift_of(page_size), table, lengths, refs, parents, new_lengths,
+                  n_slots, table_width, table_out, lengths_out, refs_out, shortfall, scratch,
+                  (hipStream_t)stream};
   return launched(va::launch_pages_remap(a), what);
+}
+
+int compact_checked(void* pages, uint8_t* exps, bool bytes, int64_t outer, int32_t n_pages,
+                    int32_t kv_heads, int32_t page_size, int32_t head_dim, const int32_t* table,
+                    const int32_t* lengths, const int32_t* refs, int32_t n_slots,
+                    int32_t table_width, int32_t* table_out, int32_t* refs_out, int32_t* live,
+                    int32_t* scratch, int64_t scratch_words, void* stream, const char* what) {
+  int rc = check_pages(pages, outer, n_pages, kv_heads, page_size, head_dim, n_slots, table_width,
+                       scratch_words, what);
+  if (rc) return rc;
+  if (bytes && n_pages > 0 && outer > 0 && (rc = check_buffers({exps}, what))) return rc;
+  if ((rc = check_words({live, scratch}, what))) return rc;
+  if (n_slots > 0 && (rc = check_words({lengths}, what))) return rc;
+  if (n_slots > 0 && table_width > 0 && (rc = check_words({table, table_out}, what))) return rc;
+  if (n_pages > 0 && (rc = check_words({refs, refs_out}, what))) return rc;
+  if ((table != nullptr && table == table_out) || (refs != nullptr && refs == refs_out))
+    return va::fail(VA_EINVAL, "%s: outputs may not be the inputs", what);
+  va::PagesArgs a{pages, bytes ? exps : nullptr, va::kHeadDim / (bytes ? 16 : 8), outer, n_pages,
+                  kv_heads, shift_of(page_size), table, lengths, refs, nullptr, nullptr, n_slots,
+                  table_width, table_out, nullptr, refs_out, live, scratch, (hipStream_t)stream};
+  return launched(va::launch_pages_compact(a), what);
+}
+
+}  // namespace
+
+extern "C" int va_pages_remap(void* pages, int64_t outer, int32_t n_pages, int32_t kv_heads,
+                              int32_t page_size, int32_t head_dim, const int32_t* table,
+                              const int32_t* lengths, const int32_t* refs, const int32_t* parents,
+                              const int32_t* new_lengths, int32_t n_slots, int32_t table_width,
+                              int32_t* table_out, int32_t* lengths_out, int32_t* refs_out,
+                              int32_t* shortfall, int32_t* scratch, int64_t scratch_words,
+                              void* stream) {
+  return remap_checked(pages, nullptr, false, outer, n_pages, kv_heads, page_size, head_dim, table,
+                       lengths, refs, parents, new_lengths, n_slots, table_width, table_out,
+                       lengths_out, refs_out, shortfall, scratch, scratch_words, stream,
+                       "va_pages_remap");
+}
+
+extern "C" int va_pages_remap8(void* pages, uint8_t* exps, int64_t outer, int32_t n_pages,
+                               int32_t kv_heads, int32_t page_size, int32_t head_dim,
+                               const int32_t* table, const int32_t* lengths, const int32_t* refs,
+                               const int32_t* parents, const int32_t* new_lengths, int32_t n_slots,
+                               int32_t table_width, int32_t* table_out, int32_t* lengths_out,
+                               int32_t* refs_out, int32_t* shortfall, int32_t* scratch,
+                               int64_t scratch_words, void* stream) {
+  return remap_checked(pages, exps, true, outer, n_pages, kv_heads, page_size, head_dim, table,
+                       lengths, refs, parents, new_lengths, n_slots, table_width, table_out,
+                       lengths_out, refs_out, shortfall, scratch, scratch_words, stream,
+                       "va_pages_remap8");
 }
 
 extern "C" int va_pages_compact(void* pages, int64_t outer, int32_t n_pages, int32_t kv_heads,
@@ -255,18 +398,42 @@ extern "C" int va_pages_compact(void* pages, int64_t outer, int32_t n_pages, int
                                 int32_t table_width, int32_t* table_out, int32_t* refs_out,
                                 int32_t* live, int32_t* scratch, int64_t scratch_words,
                                 void* stream) {
-  const char* what = "va_pages_compact";
-  int rc = check_pages(pages, outer, n_pages, kv_heads, page_size, head_dim, n_slots, table_width,
-                       scratch_words, what);
+  return compact_checked(pages, nullptr, false, outer, n_pages, kv_heads, page_size, head_dim,
+                         table, lengths, refs, n_slots, table_width, table_out, refs_out, live,
+                         scratch, scratch_words, stream, "va_pages_compact");
+}
+
+extern "C" int va_pages_compact8(void* pages, uint8_t* exps, int64_t outer, int32_t n_pages,
+                                 int32_t kv_heads, int32_t page_size, int32_t head_dim,
+                                 const int32_t* table, const int32_t* lengths, const int32_t* refs,
+                                 int32_t n_slots, int32_t table_width, int32_t* table_out,
+                                 int32_t* refs_out, int32_t* live, int32_t* scratch,
+                                 int64_t scratch_words, void* stream) {
+  return compact_checked(pages, exps, true, outer, n_pages, kv_heads, page_size, head_dim, table,
+                         lengths, refs, n_slots, table_width, table_out, refs_out, live, scratch,
+                         scratch_words, stream, "va_pages_compact8");
+}
+
+extern "C" int va_paged_accept(const va_paged_step* step, const int32_t* tree, void* pages,
+                               uint8_t* exps, int64_t outer, int32_t n_pages, int32_t kv_heads,
+                               int32_t head_dim, const int32_t* lengths, const int32_t* accepted,
+                               int32_t* lengths_out, void* stream) {
+  const char* what = "va_paged_accept";
+  int rc = check_step(step, what);
   if (rc) return rc;
-  if ((rc = check_words({live, scratch}, what))) return rc;
-  if (n_slots > 0 && (rc = check_words({lengths}, what))) return rc;
-  if (n_slots > 0 && table_width > 0 && (rc = check_words({table, table_out}, what))) return rc;
-  if (n_pages > 0 && (rc = check_words({refs, refs_out}, what))) return rc;
-  if ((table != nullptr && table == table_out) || (refs != nullptr && refs == refs_out))
-    return va::fail(VA_EINVAL, "%s: outputs may not be the inputs", what);
-  va::PagesArgs a{pages, outer, n_pages, kv_heads, shift_of(page_size), table, lengths, refs,
-                  nullptr, nullptr, n_slots, table_width, table_out, nullptr, refs_out, live,
-                  scratch, (hipStream_t)stream};
-  return launched(va::launch_pages_compact(a), what);
+  const va_paged_step& s = *step;
+  if ((rc = check_pages(pages, outer, n_pages, kv_heads, s.page_size, head_dim, s.n_seqs,
+                        s.table_width, INT64_MAX, what)))
+    return rc;
+  if (exps != nullptr && (rc = check_buffers({exps}, what))) return rc;
+  if (s.n_seqs == 0) return VA_OK;
+  if ((rc = check_words({lengths, accepted, lengths_out}, what))) return rc;
+  if (s.table_width > 0 && (rc = check_words({s.page_table}, what))) return rc;
+  if (s.n_tokens > 0 && (rc = check_buffers({s.plan}, what))) return rc;
+  if (tree != nullptr && (rc = check_buffers({tree}, what))) return rc;
+  va::PagedAcceptArgs a{s.plan, layout_of(s), tree, s.page_table, s.n_seqs, (int)s.n_tokens,
+                        s.table_width, shift_of(s.page_size), pages, exps,
+                        va::kHeadDim / (exps == nullptr ? 8 : 16), outer, n_pages, kv_heads,
+                        lengths, accepted, lengths_out, (hipStream_t)stream};
+  return launched(va::launch_paged_accept(a), what);
 }

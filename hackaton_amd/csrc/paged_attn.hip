@@ -18,6 +18,16 @@
 // P^T reads V^T from the row-major tile with transposed LDS reads. A tile's rows are stored in groups of
 // 4 (1 KB, one copy instruction) 1088 bytes apart, chunk c of row r at c ^ (r & 3), so that both reads
 // touch all banks.
+//
+// 8-bit pages: an e4m3 number times a power of two is a 16-bit number exactly (four significant bits), so
+// rows are turned into 16-bit ones on the way, two numbers and their power by one instruction, and the
+// products are those of 16-bit pages. Copies go through registers: a wave turns its share of a tile into
+// LDS rows while the next tile's loads are in flight. Few rows take keys as the matrix operand straight
+// from memory (a lane holds a key's numbers in memory's order, the queries follow it) and only the values,
+// which the product needs transposed, through LDS.
+//
+// Trees of new tokens: the tiles that reach past the cached rows read, for every row, the bits of the
+// tokens on its path (paged_tree_kernel) instead of comparing places.
 #include <climits>
 
 #include "../../include/varlen_attn.h"
@@ -254,6 +264,56 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
 }
 
 // ------------------------------------------------------------------------------------------------
+// trees
+// ------------------------------------------------------------------------------------------------
+// A work-group per sequence: the paths of its new tokens by doubling (after round r a token knows the 2^r
+// next ones on its way to the root, and the one behind them), in LDS; the other work-groups mark the
+// padding rows. Bounded by its launch and the rounds' barriers.
+static_assert(PT == kTreeTokens, "a thread per token");
+__global__ __launch_bounds__(PT) void paged_tree_kernel(PagedTreeArgs a) {
+  __shared__ uint32_t s_path[PT][kTreeWords + 1];
+  __shared__ int s_next[PT];
+  const int tid = threadIdx.x, s = blockIdx.x;
+  int32_t* positions = a.tree + tree_positions(a.n_tokens);
+  if (s >= a.n_seqs) {
+    const int n = (s - a.n_seqs) * PT + tid;
+    if (n < a.n_tokens && n >= a.plan[a.n_seqs]) positions[n] = -1;
+    return;
+  }
+  const int first = min(max(a.plan[s], 0), a.n_tokens), count = min(a.plan[s + 1], a.n_tokens) - first;
+  if (count <= 0) return;
+  const int32_t* pos = a.plan + a.layout.pos + first;
+  if (count > kTreeTokens) {
+    for (int j = tid; j < count; j += PT) positions[first + j] = pos[j];
+    return;
+  }
+  uint32_t path[kTreeWords];
+#pragma unroll
+  for (int w = 0; w < kTreeWords; ++w) path[w] = tid >> 5 == w ? 1u << (tid & 31) : 0u;
+  int next = tid < count ? a.parents[first + tid] : -1;
+  if (next < 0 || next >= tid) next = -1;
+  while (__syncthreads_or(next >= 0)) {  // (at most 8 rounds: a parent comes before its token)
+#pragma unroll
+    for (int w = 0; w < kTreeWords; ++w) s_path[tid][w] = path[w];
+    s_next[tid] = next;
+    __syncthreads();
+    if (next >= 0) {
+#pragma unroll
+      for (int w = 0; w < kTreeWords; ++w) path[w] |= s_path[next][w];
+      next = s_next[next];
+    }
+  }
+  if (tid >= count) return;
+  int depth = -1;
+#pragma unroll
+  for (int w = 0; w < kTreeWords; ++w) depth += __builtin_popcount(path[w]);
+  u32x4* words = reinterpret_cast<u32x4*>(a.tree + (long)(first + tid) * kTreeWords);
+  words[0] = u32x4{path[0], path[1], path[2], path[3]};
+  words[1] = u32x4{path[4], path[5], path[6], path[7]};
+  positions[first + tid] = pos[0] + depth;
+}
+
+// ------------------------------------------------------------------------------------------------
 // attention
 // ------------------------------------------------------------------------------------------------
 constexpr int D = kHeadDim;
@@ -347,18 +407,75 @@ __device__ inline void scores(const lds_u16* kb, const Offsets& o, const u32x4 (
   }
 }
 
-// Mask (keys past `lim` of the tile), running maximum and sum, weights of one tile. The maximum moves
-// when some row's tile maximum exceeds its own by more than 2^margin.
-template <class E, int BLOCKS>
-__device__ inline void soften(f32x16 (&s)[BLOCKS], bool mask, int lim, int hi, float scale_log2,
-                              float margin, State& st, u32x4 (&pf)[BLOCKS][2]) {
-  if (mask) {
+// What a row sees of a tile's keys: those up to `lim` of the tile, or, with a tree, the ones whose bits are
+// set in the words of its path. Key k of the cache is new token k - pos0; earlier keys are seen by all.
+struct Chain {
+  int lim;
+  template <int BLOCKS>
+  __device__ inline void hide(f32x16 (&s)[BLOCKS], int hi) const {
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
       for (int j = 0; j < 16; ++j)
         if (32 * b + reg_row(j, hi) > lim) s[b][j] = -INFINITY;
   }
+};
+struct Path {
+  const uint32_t* words;  // the row's (null: the sequence's new tokens are a chain)
+  int first;              // number of the tile's first key among the new tokens
+  int lim;
+  // keys o to o + 31 by number (o the same in all lanes)
+  __device__ inline uint32_t bits(int o) const {
+    if (o <= -32) return ~0u;
+    if (o < 0) return words[0] << -o | ((1u << -o) - 1);
+    const int w = o >> 5;
+    const uint32_t lo = w < kTreeWords ? words[w] : 0u, up = w + 1 < kTreeWords ? words[w + 1] : 0u;
+    return __builtin_amdgcn_alignbit(up, lo, o & 31);
+  }
+  template <int BLOCKS>
+  __device__ inline void hide(f32x16 (&s)[BLOCKS], int hi) const {
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+      const int n = lim - 32 * b;
+      const uint32_t seen = words != nullptr ? bits(first + 32 * b)
+                            : n >= 31        ? ~0u
+                            : n < 0          ? 0u
+                                             : (2u << n) - 1;
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (!(seen >> reg_row(j, hi) & 1)) s[b][j] = -INFINITY;
+    }
+  }
+};
+// How an item's rows see its keys.
+template <bool TREE>
+struct Sight {
+  const uint32_t* words;  // of the lane's row
+  int lim, pos0, from;    // the row's last key; the cached rows; tiles that end behind `from` are masked
+  __device__ Sight(const PagedAttnArgs& a, const Item& it, int tok, int lim, int first_lim)
+      : words(nullptr), lim(lim), pos0(it.pos0), from(first_lim) {
+    if constexpr (TREE) {
+      if (scalar_count(a, it.seq) <= kTreeTokens) {
+        words = reinterpret_cast<const uint32_t*>(a.tree) + (long)(it.token0 + tok) * kTreeWords;
+        from = it.pos0 - 1;
+      }
+    }
+  }
+  __device__ static inline int scalar_count(const PagedAttnArgs& a, int seq) {
+    return __builtin_amdgcn_readfirstlane(a.plan[seq + 1] - a.plan[seq]);
+  }
+  __device__ inline auto of(int key) const {  // the tile from `key` on
+    if constexpr (TREE) return Path{words, key - pos0, lim - key};
+    else return Chain{lim - key};
+  }
+};
+
+// Mask, running maximum and sum, weights of one tile. The maximum moves when some row's tile maximum
+// exceeds its own by more than 2^margin.
+template <class E, int BLOCKS, class Seen>
+__device__ inline void soften(f32x16 (&s)[BLOCKS], bool mask, const Seen& seen, int hi, float scale_log2,
+                              float margin, State& st, u32x4 (&pf)[BLOCKS][2]) {
+  if (mask) seen.hide(s, hi);
   float mt = -INFINITY;
 #pragma unroll
   for (int b = 0; b < BLOCKS; ++b)
@@ -407,9 +524,9 @@ struct Head {
   uint64_t k, v;  // addresses of the head's rows in page 0
   uint32_t k_stride, v_stride, mask;
   int n_pages, end;  // the range's end
-  __device__ Head(const PagedAttnArgs& a, const Item& it, int head)
-      : k((uint64_t)a.k + ((uint64_t)(head << a.pool.page_shift) * (D * 2))),
-        v((uint64_t)a.v + ((uint64_t)(head << a.pool.page_shift) * (D * 2))),
+  __device__ Head(const PagedAttnArgs& a, const Item& it, int head, int row_bytes = D * 2)
+      : k((uint64_t)a.k + ((uint64_t)(head << a.pool.page_shift) * row_bytes)),
+        v((uint64_t)a.v + ((uint64_t)(head << a.pool.page_shift) * row_bytes)),
         k_stride(a.pool.k_stride), v_stride(a.pool.v_stride), mask((1u << a.pool.page_shift) - 1),
         n_pages(a.pool.n_pages), end(it.key_end) {}
   // The page of the row at `pos`; -1 where there is none, or the range has ended.
@@ -417,10 +534,21 @@ struct Head {
     const int p = pos < end ? table[pos >> shift] : -1;
     return (uint32_t)p < (uint32_t)n_pages ? p : -1;
   }
+  // 8-bit pages: where the row at `pos` of this page lies (of page 0 where there is none: what is read
+  // there is not used), and its power of two, as a float, from the exponent byte. (Bytes that no row was
+  // written with, behind a sequence's end, may be anything: 255 would be no number.)
+  __device__ inline const uint8_t* row8(uint64_t base, uint32_t stride, int page, int pos) const {
+    return reinterpret_cast<const uint8_t*>(base + (uint64_t)(uint32_t)max(page, 0) * stride +
+                                            ((uint32_t)pos & mask) * D);
+  }
+  __device__ inline uint32_t exp8(const uint8_t* base, uint32_t stride, int head, int shift, int page, int pos) const {
+    return base[(uint64_t)(uint32_t)max(page, 0) * stride + ((uint32_t)(head << shift) + ((uint32_t)pos & mask))];
+  }
   // The rows from `pos` on: the page's, up to 16 and up to the range's end; the others read as zeros.
+  template <int ROW = D * 2>
   __device__ inline void rows(int page, int pos, u32x4& rk, u32x4& rv) const {
-    const uint32_t in = ((uint32_t)pos & mask) * (D * 2), p = (uint32_t)max(page, 0);
-    const uint32_t bytes = page < 0 ? 0 : (uint32_t)min(end - pos, 16) * (D * 2);
+    const uint32_t in = ((uint32_t)pos & mask) * ROW, p = (uint32_t)max(page, 0);
+    const uint32_t bytes = page < 0 ? 0 : (uint32_t)min(end - pos, 16) * ROW;
     const uint64_t ak = k + (uint64_t)p * k_stride + in, av = v + (uint64_t)p * v_stride + in;
     rk = u32x4{(uint32_t)scalar((int)ak), (uint32_t)scalar((int)(ak >> 32)) & 0xffffu,
                (uint32_t)scalar((int)bytes), 0x00020000u};
@@ -442,90 +570,14 @@ struct RowMap {
   }
 };
 
+// The waves of a few-row tile meet.
 template <class E, int W>
-__device__ inline void few_rows(const PagedAttnArgs& a, const Item& it, lds_u16* smem, char* smem_raw) {
+__device__ inline void join_waves(const PagedAttnArgs& a, const Item& it, const RowMap& map, int head,
+                                  int n_rows, char* smem_raw, const State& st) {
   constexpr int NW = W;
-  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5, group = map.group;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int head = it.head & 0xffff, group = a.hq / a.hkv, n_rows = it.row_end - it.row;
-  const float scale_log2 = a.scale * kLog2e;
-  const RowMap map(it.row, group);
-  const Offsets off = offsets_of(lane);
-  const int32_t* table = a.pool.table + (long)it.seq * a.pool.table_width;
-  const int n_tiles = (it.key_end - it.key + 31) >> 5;
-
-  // This wave's rows: all waves hold the same queries.
-  u32x4 qf[8];
-  int my_lim = -1;
-  {
-    int tok, h;
-    map.at(l32, tok, h);
-    if (l32 < n_rows) my_lim = it.pos0 + tok;
-    const uint16_t* q = (const uint16_t*)a.q + ((long)(it.token0 + tok) * a.hq + head * group + h) * D;
-#pragma unroll
-    for (int kk = 0; kk < 8; ++kk) {
-      qf[kk] = u32x4{0u, 0u, 0u, 0u};
-      if (l32 < n_rows) qf[kk] = gload16(q + 16 * kk + 8 * hi);
-    }
-  }
-  // Page numbers of this wave's next 32 tiles, two per tile (16 rows each): lane 2 i + h holds half h.
-  const Head rows(a, it, head);
-  auto load_pages = [&](int t) {
-    return rows.page(table, a.pool.page_shift, it.key + 32 * (t + NW * (lane >> 1)) + 16 * (lane & 1));
-  };
-  const uint32_t kl = lds_addr(smem + wave * (TILE)), vl = lds_addr(smem + wave * TILE + TILE / 2);
-  const lds_u16* kb = smem + wave * TILE;
-  const lds_u16* vb = kb + TILE / 2;
-  const int c_row = lane >> 4, coff = (c_row * D + 8 * ((lane & 15) ^ c_row)) * 2;
-  auto copy = [&](const u32x4 (&from)[2], uint32_t dst) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        dma16_opaque(from[h], dst + (4 * h + j) * GRP * 2, coff + j * 4 * D * 2);
-  };
-  State st;
-  start(st);
-  int pages = 0, i = 0;  // i: this wave's tiles so far
-  u32x4 rk[2], rv[2];
-  auto locate = [&](int t, int n) {  // this wave's n-th tile, tile t of the item
-    if ((n & 31) == 0) pages = load_pages(t);
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      rows.rows(__builtin_amdgcn_readlane(pages, 2 * (n & 31) + h), it.key + 32 * t + 16 * h, rk[h], rv[h]);
-  };
-  if (wave < n_tiles) {
-    locate(wave, 0);
-    copy(rk, kl);
-    copy(rv, vl);
-  }
-#pragma unroll
-  for (int kk = 0; kk < 8; ++kk) settle(qf[kk]);
-  const int first_lim = it.pos0 + map.token;  // the first row's last key: keys past it need the mask
-  for (int t = wave; t < n_tiles; t += NW, ++i) {
-    const bool more = t + NW < n_tiles;
-    asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // this tile's K; its V (8 copies) may be in flight
-    f32x16 s[1];
-    scores<E, 1>(kb, off, qf, s);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K read: its place is free
-    if (more) {
-      locate(t + NW, i + 1);
-      copy(rk, kl);
-    }
-    const int kv0 = it.key + 32 * t;
-    u32x4 pf[1][2];
-    soften<E, 1>(s, kv0 + 31 > first_lim, my_lim - kv0, hi, scale_log2, 0.f, st, pf);
-    if (more) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // V; the next K in flight
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    u32x4 va[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) va[j] = read_v(vb, off, j);
-    weigh<E, 1>(vb, off, pf, va, st);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V read
-    if (more) copy(rv, vl);
-  }
-
-  // The waves meet: fp32 rows of 132 words per wave, then their maxima and sums.
+  // fp32 rows of 132 words per wave, then their maxima and sums
   constexpr int LT = D + 4;
   float* xo = reinterpret_cast<float*>(smem_raw);
   float* xs = xo + NW * 32 * LT;
@@ -586,7 +638,226 @@ __device__ inline void few_rows(const PagedAttnArgs& a, const Item& it, lds_u16*
                                    o[2 * e + 1][2] * inv, o[2 * e + 1][3] * inv));
 }
 
-template <class E, int W>
+template <class E, int W, bool TREE>
+__device__ inline void few_rows(const PagedAttnArgs& a, const Item& it, lds_u16* smem, char* smem_raw) {
+  constexpr int NW = W;
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int head = it.head & 0xffff, group = a.hq / a.hkv, n_rows = it.row_end - it.row;
+  const float scale_log2 = a.scale * kLog2e;
+  const RowMap map(it.row, group);
+  const Offsets off = offsets_of(lane);
+  const int32_t* table = a.pool.table + (long)it.seq * a.pool.table_width;
+  const int n_tiles = (it.key_end - it.key + 31) >> 5;
+
+  // This wave's rows: all waves hold the same queries.
+  u32x4 qf[8];
+  int my_lim = -1, my_tok = map.token;
+  {
+    int tok, h;
+    map.at(l32, tok, h);
+    if (l32 < n_rows) my_lim = it.pos0 + tok, my_tok = tok;
+    const uint16_t* q = (const uint16_t*)a.q + ((long)(it.token0 + tok) * a.hq + head * group + h) * D;
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) {
+      qf[kk] = u32x4{0u, 0u, 0u, 0u};
+      if (l32 < n_rows) qf[kk] = gload16(q + 16 * kk + 8 * hi);
+    }
+  }
+  // Page numbers of this wave's next 32 tiles, two per tile (16 rows each): lane 2 i + h holds half h.
+  const Head rows(a, it, head);
+  auto load_pages = [&](int t) {
+    return rows.page(table, a.pool.page_shift, it.key + 32 * (t + NW * (lane >> 1)) + 16 * (lane & 1));
+  };
+  const uint32_t kl = lds_addr(smem + wave * (TILE)), vl = lds_addr(smem + wave * TILE + TILE / 2);
+  const lds_u16* kb = smem + wave * TILE;
+  const lds_u16* vb = kb + TILE / 2;
+  const int c_row = lane >> 4, coff = (c_row * D + 8 * ((lane & 15) ^ c_row)) * 2;
+  auto copy = [&](const u32x4 (&from)[2], uint32_t dst) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        dma16_opaque(from[h], dst + (4 * h + j) * GRP * 2, coff + j * 4 * D * 2);
+  };
+  State st;
+  start(st);
+  int pages = 0, i = 0;  // i: this wave's tiles so far
+  u32x4 rk[2], rv[2];
+  auto locate = [&](int t, int n) {  // this wave's n-th tile, tile t of the item
+    if ((n & 31) == 0) pages = load_pages(t);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      rows.rows(__builtin_amdgcn_readlane(pages, 2 * (n & 31) + h), it.key + 32 * t + 16 * h, rk[h], rv[h]);
+  };
+  if (wave < n_tiles) {
+    locate(wave, 0);
+    copy(rk, kl);
+    copy(rv, vl);
+  }
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) settle(qf[kk]);
+  const Sight<TREE> sight(a, it, my_tok, my_lim, it.pos0 + map.token);  // (the first row's last key)
+  for (int t = wave; t < n_tiles; t += NW, ++i) {
+    const bool more = t + NW < n_tiles;
+    asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // this tile's K; its V (8 copies) may be in flight
+    f32x16 s[1];
+    scores<E, 1>(kb, off, qf, s);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K read: its place is free
+    if (more) {
+      locate(t + NW, i + 1);
+      copy(rk, kl);
+    }
+    const int kv0 = it.key + 32 * t;
+    u32x4 pf[1][2];
+    soften<E, 1>(s, kv0 + 31 > sight.from, sight.of(kv0), hi, scale_log2, 0.f, st, pf);
+    if (more) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // V; the next K in flight
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    u32x4 va[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) va[j] = read_v(vb, off, j);
+    weigh<E, 1>(vb, off, pf, va, st);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V read
+    if (more) copy(rv, vl);
+  }
+
+  join_waves<E, W>(a, it, map, head, n_rows, smem_raw, st);
+}
+
+// 8-bit pages. Keys: lane (row, hi) of the operand loads its row's 16-byte pieces 2 i + hi, i = 0..3; piece
+// i serves two products, whose k slots 8 hi + 0..7 are then numbers 16 (2 i + hi) + 8 half + 0..7 of a row,
+// in the queries too. Values: 16 numbers of row 8 j + lane / 8 per lane and load, turned into 16-bit rows of
+// the wave's own LDS tile. A tile's loads are issued when the registers of the one before are free: keys
+// after its products, values after their rows are in LDS, so that 8 KB per wave are in flight but for the
+// conversions.
+template <class E>
+__device__ inline u32x4 numbers8(uint32_t lo, uint32_t hi, float power) {
+  return u32x4{E::from_e4m3(lo, power, false), E::from_e4m3(lo, power, true),
+               E::from_e4m3(hi, power, false), E::from_e4m3(hi, power, true)};
+}
+__device__ inline float power_of(uint32_t byte) {
+  return __builtin_bit_cast(float, min(byte, 254u) << 23);
+}
+__device__ inline float from_lane(int lane, float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(4 * lane, __builtin_bit_cast(int, x)));
+}
+
+template <class E, int W, bool TREE>
+__device__ inline void few_rows8(const PagedAttnArgs& a, const Item& it, lds_u16* smem, char* smem_raw) {
+  constexpr int NW = W;
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int head = it.head & 0xffff, group = a.hq / a.hkv, n_rows = it.row_end - it.row;
+  const int shift = a.pool.page_shift;
+  const float scale_log2 = a.scale * kLog2e;
+  const RowMap map(it.row, group);
+  const Offsets off = offsets_of(lane);
+  const int32_t* table = a.pool.table + (long)it.seq * a.pool.table_width;
+  const int n_tiles = (it.key_end - it.key + 31) >> 5;
+
+  u32x4 qf[8];
+  int my_lim = -1, my_tok = map.token;
+  {
+    int tok, h;
+    map.at(l32, tok, h);
+    if (l32 < n_rows) my_lim = it.pos0 + tok, my_tok = tok;
+    const uint16_t* q = (const uint16_t*)a.q + ((long)(it.token0 + tok) * a.hq + head * group + h) * D;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      qf[i] = u32x4{0u, 0u, 0u, 0u};
+      if (l32 < n_rows) qf[i] = gload16(q + 16 * (2 * (i >> 1) + hi) + 8 * (i & 1));
+    }
+  }
+  const Head rows(a, it, head, D);
+  int pages = 0;
+  auto load_pages = [&](int t) {
+    return rows.page(table, shift, it.key + 32 * (t + NW * (lane >> 1)) + 16 * (lane & 1));
+  };
+  const int k_row = perm32(l32);
+  lds_u16* const vt = smem + wave * (TILE / 2);
+  // this lane's rows of the value tile: row 8 j + lane / 8, numbers 16 m .. 16 m + 15
+  const int v_row = lane >> 3, m = lane & 7;
+  const Sight<TREE> sight(a, it, my_tok, my_lim, it.pos0 + map.token);
+  State st;
+  start(st);
+
+  u32x4 kr[4], vr[4];
+  uint32_t ke = 0, ve = 0;
+  int pg[2] = {-1, -1};  // pages of the tile whose keys are in flight, and of the one whose values are
+  auto locate = [&](int t, int n) {  // this wave's n-th tile, tile t of the item
+    if ((n & 31) == 0) pages = load_pages(t);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) pg[h] = __builtin_amdgcn_readlane(pages, 2 * (n & 31) + h);
+  };
+  auto fetch_keys = [&](int t) {
+    const int pos = it.key + 32 * t;
+    const uint8_t* p0 = rows.row8(rows.k, rows.k_stride, pg[0], pos);
+    const uint8_t* p1 = rows.row8(rows.k, rows.k_stride, pg[1], pos + 16);
+    const uint8_t* p = (k_row < 16 ? p0 : p1) + (k_row & 15) * D + 16 * hi;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) kr[i] = *reinterpret_cast<const u32x4*>(p + 32 * i);
+    ke = rows.exp8(a.pool.k_exp, a.pool.k_exp_stride, head, shift, k_row < 16 ? pg[0] : pg[1], pos + k_row);
+  };
+  auto fetch_values = [&](int t) {
+    const int pos = it.key + 32 * t;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      u32x4 rk, rv;
+      rows.rows<D>(pg[h], pos + 16 * h, rk, rv);
+      const brsrc r = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)((uint64_t)rv[0] | (uint64_t)rv[1] << 32), (short)0, (int)rv[2], 0x00020000);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) vr[2 * h + j] = bload16(r, 16 * lane + 1024 * j);
+    }
+    ve = rows.exp8(a.pool.v_exp, a.pool.v_exp_stride, head, shift, l32 < 16 ? pg[0] : pg[1], pos + l32);
+  };
+  int i = 0;  // this wave's tiles so far
+  if (wave < n_tiles) {
+    locate(wave, 0);
+    fetch_keys(wave);
+    fetch_values(wave);
+  }
+  for (int t = wave; t < n_tiles; t += NW, ++i) {
+    const bool more = t + NW < n_tiles;
+    const int kv0 = it.key + 32 * t;
+    f32x16 s[1] = {f32x16{}};
+    {
+      const float power = power_of(ke);
+      if ((pg[0] | pg[1]) < 0) {  // (rows that no page holds are zeros; those behind the end are not seen)
+        const bool gone = (k_row < 16 ? pg[0] : pg[1]) < 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) kr[j] = gone ? u32x4{0u, 0u, 0u, 0u} : kr[j];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        s[0] = E::mfma(numbers8<E>(kr[j >> 1][2 * (j & 1)], kr[j >> 1][2 * (j & 1) + 1], power), qf[j], s[0]);
+    }
+    if (more) {
+      locate(t + NW, i + 1);
+      fetch_keys(t + NW);
+    }
+    u32x4 pf[1][2];
+    soften<E, 1>(s, kv0 + 31 > sight.from, sight.of(kv0), hi, scale_log2, 0.f, st, pf);
+    const float power = power_of(ve);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = 8 * j + v_row;
+      const float f = from_lane(r, power);
+      lds_u16* row = vt + (r >> 2) * GRP + (r & 3) * D;
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        st128(row + 8 * ((2 * m + c) ^ (r & 3)), numbers8<E>(vr[j][2 * c], vr[j][2 * c + 1], f));
+    }
+    if (more) fetch_values(t + NW);
+    u32x4 va[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) va[j] = read_v(vt, off, j);
+    weigh<E, 1>(vt, off, pf, va, st);
+  }
+  join_waves<E, W>(a, it, map, head, n_rows, smem_raw, st);
+}
+
+template <class E, int W, bool P8, bool TREE>
 __device__ inline void many_rows(const PagedAttnArgs& a, const Item& it, lds_u16* smem) {
   using S = Shape<W>;
   constexpr int KEYS = 64, STAGE = 2 * TILE, STAGES = S::STAGES, BLOCKS = S::BLOCKS, GROUPS = S::GROUPS;
@@ -602,8 +873,52 @@ __device__ inline void many_rows(const PagedAttnArgs& a, const Item& it, lds_u16
 
   // Copies, in tile order: wave w moves 4 GROUPS rows of K and of V, which lie in one page; the page
   // numbers of its next 64 tiles are in its lanes.
-  const Head rows(a, it, head);
+  const Head rows(a, it, head, P8 ? D : D * 2);
   int pages = 0, tc = 0;
+  // 8-bit pages: a wave fetches 4 GROUPS rows of K and of V into registers (16 numbers of row 8 j + lane / 8
+  // per lane and load; the powers of K rows in lanes 0 to 15, of V rows in lanes 16 to 31) and places them
+  // as 16-bit rows in their stage.
+  constexpr int PIECES = 4 * GROUPS / 8;
+  u32x4 kr[PIECES], vr[PIECES];
+  uint32_t ex = 0;
+  int tp = 0;  // tiles placed
+  auto fetch_next = [&]() {
+    const int pos = it.key + 4 * GROUPS * wave + KEYS * tc, shift = a.pool.page_shift;
+    if ((tc & 63) == 0) pages = rows.page(table, shift, pos + KEYS * lane);
+    const int page = __builtin_amdgcn_readlane(pages, tc & 63);
+    u32x4 r[2];
+    rows.template rows<D>(page, pos, r[0], r[1]);
+    brsrc b[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      b[i] = __builtin_amdgcn_make_buffer_rsrc((void*)((uint64_t)r[i][0] | (uint64_t)r[i][1] << 32), (short)0,
+                                               (int)r[i][2], 0x00020000);
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) kr[j] = bload16(b[0], 16 * lane + 1024 * j);
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) vr[j] = bload16(b[1], 16 * lane + 1024 * j);
+    const bool is_v = lane & 16;
+    ex = rows.exp8(is_v ? a.pool.v_exp : a.pool.k_exp, is_v ? a.pool.v_exp_stride : a.pool.k_exp_stride, head,
+                   shift, page, pos + (lane & (4 * GROUPS - 1)));
+    ++tc;
+  };
+  auto place_next = [&]() {
+    const float power = power_of(ex);
+    lds_u16* const stage = smem + (tp & (STAGES - 1)) * STAGE + GROUPS * wave * GRP;
+    const int m = lane & 7;
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+      const int r = 8 * j + (lane >> 3);
+      const float fk = from_lane(r, power), fv = from_lane(16 + r, power);
+      lds_u16* row = stage + (r >> 2) * GRP + (r & 3) * D;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        st128(row + 8 * ((2 * m + c) ^ (r & 3)), numbers8<E>(kr[j][2 * c], kr[j][2 * c + 1], fk));
+        st128(row + TILE + 8 * ((2 * m + c) ^ (r & 3)), numbers8<E>(vr[j][2 * c], vr[j][2 * c + 1], fv));
+      }
+    }
+    ++tp;
+  };
   const int coff = (c_row * D + 8 * ((lane & 15) ^ c_row)) * 2;
   auto copy_next = [&]() {
     const int pos = it.key + 4 * GROUPS * wave + KEYS * tc;
@@ -632,7 +947,14 @@ __device__ inline void many_rows(const PagedAttnArgs& a, const Item& it, lds_u16
       dma16_opaque(rq, lds_addr(smem + STAGE + g * GRP), r < n_rows ? o : 0x7fffff00);
     }
   }
-  if (n_tiles > 0) copy_next();
+  if constexpr (P8) {
+    if (n_tiles > 0) {
+      fetch_next();
+      place_next();
+    }
+  } else {
+    if (n_tiles > 0) copy_next();
+  }
   wait_vmcnt<0>();
   __syncthreads();
   u32x4 qf[8];
@@ -645,9 +967,13 @@ __device__ inline void many_rows(const PagedAttnArgs& a, const Item& it, lds_u16
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk) settle(qf[kk]);
   __syncthreads();  // every wave holds its rows before the second stage is written
+  if constexpr (P8) {
+    if (1 < n_tiles) fetch_next();
+  } else {
 #pragma unroll
-  for (int t = 1; t < STAGES - 1; ++t)
-    if (t < n_tiles) copy_next();
+    for (int t = 1; t < STAGES - 1; ++t)
+      if (t < n_tiles) copy_next();
+  }
 
   int my_tok, my_h;
   map.at(32 * strip + l32, my_tok, my_h);
@@ -655,15 +981,27 @@ __device__ inline void many_rows(const PagedAttnArgs& a, const Item& it, lds_u16
   const int left = n_rows - 32 * strip;  // rows of this strip
   const int first_lim = __builtin_amdgcn_readfirstlane(my_lim);
   const int last_lim = __builtin_amdgcn_readlane(my_lim, max(0, min(31, left - 1)));
+  const Sight<TREE> sight(a, it, l32 < left ? my_tok : map.token, my_lim, first_lim);
   const int key0 = it.key + 32 * BLOCKS * half;  // this wave's keys of the first tile
   const int n_live = left <= 0 || last_lim < key0 ? 0 : min((last_lim - key0) / KEYS + 1, n_tiles);
   State st;
   start(st);
   // This wave's copies of tile t + 1 have landed; those of the tiles behind it stay in flight.
   auto next = [&](int t) {
-    if (t + STAGES - 1 < n_tiles) wait_vmcnt<(STAGES - 2) * 2 * GROUPS>();
+    if constexpr (P8) {
+    } else if (t + STAGES - 1 < n_tiles) wait_vmcnt<(STAGES - 2) * 2 * GROUPS>();
     else wait_vmcnt<0>();
     __syncthreads();
+  };
+  // While tile t is worked on: the copies of the tile STAGES - 1 behind it begin, or (8-bit) tile t + 1 is
+  // placed, in the stage that no wave has read since a barrier, and tile t + 2 fetched.
+  auto advance = [&](int t) {
+    if constexpr (P8) {
+      if (t + 1 < n_tiles) place_next();
+      if (t + 2 < n_tiles) fetch_next();
+    } else {
+      if (t + STAGES - 1 < n_tiles) copy_next();
+    }
   };
   int t = 0;
   for (; t < n_live; ++t) {
@@ -674,12 +1012,12 @@ __device__ inline void many_rows(const PagedAttnArgs& a, const Item& it, lds_u16
     __builtin_amdgcn_s_setprio(1);
     scores<E, BLOCKS>(kb, off, qf, s);
     __builtin_amdgcn_s_setprio(0);
-    if (t + STAGES - 1 < n_tiles) copy_next();
+    advance(t);
     u32x4 va[4], pf[BLOCKS][2];
 #pragma unroll
     for (int j = 0; j < 4; ++j) va[j] = read_v(kb + TILE, off, j);
     const int kv0 = key0 + KEYS * t;
-    soften<E, BLOCKS>(s, kv0 + 32 * BLOCKS - 1 > first_lim, my_lim - kv0, hi, scale_log2,
+    soften<E, BLOCKS>(s, kv0 + 32 * BLOCKS - 1 > sight.from, sight.of(kv0), hi, scale_log2,
                       kRescaleLog2, st, pf);
     __builtin_amdgcn_s_setprio(1);
     weigh<E, BLOCKS>(kb + TILE, off, pf, va, st);
@@ -687,7 +1025,7 @@ __device__ inline void many_rows(const PagedAttnArgs& a, const Item& it, lds_u16
     next(t);
   }
   for (; t < n_tiles; ++t) {  // past this strip's keys the wave only copies
-    if (t + STAGES - 1 < n_tiles) copy_next();
+    advance(t);
     next(t);
   }
 
@@ -787,7 +1125,7 @@ __device__ inline bool inside(const PagedAttnArgs& a, const Merge& m) {
          m.part_row + (m.parts - 1) * (long)m.stride + m.rows <= a.layout.max_part_rows;
 }
 
-template <class E, int W>
+template <class E, int W, bool P8 = false, bool TREE = false>
 __global__ __launch_bounds__(Shape<W>::THREADS, 2) void paged_attn_kernel(PagedAttnArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t smem_raw[Shape<W>::LDS];
   lds_u16* smem = (lds_u16*)smem_raw;
@@ -800,9 +1138,10 @@ __global__ __launch_bounds__(Shape<W>::THREADS, 2) void paged_attn_kernel(PagedA
   const int kind = it.head >> 16;
   if (!inside(a, it, kind)) return;  // (the same in all threads)
   if (kind == kMany) {
-    many_rows<E, W>(a, it, smem);
+    many_rows<E, W, P8, TREE>(a, it, smem);
   } else if (kind == kFew) {
-    few_rows<E, W>(a, it, smem, (char*)smem_raw);
+    if constexpr (P8) few_rows8<E, W, TREE>(a, it, smem, (char*)smem_raw);
+    else few_rows<E, W, TREE>(a, it, smem, (char*)smem_raw);
   } else if (kind == kPad) {
     u32x4* out = (u32x4*)a.out + (long)it.row * a.hq * (D / 8);
     const int chunks = (it.row_end - it.row) * a.hq * (D / 8);
@@ -903,9 +1242,22 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a) {
   }
 }
 
-template <class E>
+// A pool without pages: every key and value is zero, and so is every row.
+__global__ __launch_bounds__(256) void paged_zero_kernel(u32x4* out, long chunks) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i < chunks) out[i] = u32x4{0u, 0u, 0u, 0u};
+}
+
+template <class E, bool P8, bool TREE>
 hipError_t launch_attention(const PagedAttnArgs& a) {
-  const auto kernel = a.layout.wide ? paged_attn_kernel<E, 8> : paged_attn_kernel<E, 4>;
+  if (P8 && a.pool.n_pages == 0) {
+    const long chunks = (long)a.n_tokens * a.hq * (D / 8);
+    hipLaunchKernelGGL(paged_zero_kernel, dim3((unsigned)((chunks + 255) / 256)), dim3(256), 0, a.stream,
+                       (u32x4*)a.out, chunks);
+    return hipGetLastError();
+  }
+  const auto kernel =
+      a.layout.wide ? paged_attn_kernel<E, 8, P8, TREE> : paged_attn_kernel<E, 4, P8, TREE>;
   const int threads = a.layout.wide ? Shape<8>::THREADS : Shape<4>::THREADS;
   hipLaunchKernelGGL(kernel, dim3((unsigned)a.layout.max_items), dim3(threads), 0, a.stream, a);
   if (a.layout.max_merges > 0) {
@@ -913,6 +1265,12 @@ hipError_t launch_attention(const PagedAttnArgs& a) {
     hipLaunchKernelGGL(paged_merge_kernel<E>, dim3(groups), dim3(256), 0, a.stream, a);
   }
   return hipGetLastError();
+}
+template <class E>
+hipError_t launch_attention(const PagedAttnArgs& a) {
+  if (a.pool.k_exp != nullptr || a.pool.k_exp_stride != 0)  // (a pool without pages may have no address)
+    return a.tree == nullptr ? launch_attention<E, true, false>(a) : launch_attention<E, true, true>(a);
+  return a.tree == nullptr ? launch_attention<E, false, false>(a) : launch_attention<E, false, true>(a);
 }
 
 }  // namespace
@@ -925,6 +1283,11 @@ hipError_t launch_paged_plan(const PagedPlanArgs& a) {
                       : a.n_seqs <= 4 * PT ? paged_plan_kernel<4>
                                            : paged_plan_kernel<kPagedMaxSeqs / PT>;
   hipLaunchKernelGGL(kernel, dim3(2 * writers + placers), dim3(PT), 0, a.stream, a, writers);
+  return hipGetLastError();
+}
+
+hipError_t launch_paged_tree(const PagedTreeArgs& a) {
+  hipLaunchKernelGGL(paged_tree_kernel, dim3(a.n_seqs + (a.n_tokens + PT - 1) / PT), dim3(PT), 0, a.stream, a);
   return hipGetLastError();
 }
 

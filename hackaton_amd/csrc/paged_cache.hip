@@ -269,7 +269,7 @@ __global__ __launch_bounds__(T) void remap_finish_kernel(PagesArgs a) {
   }
   if (failed) return;
   const long units = (long)sc.totals[kCopies] * a.outer;
-  const int ps = 1 << a.page_shift, row_chunks = kHeadDim / 8;
+  const int ps = 1 << a.page_shift, row_chunks = a.row_chunks;
   const long page_chunks = (long)a.kv_heads * ps * row_chunks;
   u32x4* pages = (u32x4*)a.pages;
   for (long u = blockIdx.x - a.n_slots; u < units; u += kCopyGroups) {
@@ -283,6 +283,15 @@ __global__ __launch_bounds__(T) void remap_finish_kernel(PagesArgs a) {
     for (int i = tid; i < run * a.kv_heads; i += T) {
       const int at = i / run * (ps * row_chunks) + i % run;
       to[at] = from[at];
+    }
+    if (a.exps != nullptr) {  // (a byte per row)
+      const int rows = s.kept & (ps - 1);
+      const uint8_t* x = a.exps + (o * a.n_pages + src) * a.kv_heads * ps;
+      uint8_t* y = a.exps + (o * a.n_pages + dst) * a.kv_heads * ps;
+      for (int i = tid; i < rows * a.kv_heads; i += T) {
+        const int at = i / rows * ps + i % rows;
+        y[at] = x[at];
+      }
     }
   }
 }
@@ -362,7 +371,8 @@ __global__ __launch_bounds__(T) void compact_move_kernel(PagesArgs a, int count_
     a.refs_out[p] = p >= n_live ? 0 : own > 0 ? own : a.refs[mv.other[p]];
     return;
   }
-  const long page_chunks = (long)a.kv_heads * (kHeadDim / 8) << a.page_shift;
+  const long page_chunks = (long)a.kv_heads * a.row_chunks << a.page_shift;
+  const long page_exps = (long)a.kv_heads << a.page_shift;  // (a multiple of 16)
   u32x4* pages = (u32x4*)a.pages;
   const long units = (long)moves * a.outer;
   for (long u = blockIdx.x - a.n_slots - count_groups; u < units; u += kCopyGroups) {
@@ -371,10 +381,122 @@ __global__ __launch_bounds__(T) void compact_move_kernel(PagesArgs a, int count_
     const u32x4* x = pages + (layer + src) * page_chunks;
     u32x4* y = pages + (layer + mv.other[src]) * page_chunks;
     for (long i = tid; i < page_chunks; i += T) y[i] = x[i];
+    if (a.exps != nullptr) {
+      const u32x4* from = reinterpret_cast<const u32x4*>(a.exps + (layer + src) * page_exps);
+      u32x4* to = reinterpret_cast<u32x4*>(a.exps + (layer + mv.other[src]) * page_exps);
+      for (long i = tid; i < page_exps / 16; i += T) to[i] = from[i];
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// accepted paths: a work-group per sequence and (layer, keys or values). Token path[i] of the sequence's
+// new ones goes to place i behind the cached rows; path[i] >= i and ascending, so that rows read together
+// may be written together once all of them are in registers, front to back. Bounded by its launch for
+// the paths that drafted trees have (tens of rows of a few hundred bytes).
+// ------------------------------------------------------------------------------------------------
+constexpr int kAcceptLoads = 4;  // 16-byte pieces per thread between two barriers
+__global__ __launch_bounds__(T) void accept_kernel(PagedAcceptArgs a) {
+  __shared__ int s_path[kTreeTokens], s_page_of[2][kTreeTokens];
+  const int s = blockIdx.y, tid = threadIdx.x;
+  const long o = blockIdx.x;
+  int first = 0, count = 0;
+  if (a.n_tokens > 0) {
+    first = min(max(a.plan[s], 0), a.n_tokens);
+    count = max(min(a.plan[s + 1], a.n_tokens) - first, 0);
+  }
+  const int last = a.accepted[s];
+  const bool some = last >= 0 && last < count;
+  const bool chain = a.tree == nullptr || count > kTreeTokens;
+  int kept = !some ? 0 : last + 1, moved = 0;  // rows that stay; of them, those that are in place
+  if (some && !chain) {
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(a.tree) + (long)(first + last) * kTreeWords;
+    int before = 0;
+    kept = 0;
+#pragma unroll
+    for (int w = 0; w < kTreeWords; ++w) {
+      const uint32_t x = words[w];
+      const int mine = tid >> 5;
+      if (w < mine) before += __builtin_popcount(x);
+      if (w == mine) before += __builtin_popcount(x & ((1u << (tid & 31)) - 1));
+      kept += __builtin_popcount(x);
+    }
+    if (words[tid >> 5] >> (tid & 31) & 1) s_path[before] = tid;
+    // (a token is in place where all before it are on the path)
+    moved = kept;
+    for (int w = kTreeWords - 1; w >= 0; --w)
+      if (~words[w] != 0) moved = min(kept, 32 * w + __builtin_ctz(~words[w]));
+  }
+  if (tid == 0 && o == 0) {
+    const int had = a.lengths[s];
+    a.lengths_out[s] = count == 0 ? had : max(had - count, 0) + kept;
+  }
+  if (!some || chain || moved >= kept || o >= a.outer) return;  // (the same in all threads)
+  __syncthreads();
+  const int pos0 = a.plan[a.layout.pos + first], ps = 1 << a.page_shift;
+  if (tid < kept) {  // pages of the path's rows and of their new places
+    const int32_t* row = a.table + (long)s * a.width;
+    const int from = pos0 + s_path[tid], to = pos0 + tid;
+    const int x = from >= 0 && from >> a.page_shift < a.width ? row[from >> a.page_shift] : -1;
+    const int y = to >= 0 && to >> a.page_shift < a.width ? row[to >> a.page_shift] : -1;
+    s_page_of[0][tid] = x < a.n_pages ? x : -1;
+    s_page_of[1][tid] = y < a.n_pages ? y : -1;
+  }
+  __syncthreads();
+  u32x4* const pages = (u32x4*)a.pages + o * a.n_pages * a.kv_heads * ps * a.row_chunks;
+  const int per_row = a.kv_heads * a.row_chunks, pieces = (kept - moved) * per_row;
+  // piece i: chunk i % row_chunks of head i / row_chunks % kv_heads of the (i / per_row)-th row that moves
+  auto at = [&](int i, int side) -> long {
+    const int r = moved + i / per_row, in = i % per_row, page = s_page_of[side][r];
+    const int place = pos0 + (side == 0 ? s_path[r] : r);
+    if (page < 0) return -1;
+    return (((long)page * a.kv_heads + in / a.row_chunks) * ps + (place & (ps - 1))) * a.row_chunks +
+           in % a.row_chunks;
+  };
+  for (int base = 0; base < pieces; base += kAcceptLoads * T) {
+    u32x4 x[kAcceptLoads];
+    bool have[kAcceptLoads];
+#pragma unroll
+    for (int l = 0; l < kAcceptLoads; ++l) {
+      const int i = base + l * T + tid;
+      const long from = i < pieces ? at(i, 0) : -1;
+      have[l] = from >= 0;
+      if (have[l]) x[l] = pages[from];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int l = 0; l < kAcceptLoads; ++l) {
+      const long to = have[l] ? at(base + l * T + tid, 1) : -1;
+      if (to >= 0) pages[to] = x[l];
+    }
+    __syncthreads();
+  }
+  if (a.exps == nullptr) return;
+  uint8_t* const exps = a.exps + o * a.n_pages * a.kv_heads * ps;
+  const int bytes = (kept - moved) * a.kv_heads;
+  auto exp_at = [&](int i, int side) -> long {
+    const int r = moved + i / a.kv_heads, page = s_page_of[side][r];
+    const int place = pos0 + (side == 0 ? s_path[r] : r);
+    return page < 0 ? -1 : ((long)page * a.kv_heads + i % a.kv_heads) * ps + (place & (ps - 1));
+  };
+  for (int base = 0; base < bytes; base += T) {
+    const int i = base + tid;
+    const long from = i < bytes ? exp_at(i, 0) : -1;
+    const uint8_t x = from >= 0 ? exps[from] : 0;
+    __syncthreads();
+    const long to = from >= 0 ? exp_at(i, 1) : -1;
+    if (to >= 0) exps[to] = x;
+    __syncthreads();
   }
 }
 
 }  // namespace
+
+hipError_t launch_paged_accept(const PagedAcceptArgs& a) {
+  const bool moves = a.tree != nullptr && a.outer > 0 && a.n_pages > 0;
+  hipLaunchKernelGGL(accept_kernel, dim3(moves ? (unsigned)a.outer : 1, a.n_seqs), dim3(T), 0, a.stream, a);
+  return hipGetLastError();
+}
 
 hipError_t launch_pages_growth(const PagesGrowthArgs& a) {
   hipLaunchKernelGGL(growth_kernel, dim3(1), dim3(ST), 0, a.stream, a);

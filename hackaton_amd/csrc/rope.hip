@@ -284,12 +284,36 @@ __global__ __launch_bounds__(kRopeThreads) void rope_fwd_padded_kernel(RopeArgs 
 // A step's new rows into a paged cache: one wave per row, as above; q rows are written packed, k and v
 // rows where the page table says. A row without a place (padding, a position before the sequence,
 // past the tables or the table row, a page outside the pool) writes no key or value.
-template <int IN, int OUT>
+//
+// Rows of 8-bit pages (P8) are held as e4m3 numbers over a power of two of their own: the 8 lanes of a row
+// find its largest finite number by three exchanges in registers, divide by the power of two (exact), and
+// round once, to nearest even. The power is formed from the number's exponent and fraction alone.
+__device__ inline float max_of_8(float x) {
+  x = fmaxf(x, dpp_mov<0xb1>(x));   // quad_perm [1, 0, 3, 2]
+  x = fmaxf(x, dpp_mov<0x4e>(x));   // quad_perm [2, 3, 0, 1]
+  return fmaxf(x, dpp_mov<0x141>(x));  // row_half_mirror
+}
+// 8 numbers of a row whose power of two has 1 / power = inv: e4m3, what is not finite as not a number.
+__device__ inline u32x2 quantize8(const float (&x)[8], float inv) {
+  float y[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = __builtin_isfinite(x[e]) ? x[e] * inv : __builtin_nanf("");
+  u32x2 r;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * w], y[4 * w + 1], 0, false);
+    r[w] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * w + 2], y[4 * w + 3], lo, true);
+  }
+  return r;
+}
+
+template <int IN, int OUT, bool P8>
 __global__ __launch_bounds__(kRopeThreads) void rope_paged_kernel(PagedAppendArgs a) {
   const TokenLanes tl = token_lanes(a.n_tokens);
   if (!tl.valid) return;
-  const int c0 = 8 * tl.j, seq = a.seq[tl.pid], pos = a.pos[tl.pid];
-  const bool placed = seq >= 0 && seq < a.n_seqs && pos >= 0 && (a.cos_rows == 0 || pos < a.cos_rows);
+  const int c0 = 8 * tl.j, seq = a.seq[tl.pid], pos = a.pos[tl.pid], rot = a.rot[tl.pid];
+  const bool placed = seq >= 0 && seq < a.n_seqs && pos >= 0 && rot >= 0 &&
+                      (a.cos_rows == 0 || rot < a.cos_rows);
   int page = -1;
   const int at = pos >> a.pool.page_shift, ps = 1 << a.pool.page_shift;
   if (placed && at < a.pool.table_width)
@@ -297,7 +321,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_paged_kernel(PagedAppendArg
   const bool in_pool = page >= 0 && page < a.pool.n_pages;
   Tables tb;
   if (placed) {
-    const long cb = seq * a.cos_batch_stride + pos * a.cos_seq_stride + tl.pid * a.cos_token_stride;
+    const long cb = seq * a.cos_batch_stride + rot * a.cos_seq_stride + tl.pid * a.cos_token_stride;
     load_table8(a.cos, cb + c0, tb.cs1);
     load_table8(a.cos, cb + HALF + c0, tb.cs2);
     load_table8(a.sin, cb + c0, tb.sn1);
@@ -324,6 +348,33 @@ __global__ __launch_bounds__(kRopeThreads) void rope_paged_kernel(PagedAppendArg
       }
       y1[e] = r1;
       y2[e] = r2;
+    }
+    if constexpr (P8) {
+      const int size = (int)uniform(a.heads) * D;
+      if (is_q) {
+        store8<OUT>((gvoid)a.q_out, tl.pid * size + head * D + c0, y1);
+        store8<OUT>((gvoid)a.q_out, tl.pid * size + head * D + HALF + c0, y2);
+        continue;
+      }
+      float top = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        top = fmaxf(top, __builtin_isfinite(y1[e]) ? fabsf(y1[e]) : 0.f);
+        top = fmaxf(top, __builtin_isfinite(y2[e]) ? fabsf(y2[e]) : 0.f);
+      }
+      const uint32_t bits = __builtin_bit_cast(uint32_t, max_of_8(top));
+      // top = 1.f * 2^(E - 127) is at most 1.75 * 2^(8 + power): power = E - 135, one more past 1.75
+      const int exp = max((int)(bits >> 23) - 135 + ((bits & 0x7fffff) > 0x600000) + kExpBias, kExpMin);
+      const float inv = __builtin_bit_cast(float, (uint32_t)(2 * kExpBias - exp) << 23);
+      const long in_page = (long)head * ps + (pos & (ps - 1));
+      VA_GLOBAL uint8_t* codes = reinterpret_cast<VA_GLOBAL uint8_t*>(pick3(false, is_v, a.q_out, a.k_pages, a.v_pages));
+      VA_GLOBAL uint8_t* exps = reinterpret_cast<VA_GLOBAL uint8_t*>(pick3(false, is_v, a.q_out, a.pool.k_exp, a.pool.v_exp));
+      codes += page * (long)(is_v ? uniform(a.pool.v_stride) : uniform(a.pool.k_stride)) + in_page * D + c0;
+      exps += page * (long)(is_v ? uniform(a.pool.v_exp_stride) : uniform(a.pool.k_exp_stride)) + in_page;
+      *reinterpret_cast<VA_GLOBAL u32x2*>(codes) = quantize8(y1, inv);
+      *reinterpret_cast<VA_GLOBAL u32x2*>(codes + HALF) = quantize8(y2, inv);
+      if (tl.j == 0) *exps = (uint8_t)exp;
+      continue;
     }
     const gvoid y = pick3(is_q, is_v, a.q_out, a.k_pages, a.v_pages);
     const long stride = (is_v ? uniform(a.pool.v_stride) : uniform(a.pool.k_stride)) / 2;  // elements
@@ -529,16 +580,23 @@ hipError_t launch_rope(const RopeArgs& a, bool fwd) {
 hipError_t launch_rope_fwd(const RopeArgs& a) { return launch_rope(a, true); }
 hipError_t launch_rope_bwd(const RopeArgs& a) { return launch_rope(a, false); }
 
-hipError_t launch_paged_append(const PagedAppendArgs& a) {
+template <int IN, int OUT>
+static void append_rows(const PagedAppendArgs& a) {
   const dim3 grid((unsigned)((a.n_tokens + kTokensPerGroup - 1) / kTokensPerGroup));
   const auto kernel =
-      a.out_dtype == kF16 ? (a.in_dtype == kF16    ? rope_paged_kernel<kF16, kF16>
-                             : a.in_dtype == kBF16 ? rope_paged_kernel<kBF16, kF16>
-                                                   : rope_paged_kernel<kF32, kF16>)
-                          : (a.in_dtype == kF16    ? rope_paged_kernel<kF16, kBF16>
-                             : a.in_dtype == kBF16 ? rope_paged_kernel<kBF16, kBF16>
-                                                   : rope_paged_kernel<kF32, kBF16>);
+      a.pool.k_exp != nullptr ? rope_paged_kernel<IN, OUT, true> : rope_paged_kernel<IN, OUT, false>;
   hipLaunchKernelGGL(kernel, grid, dim3(kRopeThreads), 0, a.stream, a);
+}
+
+hipError_t launch_paged_append(const PagedAppendArgs& a) {
+  const auto run =
+      a.out_dtype == kF16 ? (a.in_dtype == kF16    ? append_rows<kF16, kF16>
+                             : a.in_dtype == kBF16 ? append_rows<kBF16, kF16>
+                                                   : append_rows<kF32, kF16>)
+                          : (a.in_dtype == kF16    ? append_rows<kF16, kBF16>
+                             : a.in_dtype == kBF16 ? append_rows<kBF16, kBF16>
+                                                   : append_rows<kF32, kBF16>);
+  run(a);
   return hipGetLastError();
 }
 

@@ -33,6 +33,11 @@ struct F16 {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
+  // Two e4m3 numbers of x (the lower or the upper two) times a power of two, as two 16-bit ones.
+  __device__ static inline uint32_t from_e4m3(uint32_t x, float power, bool upper) {
+    return __builtin_bit_cast(uint32_t, upper ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, power, true)
+                                              : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, power, false));
+  }
   // acc + the two 16-bit values packed in x (v_dot2_f32_f16 with (1, 1)).
   __device__ static inline float sum2(uint32_t x, float acc) {
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, x), f16x2_t{1, 1}, acc, false);
@@ -55,6 +60,11 @@ struct BF16 {
   __device__ static inline f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  // Two e4m3 numbers of x (the lower or the upper two) times a power of two, as two 16-bit ones.
+  __device__ static inline uint32_t from_e4m3(uint32_t x, float power, bool upper) {
+    return __builtin_bit_cast(uint32_t, upper ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, power, true)
+                                              : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, power, false));
   }
   // acc + the two 16-bit values packed in x (v_dot2_f32_bf16 with (1, 1)).
   __device__ static inline float sum2(uint32_t x, float acc) {

@@ -92,13 +92,37 @@ struct PagedPlanArgs {
   hipStream_t stream;
 };
 
-// Pages of one layer.
+// Pages of one layer. 8-bit pages have a byte per row beside them, the exponent of its power of two.
 struct PagedPool {
   const int32_t* table;
   int table_width;
   int n_pages;
   int page_shift;               // log2 of page_size
   uint32_t k_stride, v_stride;  // bytes from page to page
+  uint8_t* k_exp;               // null: 16-bit pages
+  uint8_t* v_exp;
+  uint32_t k_exp_stride, v_exp_stride;
+};
+
+// Rows of 8-bit pages are e4m3 numbers (up to 448 = 1.75 * 2^8) times 2^(byte - 127), the smallest such
+// power that brings a row's largest finite number to 448 or less, from 2^-100 on (what is smaller than
+// 448 * 2^-100 loses digits; 16-bit floats end far above).
+constexpr int kExpBias = 127, kExpMin = 27;
+
+// A step's tree: eight words per row, bit i of which says that token i of the row's sequence (of its new
+// ones) lies on the row's path, itself included; then the position of every row, -1 for padding. The new
+// tokens of a sequence of more than kTreeTokens are a chain and their words are not read.
+constexpr int kTreeTokens = 256, kTreeWords = kTreeTokens / 32;
+constexpr int64_t tree_positions(int64_t n_tokens) { return n_tokens * kTreeWords; }
+inline int64_t tree_words(int64_t n_tokens) { return tree_positions(n_tokens) + up4(n_tokens); }
+
+struct PagedTreeArgs {
+  const int32_t* plan;
+  PagedLayout layout;
+  const int32_t* parents;
+  int n_seqs, n_tokens;
+  int32_t* tree;
+  hipStream_t stream;
 };
 
 struct PagedAttnArgs {
@@ -116,6 +140,7 @@ struct PagedAttnArgs {
   void* out;
   float* workspace;
   hipStream_t stream;
+  const int32_t* tree;  // null: the new tokens of every sequence are a chain
 };
 
 struct PagedAppendArgs {
@@ -126,8 +151,9 @@ struct PagedAppendArgs {
   const float* sin;
   int64_t cos_batch_stride, cos_seq_stride, cos_token_stride;
   int64_t cos_rows;  // 0: positions are not bounded by the tables
-  const int32_t* seq;  // plan: sequence and position of every row
+  const int32_t* seq;  // plan: sequence and place of every row
   const int32_t* pos;
+  const int32_t* rot;  // the position that it is rotated by
   PagedPool pool;
   void* q_out;
   void* k_pages;
@@ -138,9 +164,12 @@ struct PagedAppendArgs {
   hipStream_t stream;
 };
 
-// Page bookkeeping: outer x n_pages x (kv_heads, page_size) rows of kHeadDim 16-bit elements.
+// Page bookkeeping: outer x n_pages x (kv_heads, page_size) rows of row_chunks times 16 bytes (kHeadDim
+// 16-bit elements, or 8-bit ones with an exponent byte per row in `exps`).
 struct PagesArgs {
   void* pages;
+  uint8_t* exps;  // null: 16-bit pages
+  int row_chunks;
   int64_t outer;
   int n_pages, kv_heads;
   int page_shift;
@@ -171,7 +200,27 @@ struct PagesGrowthArgs {
   hipStream_t stream;
 };
 
+// Rows of an accepted path: moved together behind the sequence's cached rows.
+struct PagedAcceptArgs {
+  const int32_t* plan;
+  PagedLayout layout;
+  const int32_t* tree;  // null: chains, nothing moves
+  const int32_t* table;
+  int n_seqs, n_tokens, width, page_shift;
+  void* pages;
+  uint8_t* exps;
+  int row_chunks;
+  int64_t outer;
+  int n_pages, kv_heads;
+  const int32_t* lengths;
+  const int32_t* accepted;
+  int32_t* lengths_out;
+  hipStream_t stream;
+};
+
 hipError_t launch_paged_plan(const PagedPlanArgs& a);
+hipError_t launch_paged_tree(const PagedTreeArgs& a);
+hipError_t launch_paged_accept(const PagedAcceptArgs& a);
 hipError_t launch_paged_attention(const PagedAttnArgs& a);
 hipError_t launch_paged_append(const PagedAppendArgs& a);
 hipError_t launch_pages_growth(const PagesGrowthArgs& a);

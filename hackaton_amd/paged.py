@@ -3,12 +3,14 @@ tokens of every sequence of a step are appended to pages and attend to them, one
 drafted ones or a prompt's chunk, all in one call. Hand-written gfx950 kernels through the C ABI; the
 reference trains only and has no counterpart.
 
-    paged_plan(page_table, q_lengths, kv_lengths, n_tokens, heads, kv_heads, page_size)
-    paged_append(q, k, v, cos, sin, k_pages, v_pages, plan)
+    paged_plan(page_table, q_lengths, kv_lengths, n_tokens, heads, kv_heads, page_size, tree)
+    paged_append(q, k, v, cos, sin, k_pages, v_pages, plan, dtype)
     paged_attention(query, k_pages, v_pages, plan, scale)
+    paged_accept(pages, plan, lengths, accepted)
     remap_pages(pages, table, lengths, refs, parents, new_lengths)
     compact_pages(pages, table, lengths, refs)
     PagedCache       a pool, its page tables and the calls above on them
+    QuantizedPages   pages in 8 bits, where these calls take pages
 
 Pages hold `page_size` rows (a power of two, 16 to 256) of every key/value head: one layer's keys are
 (n_pages, kv_heads, page_size, 128). Row t of a sequence lies in page `page_table[sequence, t //
@@ -19,6 +21,7 @@ has a backward or a forward-mode derivative; tensors that ask for one are refuse
 
 import ctypes
 import functools
+from typing import NamedTuple
 
 import torch
 from torch.autograd import forward_ad
@@ -28,6 +31,28 @@ from ._lib import check, lib
 from .attention import _DTYPES, HEAD_DIM, _attn_dtype, _rope_strides, _tables
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
+TREE_TOKENS = _lib.VA_TREE_TOKENS  # the most new tokens of a sequence that form a tree
+
+
+class QuantizedPages(NamedTuple):
+    """Pages in 8 bits: `codes` (..., n_pages, kv_heads, page_size, 128) float8_e4m3fn and `exponents`
+    (..., n_pages, kv_heads, page_size) float8_e8m0fnu. A row's values are its codes times its power of
+    two, the smallest from 2^-100 on that brings the row's largest finite number to 448 or less; numbers
+    are rounded once, to nearest even, and what is not finite is held as not a number. A row takes 129
+    bytes instead of 256. One layer's keys or values for `paged_append` and `paged_attention`, the whole
+    pool (layers, 2, ...) for the page bookkeeping."""
+
+    codes: torch.Tensor
+    exponents: torch.Tensor
+
+    def dequantize(self, dtype=torch.float32):
+        """The values, as one tensor of another type."""
+        return (self.codes.float() * self.exponents.float()[..., None]).to(dtype)
+
+
+def _split(pages):
+    """(pages or codes, exponents or None)."""
+    return pages if isinstance(pages, QuantizedPages) else (pages, None)
 
 
 def _no_grad(*tensors):
@@ -127,7 +152,7 @@ class PagedPlan:
 
     __slots__ = ("page_table", "words", "n_tokens", "n_seqs", "heads", "kv_heads", "page_size",
                  "workspace_bytes", "_step", "_page", "_strides", "_stream",
-                 "_capture")
+                 "_capture", "_tree", "_paths")
 
     def _rows(self, which):
         rows = -(-self.n_tokens // 4) * 4
@@ -141,7 +166,17 @@ class PagedPlan:
 
     @property
     def positions(self):
-        """(n_tokens) int32: the position of every row in its sequence, -1 for padding."""
+        """(n_tokens) int32: the position of every row in its sequence, -1 for padding. With a tree:
+        the tokens that come before it, cached ones and those on its path."""
+        if self._tree is None:
+            return self._rows(1)
+        at = self.n_tokens * (TREE_TOKENS // 32)
+        return self._paths[at:at + self.n_tokens]
+
+    @property
+    def places(self):
+        """(n_tokens) int32: where every row lies in its sequence's pages, -1 for padding: its position,
+        but for the tokens of a tree, which lie in the order of the rows."""
         return self._rows(1)
 
     def _use(self):
@@ -157,21 +192,62 @@ class PagedPlan:
             current = torch.cuda.current_stream()
             self.words.record_stream(current)
             self.page_table.record_stream(current)
+            if self._paths is not None:
+                self._paths.record_stream(current)
         return stream
 
 
-def paged_plan(page_table, q_lengths, kv_lengths, n_tokens, heads, kv_heads, page_size):
+def _parents(tree, q_lengths, n_tokens, device):
+    """A step's tree as (n_tokens) int32 on the device, from such a tensor or from a host list."""
+    if isinstance(tree, torch.Tensor):
+        if tree.device != device:
+            raise ValueError(f"tree on {tree.device}, page_table on {device}")
+        _int32("tree", tree, n_tokens)
+        return tree
+    tree = [int(x) for x in tree]
+    if len(tree) > n_tokens:
+        raise ValueError(f"a tree of {len(tree)} rows, the step has {n_tokens}")
+    if not isinstance(q_lengths, torch.Tensor):
+        at = 0
+        for count in (int(x) for x in q_lengths):
+            rows, at = tree[at:at + count], at + count
+            if len(rows) < count:
+                raise ValueError(f"a tree of {len(tree)} rows for {sum(map(int, q_lengths))} new tokens")
+            if any(p >= j for j, p in enumerate(rows)):
+                raise ValueError("a token of a tree follows an earlier one of its sequence, or none (-1)")
+            if count > TREE_TOKENS and any(p != j - 1 for j, p in enumerate(rows)):
+                raise ValueError(f"a tree of {count} tokens: at most {TREE_TOKENS} of a sequence form one")
+    out = torch.tensor(tree + [-1] * (n_tokens - len(tree)), dtype=torch.int64)
+    return out.clamp(-1, 2 ** 31 - 1).to(device=device, dtype=torch.int32)
+
+
+@functools.lru_cache(maxsize=256)
+def _tree_words(n_seqs, n_tokens, heads, kv_heads, page_size, width):
+    words = ctypes.c_int64()
+    step = _lib.PagedStep(None, None, n_tokens, n_seqs, width, page_size, heads, kv_heads)
+    check(lib().va_paged_tree_words(step, ctypes.byref(words)), "va_paged_tree_words")
+    return words.value
+
+
+def paged_plan(page_table, q_lengths, kv_lengths, n_tokens, heads, kv_heads, page_size, tree=None):
     """The plan of a step: `q_lengths[s]` new tokens of every sequence (packed rows, one sequence
     after the other, `n_tokens` rows in all; rows behind the last sequence are padding) and
     `kv_lengths[s]` cached tokens with the new ones included. Both are host lists or device tensors
     (for a captured step: device tensors); `page_table` is (sequences, pages per sequence) int32 on
     the GPU, at most 4096 sequences. Device lengths are not read back: negative ones count as 0, kv
-    lengths end with the table row, new tokens with the rows. One launch."""
+    lengths end with the table row, new tokens with the rows. One launch.
+
+    `tree`: the new tokens of a sequence form trees instead of following each other: of every row the
+    number, among its sequence's new tokens, of the earlier one that it follows, or -1 where it follows the
+    cached tokens directly; (n_tokens) int32 on the GPU or a host list. A row then sees the tokens cached
+    before the step, those on its path, and itself. At most 256 new tokens of a sequence form a tree; those
+    of a longer one follow each other whatever `tree` holds (host lists that say otherwise are refused,
+    device ones are not read; there, what names no earlier token counts as -1). Another launch."""
     device = _one_device(page_table)
     if device.index != _current_device():  # launches and allocations go to the tensors' device
         with torch.cuda.device(device):
             return paged_plan(page_table, q_lengths, kv_lengths, n_tokens, heads, kv_heads,
-                              page_size)
+                              page_size, tree)
     if page_table.dim() != 2:
         raise ValueError(f"page_table must be (sequences, pages), got {tuple(page_table.shape)}")
     n_seqs, width = page_table.shape
@@ -179,6 +255,7 @@ def paged_plan(page_table, q_lengths, kv_lengths, n_tokens, heads, kv_heads, pag
     page_size, n_tokens = _page_size(page_size), int(n_tokens)
     _check_host_lengths(q_lengths, kv_lengths, n_tokens, width * page_size)
     plan = PagedPlan()
+    parents = None if tree is None else _parents(tree, q_lengths, n_tokens, device)
     n_words, plan.workspace_bytes = _plan_sizes(n_seqs, n_tokens, heads, kv_heads, page_size, width)
     q_lengths = _lengths("q_lengths", q_lengths, n_seqs, device)
     kv_lengths = _lengths("kv_lengths", kv_lengths, n_seqs, device)
@@ -193,6 +270,13 @@ def paged_plan(page_table, q_lengths, kv_lengths, n_tokens, heads, kv_heads, pag
                                 page_size, heads, kv_heads)
     check(lib().va_paged_plan(plan._step, q_lengths.data_ptr(), kv_lengths.data_ptr(), n_words,
                               plan._stream), "va_paged_plan")
+    plan._tree = plan._paths = None
+    if parents is not None:
+        n_words = _tree_words(n_seqs, n_tokens, heads, kv_heads, page_size, width)
+        plan._paths = torch.empty(n_words, dtype=torch.int32, device=device)
+        plan._tree = plan._paths.data_ptr()
+        check(lib().va_paged_tree(plan._step, parents.data_ptr(), plan._tree, n_words, plan._stream),
+              "va_paged_tree")
     return plan
 
 
@@ -215,18 +299,52 @@ def _pages_of(k_pages, v_pages, plan):
     return k_stride[0], v_stride[0], shape[0]
 
 
-def paged_append(q, k, v, cos, sin, k_pages, v_pages, plan):
+def _exponents_of(pages, plan):
+    """Elements from one page's exponents to the next."""
+    codes, exponents = pages
+    if codes.dtype != torch.float8_e4m3fn or exponents.dtype != torch.float8_e8m0fnu:
+        raise ValueError("8-bit pages are float8_e4m3fn codes and float8_e8m0fnu exponents, got "
+                         f"{codes.dtype} and {exponents.dtype}")
+    if exponents.device != codes.device:
+        raise ValueError(f"tensors on {codes.device} and {exponents.device}")
+    shape, stride = exponents.shape, exponents.stride()
+    if shape != codes.shape[:-1]:
+        raise ValueError(f"exponents must be {tuple(codes.shape[:-1])}, got {tuple(shape)}")
+    if stride[2] != 1 or (stride[1] != plan.page_size and plan.kv_heads != 1):
+        raise ValueError(f"every page's exponents must be contiguous, got strides {stride}")
+    least = plan.kv_heads * plan.page_size
+    return max(stride[0], least) if shape[0] <= 1 else stride[0]
+
+
+def _layer(k_pages, v_pages, plan):
+    """va_paged_pages of one layer's keys and values, in 8 bits or in 16."""
+    if isinstance(k_pages, QuantizedPages) != isinstance(v_pages, QuantizedPages):
+        raise ValueError("keys and values must both be pages in 8 bits, or neither")
+    (k, k_exps), (v, v_exps) = _split(k_pages), _split(v_pages)
+    k_stride, v_stride, n_pages = _pages_of(k, v, plan)
+    if k_exps is None:
+        return _lib.PagedPages(k.data_ptr(), v.data_ptr(), None, None, k_stride, v_stride, 0, 0, n_pages,
+                               _attn_dtype(k))
+    return _lib.PagedPages(k.data_ptr(), v.data_ptr(), k_exps.data_ptr(), v_exps.data_ptr(), k_stride,
+                           v_stride, _exponents_of(k_pages, plan), _exponents_of(v_pages, plan), n_pages,
+                           _lib.VA_E4M3)
+
+
+def paged_append(q, k, v, cos, sin, k_pages, v_pages, plan, dtype=None):
     """The step's new rows: q (n_tokens, heads * 128), k and v (n_tokens, kv_heads * 128) projections
     in fp16, bf16 or fp32. Returns q rotated, (n_tokens, heads, 128) in the pages' type; k rotated and
     v go into `k_pages` / `v_pages` (n_pages, kv_heads, page_size, 128) at the rows' positions, rotated
     in fp32 and rounded once. cos / sin: (1 or sequences, T, 128) read by position, or (n_tokens, 128)
     read by row. Rows without a place (padding, positions past the tables or in no page) write
-    nothing; padding and positions outside the cos / sin table give zeros in q."""
-    device = _one_device(q, k, v, cos, sin, k_pages, v_pages, plan.words)
+    nothing; padding and positions outside the cos / sin table give zeros in q. Pages may be
+    `QuantizedPages`: keys, rotated, and values go into them in 8 bits. `dtype` is then q's, fp16 or bf16
+    (None: the projections' type, fp16 for fp32 ones)."""
+    keys, values = _split(k_pages)[0], _split(v_pages)[0]
+    device = _one_device(q, k, v, cos, sin, keys, values, plan.words)
     if device.index != _current_device():  # launches and allocations go to the tensors' device
         with torch.cuda.device(device):
-            return paged_append(q, k, v, cos, sin, k_pages, v_pages, plan)
-    _no_grad(q, k, v, k_pages, v_pages)
+            return paged_append(q, k, v, cos, sin, k_pages, v_pages, plan, dtype)
+    _no_grad(q, k, v, keys, values)
     if forward_ad._current_level >= 0:  # (the tables are constants, as in qkv_rotate)
         _no_tangent(cos, sin)
     n, heads, kv_heads = plan.n_tokens, plan.heads, plan.kv_heads
@@ -237,8 +355,16 @@ def paged_append(q, k, v, cos, sin, k_pages, v_pages, plan):
     if not (q.dtype == k.dtype == v.dtype) or q.dtype not in _DTYPES:
         raise ValueError(f"q, k and v must share a dtype (fp16, bf16 or fp32), got {q.dtype}, "
                          f"{k.dtype}, {v.dtype}")
-    out_dtype = _attn_dtype(k_pages)
-    k_stride, v_stride, n_pages = _pages_of(k_pages, v_pages, plan)
+    plain = plan._tree is None and keys is k_pages and values is v_pages  # 16 bits, no tree
+    if dtype is None:
+        dtype = keys.dtype if keys is k_pages else q.dtype if q.dtype != torch.float32 else torch.float16
+    elif dtype not in (torch.float16, torch.bfloat16) or (keys is k_pages and dtype != keys.dtype):
+        raise ValueError(f"queries in {dtype} over pages in {keys.dtype}")
+    if plain:
+        out_dtype = _attn_dtype(k_pages)
+        k_stride, v_stride, n_pages = _pages_of(k_pages, v_pages, plan)
+    else:
+        out_dtype, layer = _DTYPES[dtype], _layer(k_pages, v_pages, plan)
     by_row = cos.dim() == 2
     if by_row and (tuple(cos.shape) != (n, HEAD_DIM) or sin.shape != cos.shape):
         raise ValueError(f"cos/sin by row must be ({n}, {HEAD_DIM}), got {tuple(cos.shape)}, "
@@ -246,13 +372,20 @@ def paged_append(q, k, v, cos, sin, k_pages, v_pages, plan):
     cos, sin = _tables(cos[None] if by_row else cos, sin[None] if by_row else sin)
     if not by_row and cos.shape[0] not in (1, plan.n_seqs):
         raise ValueError(f"cos/sin for {cos.shape[0]} sequences, the plan has {plan.n_seqs}")
-    query = torch.empty((n, heads, HEAD_DIM), dtype=k_pages.dtype, device=device)
+    query = torch.empty((n, heads, HEAD_DIM), dtype=dtype, device=device)
     if n == 0:
         return query
     if cos.shape[1] == 0:
         raise ValueError("cos/sin hold no positions")
     batch, row = (0, 0) if by_row else _rope_strides(cos)
     q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    if not plain:
+        check(lib().va_paged_append_pages(
+            plan._step, plan._tree, q.data_ptr(), k.data_ptr(), v.data_ptr(), cos.data_ptr(),
+            sin.data_ptr(), batch, row, HEAD_DIM if by_row else 0, 0 if by_row else cos.shape[1],
+            query.data_ptr(), layer, HEAD_DIM, _DTYPES[q.dtype], out_dtype, plan._use()),
+            "va_paged_append_pages")
+        return query
     check(lib().va_paged_append(
         plan._step, q.data_ptr(), k.data_ptr(), v.data_ptr(), cos.data_ptr(), sin.data_ptr(), batch,
         row, HEAD_DIM if by_row else 0, 0 if by_row else cos.shape[1], query.data_ptr(),
@@ -268,26 +401,39 @@ def paged_attention(query, k_pages, v_pages, plan, scale):
     page holds behind its sequence's end is never read. (Keys that a row does not see never reach it,
     whatever they hold. Values that are infinite or not a number do where they lie in a 64-key tile that
     another of the 32 rows computed together sees, rows being pairs of a token and a query head of the
-    group: in rows of the same sequence up to 63 + ceil(31 kv_heads / heads) positions before their own.)
-    The same step gives the same bits; the same sequence in another step agrees to rounding."""
-    device = _one_device(query, k_pages, v_pages, plan.words)
+    group: in rows of the same sequence up to 63 + ceil(31 kv_heads / heads) positions before their own;
+    with a tree, places before or behind it: rows that do not see each other share tiles.)
+    The same step gives the same bits; the same sequence in another step agrees to rounding. Pages may be
+    `QuantizedPages`, under queries in fp16 or bf16: their values are multiplied as numbers of that type,
+    exactly but for what passes fp16's range."""
+    keys, values = _split(k_pages)[0], _split(v_pages)[0]
+    device = _one_device(query, keys, values, plan.words)
     if device.index != _current_device():  # launches and allocations go to the tensors' device
         with torch.cuda.device(device):
             return paged_attention(query, k_pages, v_pages, plan, scale)
-    _no_grad(query, k_pages, v_pages)
+    _no_grad(query, keys, values)
     dtype = _attn_dtype(query)
-    if k_pages.dtype != query.dtype:
-        raise ValueError(f"query in {query.dtype}, pages in {k_pages.dtype}")
+    if keys is k_pages and keys.dtype != query.dtype:
+        raise ValueError(f"query in {query.dtype}, pages in {keys.dtype}")
     n, heads = plan.n_tokens, plan.heads
     if query.shape != (n, heads, HEAD_DIM):
         raise ValueError(f"query must be ({n}, {heads}, {HEAD_DIM}), got {tuple(query.shape)}")
-    k_stride, v_stride, n_pages = _pages_of(k_pages, v_pages, plan)
+    plain = plan._tree is None and keys is k_pages and values is v_pages  # 16 bits, no tree
+    if plain:
+        k_stride, v_stride, n_pages = _pages_of(k_pages, v_pages, plan)
+    else:
+        layer = _layer(k_pages, v_pages, plan)
     query = query.contiguous()
     out = torch.empty((n, heads * HEAD_DIM), dtype=query.dtype, device=device)
     if n == 0:
         return out
     nbytes = plan.workspace_bytes
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    if not plain:
+        check(lib().va_paged_attention_pages(
+            plan._step, plan._tree, query.data_ptr(), layer, HEAD_DIM, scale, dtype, out.data_ptr(),
+            ws.data_ptr() if nbytes else None, nbytes, plan._use()), "va_paged_attention_pages")
+        return out
     check(lib().va_paged_attention(
         plan._step, query.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_stride, v_stride,
         n_pages, HEAD_DIM, scale, dtype, out.data_ptr(), ws.data_ptr() if nbytes else None, nbytes,
@@ -299,14 +445,31 @@ def paged_attention(query, k_pages, v_pages, plan, scale):
 # page bookkeeping
 # ------------------------------------------------------------------------------------------------
 def _pool_of(pages):
+    """(layers * 2, n_pages, kv_heads, page_size) of a whole pool."""
+    pages, exponents = _split(pages)
     shape = pages.shape
     if len(shape) != 6 or shape[1] != 2 or shape[5] != HEAD_DIM:
         raise ValueError(f"pages must be (layers, 2, n_pages, kv_heads, page_size, {HEAD_DIM}), got "
                          f"{tuple(shape)}")
     if not pages.is_contiguous():
         raise ValueError(f"pages must be contiguous, got strides {pages.stride()}")
-    _attn_dtype(pages)
+    if exponents is None:
+        _attn_dtype(pages)
+    elif pages.dtype != torch.float8_e4m3fn or exponents.dtype != torch.float8_e8m0fnu:
+        raise ValueError("8-bit pages are float8_e4m3fn codes and float8_e8m0fnu exponents, got "
+                         f"{pages.dtype} and {exponents.dtype}")
+    elif (exponents.shape != shape[:-1] or not exponents.is_contiguous()
+          or exponents.device != pages.device):
+        raise ValueError(f"exponents must be {tuple(shape[:-1])}, contiguous, on {pages.device}, got "
+                         f"{tuple(exponents.shape)}, strides {exponents.stride()} on {exponents.device}")
     return 2 * shape[0], shape[2], shape[3], _page_size(shape[4])
+
+
+def _pool_args(pages):
+    """(the library's suffix, the pool's addresses)."""
+    pages, exponents = _split(pages)
+    return ("", (pages.data_ptr(),)) if exponents is None else \
+        ("8", (pages.data_ptr(), exponents.data_ptr()))
 
 
 def _state_of(n_pages, table, lengths, refs, **more):
@@ -349,12 +512,12 @@ def remap_pages(pages, table, lengths, refs, parents=None, new_lengths=None):
     slot that ends in it if nobody else holds it, and the others get a copy of its filled rows, in
     every layer. Free pages are handed out in ascending order, slot after slot. shortfall (1): 0, or
     how many pages the pool or the table rows lack, in which case nothing changes."""
-    device = _one_device(pages, table, lengths, refs,
+    device = _one_device(_split(pages)[0], table, lengths, refs,
                          *(t for t in (parents, new_lengths) if t is not None))
     if device.index != _current_device():  # launches and allocations go to the tensors' device
         with torch.cuda.device(device):
             return remap_pages(pages, table, lengths, refs, parents, new_lengths)
-    _no_grad(pages)
+    _no_grad(_split(pages)[0])
     outer, n_pages, kv_heads, page_size = _pool_of(pages)
     slots, width = _state_of(n_pages, table, lengths, refs, parents=parents, new_lengths=new_lengths)
     table_out, lengths_out, refs_out = (torch.empty_like(table), torch.empty_like(lengths),
@@ -362,12 +525,13 @@ def remap_pages(pages, table, lengths, refs, parents=None, new_lengths=None):
     shortfall = torch.empty(1, dtype=torch.int32, device=device)
     words = _scratch_words(slots, n_pages)
     scratch = torch.empty(words, dtype=torch.int32, device=device)
-    check(lib().va_pages_remap(
-        pages.data_ptr(), outer, n_pages, kv_heads, page_size, HEAD_DIM, table.data_ptr(),
+    bits, pool = _pool_args(pages)
+    check(getattr(lib(), "va_pages_remap" + bits)(
+        *pool, outer, n_pages, kv_heads, page_size, HEAD_DIM, table.data_ptr(),
         lengths.data_ptr(), refs.data_ptr(), None if parents is None else parents.data_ptr(),
         None if new_lengths is None else new_lengths.data_ptr(), slots, width, table_out.data_ptr(),
         lengths_out.data_ptr(), refs_out.data_ptr(), shortfall.data_ptr(), scratch.data_ptr(), words,
-        _current_stream(device.index)), "va_pages_remap")
+        _current_stream(device.index)), "va_pages_remap" + bits)
     return table_out, lengths_out, refs_out, shortfall
 
 
@@ -376,29 +540,60 @@ def compact_pages(pages, table, lengths, refs):
     moves to the k-th free page below it, in every layer. Arguments as for `remap_pages`. Returns
     new (table, refs, live); live (1): how many pages are in use, all of them below that number. Pages
     that the program holds without a table row move too: a row of their own keeps track of them."""
-    device = _one_device(pages, table, lengths, refs)
+    device = _one_device(_split(pages)[0], table, lengths, refs)
     if device.index != _current_device():  # launches and allocations go to the tensors' device
         with torch.cuda.device(device):
             return compact_pages(pages, table, lengths, refs)
-    _no_grad(pages)
+    _no_grad(_split(pages)[0])
     outer, n_pages, kv_heads, page_size = _pool_of(pages)
     slots, width = _state_of(n_pages, table, lengths, refs)
     table_out, refs_out = torch.empty_like(table), torch.empty_like(refs)
     live = torch.empty(1, dtype=torch.int32, device=device)
     words = _scratch_words(slots, n_pages)
     scratch = torch.empty(words, dtype=torch.int32, device=device)
-    check(lib().va_pages_compact(
-        pages.data_ptr(), outer, n_pages, kv_heads, page_size, HEAD_DIM, table.data_ptr(),
+    bits, pool = _pool_args(pages)
+    check(getattr(lib(), "va_pages_compact" + bits)(
+        *pool, outer, n_pages, kv_heads, page_size, HEAD_DIM, table.data_ptr(),
         lengths.data_ptr(), refs.data_ptr(), slots, width, table_out.data_ptr(), refs_out.data_ptr(),
         live.data_ptr(), scratch.data_ptr(), words, _current_stream(device.index)),
-        "va_pages_compact")
+        "va_pages_compact" + bits)
     return table_out, refs_out, live
+
+
+def paged_accept(pages, plan, lengths, accepted):
+    """The end of a step whose new tokens were drafted: the tokens up to `accepted[s]` on its path stay.
+    pages: the whole pool, (layers, 2, n_pages, kv_heads, page_size, 128) or `QuantizedPages`; plan: the
+    step's, with its tree (or without: the tokens follow each other); lengths (sequences) int32: the cached
+    tokens, the new ones included; accepted (sequences) int32: the number of a new token of the sequence,
+    anything else: none stays. The rows that stay move together behind the tokens cached before, in order
+    and in every layer; rows behind them hold what they held or what moved over them. Returns the lengths
+    (sequences) int32; sequences without new tokens keep theirs. Pages past them are given back by
+    `remap_pages(pages, table, lengths, refs, None, new_lengths)` over the lengths of before the call."""
+    codes, exponents = _split(pages)
+    device = _one_device(codes, plan.words, lengths, accepted)
+    if device.index != _current_device():  # launches and allocations go to the tensors' device
+        with torch.cuda.device(device):
+            return paged_accept(pages, plan, lengths, accepted)
+    _no_grad(codes)
+    outer, n_pages, kv_heads, page_size = _pool_of(pages)
+    if (kv_heads, page_size) != (plan.kv_heads, plan.page_size):
+        raise ValueError(f"pages of {page_size} rows of {kv_heads} heads, the plan's have "
+                         f"{plan.page_size} of {plan.kv_heads}")
+    _int32("lengths", lengths, plan.n_seqs)
+    _int32("accepted", accepted, plan.n_seqs)
+    out = torch.empty_like(lengths)
+    check(lib().va_paged_accept(
+        plan._step, plan._tree, codes.data_ptr(), None if exponents is None else exponents.data_ptr(),
+        outer, n_pages, kv_heads, HEAD_DIM, lengths.data_ptr(), accepted.data_ptr(), out.data_ptr(),
+        plan._use()), "va_paged_accept")
+    return out
 
 
 class PagedCache:
     """Keys and values of `layers` layers in one pool of `n_pages` pages, and up to `slots` sequences
-    of at most `max_length` tokens (rounded up to whole pages) in it. State, all on the GPU: `pages`,
-    `table`, `lengths`, `refs`. Every call updates it in place on the current stream, so the calls of one
+    of at most `max_length` tokens (rounded up to whole pages) in it, in fp16, bf16 or, with
+    `dtype=torch.float8_e4m3fn`, in 8 bits (`QuantizedPages`). State, all on the GPU: `pages` (8 bits: the
+    codes, and `exponents`), `table`, `lengths`, `refs`. Every call updates it in place on the current stream, so the calls of one
     cache belong on one stream or in order across streams, and a captured step replays on the state it
     finds. A call that lacks pages (or a step that lacks rows) changes nothing; `check()` reports it."""
 
@@ -408,7 +603,11 @@ class PagedCache:
         width = -(-int(max_length) // self.page_size)
         self.pages = torch.empty(layers, 2, n_pages, kv_heads, page_size, HEAD_DIM, dtype=dtype,
                                  device=device)
-        _attn_dtype(self.pages)
+        self.exponents = None
+        if dtype == torch.float8_e4m3fn:
+            self.exponents = torch.empty(self.pages.shape[:-1], dtype=torch.float8_e8m0fnu, device=device)
+        else:
+            _attn_dtype(self.pages)
         ints = {"dtype": torch.int32, "device": self.pages.device}
         self.table = torch.full((slots, width), -1, **ints)
         self.lengths = torch.zeros(slots, **ints)
@@ -421,11 +620,20 @@ class PagedCache:
     def slots(self):
         return self.table.shape[0]
 
+    @property
+    def pool(self):
+        """All pages, as the page bookkeeping takes them."""
+        return self.pages if self.exponents is None else QuantizedPages(self.pages, self.exponents)
+
+    def _of(self, layer, which):
+        pages = self.pages[layer, which]
+        return pages if self.exponents is None else QuantizedPages(pages, self.exponents[layer, which])
+
     def keys(self, layer):
-        return self.pages[layer, 0]
+        return self._of(layer, 0)
 
     def values(self, layer):
-        return self.pages[layer, 1]
+        return self._of(layer, 1)
 
     def _slots(self, values, fill):
         """One int32 per slot: a device tensor as it is, or `fill` with a host dict's entries."""
@@ -442,7 +650,7 @@ class PagedCache:
         """`remap_pages` on the cache's state. parents: (slots) int32 tensor or a dict {slot: parent}
         (the other slots go on as themselves); new_lengths: (slots) int32 tensor or None."""
         parents = self._slots(parents, range(self.slots))
-        table, lengths, refs, shortfall = remap_pages(self.pages, self.table, self.lengths,
+        table, lengths, refs, shortfall = remap_pages(self.pool, self.table, self.lengths,
                                                       self.refs, parents, new_lengths)
         self.table.copy_(table)
         self.lengths.copy_(lengths)
@@ -459,20 +667,29 @@ class PagedCache:
         """The sequences of these slots are given up."""
         self.remap({s: -1 for s in slots})
 
-    def step(self, q_lengths, n_tokens, heads):
+    def step(self, q_lengths, n_tokens, heads, tree=None):
         """Room for `q_lengths[s]` new tokens of every slot, and the step's plan: `n_tokens` rows in
         all, no fewer than their sum. At most 4096 slots. Where pages are lacking, or device lengths sum
         to more than `n_tokens` (host lists are refused), no slot grows and every row of the plan is
-        padding."""
+        padding. `tree` as for `paged_plan`; `accept` then keeps a path of it."""
         n_tokens, kv_heads = int(n_tokens), self.pages.shape[3]
         _check_host_lengths(q_lengths, self.lengths, n_tokens, 0)
         # (a step that the plan would refuse is refused before a slot has grown)
         _plan_sizes(self.slots, n_tokens, heads, kv_heads, self.page_size, self.table.shape[1])
+        if tree is not None:
+            tree = _parents(tree, q_lengths, n_tokens, self.table.device)
         q = _lengths("q_lengths", q_lengths, self.slots, self.table.device)
         before = self.lengths.clone()
         self.remap(None, self._grown(q, n_tokens))
         return paged_plan(self.table, self.lengths - before, self.lengths, n_tokens, heads, kv_heads,
-                          self.page_size)
+                          self.page_size, tree)
+
+    def accept(self, plan, accepted):
+        """Of the last step's new tokens (`plan`: what `step` returned) those up to `accepted[s]` on its
+        path stay, `paged_accept`; pages that are not needed any more are given back. accepted: (slots)
+        int32 tensor, or a dict {slot: number} (the other slots' new tokens go)."""
+        accepted = self._slots(accepted, [-1] * self.slots)
+        self.remap(None, paged_accept(self.pool, plan, self.lengths, accepted))
 
     def _grown(self, q_lengths, n_tokens):
         """The slots' lengths with their new tokens, or as they are where those pass the rows."""
@@ -488,7 +705,7 @@ class PagedCache:
 
     def compact(self):
         """The live pages to the front of the pool; returns their number as a (1) int32 tensor."""
-        table, refs, live = compact_pages(self.pages, self.table, self.lengths, self.refs)
+        table, refs, live = compact_pages(self.pool, self.table, self.lengths, self.refs)
         self.table.copy_(table)
         self.refs.copy_(refs)
         return live

@@ -50,7 +50,7 @@ enum {
   VA_ECAPACITY = -5  /* output buffer too small (plan items, workspace) */
 };
 
-enum { VA_F16 = 0, VA_BF16 = 1, VA_F32 = 2 };
+enum { VA_F16 = 0, VA_BF16 = 1, VA_F32 = 2, VA_E4M3 = 3 };
 enum { VA_PLAN_FWD = 0, VA_PLAN_BWD = 1, VA_PLAN_BWD_HEADS = 2, VA_PLAN_BWD_PAIRS = 3,
        VA_PLAN_BWD_GROUPS = 4, VA_PLAN_BWD_GROUPS_ALL = 5, VA_PLAN_FWD_NARROW = 6 };
 enum { VA_BWD_PAIR_MIN_ITEMS = 1024 };
@@ -382,6 +382,75 @@ int va_pages_compact(void* pages, int64_t outer, int32_t n_pages, int32_t kv_hea
                      const int32_t* lengths, const int32_t* refs, int32_t n_slots,
                      int32_t table_width, int32_t* table_out, int32_t* refs_out, int32_t* live,
                      int32_t* scratch, int64_t scratch_words, void* stream);
+
+/* ---- 8-bit pages and trees of new tokens --------------------------------------------------------
+ * The calls above for caches whose rows are held in 8 bits and for steps whose new tokens form trees.
+ * Pages of one layer are given in one struct: dtype VA_F16 or VA_BF16 (exponents NULL, as above) or
+ * VA_E4M3: rows of 128 e4m3 numbers (1-4-3 bits, bias 7, largest 448, no infinities), each row with an
+ * exponent byte e beside it in (n_pages, Hkv, page_size) bytes, k_exp_stride / v_exp_stride apart
+ * (at least Hkv page_size, under 2^31): the row's values are its numbers times 2^(e - 127). e is the smallest
+ * from 27 on that brings the row's largest finite number to 448 or less; what is not finite is held as
+ * not a number. Strides are in elements (multiples of 8; of 16 for VA_E4M3).
+ * `tree` is NULL (the new tokens of every sequence follow each other) or what va_paged_tree wrote:
+ * va_paged_tree_words int32 of device memory, 16-byte aligned, for the plan that it was given with.
+ * parents (n_tokens): of every row the number, among the new tokens of its sequence, of the one that it
+ * follows (an earlier one); anything else: it follows the cached rows directly. A row then sees the rows
+ * cached before the step, the tokens on its path and itself; its position, which it is rotated by, is
+ * the cached length plus the tokens on its path before it, while its place in the cache is that of its
+ * number. Sequences of more than VA_TREE_TOKENS new tokens are chains whatever parents hold.
+ * Replaces nothing in the reference, which trains only. */
+enum { VA_TREE_TOKENS = 256 };
+typedef struct va_paged_pages {
+  void* k_pages;
+  void* v_pages;
+  uint8_t* k_exps;
+  uint8_t* v_exps;
+  int64_t k_stride, v_stride;
+  int64_t k_exp_stride, v_exp_stride;
+  int32_t n_pages;
+  int32_t dtype;
+} va_paged_pages;
+int va_paged_tree_words(const va_paged_step* step, int64_t* words);
+int va_paged_tree(const va_paged_step* step, const int32_t* parents, int32_t* tree,
+                  int64_t tree_words, void* stream);
+
+/* va_paged_append into pages of either kind; out_dtype is q_out's type (that of 16-bit pages). */
+int va_paged_append_pages(const va_paged_step* step, const int32_t* tree, const void* q, const void* k,
+                          const void* v, const float* cos, const float* sin, int64_t cos_batch_stride,
+                          int64_t cos_seq_stride, int64_t cos_token_stride, int64_t cos_rows,
+                          void* q_out, const va_paged_pages* pages, int32_t head_dim,
+                          int32_t in_dtype, int32_t out_dtype, void* stream);
+
+/* va_paged_attention over pages of either kind; dtype is that of q and out (that of 16-bit pages). 8-bit
+ * rows are multiplied as 16-bit numbers of that type: exactly, but for what passes VA_F16's range. */
+int va_paged_attention_pages(const va_paged_step* step, const int32_t* tree, const void* q,
+                             const va_paged_pages* pages, int32_t head_dim, float scale,
+                             int32_t dtype, void* out, void* workspace, int64_t workspace_bytes,
+                             void* stream);
+
+/* The end of a step of drafted tokens. accepted (n_seqs): the number of the last new token of every
+ * sequence that stays; the ones on its path stay with it and their rows, in every one of the `outer`
+ * (keys and values of every layer) x n_pages pages, move together behind the cached rows, in order;
+ * anything else: none stays. lengths (n_seqs): the cached tokens, the new ones included; lengths_out
+ * those that stay. Rows behind them keep what they held or what moved over them. `pages` as in
+ * va_pages_remap, or 8-bit rows with their exponents (outer, n_pages, kv_heads, page_size). */
+int va_paged_accept(const va_paged_step* step, const int32_t* tree, void* pages, uint8_t* exps,
+                    int64_t outer, int32_t n_pages, int32_t kv_heads, int32_t head_dim,
+                    const int32_t* lengths, const int32_t* accepted, int32_t* lengths_out,
+                    void* stream);
+
+/* va_pages_remap and va_pages_compact for 8-bit pages: a row's exponent goes with it. */
+int va_pages_remap8(void* pages, uint8_t* exps, int64_t outer, int32_t n_pages, int32_t kv_heads,
+                    int32_t page_size, int32_t head_dim, const int32_t* table,
+                    const int32_t* lengths, const int32_t* refs, const int32_t* parents,
+                    const int32_t* new_lengths, int32_t n_slots, int32_t table_width,
+                    int32_t* table_out, int32_t* lengths_out, int32_t* refs_out,
+                    int32_t* shortfall, int32_t* scratch, int64_t scratch_words, void* stream);
+int va_pages_compact8(void* pages, uint8_t* exps, int64_t outer, int32_t n_pages, int32_t kv_heads,
+                      int32_t page_size, int32_t head_dim, const int32_t* table,
+                      const int32_t* lengths, const int32_t* refs, int32_t n_slots,
+                      int32_t table_width, int32_t* table_out, int32_t* refs_out, int32_t* live,
+                      int32_t* scratch, int64_t scratch_words, void* stream);
 
 /* ---- machine-ceiling probes (diagnostics) ----------------------------------------------------
  * No counterpart in the reference: the benchmark measures with them the two ceilings it quotes

@@ -1,0 +1,514 @@
+"""Steps whose new tokens form trees, on the GPU against plain references: attention along the paths over
+16-bit and 8-bit pages, positions, the append, the rows of an accepted path, and a cache that drafts."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from hackaton_amd import (PagedCache, QuantizedPages, paged_accept, paged_append, paged_attention,
+                          paged_plan)
+from tests import paged8_oracle as o8
+from tests import paged_oracle as orc
+from tests.paged_oracle import DIM, SCALE
+from tests.test_gpu_paged import append_case, banner, ints
+from tests.test_gpu_paged8 import cuda, random_pool
+
+pytestmark = pytest.mark.gpu
+
+FP16, BF16 = torch.float16, torch.bfloat16
+
+
+def chain(n):
+    return [j - 1 for j in range(n)]
+
+
+def case(bits, seed, q, kv, heads, kv_heads, dtype, ps, padding=0, width=None):
+    """(query, k pages, v pages on the GPU, values in 64 bits, table)."""
+    if bits == 8:
+        query, k, v, exact, table = o8.case8(seed, q, kv, heads, kv_heads, dtype, ps, padding, width)
+        return query, cuda(k), cuda(v), exact, table
+    query, k, v, table = orc.paged_case(seed, q, kv, heads, kv_heads, dtype, ps, padding, width=width)
+    return query, k.cuda(), v.cuda(), [torch.nan_to_num(x.double()) for x in (k, v)], table
+
+
+def check_tree(bits, trees, kv, heads, kv_heads, dtype, ps, padding=0):
+    """trees: parents per sequence (empty: no new token)."""
+    q = [len(t) for t in trees]
+    banner("tree", bits, q[:20], kv[:20], heads, kv_heads, dtype, ps)
+    query, k, v, exact, table = case(bits, sum(kv) + heads, q, kv, heads, kv_heads, dtype, ps, padding)
+    n = sum(q) + padding
+    parents = ints([p for t in trees for p in t] + [3] * padding)
+    plan = paged_plan(table.cuda(), ints(q), ints(kv), n, heads, kv_heads, ps, parents)
+    out = paged_attention(query.cuda(), k, v, plan, SCALE).view(n, heads, DIM)
+    again = paged_attention(query.cuda(), k, v, plan, SCALE).view(n, heads, DIM)
+    ref, size = o8.attention(query, *exact, table, q, kv, [t if len(t) <= 256 else chain(len(t)) for t in trees])
+    got = out.cpu().double()
+    assert torch.isfinite(got).all()
+    excess = (got - ref).abs() - orc.attention_bound(ref, size, dtype)
+    assert float(excess.max()) <= 0, float((got - ref).abs().max())
+    assert torch.equal(out, again) and not out[sum(q):].any()
+    # positions and places
+    seq = [s for s, c in enumerate(q) for _ in range(c)]
+    places = [x - c + j for c, x in zip(q, kv) for j in range(c)]
+    depth = [int(o8.paths(t if len(t) <= 256 else chain(len(t)))[j].sum()) - 1 for t in trees for j in range(len(t))]
+    assert plan.sequences.tolist() == seq + [-1] * padding
+    assert plan.places.tolist() == places + [-1] * padding
+    assert plan.positions.tolist() == [kv[s] - q[s] + d for s, d in zip(seq, depth)] + [-1] * padding
+    return out
+
+
+HEADS = [(12, 2, FP16), (28, 4, BF16), (4, 4, BF16), (3, 1, FP16), (40, 1, BF16)]
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("ps", [16, 64])
+@pytest.mark.parametrize("heads,kv_heads,dtype", HEADS)
+def test_trees_of_all_sizes(heads, kv_heads, dtype, ps, bits):
+    """Trees around the words' and the tiles' borders beside idle sequences, single tokens and prompts."""
+    rng = np.random.default_rng(heads * ps + bits)
+    sizes = [1, 0, 2, 3, 5, 8, 31, 32, 33, 64, 100, 1, 65]
+    past = [0, 40, 7, 300, 31, 33, 64, 1, 200, 63, 95, 700, 17]
+    trees = [o8.random_tree(rng, n, 6) for n in sizes]
+    check_tree(bits, trees, [n + p for n, p in zip(sizes, past)], heads, kv_heads, dtype, ps, padding=5)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("past", [0, 1, 31, 32, 33, 63, 64, 65, 500])
+def test_every_border_of_the_cached_rows(past, bits):
+    """The tree begins at any row of a tile: words are read across their borders."""
+    rng = np.random.default_rng(past)
+    trees = [o8.random_tree(rng, n, 40) for n in (4, 70, 255, 256)]
+    check_tree(bits, trees, [len(t) + past for t in trees], 6, 2, FP16, 16)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_long_contexts_and_prompts_beside_trees(bits):
+    """Split key ranges, both shapes of work-groups; more than 256 new tokens are a chain."""
+    rng = np.random.default_rng(bits)
+    few, wide = o8.random_tree(rng, 3, 3), o8.random_tree(rng, 60, 20)
+    check_tree(bits, [few, wide, [-1]], [9003, 5060, 2001], 12, 2, BF16, 64)
+    check_tree(bits, [o8.random_tree(rng, 300, 300), wide, few], [700, 1060, 40], 8, 4, FP16, 16)
+    check_tree(bits, [o8.random_tree(rng, 24, 12) for _ in range(40)], [24 + 37 * i for i in range(40)], 28, 4,
+               BF16, 16)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("heads,kv_heads", [(12, 2), (4, 4)])
+def test_a_chain_is_a_step_without_a_tree(heads, kv_heads, bits):
+    banner("chain", bits, heads)
+    q, kv = [1, 5, 40, 256, 300, 0], [900, 70, 40, 700, 300, 9]
+    query, k, v, _, table = case(bits, 5, q, kv, heads, kv_heads, BF16, 32)
+    args = (table.cuda(), q, kv, sum(q), heads, kv_heads, 32)
+    plain, tree = paged_plan(*args), paged_plan(*args, [p for n in q for p in chain(n)])
+    assert torch.equal(plain.positions, tree.positions) and torch.equal(plain.places, tree.places)
+    assert torch.equal(plain.positions, plain.places)
+    assert torch.equal(*(paged_attention(query.cuda(), k, v, p, SCALE) for p in (plain, tree)))
+
+
+def test_parents_that_name_no_earlier_token():
+    """On the device they count as none; more new tokens than the cache counts lie before the sequence."""
+    banner("parents outside")
+    trees = [[5, 0, 2, -7, 3, 1 << 30, -(1 << 31), 1], [0, 1, 2], [-1, 0, 0, 2, 2, 1]]
+    check_tree(16, trees, [20, 3, 46], 12, 2, FP16, 16)
+    q, kv = [8, 6], [5, 2]
+    query, k, v, exact, table = case(16, 4, q, kv, 12, 2, FP16, 16)
+    trees = [[-1, 0, 0, 2, 2, 1, 5, 3], [-1, 0, 1, 2, 3, 4]]
+    plan = paged_plan(table.cuda(), ints(q), ints(kv), 14, 12, 2, 16, ints(sum(trees, [])))
+    out = paged_attention(query.cuda(), k, v, plan, SCALE).cpu().double().view(14, 12, DIM)
+    ref, size = o8.attention(query, *exact, table, q, kv, trees)
+    assert torch.isfinite(out).all() and ((out - ref).abs() <= orc.attention_bound(ref, size, FP16)).all()
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("count", [4, 40])
+def test_keys_of_other_branches_never_reach_a_row(count, bits):
+    """Two branches: the keys of one are not a number, and the rows of the other come out as they were."""
+    banner("branches", count, bits)
+    tree = [-1] + [max(0, j - 2) if j > 2 else 0 for j in range(1, count)]  # odd and even numbers
+    q, kv, ps = [count], [count + 37], 16
+    query, k, v, _, table = case(bits, 6, q, kv, 12, 2, FP16, ps)
+    plan = paged_plan(table.cuda(), q, kv, count, 12, 2, ps, tree)
+    want = paged_attention(query.cuda(), k, v, plan, SCALE).view(count, 12, DIM)
+    codes = k if bits == 16 else k.codes.view(torch.uint8)
+    for j in range(1, count, 2):
+        at = 37 + j
+        codes[int(table[0, at // ps]), :, at % ps] = math.nan if bits == 16 else 0x7f
+    out = paged_attention(query.cuda(), k, v, plan, SCALE).view(count, 12, DIM)
+    assert torch.equal(out[0::2], want[0::2])
+    assert torch.isnan(out[1::2]).all()
+
+
+def test_append_rotates_by_position_and_writes_by_place():
+    banner("append of a tree")
+    rng = np.random.default_rng(1)
+    trees = [o8.random_tree(rng, n, 4) for n in (7, 1, 30)]
+    q, kv, heads, kv_heads, ps = [7, 1, 30], [60, 9, 35], 12, 2, 16
+    qkv, cos, sin, table, pages = append_case(q, kv, heads, kv_heads, ps, FP16, 4)
+    parents = ints([p for t in trees for p in t])
+    plan = paged_plan(table.cuda(), q, kv, sum(q), heads, kv_heads, ps, parents)
+    pos = plan.positions.long().cpu()
+    assert not torch.equal(pos, plan.places.long().cpu())
+    flat = paged_plan(table.cuda(), q, kv, sum(q), heads, kv_heads, ps)
+    results = []
+    for p, tables in ((plan, (cos, sin)), (plan, (cos[0, pos], sin[0, pos])), (flat, (cos[0, pos], sin[0, pos]))):
+        dev = torch.zeros(2, pages, kv_heads, ps, DIM, dtype=FP16, device="cuda")
+        out = paged_append(*(x.cuda() for x in qkv), *(x.cuda() for x in tables), dev[0], dev[1], p)
+        results.append((out, dev))
+    for got in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got, results[0]))
+    short = paged_append(*(x.cuda() for x in qkv), cos[:, :40].cuda(), sin[:, :40].cuda(), dev[0], dev[1], plan)
+    assert [not r.any() for r in short.cpu()] == (pos >= 40).tolist()
+
+
+# ------------------------------------------------------------------------------------------------
+# accepted paths
+# ------------------------------------------------------------------------------------------------
+def accept_want(pool, table, q, kv, trees, accepted, ps):
+    """(pool, lengths) from lists; pool: byte or 16-bit tensors with (layers, 2, pages, heads, rows, ...)."""
+    pool, lengths = [x.clone() for x in pool], []
+    for s, (n, length, tree, last) in enumerate(zip(q, kv, trees, accepted)):
+        if not n:
+            lengths.append(length)
+            continue
+        path = []
+        while 0 <= last < n:
+            path.insert(0, last)
+            last = tree[last] if 0 <= tree[last] < last else -1
+        for i, j in enumerate(path):
+            (a, x), (b, y) = divmod(length - n + j, ps), divmod(length - n + i, ps)
+            for p in pool:
+                p[:, :, int(table[s, b]), :, y] = p[:, :, int(table[s, a]), :, x]
+        lengths.append(length - n + len(path))
+    return pool, lengths
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("kv_heads,ps,layers,span", [(2, 16, 3, 4), (4, 64, 1, 2), (1, 256, 2, 40), (8, 32, 2, 1)])
+def test_accept(kv_heads, ps, layers, span, bits):
+    banner("accept", bits, kv_heads, ps, layers, span)
+    rng = np.random.default_rng(ps + bits)
+    q = [1, 0, 5, 33, 64, 256, 2, 17, 300, 24, 24, 24, 0]
+    kv = [n + int(rng.integers(0, 90)) for n in q]
+    trees = [o8.random_tree(rng, n, span) if n <= 256 else chain(n) for n in q]
+    accepted = [int(rng.integers(0, n)) if n else 0 for n in q]
+    accepted[4], accepted[5], accepted[8], accepted[9], accepted[10] = 63, 255, 200, -1, 24
+    counts = [-(-x // ps) for x in kv]
+    order, table = rng.permutation(sum(counts) + 4).tolist(), np.full((len(q), max(counts) + 1), -1, np.int32)
+    for s, c in enumerate(counts):
+        table[s, :c] = [order.pop() for _ in range(c)]
+    pool = random_pool(layers, sum(counts) + 4, kv_heads, ps)
+    plain = pool.codes.view(torch.uint8) if bits == 8 else torch.randn(pool.codes.shape, device="cuda").to(BF16)
+    parts = [plain, pool.exponents.view(torch.uint8)] if bits == 8 else [plain]
+    want, lengths = accept_want(parts, table, q, kv, trees, accepted, ps)
+    plan = paged_plan(torch.from_numpy(table).cuda(), q, kv, sum(q) + 3, 2 * kv_heads, kv_heads, ps,
+                      [p for t in trees for p in t])
+    got = paged_accept(pool if bits == 8 else plain, plan, ints(kv), ints(accepted))
+    assert got.tolist() == lengths
+    assert all(torch.equal(a, b) for a, b in zip(parts, want))
+    # the same step without a tree: the tokens up to the accepted one stay where they are
+    flat = paged_plan(torch.from_numpy(table).cuda(), q, kv, sum(q) + 3, 2 * kv_heads, kv_heads, ps)
+    got = paged_accept(pool if bits == 8 else plain, flat, ints(kv), ints(accepted))
+    assert got.tolist() == [x if not n else x - n + (a + 1 if 0 <= a < n else 0)
+                            for x, n, a in zip(kv, q, accepted)]
+    assert all(torch.equal(a, b) for a, b in zip(parts, want))
+
+
+def test_accept_over_missing_pages_and_empty_steps():
+    banner("accept without pages")
+    pool = torch.randn(2, 2, 5, 2, 16, DIM, device="cuda").to(FP16)
+    before = pool.clone()
+    table = ints([[0, -1, 99], [1, 2, 3]])
+    tree = [-1, 0, 0, 2, 3, 4, 5, 6] + [-1, -1, 1]
+    plan = paged_plan(table, [8, 3], [24, 20], 11, 4, 2, 16, tree)
+    got = paged_accept(pool, plan, ints([24, 20]), ints([7, 2]))
+    # path 0, 2, 3, ... of rows 16 to 23 (no page); path 1, 2 of rows 17 to 19 of the second: one page
+    assert got.tolist() == [23, 19]
+    for i, j in enumerate((1, 2)):
+        before[:, :, 2, :, 1 + i] = before[:, :, 2, :, 1 + j]
+    assert torch.equal(pool, before)
+    plan = paged_plan(table, [0, 0], [24, 20], 0, 4, 2, 16, [])
+    assert paged_accept(pool, plan, ints([24, 20]), ints([7, 2])).tolist() == [24, 20]
+    none = paged_plan(table[:0], [], [], 4, 4, 2, 16, [])
+    assert paged_accept(pool, none, ints([]), ints([])).shape == (0,) and torch.equal(pool, before)
+    empty = paged_plan(table, ints([8, 3]), ints([24, 20]), 11, 4, 2, 16, tree)
+    assert paged_accept(pool[:, :, :0], empty, ints([24, 20]), ints([7, 2])).tolist() == [23, 19]
+    assert paged_accept(pool[:0], empty, ints([24, 20]), ints([7, 2])).tolist() == [23, 19]
+
+
+# ------------------------------------------------------------------------------------------------
+# graphs, streams, refusals
+# ------------------------------------------------------------------------------------------------
+def test_captured_steps_follow_the_tree():
+    """Two captured steps; trees, lengths and queries change between the replays."""
+    banner("captured trees")
+    heads, kv_heads, ps = 12, 2, 16
+    rng = np.random.default_rng(0)
+    q, kv = [20, 30, 10], [1500, 90, 64]
+    query, k, v, _, table = case(8, 10, q, kv, heads, kv_heads, FP16, ps, 4, width=100)
+    query, table, q_len, kv_len, parents = query.cuda(), table.cuda(), ints(q), ints(kv), ints([-1] * 64)
+
+    def step(x):
+        plan = paged_plan(table, q_len, kv_len, 64, heads, kv_heads, ps, parents)
+        return paged_attention(x, k, v, plan, SCALE), plan.positions
+
+    graphs, static = [], [query.clone(), query * 0.5]
+    for x in static:
+        step(x)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step(x)
+        graphs.append((graph, got))
+    for new, total in ((q, kv), ([1, 60, 1], [1400, 90, 60]), ([0, 0, 0], [5, 6, 7]), ([64, 0, 0], [70, 8, 9])):
+        q_len.copy_(ints(new))
+        kv_len.copy_(ints(total))
+        parents.copy_(ints(sum((o8.random_tree(rng, n, 5) for n in new), [])
+                           + [-1] * (64 - sum(new))))
+        for (graph, got), x in zip(graphs, static):
+            want = step(x)
+            for _ in range(3):
+                graph.replay()
+                torch.cuda.synchronize()
+                assert all(torch.equal(a, b) for a, b in zip(got, want)), (new, total)
+                x.mul_(1.0)  # eager work between the replays
+
+
+def test_a_graph_keeps_the_tree_that_it_reads():
+    """A call captured over a plan with a tree that was made before and is dropped."""
+    from hackaton_amd import attention as att
+
+    banner("captured call over an eager tree")
+    rng = np.random.default_rng(2)
+    q, kv = [20, 50], [1400, 90]
+    query, k, v, _, table = case(16, 12, q, kv, 12, 2, FP16, 16)
+    tree = sum((o8.random_tree(rng, n, 5) for n in q), [])
+    plan = paged_plan(table.cuda(), q, kv, 70, 12, 2, 16, tree)
+    query = query.cuda()
+    want = paged_attention(query, k, v, plan, SCALE)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = paged_attention(query, k, v, plan, SCALE)
+    size = plan._paths.numel()
+    del plan
+    fill = [torch.full((size,), 0, dtype=torch.int32, device="cuda") for _ in range(8)]
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    del fill, graph
+    att.release_captured_plans()
+
+
+def test_another_stream_and_calls_at_once():
+    banner("tree on streams")
+    rng = np.random.default_rng(3)
+    q, kv = [20, 30, 1], [800, 90, 65]
+    query, k, v, _, table = case(8, 11, q, kv, 12, 2, BF16, 16)
+    query, table, parents = query.cuda(), table.cuda(), ints(sum((o8.random_tree(rng, n, 5) for n in q), []))
+
+    def step():
+        return paged_plan(table, ints(q), ints(kv), sum(q), 12, 2, 16, parents)
+
+    want = paged_attention(query, k, v, step(), SCALE)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    for _ in range(4):
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                got.append(paged_attention(query, k, v, step(), SCALE))
+    plan = step()  # made here, used there, dropped at once
+    streams[0].wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(streams[0]):
+        got.append(paged_attention(query, k, v, plan, SCALE))
+        del plan
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want) for x in got)
+
+
+def test_refusals():
+    table = ints([[0, 1], [2, 3]])
+    args = (table, [3, 2], [30, 20], 6, 4, 2, 16)
+    for bad in ([-1, 0, 3, -1, 0], [-1, 0, 2, -1, 0], [-1, 0, 1, 0, 0], [-1, 0], [-1] * 7, ints([-1] * 5),
+                ints([-1] * 6).long(), ints([-1] * 12)[::2], torch.zeros(6, dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            paged_plan(*args, bad)
+    wide = ints([list(range(20))])
+    with pytest.raises(ValueError, match="256"):
+        paged_plan(wide, [257], [300], 257, 4, 2, 16, [-1] * 257)
+    paged_plan(wide, [257], [300], 257, 4, 2, 16, chain(257))
+    plan = paged_plan(*args, [-1, 0, 1, -1, 0])
+    pool = torch.zeros(1, 2, 4, 2, 16, DIM, dtype=FP16, device="cuda")
+    for bad in ((pool[:, :, :, :1].contiguous(), ints([30, 20]), ints([0, 0])),
+                (pool[0], ints([30, 20]), ints([0, 0])), (pool, ints([30]), ints([0, 0])),
+                (pool, ints([30, 20]), ints([0, 0]).long()), (pool, ints([30, 20]), ints([0, 0]).cpu()),
+                (pool.float(), ints([30, 20]), ints([0, 0])),
+                (QuantizedPages(pool, pool[..., 0]), ints([30, 20]), ints([0, 0]))):
+        with pytest.raises(ValueError):
+            paged_accept(bad[0], plan, *bad[1:])
+    with pytest.raises(RuntimeError, match="no backward"):
+        paged_accept(pool.clone().requires_grad_(), plan, ints([30, 20]), ints([0, 0]))
+    cache = PagedCache(1, 8, 16, 1, 2, 64)
+    for bad in ([0, -1], [-1]):
+        with pytest.raises(ValueError):
+            cache.step([1, 1], 2, 2, bad)
+    assert cache.lengths.tolist() == [0, 0]
+    with pytest.raises(ValueError):
+        cache.accept(cache.step([1, 1], 2, 2, [-1, -1]), {2: 0})
+
+
+# ------------------------------------------------------------------------------------------------
+# together
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,held,page_size", [(FP16, FP16, 16), (BF16, o8.E4M3, 16), (FP16, o8.E4M3, 64)])
+def test_a_program_that_drafts(dtype, held, page_size):
+    """Prompts, drafted trees of which a path is accepted, a fork, single tokens, freed slots and a
+    compaction over one cache, against attention over the rows that are held: as a plain list per slot."""
+    banner("a drafting run", dtype, held, page_size)
+    layers, heads, kv_heads, slots = 2, 6, 2, 4
+    rng = np.random.default_rng(page_size)
+    gen = torch.Generator().manual_seed(page_size)
+    cache = PagedCache(layers, 640 // page_size, page_size, kv_heads, slots, 256, held)
+    if held == o8.E4M3:
+        cache.pages.view(torch.uint8).fill_(0x7f)
+        cache.exponents.view(torch.uint8).fill_(0xff)
+    else:
+        cache.pages.fill_(math.nan)
+    angle = torch.arange(256)[:, None] * (1e4 ** (-torch.arange(64) / 64.0))[None]
+    angle = torch.cat((angle, angle), -1)[None]
+    cos, sin = angle.cos().cuda(), angle.sin().cuda()
+    mirror = [[[] for _ in range(slots)] for _ in range(layers)]  # (k, v) that the cache holds, per token
+
+    def held_rows(layer, slot, count):
+        """The last `count` rows of a slot as they lie in the pages."""
+        length, row = int(cache.lengths[slot]), cache.table[slot].tolist()
+        rows = []
+        for t in range(length - count, length):
+            pair = []
+            for which in (0, 1):
+                at = (layer, which, row[t // page_size], slice(None), t % page_size)
+                x = cache.pages[at].double()
+                if held == o8.E4M3:
+                    x = x * cache.exponents[at].double()[:, None]
+                pair.append(x.cpu())
+            rows.append(pair)
+        return rows
+
+    def go(q, trees):
+        n = sum(q) + 2
+        plan = cache.step(ints(q), n, heads, ints(sum(trees, []) + [0, 0]))
+        assert cache.lengths.tolist() == [len(mirror[0][s]) + c for s, c in enumerate(q)]
+        pos = plan.positions.tolist()
+        for layer in range(layers):
+            proj = [torch.randn(n, h * DIM, generator=gen).to(dtype) for h in (heads, kv_heads, kv_heads)]
+            keys, values = cache.keys(layer), cache.values(layer)
+            query = paged_append(*(x.cuda() for x in proj), cos, sin, keys, values, plan)
+            assert query.dtype == dtype
+            out = paged_attention(query, keys, values, plan, SCALE).cpu().double().view(n, heads, DIM)
+            assert not out[sum(q):].any()
+            at, got_q = 0, query.cpu()
+            for s, (count, tree) in enumerate(zip(q, trees)):
+                on, new = o8.paths(tree), held_rows(layer, s, count) if count else []
+                for j in range(count):
+                    # what the pages hold is what was given, rotated and rounded to their type
+                    k = orc.rotate(proj[1][at + j].double().view(1, kv_heads, DIM), *(
+                        x[0, pos[at + j]][None].cpu() for x in (cos, sin)))[0]
+                    for mine, given in ((new[j][0], k), (new[j][1], proj[2][at + j].double().view(kv_heads, DIM))):
+                        # (half a step: 2^-4 of a number, or of a row's largest by 448 / 2^-6 in steps of 2^-9)
+                        size = given.abs()
+                        loss = (size * 2.0 ** -4 + size.amax(-1, keepdim=True) * 2.0 ** -17 if held == o8.E4M3
+                                else size * orc.HALF_STEP[dtype])
+                        assert ((mine - given).abs() <= loss * (1 + 2.0 ** -8) + 2.0 ** -20).all()
+                    seen = mirror[layer][s] + [new[i] for i in range(j + 1) if on[j][i]]
+                    k, v = (torch.stack([r[i] for r in seen], 1) for i in (0, 1))
+                    for h in range(heads):
+                        w = torch.softmax(k[h // 3] @ got_q[at + j, h].double() * SCALE, 0)
+                        want, size = w @ v[h // 3], w @ v[h // 3].abs()
+                        assert ((out[at + j, h] - want).abs() <= orc.attention_bound(want, size, dtype)).all()
+                at += count
+        return plan
+
+    def accept(plan, q, trees, last):
+        rows = [[held_rows(layer, s, c) if c else [] for s, c in enumerate(q)] for layer in range(layers)]
+        cache.accept(plan, {s: x for s, x in enumerate(last)})
+        for layer in range(layers):
+            for s, (tree, x) in enumerate(zip(trees, last)):
+                path = [] if not 0 <= x < q[s] else np.nonzero(o8.paths(tree)[x])[0].tolist()
+                mirror[layer][s] += [rows[layer][s][j] for j in path]
+        assert cache.lengths.tolist() == [len(x) for x in mirror[0]]
+        for layer in range(layers):  # what the cache holds now
+            for s in range(slots):
+                for a, b in zip(held_rows(layer, s, len(mirror[layer][s])), mirror[layer][s]):
+                    assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+    def turn(q, span, last):
+        trees = [o8.random_tree(rng, n, span) if span else chain(n) for n in q]
+        accept(go(q, trees), q, trees, last)
+
+    turn([37, 20, 5, 0], 0, [36, 19, 4, 0])
+    turn([9, 1, 30, 0], 3, [8, 0, 17, -1])
+    cache.fork(0, [3])
+    for layer in mirror:
+        layer[3] = list(layer[0])
+    turn([12, 12, 12, 12], 4, [11, 6, -1, 9])
+    turn([1, 1, 1, 1], 0, [0, 0, 0, 0])
+    cache.free([1])
+    for layer in mirror:
+        layer[1] = []
+    assert int(cache.compact()) == int((cache.refs > 0).sum())
+    turn([24, 3, 8, 24], 8, [23, 2, 5, 20])
+    cache.check()
+    refs = torch.bincount(cache.table[cache.table >= 0].long(), minlength=cache.refs.numel())
+    assert torch.equal(refs.int(), cache.refs)
+
+
+def test_a_captured_drafting_step_runs_on():
+    """step with a tree, append, attention and accept captured once and replayed over changing trees; the
+    same steps run eagerly give the same cache and outputs."""
+    banner("captured drafting")
+    heads, kv_heads, slots, n = 12, 2, 3, 30
+    rng, gen = np.random.default_rng(4), torch.Generator().manual_seed(4)
+    angle = torch.rand(1, 400, DIM, generator=gen) * 6
+    cos, sin = angle.cos().cuda(), angle.sin().cuda()
+    caches = [PagedCache(1, 80, 16, kv_heads, slots, 400, o8.E4M3) for _ in range(2)]
+    rows = [torch.zeros(n, h * DIM, dtype=BF16, device="cuda") for h in (heads, kv_heads, kv_heads)]
+    q, parents, last = ints([1, 0, 1]), ints([-1] * n), ints([0, 0, 0])
+
+    def step(cache):
+        plan = cache.step(q, n, heads, parents)
+        query = paged_append(*rows, cos, sin, cache.keys(0), cache.values(0), plan)
+        out = paged_attention(query, cache.keys(0), cache.values(0), plan, SCALE)
+        cache.accept(plan, last)
+        return out
+
+    for cache in caches:
+        cache.pages.view(torch.uint8).zero_()
+        cache.exponents.view(torch.uint8).fill_(127)
+        cache.remap(None, ints([20, 0, 0]))
+    step(caches[0])
+    caches[0].remap(None, ints([20, 0, 0]))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(caches[0])
+    for x in ("pages", "exponents"):
+        getattr(caches[0], x).view(torch.uint8).copy_(getattr(caches[1], x).view(torch.uint8))
+    for i in range(20):
+        new = [int(x) for x in rng.integers(0, 11, slots)]
+        q.copy_(ints(new))
+        parents.copy_(ints(sum((o8.random_tree(rng, c, 4) for c in new), []) + [-1] * (n - sum(new))))
+        last.copy_(ints([int(rng.integers(-1, c + 1)) for c in new]))
+        for x in rows:
+            x.copy_(torch.randn(x.shape, generator=gen).to(BF16))
+        graph.replay()
+        want = step(caches[1])
+        torch.cuda.synchronize()
+        assert torch.equal(got, want), i
+        for name in ("table", "lengths", "refs", "pages", "exponents"):
+            a, b = (getattr(c, name) for c in caches)
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)), (i, name)
+    for cache in caches:
+        cache.check()
