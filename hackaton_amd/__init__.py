@@ -7,6 +7,7 @@ of the reference (MLP, loss, norms, NF4, trainer) are outside this package's sco
 
 from .attention import (PackedAttention, PackRows, QKVRotate, VarlenAttention, pack_rows,
                         packed_attention, qkv_rotate, varlen_attention)
+from .beams import select_beams
 from .paged import (PagedCache, PagedPlan, QuantizedPages, compact_pages, paged_accept, paged_append,
                     paged_attention, paged_plan, remap_pages)
 from .patches import patch_qwen2_attention
@@ -14,7 +15,8 @@ from .patches import patch_qwen2_attention
 __all__ = ["apply", "patch_qwen2_attention", "packed_attention", "varlen_attention",
            "qkv_rotate", "pack_rows", "PackedAttention", "VarlenAttention", "QKVRotate",
            "PackRows", "paged_plan", "paged_append", "paged_attention", "remap_pages", "compact_pages",
-           "PagedCache", "PagedPlan", "QuantizedPages", "paged_accept"]
+           "PagedCache", "PagedPlan", "QuantizedPages", "paged_accept",
+           "select_beams"]
 
 
 def apply():

@@ -119,6 +119,9 @@ SIGNATURES = {
                                        _i32, _i32, _p, _p, _p, _p, _p, _i64, _p]),
     "va_pages_compact8": (ctypes.c_int, [_p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _i32,
                                          _i32, _p, _p, _p, _p, _i64, _p]),
+    "va_select_beams_workspace": (ctypes.c_int, [_i64, _i32, _i32, _pi64]),
+    "va_select_beams": (ctypes.c_int, [_p, _i32, _i64, _i64, _i32, _i32, _p, _p, _i32, _i32, _p, _p,
+                                       _p, _p, _i64, _p]),
     "va_probe_mfma": (ctypes.c_int, [_i32, _i32, _i32, _p, _p]),
     "va_probe_copy": (ctypes.c_int, [_p, _p, _i64, _i32, _p]),
 }

@@ -29,6 +29,7 @@ from torch.autograd import forward_ad
 from . import _lib, attention
 from ._lib import check, lib
 from .attention import _DTYPES, HEAD_DIM, _attn_dtype, _rope_strides, _tables
+from .beams import select_beams
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 TREE_TOKENS = _lib.VA_TREE_TOKENS  # the most new tokens of a sequence that form a tree
@@ -702,6 +703,18 @@ class PagedCache:
                                     out.data_ptr(), self.excess.data_ptr(),
                                     _current_stream(device.index)), "va_pages_growth")
         return out
+
+    def select(self, logits, scores, beams, ended=None, end_token=None):
+        """Beam search over the slots, `beams` of them a prompt: `select_beams` on the slots' next-token
+        logits (slots, vocab) and scores (slots), and every slot goes on as the one that it continues.
+        Returns (scores, parents, tokens), each (slots): the slots' scores, the slots that they were, and
+        their next tokens."""
+        if logits.dim() != 2 or logits.shape[0] != self.slots:
+            raise ValueError(f"logits must be ({self.slots}, vocab), got {tuple(logits.shape)}")
+        scores, parents, tokens = (x.view(-1) for x in select_beams(logits, scores, beams, None, ended,
+                                                                    end_token))
+        self.remap(parents)
+        return scores, parents, tokens
 
     def compact(self):
         """The live pages to the front of the pool; returns their number as a (1) int32 tensor."""

@@ -452,6 +452,24 @@ int va_pages_compact8(void* pages, uint8_t* exps, int64_t outer, int32_t n_pages
                       int32_t table_width, int32_t* table_out, int32_t* refs_out, int32_t* live,
                       int32_t* scratch, int64_t scratch_words, void* stream);
 
+/* ---- beam search's selection ------------------------------------------------------------------
+ * Of all continuations of a prompt's beams the best `count` (1 to 64). logits: rows of vocab (at most
+ * 2^18) elements of dtype (VA_F16, VA_BF16 or VA_F32), row_stride elements apart, at any address of an
+ * element; row g * beams + b is beam b (of up to 64) of prompt g; scores: the beams' sums of log
+ * probabilities so far. A continuation's score is score + (logit - log of the sum of the row's
+ * exponentials), formed and compared in 64 bits and rounded once; what is not a number counts as
+ * -infinity. Outputs (groups, count), best first, ties to the lowest row and token: scores, rows that they
+ * continue (among all rows) and tokens. ended (a byte per row, may be NULL): rows that are not 0 have
+ * ended; their logits are not read, they go on with end_token at their score, and as -infinity with every
+ * other token. The order is that of a full sort of all continuations. Deterministic. Workspace:
+ * va_select_beams_workspace bytes, 16-byte aligned; calls that may overlap need one each. No counterpart in
+ * the reference (its generation goes through transformers). */
+int va_select_beams_workspace(int64_t groups, int32_t beams, int32_t vocab, int64_t* bytes);
+int va_select_beams(const void* logits, int32_t dtype, int64_t row_stride, int64_t groups,
+                    int32_t beams, int32_t vocab, const float* scores, const uint8_t* ended,
+                    int32_t end_token, int32_t count, float* scores_out, int32_t* parents_out,
+                    int32_t* tokens_out, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- machine-ceiling probes (diagnostics) ----------------------------------------------------
  * No counterpart in the reference: the benchmark measures with them the two ceilings it quotes
  * its roofline fractions against, on the box it runs on, beside the data-sheet figures.
