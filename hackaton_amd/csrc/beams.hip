@@ -9,8 +9,11 @@
 // numbers, and the best numbers in them. Scores are formed and compared in 64 bits, score + (number - log
 // of the sum): a rounding to 32 would make ties of continuations that are not as good.
 //
-// The first kernel is bounded by memory (its arithmetic, 11 instructions a number, takes 2/3 as long); the
-// second by the latency of its steps.
+// The first kernel is bounded by memory, and for 16-bit numbers nearly as much by its arithmetic (a power of
+// two, 16 cycles of a wave, and six other instructions a number): 512 rows of 150,016 numbers (154 MB) 34 us,
+// 4.6 TB/s; of 75,008 fp32 numbers, as many bytes, 30 us. 1, 2 and 4 pieces on their way and 1024 to 8192
+// work-groups measured 34 to 47. The second kernel is bounded by the latency of its steps: 9 us for a prompt
+// of four beams, 11 us for 64 of eight (13.8 and 33.7 with 256 threads, which computed each key twice).
 #include <climits>
 #include <type_traits>
 
@@ -26,12 +29,12 @@ constexpr int kNumbers = 8;  // per lane and load
 
 enum { kF16 = 0, kBF16 = 1, kF32 = 2 };
 
-// 8 numbers from `p` on, at any alignment of the element.
+// 8 numbers of a row, as loaded.
 template <int DT>
 struct Numbers {
   static constexpr int W = DT == kF32 ? 8 : 4;  // words
   uint32_t w[W];
-  __device__ inline void load(const void* base, int64_t at) {
+  __device__ inline void load(const void* base, int64_t at) {  // at any address of an element
     __builtin_memcpy(w, (const char*)base + at * (DT == kF32 ? 4 : 2), 4 * W);
   }
   __device__ inline void load_some(const void* base, int64_t at, int count) {  // the others: -infinity
@@ -52,6 +55,30 @@ struct Numbers {
   }
 };
 
+// The same on the way: 16-bit numbers that begin in the middle of a word (ODD) are loaded as the words that
+// they lie in, from the number before them to the one behind them, and shifted when they are used (512 rows
+// of 150,001: 36 us, 39 with loads that straddle words). Not by cells that begin elsewhere: rows that hold the
+// same numbers have the same sum to the last bit, or equal scores would be no ties.
+template <int DT, bool ODD>
+struct Coming {
+  Numbers<DT> x;
+  uint32_t last;
+  // numbers i to i + 7 of the row at `row`, of which the one before and the one behind exist if ODD
+  __device__ inline void load(const void* logits, int64_t row, int i) {
+    x.load(logits, row + i - ODD);
+    if constexpr (ODD) __builtin_memcpy(&last, (const char*)logits + 2 * (row + i + kNumbers - 1), 4);
+  }
+  __device__ inline Numbers<DT> numbers() const {
+    Numbers<DT> y = x;
+    if constexpr (ODD) {
+#pragma unroll
+      for (int k = 0; k < Numbers<DT>::W; ++k)
+        y.w[k] = __builtin_amdgcn_alignbit(k + 1 < Numbers<DT>::W ? x.w[k + 1] : last, x.w[k], 16);
+    }
+    return y;
+  }
+};
+
 // The largest number of a wave, in all lanes (not-a-numbers are passed over).
 __device__ inline float wave_max(float x) {
   x = fmaxf(x, dpp_mov<0xb1>(x));
@@ -62,6 +89,129 @@ __device__ inline float wave_max(float x) {
   return max_with_other_half(x);
 }
 
+// The same in the last lane only, without LDS.
+template <int CTRL, int ROWS>
+__device__ inline float dpp_max(float x) {
+  const int i = __builtin_bit_cast(int, x);
+  return fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, CTRL, ROWS, 0xf, false)));
+}
+__device__ inline float wave_max_last(float x) {
+  x = dpp_max<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8: within rows of 16 lanes
+  x = dpp_max<0x112, 0xf>(x);
+  x = dpp_max<0x114, 0xf>(x);
+  x = dpp_max<0x118, 0xf>(x);
+  x = dpp_max<0x142, 0xa>(x);  // row_bcast 15: the last lane of a row to the next one (rows 1, 3)
+  return dpp_max<0x143, 0xc>(x);  // row_bcast 31: lane 31 to rows 2, 3
+}
+
+// Exponentials are powers of two, number * kLog2e less the reference of the largest number so far. Up to 2^16
+// that is largest * kLog2e rounded, so that a power costs a fused multiply-add and one rounding, of a
+// difference; from there on, where that rounding would count, the product itself: differences of numbers
+// are taken first. kLog2e, rounded, stands for the base: the second kernel divides by it, so a shift of all
+// numbers shifts the result.
+__device__ inline bool far_out(float largest) { return fabsf(largest) >= 65536.f; }
+// Power of two by which a sum over the reference of `was` has to be multiplied for that of `is`.
+__device__ inline float rescale(float was, float is) {
+  const float a = was * kLog2e, b = is * kLog2e;
+  const float d = far_out(is) ? (far_out(was) ? (was - is) * kLog2e : __builtin_fmaf(-is, kLog2e, a))
+                              : (far_out(was) ? __builtin_fmaf(was, kLog2e, -b) : a - b);
+  return fast_exp2(d);
+}
+
+// A wave's part of a row: the largest numbers of its cells, every step-th one from c0 on, and per lane the
+// largest number and the sum. Cells are gone through in pieces of 64 kNumbers numbers, PIECES at a time (of
+// as many cells, or of one), as many on their way: a reduction over the wave, the exponentials' latency and
+// the test for a new largest number are then paid once.
+constexpr int PIECES = 2;
+template <int DT, bool ODD>
+__device__ inline void read_row(const BeamsArgs& a, int64_t base, float* tops, int c0, int step, float& top,
+                                float& sum) {
+  const BeamsLayout& l = a.layout;
+  const int lane = threadIdx.x & 63, shift = __builtin_ctz(l.cell / (64 * kNumbers));
+  const int pieces = c0 < l.cells ? ((l.cells - 1 - c0) / step + 1) << shift : 0;
+  auto cell_of = [&](int p) { return c0 + (p >> shift) * step; };
+  auto begin_of = [&](int p) { return cell_of(p) * l.cell + (p & ((1 << shift) - 1)) * (64 * kNumbers); };
+  // Loads are the same for all pieces, from inside the row; what a row's first or last piece, or one that
+  // there is not, got from elsewhere is replaced when it is used.
+  const int least = ODD, most = a.vocab - kNumbers - ODD;
+  auto plain = [&](int p) {
+    return p < pieces && begin_of(p) >= least && begin_of(p) + 64 * kNumbers <= a.vocab - ODD;
+  };
+  Coming<DT, ODD> next[PIECES];
+  auto fetch = [&](int p) {
+    if (most < least) return;  // (a row of a few numbers: replaced)
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j)
+      next[j].load(a.logits, base, max(min(begin_of(p + j) + kNumbers * lane, most), least));
+  };
+  float ref = 0.f, cell = -INFINITY;
+  bool some_far = false;  // some lane's largest number is far out
+  fetch(0);
+  for (int p = 0; p < pieces; p += PIECES) {
+    Numbers<DT> x[PIECES];
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) x[j] = next[j].numbers();
+    fetch(p + PIECES);
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j)
+      if (!plain(p + j)) {
+        const int i = p + j < pieces ? begin_of(p + j) + kNumbers * lane : a.vocab;
+        x[j].load_some(a.logits, base + min(i, a.vocab), a.vocab - i);
+      }
+    float mine[PIECES], part[PIECES];
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+      part[j] = 0.f;
+      mine[j] = x[j].get(0);
+#pragma unroll
+      for (int e = 1; e < kNumbers; ++e) mine[j] = fmaxf(mine[j], x[j].get(e));
+    }
+    float all = mine[0];
+#pragma unroll
+    for (int j = 1; j < PIECES; ++j) all = fmaxf(all, mine[j]);
+    if (__builtin_amdgcn_ballot_w64(all > top) != 0) {
+      const float more = fmaxf(top, all);
+      sum *= top == -INFINITY ? 0.f : rescale(top, more);
+      top = more;
+      ref = more == -INFINITY ? 0.f : more * kLog2e;
+      some_far = __builtin_amdgcn_ballot_w64(more != -INFINITY && far_out(more)) != 0;
+    }
+    if (!some_far) {
+#pragma unroll
+      for (int e = 0; e < kNumbers; ++e)
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) part[j] += fast_exp2(__builtin_fmaf(x[j].get(e), kLog2e, -ref));
+    } else {
+      const bool mine_far = top != -INFINITY && far_out(top);
+#pragma unroll
+      for (int e = 0; e < kNumbers; ++e)
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j)
+          part[j] += fast_exp2(mine_far ? (x[j].get(e) - top) * kLog2e
+                                        : __builtin_fmaf(x[j].get(e), kLog2e, -ref));
+    }
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) sum += part[j];
+    if (shift == 0) {
+#pragma unroll
+      for (int j = 0; j < PIECES; ++j) mine[j] = wave_max_last(mine[j]);
+#pragma unroll
+      for (int j = 0; j < PIECES; ++j)
+        if (lane == 63 && p + j < pieces) tops[cell_of(p + j)] = mine[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < PIECES; ++j) {
+        cell = fmaxf(cell, mine[j]);
+        if (((p + j + 1) & ((1 << shift) - 1)) == 0) {
+          cell = wave_max_last(cell);
+          if (lane == 63 && p + j < pieces) tops[cell_of(p + j)] = cell;
+          cell = -INFINITY;
+        }
+      }
+    }
+  }
+}
+
 template <int DT>
 __global__ __launch_bounds__(T) void beams_read_kernel(BeamsArgs a) {
   const int row = blockIdx.x, split = blockIdx.y, lane = threadIdx.x & 63;
@@ -70,29 +220,14 @@ __global__ __launch_bounds__(T) void beams_read_kernel(BeamsArgs a) {
   const int64_t base = row * a.row_stride;
   const BeamsLayout& l = a.layout;
   float* tops = a.workspace + (int64_t)row * l.cells;
-  float m = -INFINITY, sum = 0.f;  // this lane's
-  for (int c = split * kBeamsWaves + wave; c < l.cells; c += l.splits * kBeamsWaves) {
-    float top = -INFINITY;
-    for (int i = c * l.cell + kNumbers * lane; i < (c + 1) * l.cell; i += kNumbers * 64) {
-      Numbers<DT> x;
-      if (i + kNumbers <= a.vocab) x.load(a.logits, base + i);
-      else x.load_some(a.logits, base + min(i, a.vocab), a.vocab - i);
-      float mine = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < kNumbers; ++e) mine = fmaxf(mine, x.get(e));
-      top = fmaxf(top, mine);
-      // (differences, not products with the largest number taken apart: what counts is exact)
-      const float now = fmaxf(m, mine), ref = now == -INFINITY ? 0.f : now;
-      sum *= fast_exp2((m - ref) * kLog2e);
-      m = now;
-#pragma unroll
-      for (int e = 0; e < kNumbers; ++e) sum += fast_exp2((x.get(e) - ref) * kLog2e);
-    }
-    top = wave_max(top);
-    if (lane == 0) tops[c] = top;
-  }
-  const float all = wave_max(m), ref = all == -INFINITY ? 0.f : all;
-  sum *= fast_exp2((m - ref) * kLog2e);
+  float top = -INFINITY, sum = 0.f;
+  const int c0 = split * kBeamsWaves + wave, step = l.splits * kBeamsWaves;
+  if (DT != kF32 && ((((uintptr_t)a.logits >> 1) + (uint64_t)base) & 1) != 0)
+    read_row<DT, DT != kF32>(a, base, tops, c0, step, top, sum);
+  else
+    read_row<DT, false>(a, base, tops, c0, step, top, sum);
+  const float all = wave_max(top);
+  sum *= top == -INFINITY ? 1.f : rescale(top, all);  // (of -infinity: 0, or not a number)
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
   if (lane == 0) {
@@ -121,167 +256,233 @@ __device__ inline double value_of(uint64_t key) {
   return __builtin_bit_cast(double, key >> 63 ? key & ~(1ull << 63) : ~key);
 }
 
-constexpr int kPool = 4096;  // candidates that pass the threshold, at most
+constexpr int PT = 1024, PW = PT / 64;  // threads and waves of a work-group that picks
+constexpr int kPool = 4096;             // candidates that pass the threshold, at most
 struct Picks {
   Pick pool[kPool], best[64], out[kBeamsCount];
+  int rank[2][64];
   int n;
 };
 
-// The best `count` of all candidates that each(visit) shows to visit(key, index), in order, to s.out; returns how
-// many there are. Each group of 4 threads brings its best one; the count-th best of those 64 is a bound
-// that `count` candidates reach, and only those of the groups whose best reaches it: at most 4 count times the
-// candidates of a thread (kPool is no less). They are then put in order by counting who comes before.
-template <class Each>
-__device__ inline int select(Picks& s, int count, Each each) {
-  const int tid = threadIdx.x;
-  uint64_t key = 0;
-  int index = INT_MAX;
-  each([&](uint64_t k, int i) {
-    if (k != 0 && before(k, i, key, index)) key = k, index = i;
-  });
-#pragma unroll
-  for (int d = 1; d < 4; d *= 2) {
-    const uint64_t k = __shfl_xor((unsigned long long)key, d);
-    const int i = __shfl_xor(index, d);
-    if (before(k, i, key, index)) key = k, index = i;
+// How many of v[0..n) come before v[lane]: the waves share them out, ranks add up in s.
+__device__ inline void count_before(const Pick* v, int n, const Pick& mine, int* rank) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int r = 0;
+#pragma unroll 4
+  for (int j = wave; j < n; j += PW) {
+    const Pick p = v[j];
+    r += before(p.key, p.index, mine.key, mine.index);
   }
-  __syncthreads();  // (the pool and s.n may be in use from before)
-  if ((tid & 3) == 0) s.best[tid >> 2] = Pick{key, index, 0};
+  if (r != 0) atomicAdd(&rank[lane], r);
+}
+
+// The best `count` of all threads' E candidates (key 0: none), in order, to s.out; returns how many there
+// are. Each group of 16 threads brings its best one; the count-th best of those 64 is a bound that `count`
+// candidates reach, and only those of the groups whose best reaches it: at most 16 E count (and not more
+// than there are; the callers see to it that kPool is no less). They are then put in order by counting who
+// comes before. (A pool of more than 64 is slow, but takes scores whose best ones all lie with one
+// thread.)
+template <int E>
+__device__ inline int select(Picks& s, int count, const uint64_t (&key)[E], const int (&index)[E]) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  uint64_t top = 0;
+  int at = INT_MAX;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (key[e] != 0 && before(key[e], index[e], top, at)) top = key[e], at = index[e];
+#pragma unroll
+  for (int d = 1; d < 16; d *= 2) {
+    const uint64_t k = __shfl_xor((unsigned long long)top, d);
+    const int i = __shfl_xor(at, d);
+    if (before(k, i, top, at)) top = k, at = i;
+  }
+  __syncthreads();  // (the pool and the counts may be in use from before)
+  if ((tid & 15) == 0) s.best[tid >> 4] = Pick{top, at, 0};
+  if (tid < 64) s.rank[0][tid] = s.rank[1][tid] = 0;
   if (tid == 0) s.n = 0;
   __syncthreads();
-  // every wave finds the bound for itself: lane l ranks group l
-  const Pick mine = s.best[tid & 63];
-  int rank = 0;
-#pragma unroll 8
-  for (int j = 0; j < 64; ++j) {
-    const Pick p = s.best[j];
-    rank += before(p.key, p.index, mine.key, mine.index);
-  }
-  // (groups without a candidate are equal: all of them rank behind the others)
-  const uint64_t at = __builtin_amdgcn_ballot_w64(rank == count - 1 && mine.key != 0);
+  const Pick mine = s.best[lane];
+  count_before(s.best, 64, mine, s.rank[0]);
+  __syncthreads();
+  // (groups without a candidate are alike and rank behind the others)
+  const uint64_t found = __builtin_amdgcn_ballot_w64(s.rank[0][lane] == count - 1 && mine.key != 0);
   uint64_t least = 0;
   int last = INT_MAX;
-  if (at != 0) {
-    const int l = __builtin_ctzll(at);
-    least = __shfl((unsigned long long)mine.key, l);
-    last = __shfl(mine.index, l);
+  if (found != 0) {
+    const Pick p = s.best[__builtin_ctzll(found)];
+    least = p.key;
+    last = p.index;
   }
-  each([&](uint64_t k, int i) {
-    if (k != 0 && !before(least, last, k, i)) {
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (key[e] != 0 && !before(least, last, key[e], index[e])) {
       const int n = atomicAdd(&s.n, 1);
-      if (n < kPool) s.pool[n] = Pick{k, i, 0};
+      if (n < kPool) s.pool[n] = Pick{key[e], index[e], 0};
     }
-  });
   __syncthreads();
   const int n = min(s.n, kPool);
-  for (int i = tid; i < n; i += T) {
-    const Pick p = s.pool[i];
-    int r = 0;
+  if (n <= 64) {
+    const Pick p = s.pool[min(lane, n - 1)];
+    count_before(s.pool, n, p, s.rank[1]);
+    __syncthreads();
+    if (tid < n && s.rank[1][tid] < count) s.out[s.rank[1][tid]] = p;
+  } else {
+    for (int i = tid; i < n; i += PT) {
+      const Pick p = s.pool[i];
+      int r = 0;
 #pragma unroll 4
-    for (int j = 0; j < n; ++j) {
-      const Pick o = s.pool[j];
-      r += before(o.key, o.index, p.key, p.index);
+      for (int j = 0; j < n; ++j) {
+        const Pick o = s.pool[j];
+        r += before(o.key, o.index, p.key, p.index);
+      }
+      if (r < count) s.out[r] = p;
     }
-    if (r < count) s.out[r] = p;
   }
   __syncthreads();
   return min(n, count);
 }
 
-// Cells, or runs of numbers, are gone through in the order of their numbers.
-__device__ inline void in_order(const Picks& s, int n, int* order) {
+// Where the chosen runs of numbers begin, in the order of their numbers.
+template <class First>
+__device__ inline void in_order(const Picks& s, int n, int* runs, First first) {
   const int tid = threadIdx.x;
   if (tid < n) {
     int r = 0;
     for (int j = 0; j < n; ++j) r += s.out[j].index < s.out[tid].index;
-    order[r] = s.out[tid].index;
+    runs[r] = first(s.out[tid].index);
   }
   __syncthreads();
 }
 
 template <int DT>
-__global__ __launch_bounds__(T) void beams_pick_kernel(BeamsArgs a) {
+__global__ __launch_bounds__(PT) void beams_pick_kernel(BeamsArgs a) {
   __shared__ Picks s;
   __shared__ double s_score[kBeamsMost], s_sum[kBeamsMost];
+  __shared__ bool s_ended[kBeamsMost];
   __shared__ int s_runs[kBeamsCount];
+  constexpr int CELLS = kBeamsCells / PT;
   const BeamsLayout& l = a.layout;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, first = blockIdx.x * a.beams;
-  auto ended = [&](int beam) { return a.ended != nullptr && a.ended[first + beam] != 0; };
 
+  // the cells' largest numbers, on their way while the sums are formed
+  const int cells = a.beams * l.cells;
+  const float* tops = a.workspace + (int64_t)first * l.cells;
+  float top[CELLS];
+#pragma unroll
+  for (int e = 0; e < CELLS; ++e) top[e] = e * PT + tid < cells ? tops[e * PT + tid] : 0.f;
   // log of the sum of exponentials of every beam (an ended one: all of its weight on its end token)
   const int waves = l.splits * kBeamsWaves;
-  for (int b = wave; b < a.beams; b += kBeamsWaves) {
+  for (int b = wave; b < a.beams; b += PW) {
     const f32x2* sums = reinterpret_cast<const f32x2*>(a.workspace + l.sums) + (int64_t)(first + b) * waves;
-    const bool done = ended(b);
-    float m = -INFINITY;
-    for (int i = lane; i < waves && !done; i += 64) m = fmaxf(m, sums[i][0]);
-    m = wave_max(m);
-    double sum = 0;
-    for (int i = lane; i < waves && !done; i += 64) {
-      const f32x2 x = sums[i];
-      if (x[0] != -INFINITY || x[1] != 0.f) sum += (double)x[1] * exp((double)x[0] - (double)m);
+    const float score = a.scores[first + b];
+    const bool done = a.ended != nullptr && a.ended[first + b] != 0;
+    double sum = 0, ref = 0;
+    if (!done) {
+      const f32x2 none = {-INFINITY, 0.f}, mine = lane < waves ? sums[lane] : none;
+      float m = mine[0];
+      for (int i = lane + 64; i < waves; i += 64) m = fmaxf(m, sums[i][0]);
+      m = wave_max(m);
+      auto ref_of = [](float x) { return far_out(x) ? (double)x * (double)kLog2e : (double)(x * kLog2e); };
+      ref = ref_of(m);
+      // (-infinity with a sum of 0: nothing was read, or nothing but -infinity)
+      auto add = [&](const f32x2& x) {
+        if (x[0] != -INFINITY || x[1] != 0.f) sum += (double)x[1] * exp2(ref_of(x[0]) - ref);
+      };
+      add(mine);
+      for (int i = lane + 64; i < waves; i += 64) add(sums[i]);
+      for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
     }
-    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
     if (lane == 0) {
-      s_score[b] = a.scores[first + b];
-      s_sum[b] = done ? 0.0 : (double)m + log(sum);
+      s_score[b] = score;
+      s_sum[b] = done ? 0.0 : (ref + log2(sum)) / (double)kLog2e;
+      s_ended[b] = done;
     }
   }
   __syncthreads();
-  auto key = [&](int beam, float x) { return key_of(s_score[beam] + ((double)x - s_sum[beam])); };
+  auto score_of = [&](int beam, float x) { return key_of(s_score[beam] + ((double)x - s_sum[beam])); };
 
   // the best cells
-  const int cells = a.beams * l.cells;
-  int n = select(s, min(a.count, cells), [&](auto visit) {
-    for (int i = tid; i < cells; i += T) {
-      const int beam = i / l.cells, c = i % l.cells;
-      const float top = ended(beam) ? (a.end_token / l.cell == c ? 0.f : -INFINITY)
-                                    : a.workspace[(int64_t)(first + beam) * l.cells + c];
-      visit(key(beam, top), i);
+  int n;
+  {
+    // (quotients of small numbers: exact in fp32, half a unit to spare)
+    const float inv = 1.f / (float)l.cells;
+    const int end_cell = a.end_token / l.cell;
+    uint64_t key[CELLS];
+    int index[CELLS];
+#pragma unroll
+    for (int e = 0; e < CELLS; ++e) {
+      const int i = e * PT + tid;
+      index[e] = i;
+      key[e] = 0;
+      if (i < cells) {
+        const int beam = (int)(((float)i + 0.5f) * inv);
+        if (s_ended[beam]) top[e] = i - beam * l.cells == end_cell ? 0.f : -INFINITY;
+        key[e] = score_of(beam, top[e]);
+      }
     }
-  });
-  in_order(s, n, s_runs);
+    n = select(s, min(a.count, cells), key, index);
+  }
+  in_order(s, n, s_runs, [&](int i) { return i / l.cells * kBeamsVocab + i % l.cells * l.cell; });
 
-  // the largest numbers of runs of `run` numbers of them, then the numbers themselves; each thread takes
-  // kNumbers numbers at a time. Index of a number: beam * 2^18 + token (of a run: its first number's).
-  auto number = [&](int at) { return s_runs[at]; };
-  auto see = [&](int beam, int token, auto visit) {  // up to kNumbers numbers from `token` on
-    if (token >= a.vocab) return;
-    Numbers<DT> x;
+  // the best runs in them where their numbers are too many, then the numbers. Each thread takes kNumbers at a
+  // time. Index of a number: beam * 2^18 + token (of a run: its first number's).
+  auto see = [&](int at, float (&x)[kNumbers]) {  // numbers from `at` on; returns how many there are
+    const int beam = at / kBeamsVocab, token = at % kBeamsVocab, some = min(a.vocab - token, kNumbers);
+    if (some <= 0) return 0;
     const int64_t base = (int64_t)(first + beam) * a.row_stride + token;
-    const int some = min(a.vocab - token, kNumbers);
-    const bool done = ended(beam);
-    if (some == kNumbers) x.load(a.logits, base);
-    else x.load_some(a.logits, base, some);
+    const bool done = s_ended[beam];
+    Numbers<DT> w;
+    if (some == kNumbers) w.load(a.logits, base);
+    else w.load_some(a.logits, base, some);
 #pragma unroll
     for (int e = 0; e < kNumbers; ++e)
-      if (e < some) visit(done ? (token + e == a.end_token ? 0.f : -INFINITY) : x.get(e), e);
+      x[e] = !done ? w.get(e) : token + e == a.end_token ? 0.f : -INFINITY;
+    return some;
   };
-  int run = l.cell;
-  for (int i = tid; i < n; i += T) s_runs[i] = s_runs[i] / l.cells * kBeamsVocab + s_runs[i] % l.cells * l.cell;
-  __syncthreads();
-  // (what a group of 4 threads then goes through, count times, has to fit in the pool)
-  if (a.count * ((n * (run / kNumbers) + T - 1) / T) * 4 * kNumbers > kPool) {
+  int run = l.cell;  // (a power of two from here on)
+  if (n * (run / kNumbers) > PT || (16 * kNumbers * a.count > kPool && n * run > kPool)) {
+    constexpr int RUNS = 64 * kBeamsCount / PT;
     const int part = run / 64;
-    n = select(s, a.count, [&](auto visit) {
-      for (int i = tid; i < 64 * n; i += T) {
-        const int at = number(i >> 6) + (i & 63) * part, beam = at / kBeamsVocab, token = at % kBeamsVocab;
-        float top = -INFINITY;
-        for (int k = 0; k < part; k += kNumbers)
-          see(beam, token + k, [&](float x, int) { top = fmaxf(top, x); });
-        if (token < a.vocab) visit(key(beam, top), at);
+    uint64_t key[RUNS];
+    int index[RUNS];
+#pragma unroll
+    for (int e = 0; e < RUNS; ++e) {
+      const int i = e * PT + tid;
+      key[e] = 0;
+      index[e] = 0;
+      if (i < 64 * n) {
+        index[e] = s_runs[i >> 6] + (i & 63) * part;
+        float best = -INFINITY;
+        bool any = false;
+        for (int k = 0; k < part; k += kNumbers) {
+          float x[kNumbers];
+          const int some = see(index[e] + k, x);
+#pragma unroll
+          for (int j = 0; j < kNumbers; ++j)
+            if (j < some) best = fmaxf(best, x[j]);
+          any = any || some > 0;
+        }
+        if (any) key[e] = score_of(index[e] / kBeamsVocab, best);
       }
-    });
-    in_order(s, n, s_runs);
+    }
+    n = select(s, a.count, key, index);
+    in_order(s, n, s_runs, [](int i) { return i; });
     run = part;
   }
-  const int loads = run / kNumbers;
-  n = select(s, a.count, [&](auto visit) {
-    for (int i = tid; i < n * loads; i += T) {
-      const int at = number(i / loads) + i % loads * kNumbers, beam = at / kBeamsVocab;
-      see(beam, at % kBeamsVocab, [&](float x, int e) { visit(key(beam, x), at + e); });
+  {
+    const int shift = __builtin_ctz(run / kNumbers), loads = n << shift;
+    uint64_t key[kNumbers];
+    int index[kNumbers];
+    float x[kNumbers];
+    const int at = tid < loads ? s_runs[tid >> shift] + (tid & ((1 << shift) - 1)) * kNumbers : 0;
+    const int some = tid < loads ? see(at, x) : 0;
+#pragma unroll
+    for (int e = 0; e < kNumbers; ++e) {
+      index[e] = at + e;
+      key[e] = e < some ? score_of(at / kBeamsVocab, x[e]) : 0;
     }
-  });
+    n = select(s, a.count, key, index);
+  }
   if (tid < a.count) {  // (n is count: there are no fewer numbers)
     const Pick p = s.out[min(tid, n - 1)];
     const int64_t at = (int64_t)blockIdx.x * a.count + tid;
@@ -294,7 +495,7 @@ __global__ __launch_bounds__(T) void beams_pick_kernel(BeamsArgs a) {
 template <int DT>
 void select_beams(const BeamsArgs& a) {
   hipLaunchKernelGGL(beams_read_kernel<DT>, dim3(a.groups * a.beams, a.layout.splits), dim3(T), 0, a.stream, a);
-  hipLaunchKernelGGL(beams_pick_kernel<DT>, dim3(a.groups), dim3(T), 0, a.stream, a);
+  hipLaunchKernelGGL(beams_pick_kernel<DT>, dim3(a.groups), dim3(PT), 0, a.stream, a);
 }
 
 }  // namespace

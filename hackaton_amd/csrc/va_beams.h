@@ -17,8 +17,8 @@ constexpr int kBeamsWaves = 4;         // of a work-group that reads logits
 constexpr int kBeamsGroups = 2048, kBeamsFewCells = 8;
 
 // How a call's logits are cut: cells of `cell` numbers of a row (the last one may be shorter), `splits`
-// work-groups per row. Workspace: the largest number of every cell (rows x cells), then {largest number,
-// sum of exponentials over it} of every wave (rows x splits x kBeamsWaves), fp32.
+// work-groups per row. Workspace: the largest number of every cell (rows x cells), then {reference,
+// sum of powers of two over it} of every wave (rows x splits x kBeamsWaves), fp32.
 struct BeamsLayout {
   int cell, cells, splits;
   int64_t sums, words;  // offset of the waves' pairs; fp32 words in all
