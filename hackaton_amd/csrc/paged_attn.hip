@@ -59,8 +59,9 @@ static_assert(sizeof(Item) == 4 * kPagedItemWords, "item words");
 
 struct Merge {
   int token0, head, row, rows;        // 1 to 8 flattened rows
-  int part_row, stride, parts, pad;   // workspace row of the first one in the first part; rows per part;
+  int part_row, stride, parts;        // workspace row of the first one in the first part; rows per part;
                                       // parts (0: the rows' only item has written them)
+  int spread;                         // one row, whose parts are shared out
 };
 static_assert(sizeof(Merge) == 4 * kPagedMergeWords, "merge words");
 
@@ -81,6 +82,10 @@ __device__ inline int last_at_most(const int* v, int n, int x) {
   return lo;
 }
 
+// Rows of a merge record: one where few rows have many parts, which are then shared out in it. (16 trees of 32
+// tokens on 500 to 16,000, up to 26 parts: 11 us with one row each.)
+__device__ inline int merged_rows(bool few, int parts) { return parts <= (few ? 8 : 32) ? 8 : 1; }
+
 // The first `writers` work-groups write the items, as many the merge records, the others place the rows.
 // Each sums the lengths by itself (at most 32 KB of them): one launch, nothing handed from one
 // work-group to another.
@@ -100,6 +105,8 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
   // records before it, parts, keys of a part
   __shared__ int s_cu[S + 1], s_pos0[S], s_many[S], s_few[S], s_part[S], s_merge[S], s_parts[S], s_chunk[S];
   __shared__ int s_scan[10 * PT / 64];
+  __shared__ __attribute__((aligned(16))) uint32_t s_key[PT];
+  __shared__ int s_at[PT], s_items[PT];  // (one sequence per thread: their order)
   const int tid = threadIdx.x, group = a.hq / a.hkv;
   // Row offsets need sums of q; the split shares need, per kind (many rows, few rows), the tiles and
   // their keys, here from the lengths as they are given (cut to n_tokens one by one), which is no less
@@ -154,10 +161,18 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
   const bool split =
       a.max_keys > kPagedWholeKeys && ((long long)sums[1] << 15) + sums[0] <= a.n_tokens;
   int chunks[2];
+  // parts of prompt tiles that are as many as the card has places (few-row tiles behind them fill the places
+  // that shorter ones leave)
+  const long long its = (long long)sums[2] * a.hkv;
+  const long long many = min(max(sums[3] == 0 ? its : its / 2, (long long)kPagedManyParts / 4),
+                             (long long)a.layout.many_parts);
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const long long all = k == 0 ? kPagedManyParts : kPagedFewParts;
-    const long long parts = max(all - (long long)sums[2 + k] * a.hkv, all / 4);
+    const long long items = (long long)sums[2 + k] * a.hkv;
+    const long long all = k == 1         ? kPagedFewParts - max(0LL, many - kPagedManyParts)
+                          : sums[3] == 0 ? a.layout.many_base
+                                         : kPagedManyParts;
+    const long long parts = max(all - items, k == 0 ? many : all / 4);
     const long long keys =
         ((long long)sums[6 + 3 * k] << 38) + ((long long)sums[5 + 3 * k] << 19) + sums[4 + 3 * k];
     // (at most INT_MAX / 2, which no range is longer than: such a share splits nothing; a prompt of 2^20
@@ -171,7 +186,7 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
   }
   const int aligned = 8 / (a.hkv % 8 == 0 ? 8 : a.hkv % 4 == 0 ? 4 : a.hkv % 2 == 0 ? 2 : 1);
   int x[4] = {0, 0, 0, 0}, n[4];  // items of both kinds, workspace rows, merge records
-  int own[SPT][4];
+  int own[SPT][4], longest_of[SPT];
 #pragma unroll
   for (int i = 0; i < SPT; ++i) {
     const int s = tid * SPT + i, rows = n_rows[i], kind = rows <= kPagedFewRows;
@@ -184,10 +199,11 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
     s_parts[s] = parts;
     s_chunk[s] = max(c, 1);
     const int items = tiles_of(rows) * parts * a.hkv;
+    longest_of[i] = kind == 0 ? longest : 0;
     own[i][0] = kind == 0 ? items : 0;
     own[i][1] = kind == 0 ? 0 : items;
     own[i][2] = parts > 1 ? rows * parts * a.hkv : 0;
-    own[i][3] = parts > 1 ? (parts <= 8 ? (rows + 7) / 8 : rows) * a.hkv : 0;
+    own[i][3] = parts > 1 ? (rows + merged_rows(kind, parts) - 1) / merged_rows(kind, parts) * a.hkv : 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) x[k] += own[i][k];
   }
@@ -196,6 +212,7 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
   for (int i = 0; i < SPT; ++i) {
     const int s = tid * SPT + i;
     s_many[s] = x[0];
+    if constexpr (SPT == 1) s_items[s] = own[i][0];
     s_few[s] = x[1];
     s_part[s] = x[2];
     s_merge[s] = x[3];
@@ -203,6 +220,31 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
     for (int k = 0; k < 4; ++k) x[k] += own[i][k];
   }
   __syncthreads();
+  // Prompt tiles of unequal ranges, more than the card has places and nothing behind them: the sequences with the
+  // longest ranges first, so that what starts last is short (64 trees on 64 to 8192 tokens 78 -> 58 us for
+  // 1 us here; up to PT sequences, by counting).
+  bool sorted = false;
+  if constexpr (SPT == 1) {
+    sorted = n[0] > kPagedManyParts && n[1] == 0 && n[2] > 0;
+    if (sorted) {
+      // (by the range, then by number: all different)
+      const uint32_t mine = (uint32_t)min(longest_of[0], (1 << 24) - 1) << 8 | (PT - 1 - tid);
+      s_key[tid] = tid < a.n_seqs ? mine : 0;
+      __syncthreads();
+      int rank = 0;
+#pragma unroll 4
+      for (int j = 0; j < a.n_seqs; j += 4) {
+        const u32x4 k = *reinterpret_cast<const u32x4*>(s_key + j);
+        rank += (k[0] > mine) + (k[1] > mine) + (k[2] > mine) + (k[3] > mine);
+      }
+      if (tid < a.n_seqs) s_at[rank] = tid;
+      __syncthreads();
+      int y[1] = {tid < a.n_seqs ? s_items[s_at[tid]] : 0}, all[1];
+      block_exclusive_sums<PT / 64>(y, all, s_scan);
+      s_many[tid] = y[0];
+      __syncthreads();
+    }
+  }
   Item* items = reinterpret_cast<Item*>(a.plan + a.layout.items);
   Merge* merges = reinterpret_cast<Merge*>(a.plan + a.layout.merges);
   const bool merging = (int)blockIdx.x >= writers;
@@ -211,9 +253,10 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
   for (int i = first; i < n_items && !merging; i += step) {
     const bool many = i < n[0];
     const int* before = many ? s_many : s_few;
-    const int j = many ? i : i - n[0], s = last_at_most(before, a.n_seqs, j);
+    const int j = many ? i : i - n[0], nth = last_at_most(before, a.n_seqs, j);
+    const int s = SPT == 1 && many && sorted ? s_at[nth] : nth;
     const int rows = (s_cu[s + 1] - s_cu[s]) * group, parts = s_parts[s], chunk = s_chunk[s];
-    const int in = j - before[s], per_tile = parts * a.hkv, tile = tiles_of(rows) - 1 - in / per_tile;
+    const int in = j - before[nth], per_tile = parts * a.hkv, tile = tiles_of(rows) - 1 - in / per_tile;
     const int head = in % a.hkv, part = in % per_tile / a.hkv;
     Item it;
     it.token0 = s_cu[s];
@@ -233,7 +276,7 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
   for (int i = first; i < n_merges && merging; i += step) {
     const int s = last_at_most(s_merge, a.n_seqs, i), in = i - s_merge[s];
     const int rows = (s_cu[s + 1] - s_cu[s]) * group, parts = s_parts[s], chunk = s_chunk[s];
-    const int each = parts <= 8 ? 8 : 1, per_head = (rows + each - 1) / each;
+    const int each = merged_rows(rows <= kPagedFewRows, parts), per_head = (rows + each - 1) / each;
     const int head = in / per_head, row = in % per_head * each;
     const int all = keys_of(s_pos0[s], min((row / kPagedTileRows + 1) * kPagedTileRows, rows), group);
     Merge m;
@@ -244,7 +287,7 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
     m.part_row = s_part[s] + head * parts * rows + row;
     m.stride = rows;
     m.parts = all <= chunk ? 0 : (all + chunk - 1) / chunk;
-    m.pad = 0;
+    m.spread = each == 1;
     merges[i] = m;
   }
   if (blockIdx.x > 0) return;
@@ -269,7 +312,7 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
 // A work-group per sequence: the paths of its new tokens by doubling (after round r a token knows the 2^r
 // next ones on its way to the root, and the one behind them), in LDS; the other work-groups mark the
 // padding rows. Bounded by its launch and the rounds' barriers.
-static_assert(PT == kTreeTokens, "a thread per token");
+static_assert(PT == kTreeTokens && PT <= 256, "a thread per token; eight bits of a sequence's number");
 __global__ __launch_bounds__(PT) void paged_tree_kernel(PagedTreeArgs a) {
   __shared__ uint32_t s_path[PT][kTreeWords + 1];
   __shared__ int s_next[PT];
@@ -1149,8 +1192,8 @@ __global__ __launch_bounds__(Shape<W>::THREADS, 2) void paged_attn_kernel(PagedA
   }
 }
 
-// Parts of split key ranges: a record of 8 rows and up to 8 parts has 32 lanes (4 elements each) per row,
-// a record of one row and more parts shares the parts out to the 8 groups of 32 lanes.
+// Parts of split key ranges: a record of 8 rows has 32 lanes (4 elements each) per row, one of a single row and
+// many parts shares the parts out to the 8 groups of 32 lanes.
 struct Sum {
   float m, l;
   f32x4 o;
@@ -1196,7 +1239,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a) {
   for (int i = blockIdx.x; i < n; i += gridDim.x) {
     if (i != (int)blockIdx.x) mg = merges[i];
     if (!inside(a, mg)) continue;  // (the same in all threads)
-    const bool spread = mg.parts > 8;
+    const bool spread = mg.spread != 0;
     const int r = spread ? 0 : g;
     const long row = mg.part_row + r;
     Sum sum{-INFINITY, 0.f, f32x4{0.f, 0.f, 0.f, 0.f}};
@@ -1207,7 +1250,9 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttnArgs a) {
     } else if (g < mg.rows) {
       if (mg.parts <= 2) add_parts<2>(o, ml, row, mg.stride, mg.parts, d0, sum);
       else if (mg.parts <= 4) add_parts<4>(o, ml, row, mg.stride, mg.parts, d0, sum);
-      else add_parts<8>(o, ml, row, mg.stride, mg.parts, d0, sum);
+      else
+        for (int p = 0; p < mg.parts; p += 8)
+          add_parts<8>(o, ml, row + (long)p * mg.stride, mg.stride, min(8, mg.parts - p), d0, sum);
     }
     if (spread) {
       s_o[g][threadIdx.x & 31] = sum.o;

@@ -24,7 +24,11 @@ constexpr int kPagedChunkKeys = 64;  // key ranges are split at multiples of thi
 // (386) 88 / 72; 8 x 300 on 700 (240) 27.5 / 26; two chunks of 512 beside 62 answers, 28/4 heads (492) 60 /
 // 59; 2 x 1024 on 500 (456) 46.5 / 47.5; 3 x 1024 (684) 62 / 67; 4 x 1024 (912) 78 / 82; four chunks of
 // 2048 623 / 680; 64 answers of 64 to 8192 tokens 30.4 / 32.0, 16 of 1500 12.1 / 12.8, four of 512 7.9 / 7.5.
-constexpr int kPagedWideTiles = 512;
+// Steps of few prompt tiles over ranges that are split take 4 waves too, and twice the parts: two work-groups
+// of a CU wait for different barriers. us, 8 waves and 256 parts / 4 and 512, 28/4 heads: 16 trees of 24 on 4000 75
+// / 53, 8 of 48 to 64 on 28,672 to 32,768 305 / 268, 512 new tokens on 8192 98 / 86, on 4096 55 / 55, 1024 new
+// ones (the table's bound 228) on 4096 106 / 106, 8 x 300 on 700, 12/2 heads (240) 29 / 39.
+constexpr int kPagedWideTiles = 512, kPagedSplitTiles = 200;
 // Parts that a step's keys are split into, by kind of tile, the shortest part (but a range's last) and
 // the longest table row that is never split. us at 384 / 512 / 1024 few-row parts: 64 answers of 64 to
 // 8192 tokens, 12/2 heads 34 / 30 / 32, four of 65,536, 28/4 heads 103 / 97 / 100; shortest few-row part
@@ -33,7 +37,13 @@ constexpr int kPagedWideTiles = 512;
 // prompt part 256 / 512 / 704: 300 new tokens on 1000 16.8 / 17.7 / 20.4, two of 64 on 8000 26.9 / 27.0 /
 // 27.8, where 256 would make twice the parts and room for the merge. Four answers of 512, table rows of
 // 576: split 8.5, whole 7.9 and a launch less.
-constexpr int kPagedFewParts = 512, kPagedManyParts = 256;
+// Prompt tiles that are as many as the card has places (tiles x heads) are split where they are longer than the
+// average one, into up to kPagedMostParts parts: 64 trees of 24 tokens on 64 to 8192, 28/4
+// heads (512 items) 162 -> 59 us and 3 more to merge, 16 chunks of 64 to 2048 on 64 to 16,384 349 -> 220. Where
+// answers follow, which fill the places that shorter items leave, at twice the average: two chunks of 512
+// beside 62 answers 58 us, 67 at the average. Steps of prompts of one length are not split by it. (What passes
+// kPagedManyParts, few-row tiles go without, so that the room for items is the same.)
+constexpr int kPagedFewParts = 512, kPagedManyParts = 256, kPagedMostParts = 512;
 constexpr int kPagedFewKeys = 256, kPagedManyKeys = 512;
 constexpr int kPagedWholeKeys = 1024;
 constexpr int kPagedPadRows = 64;     // padding rows that one item zeroes
@@ -44,6 +54,8 @@ constexpr int kPagedItemWords = 12, kPagedMergeWords = 8;
 struct PagedLayout {
   int64_t seq, pos, counts, items, merges, words;  // offsets; cu lies at 0
   int64_t max_items, max_merges, max_part_rows;
+  int many_parts;  // parts of prompt tiles at most, and
+  int many_base;   // where there are fewer of them than that, and no few-row tiles
   bool wide;
 };
 inline int64_t up4(int64_t x) { return (x + 3) & ~int64_t(3); }
@@ -51,21 +63,27 @@ inline int64_t up4(int64_t x) { return (x + 3) & ~int64_t(3); }
 // at least its total (tiles times the longest of the sequence) / its number of parts keys, so the
 // tiles of a sequence of n > 1 parts stand for more than n - 1 >= n / 2 of them each, and all split
 // tiles have at most twice as many parts; each part holds at most the kind's rows, and a row is in at
-// most max_keys / kPagedFewKeys + 1 parts. A merge record takes 8 rows of a sequence of up to 8 parts,
-// or one row of one of more.
+// most max_keys / kPagedFewKeys + 1 parts. A merge record takes 8 rows, or one of more than 8 parts (of 32
+// in a prompt tile), which are then as many as the tile's rows by 4 (by 16) and more.
 inline PagedLayout paged_layout(int64_t n_seqs, int64_t n_tokens, int64_t hq, int64_t hkv,
                                 int64_t max_keys) {
   PagedLayout l;
   const int64_t tiles = (n_seqs < n_tokens ? n_seqs : n_tokens) + n_tokens * (hq / hkv) / kPagedTileRows;
   const bool split = max_keys > kPagedWholeKeys;
   const int64_t rows = n_tokens * hq;
-  l.wide = n_tokens > n_seqs && tiles * hkv <= kPagedWideTiles;
+  const bool prompts = n_tokens > n_seqs, few = prompts && split && tiles * hkv <= kPagedSplitTiles;
+  l.wide = prompts && !few && tiles * hkv <= kPagedWideTiles;
+  const int64_t fit = n_tokens * (hq / hkv) / (kPagedFewRows + 1);  // (prompt tiles, of more rows each)
+  const int64_t its = (fit < tiles ? fit : tiles) * hkv;
+  const int64_t many = few || its > kPagedMostParts ? kPagedMostParts : its < kPagedManyParts ? kPagedManyParts : its;
+  l.many_parts = (int)many;
+  l.many_base = few ? kPagedMostParts : kPagedManyParts;
   l.max_items = tiles * hkv + (split ? kPagedFewParts + kPagedManyParts : 0) +
                 (n_tokens + kPagedPadRows - 1) / kPagedPadRows;
-  const int64_t merges = kPagedFewParts * (kPagedFewRows / 8) + kPagedManyParts * (kPagedTileRows / 8);
+  const int64_t merges = kPagedFewParts * (kPagedFewRows / 8) + many * (kPagedTileRows / 8);
   l.max_merges = !split ? 0 : rows < merges ? rows : merges;
   const int64_t by_row = rows * (max_keys / kPagedFewKeys + 1);
-  const int64_t by_part = 2 * (kPagedFewParts * kPagedFewRows + kPagedManyParts * kPagedTileRows);
+  const int64_t by_part = 2 * (kPagedFewParts * kPagedFewRows + many * kPagedTileRows);
   l.max_part_rows = !split ? 0 : by_row < by_part ? by_row : by_part;
   l.seq = up4(n_seqs + 1);
   l.pos = l.seq + up4(n_tokens);
