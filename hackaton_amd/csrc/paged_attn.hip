@@ -580,9 +580,8 @@ struct Head {
   // 8-bit pages: where the row at `pos` of this page lies (of page 0 where there is none: what is read
   // there is not used), and its power of two, as a float, from the exponent byte. (Bytes that no row was
   // written with, behind a sequence's end, may be anything: 255 would be no number.)
-  __device__ inline const uint8_t* row8(uint64_t base, uint32_t stride, int page, int pos) const {
-    return reinterpret_cast<const uint8_t*>(base + (uint64_t)(uint32_t)max(page, 0) * stride +
-                                            ((uint32_t)pos & mask) * D);
+  __device__ inline uint64_t row8(uint64_t base, uint32_t stride, int page, int pos) const {
+    return base + (uint64_t)(uint32_t)max(page, 0) * stride + ((uint32_t)pos & mask) * D;
   }
   __device__ inline uint32_t exp8(const uint8_t* base, uint32_t stride, int head, int shift, int page, int pos) const {
     return base[(uint64_t)(uint32_t)max(page, 0) * stride + ((uint32_t)(head << shift) + ((uint32_t)pos & mask))];
@@ -834,11 +833,13 @@ __device__ inline void few_rows8(const PagedAttnArgs& a, const Item& it, lds_u16
   };
   auto fetch_keys = [&](int t) {
     const int pos = it.key + 32 * t;
-    const uint8_t* p0 = rows.row8(rows.k, rows.k_stride, pg[0], pos);
-    const uint8_t* p1 = rows.row8(rows.k, rows.k_stride, pg[1], pos + 16);
-    const uint8_t* p = (k_row < 16 ? p0 : p1) + (k_row & 15) * D + 16 * hi;
+    const uint64_t p0 = rows.row8(rows.k, rows.k_stride, pg[0], pos);
+    const uint64_t p1 = rows.row8(rows.k, rows.k_stride, pg[1], pos + 16);
+    // (as device memory: loads of any memory return out of order with LDS reads, and all are waited for)
+    typedef const __attribute__((address_space(1))) u32x4 device_u32x4;
+    device_u32x4* p = (device_u32x4*)((k_row < 16 ? p0 : p1) + (uint64_t)((k_row & 15) * D + 16 * hi));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) kr[i] = *reinterpret_cast<const u32x4*>(p + 32 * i);
+    for (int i = 0; i < 4; ++i) kr[i] = p[2 * i];
     ke = rows.exp8(a.pool.k_exp, a.pool.k_exp_stride, head, shift, k_row < 16 ? pg[0] : pg[1], pos + k_row);
   };
   auto fetch_values = [&](int t) {
@@ -861,7 +862,6 @@ __device__ inline void few_rows8(const PagedAttnArgs& a, const Item& it, lds_u16
     fetch_values(wave);
   }
   for (int t = wave; t < n_tiles; t += NW, ++i) {
-    const bool more = t + NW < n_tiles;
     const int kv0 = it.key + 32 * t;
     f32x16 s[1] = {f32x16{}};
     {
@@ -875,10 +875,10 @@ __device__ inline void few_rows8(const PagedAttnArgs& a, const Item& it, lds_u16
       for (int j = 0; j < 8; ++j)
         s[0] = E::mfma(numbers8<E>(kr[j >> 1][2 * (j & 1)], kr[j >> 1][2 * (j & 1) + 1], power), qf[j], s[0]);
     }
-    if (more) {
-      locate(t + NW, i + 1);
-      fetch_keys(t + NW);
-    }
+    // (behind the last tile too, where no page is: loads under a condition would all be waited for before the
+    // next tile's first use; with keys loaded as device memory, eight answers of 700 11.6 -> 11.0 us, four of 512 9.3 -> 9.0)
+    locate(t + NW, i + 1);
+    fetch_keys(t + NW);
     u32x4 pf[1][2];
     soften<E, 1>(s, kv0 + 31 > sight.from, sight.of(kv0), hi, scale_log2, 0.f, st, pf);
     const float power = power_of(ve);
@@ -891,7 +891,7 @@ __device__ inline void few_rows8(const PagedAttnArgs& a, const Item& it, lds_u16
       for (int c = 0; c < 2; ++c)
         st128(row + 8 * ((2 * m + c) ^ (r & 3)), numbers8<E>(vr[j][2 * c], vr[j][2 * c + 1], f));
     }
-    if (more) fetch_values(t + NW);
+    fetch_values(t + NW);
     u32x4 va[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) va[j] = read_v(vt, off, j);
