@@ -109,7 +109,7 @@ SIGNATURES = {
     "va_pages_compact": (ctypes.c_int, [_p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _i32, _i32,
                                         _p, _p, _p, _p, _i64, _p]),
     "va_paged_tree_words": (ctypes.c_int, [_pstep, _pi64]),
-    "va_paged_tree": (ctypes.c_int, [_pstep, _p, _p, _i64, _p]),
+    "va_paged_plan_tree": (ctypes.c_int, [_pstep, _p, _p, _i64, _p, _p, _i64, _p]),
     "va_paged_append_pages": (ctypes.c_int, [_pstep, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64,
                                              _p, _ppages, _i32, _i32, _i32, _p]),
     "va_paged_attention_pages": (ctypes.c_int, [_pstep, _p, _p, _ppages, _i32, _f32, _i32, _p, _p,

@@ -10,6 +10,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import check, lib
 from .attention import _DTYPES
@@ -47,6 +48,11 @@ def select_beams(logits, scores, beams, count=None, ended=None, end_token=None):
     if torch.is_grad_enabled() and (logits.requires_grad or scores.requires_grad):
         raise RuntimeError("the selection has no backward: call it under torch.no_grad() or "
                            "torch.inference_mode()")
+    if forward_ad._current_level >= 0:  # inside forward_ad.dual_level()
+        for t in (logits, scores):
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("the selection has no forward-mode derivative: pass the primals "
+                                   "(torch.autograd.forward_ad.unpack_dual)")
     if logits.dim() != 2 or logits.dtype not in _DTYPES:
         raise ValueError(f"logits must be (rows, vocab) in fp16, bf16 or fp32, got {tuple(logits.shape)} in "
                          f"{logits.dtype}")

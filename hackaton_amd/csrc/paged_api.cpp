@@ -174,21 +174,45 @@ extern "C" int va_paged_plan_words(const va_paged_step* step, int64_t* words) {
   return VA_OK;
 }
 
-extern "C" int va_paged_plan(const va_paged_step* step, const int32_t* q_lengths,
-                             const int32_t* kv_lengths, int64_t plan_words, void* stream) {
-  int rc = check_step(step, "va_paged_plan");
+namespace {
+
+int plan_checked(const va_paged_step* step, const int32_t* q_lengths, const int32_t* kv_lengths,
+                 int64_t plan_words, const int32_t* parents, int32_t* tree, int64_t tree_words,
+                 bool with_tree, void* stream, const char* what) {
+  int rc = check_step(step, what);
   if (rc) return rc;
   const va_paged_step& s = *step;
   if (s.n_tokens == 0) return VA_OK;
   const va::PagedLayout layout = layout_of(s);
   if (plan_words < layout.words)
-    return va::fail(VA_ECAPACITY, "va_paged_plan: %lld words, need %lld", (long long)plan_words,
+    return va::fail(VA_ECAPACITY, "%s: %lld words, need %lld", what, (long long)plan_words,
                     (long long)layout.words);
-  if ((rc = check_buffers({s.plan}, "va_paged_plan"))) return rc;
-  if (s.n_seqs > 0 && (rc = check_words({q_lengths, kv_lengths}, "va_paged_plan"))) return rc;
+  if (with_tree && tree_words < va::tree_words(s.n_tokens))
+    return va::fail(VA_ECAPACITY, "%s: %lld words of a tree, need %lld", what, (long long)tree_words,
+                    (long long)va::tree_words(s.n_tokens));
+  if ((rc = check_buffers({s.plan}, what))) return rc;
+  if (s.n_seqs > 0 && (rc = check_words({q_lengths, kv_lengths}, what))) return rc;
+  if (with_tree && ((rc = check_buffers({tree}, what)) || (rc = check_words({parents}, what)))) return rc;
   va::PagedPlanArgs a{q_lengths, kv_lengths, s.n_seqs, (int)s.n_tokens, s.hq, s.hkv,
-                      s.table_width * s.page_size, s.plan, layout, (hipStream_t)stream};
-  return launched(va::launch_paged_plan(a), "va_paged_plan");
+                      s.table_width * s.page_size, s.plan, layout, (hipStream_t)stream,
+                      with_tree ? parents : nullptr, with_tree ? tree : nullptr};
+  return launched(va::launch_paged_plan(a), what);
+}
+
+}  // namespace
+
+extern "C" int va_paged_plan(const va_paged_step* step, const int32_t* q_lengths,
+                             const int32_t* kv_lengths, int64_t plan_words, void* stream) {
+  return plan_checked(step, q_lengths, kv_lengths, plan_words, nullptr, nullptr, 0, false, stream,
+                      "va_paged_plan");
+}
+
+extern "C" int va_paged_plan_tree(const va_paged_step* step, const int32_t* q_lengths,
+                                  const int32_t* kv_lengths, int64_t plan_words,
+                                  const int32_t* parents, int32_t* tree, int64_t tree_words,
+                                  void* stream) {
+  return plan_checked(step, q_lengths, kv_lengths, plan_words, parents, tree, tree_words, true, stream,
+                      "va_paged_plan_tree");
 }
 
 extern "C" int va_paged_append(const va_paged_step* step, const void* q, const void* k,
@@ -253,23 +277,6 @@ extern "C" int va_paged_tree_words(const va_paged_step* step, int64_t* words) {
   if (words == nullptr) return va::fail(VA_EINVAL, "va_paged_tree_words: NULL output");
   *words = va::tree_words(step->n_tokens);
   return VA_OK;
-}
-
-extern "C" int va_paged_tree(const va_paged_step* step, const int32_t* parents, int32_t* tree,
-                             int64_t tree_words, void* stream) {
-  const char* what = "va_paged_tree";
-  int rc = check_step(step, what);
-  if (rc) return rc;
-  const va_paged_step& s = *step;
-  if (s.n_tokens == 0) return VA_OK;
-  if (tree_words < va::tree_words(s.n_tokens))
-    return va::fail(VA_ECAPACITY, "%s: %lld words, need %lld", what, (long long)tree_words,
-                    (long long)va::tree_words(s.n_tokens));
-  if ((rc = check_buffers({s.plan, tree}, what))) return rc;
-  if ((rc = check_words({parents}, what))) return rc;
-  va::PagedTreeArgs a{s.plan, layout_of(s), parents, s.n_seqs, (int)s.n_tokens, tree,
-                      (hipStream_t)stream};
-  return launched(va::launch_paged_tree(a), what);
 }
 
 namespace {

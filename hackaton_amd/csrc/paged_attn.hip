@@ -27,7 +27,7 @@
 // which the product needs transposed, through LDS.
 //
 // Trees of new tokens: the tiles that reach past the cached rows read, for every row, the bits of the
-// tokens on its path (paged_tree_kernel) instead of comparing places.
+// tokens on its path (tree_paths) instead of comparing places.
 #include <climits>
 
 #include "../../include/varlen_attn.h"
@@ -82,6 +82,51 @@ __device__ inline int last_at_most(const int* v, int n, int x) {
   return lo;
 }
 
+// ------------------------------------------------------------------------------------------------
+// trees
+// ------------------------------------------------------------------------------------------------
+// The paths of a sequence's new tokens by doubling (after round r a token knows the 2^r next ones on its way to
+// the root, and the one behind them), a work-group per sequence. Bounded by the latency of its first loads
+// and the rounds' barriers.
+static_assert(PT == kTreeTokens && PT <= 256, "a thread per token; eight bits of a sequence's number");
+struct TreeLds {
+  uint32_t path[PT][kTreeWords + 1];
+  int next[PT];
+};
+__device__ inline void tree_paths(const PagedPlanArgs& a, TreeLds& lds, int first, int count, int pos0) {
+  const int tid = threadIdx.x;
+  int32_t* positions = a.tree + tree_positions(a.n_tokens);
+  if (count <= 0) return;  // (the same in all threads)
+  if (count > kTreeTokens) {
+    for (int j = tid; j < count; j += PT) positions[first + j] = pos0 + j;
+    return;
+  }
+  uint32_t path[kTreeWords];
+#pragma unroll
+  for (int w = 0; w < kTreeWords; ++w) path[w] = tid >> 5 == w ? 1u << (tid & 31) : 0u;
+  int next = tid < count ? a.parents[first + tid] : -1;
+  if (next < 0 || next >= tid) next = -1;
+  while (__syncthreads_or(next >= 0)) {  // (at most 8 rounds: a parent comes before its token)
+#pragma unroll
+    for (int w = 0; w < kTreeWords; ++w) lds.path[tid][w] = path[w];
+    lds.next[tid] = next;
+    __syncthreads();
+    if (next >= 0) {
+#pragma unroll
+      for (int w = 0; w < kTreeWords; ++w) path[w] |= lds.path[next][w];
+      next = lds.next[next];
+    }
+  }
+  if (tid >= count) return;
+  int depth = -1;
+#pragma unroll
+  for (int w = 0; w < kTreeWords; ++w) depth += __builtin_popcount(path[w]);
+  u32x4* words = reinterpret_cast<u32x4*>(a.tree + (long)(first + tid) * kTreeWords);
+  words[0] = u32x4{path[0], path[1], path[2], path[3]};
+  words[1] = u32x4{path[4], path[5], path[6], path[7]};
+  positions[first + tid] = pos0 + depth;
+}
+
 // Rows of a merge record: one where few rows have many parts, which are then shared out in it. (16 trees of 32
 // tokens on 500 to 16,000, up to 26 parts: 11 us with one row each.)
 __device__ inline int merged_rows(bool few, int parts) { return parts <= (few ? 8 : 32) ? 8 : 1; }
@@ -98,8 +143,10 @@ __device__ inline int merged_rows(bool few, int parts) { return parts <= (few ? 
 // XCD i mod 8: with a multiple of 8 items per tile, the tiles that read the same keys run on one XCD
 // and find them in its L2, so the parts are rounded down to that where there are enough of them
 // (128 new tokens on 32,768, 28/4 heads: 9 parts per tile and head 85 us, 8 parts 80 us).
-template <int SPT>  // sequences per thread
-__global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int writers) {
+// With a tree and one sequence per thread, `n_seqs` more work-groups take a sequence's paths each (64 answers of 24
+// drafted tokens: 4 us in a launch of their own).
+template <int SPT, bool TREE>  // sequences per thread
+__global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int writers, int placers) {
   constexpr int S = PT * SPT;
   // of every sequence: first row, its position, items before it (per kind), workspace rows and merge
   // records before it, parts, keys of a part
@@ -142,6 +189,15 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
     n_rows[i] = ((int)min(at, (long long)a.n_tokens) - first) * group;
   }
   if (tid == PT - 1) s_cu[S] = (int)min(at, (long long)a.n_tokens);
+  if constexpr (TREE && SPT == 1) {
+    if ((int)blockIdx.x >= 2 * writers + placers) {
+      __shared__ TreeLds lds;
+      __syncthreads();
+      const int s = blockIdx.x - 2 * writers - placers;
+      tree_paths(a, lds, s_cu[s], s_cu[s + 1] - s_cu[s], s_pos0[s]);
+      return;
+    }
+  }
   if ((int)blockIdx.x >= 2 * writers) {
     __syncthreads();
     const int rows = s_cu[a.n_seqs], first = (blockIdx.x - 2 * writers) * kPlanRowsPerGroup;
@@ -154,6 +210,7 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
       }
       a.plan[a.layout.seq + n] = seq;
       a.plan[a.layout.pos + n] = pos;
+      if (TREE && seq < 0) a.tree[tree_positions(a.n_tokens) + n] = -1;
     }
     return;
   }
@@ -177,11 +234,11 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
         ((long long)sums[6 + 3 * k] << 38) + ((long long)sums[5 + 3 * k] << 19) + sums[4 + 3 * k];
     // (at most INT_MAX / 2, which no range is longer than: such a share splits nothing; a prompt of 2^20
     // tokens, 32/8 heads, makes 2^32. Rounded up and added to a range it stays below 2^31.)
-    const long long share =
-        split ? min(max((keys * a.hkv + parts - 1) / parts,
-                        (long long)(k == 0 ? kPagedManyKeys : kPagedFewKeys)),
-                    (long long)(INT_MAX / 2))
-              : INT_MAX / 2;
+    const long long least =
+        k == 1 ? kPagedFewKeys
+               : min(max(keys * a.hkv / kPagedShortItems, (long long)kPagedFewKeys), (long long)kPagedManyKeys);
+    const long long share = split ? min(max((keys * a.hkv + parts - 1) / parts, least), (long long)(INT_MAX / 2))
+                                  : INT_MAX / 2;
     chunks[k] = (int)((share + kPagedChunkKeys - 1) / kPagedChunkKeys * kPagedChunkKeys);
   }
   const int aligned = 8 / (a.hkv % 8 == 0 ? 8 : a.hkv % 4 == 0 ? 4 : a.hkv % 2 == 0 ? 2 : 1);
@@ -306,54 +363,11 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
   }
 }
 
-// ------------------------------------------------------------------------------------------------
-// trees
-// ------------------------------------------------------------------------------------------------
-// A work-group per sequence: the paths of its new tokens by doubling (after round r a token knows the 2^r
-// next ones on its way to the root, and the one behind them), in LDS; the other work-groups mark the
-// padding rows. Bounded by its launch and the rounds' barriers.
-static_assert(PT == kTreeTokens && PT <= 256, "a thread per token; eight bits of a sequence's number");
-__global__ __launch_bounds__(PT) void paged_tree_kernel(PagedTreeArgs a) {
-  __shared__ uint32_t s_path[PT][kTreeWords + 1];
-  __shared__ int s_next[PT];
-  const int tid = threadIdx.x, s = blockIdx.x;
-  int32_t* positions = a.tree + tree_positions(a.n_tokens);
-  if (s >= a.n_seqs) {
-    const int n = (s - a.n_seqs) * PT + tid;
-    if (n < a.n_tokens && n >= a.plan[a.n_seqs]) positions[n] = -1;
-    return;
-  }
-  const int first = min(max(a.plan[s], 0), a.n_tokens), count = min(a.plan[s + 1], a.n_tokens) - first;
-  if (count <= 0) return;
-  const int32_t* pos = a.plan + a.layout.pos + first;
-  if (count > kTreeTokens) {
-    for (int j = tid; j < count; j += PT) positions[first + j] = pos[j];
-    return;
-  }
-  uint32_t path[kTreeWords];
-#pragma unroll
-  for (int w = 0; w < kTreeWords; ++w) path[w] = tid >> 5 == w ? 1u << (tid & 31) : 0u;
-  int next = tid < count ? a.parents[first + tid] : -1;
-  if (next < 0 || next >= tid) next = -1;
-  while (__syncthreads_or(next >= 0)) {  // (at most 8 rounds: a parent comes before its token)
-#pragma unroll
-    for (int w = 0; w < kTreeWords; ++w) s_path[tid][w] = path[w];
-    s_next[tid] = next;
-    __syncthreads();
-    if (next >= 0) {
-#pragma unroll
-      for (int w = 0; w < kTreeWords; ++w) path[w] |= s_path[next][w];
-      next = s_next[next];
-    }
-  }
-  if (tid >= count) return;
-  int depth = -1;
-#pragma unroll
-  for (int w = 0; w < kTreeWords; ++w) depth += __builtin_popcount(path[w]);
-  u32x4* words = reinterpret_cast<u32x4*>(a.tree + (long)(first + tid) * kTreeWords);
-  words[0] = u32x4{path[0], path[1], path[2], path[3]};
-  words[1] = u32x4{path[4], path[5], path[6], path[7]};
-  positions[first + tid] = pos[0] + depth;
+// Trees of steps of more sequences than a planning work-group of one each has threads (one launch more).
+__global__ __launch_bounds__(PT) void paged_tree_kernel(PagedPlanArgs a) {
+  __shared__ TreeLds lds;
+  const int s = blockIdx.x, first = a.plan[s];
+  tree_paths(a, lds, first, a.plan[s + 1] - first, a.plan[a.layout.pos + min(first, a.n_tokens - 1)]);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -1324,15 +1338,14 @@ hipError_t launch_paged_plan(const PagedPlanArgs& a) {
   const int placers = (a.n_tokens + kPlanRowsPerGroup - 1) / kPlanRowsPerGroup;
   const int64_t wanted = (a.layout.max_items + PT - 1) / PT;
   const int writers = (int)(wanted < kPlanWriters ? wanted : kPlanWriters);
-  const auto kernel = a.n_seqs <= PT       ? paged_plan_kernel<1>
-                      : a.n_seqs <= 4 * PT ? paged_plan_kernel<4>
-                                           : paged_plan_kernel<kPagedMaxSeqs / PT>;
-  hipLaunchKernelGGL(kernel, dim3(2 * writers + placers), dim3(PT), 0, a.stream, a, writers);
-  return hipGetLastError();
-}
-
-hipError_t launch_paged_tree(const PagedTreeArgs& a) {
-  hipLaunchKernelGGL(paged_tree_kernel, dim3(a.n_seqs + (a.n_tokens + PT - 1) / PT), dim3(PT), 0, a.stream, a);
+  const bool tree = a.parents != nullptr, within = tree && a.n_seqs <= PT;
+  const auto kernel = a.n_seqs <= PT       ? (tree ? paged_plan_kernel<1, true> : paged_plan_kernel<1, false>)
+                      : a.n_seqs <= 4 * PT ? (tree ? paged_plan_kernel<4, true> : paged_plan_kernel<4, false>)
+                      : tree               ? paged_plan_kernel<kPagedMaxSeqs / PT, true>
+                                           : paged_plan_kernel<kPagedMaxSeqs / PT, false>;
+  hipLaunchKernelGGL(kernel, dim3(2 * writers + placers + (within ? a.n_seqs : 0)), dim3(PT), 0, a.stream, a,
+                     writers, placers);
+  if (tree && !within) hipLaunchKernelGGL(paged_tree_kernel, dim3(a.n_seqs), dim3(PT), 0, a.stream, a);
   return hipGetLastError();
 }
 

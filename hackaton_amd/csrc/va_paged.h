@@ -44,7 +44,10 @@ constexpr int kPagedWideTiles = 512, kPagedSplitTiles = 200;
 // beside 62 answers 58 us, 67 at the average. Steps of prompts of one length are not split by it. (What passes
 // kPagedManyParts, few-row tiles go without, so that the room for items is the same.)
 constexpr int kPagedFewParts = 512, kPagedManyParts = 256, kPagedMostParts = 512;
-constexpr int kPagedFewKeys = 256, kPagedManyKeys = 512;
+// Prompt parts are shorter than kPagedManyKeys, down to kPagedFewKeys, while that makes no more than
+// kPagedShortItems of them (us with the merge, 512 / shorter: 300 new tokens on 700, 12/2 heads 19.6 / 16.5; with
+// 384 items 512 on 1536 23.3 / 27.3, two of 64 on 8000 25.3 / 28.0).
+constexpr int kPagedFewKeys = 256, kPagedManyKeys = 512, kPagedShortItems = 192;
 constexpr int kPagedWholeKeys = 1024;
 constexpr int kPagedPadRows = 64;     // padding rows that one item zeroes
 
@@ -108,6 +111,8 @@ struct PagedPlanArgs {
   int32_t* plan;
   PagedLayout layout;
   hipStream_t stream;
+  const int32_t* parents;  // null: no tree
+  int32_t* tree;
 };
 
 // Pages of one layer. 8-bit pages have a byte per row beside them, the exponent of its power of two.
@@ -134,14 +139,6 @@ constexpr int kTreeTokens = 256, kTreeWords = kTreeTokens / 32;
 constexpr int64_t tree_positions(int64_t n_tokens) { return n_tokens * kTreeWords; }
 inline int64_t tree_words(int64_t n_tokens) { return tree_positions(n_tokens) + up4(n_tokens); }
 
-struct PagedTreeArgs {
-  const int32_t* plan;
-  PagedLayout layout;
-  const int32_t* parents;
-  int n_seqs, n_tokens;
-  int32_t* tree;
-  hipStream_t stream;
-};
 
 struct PagedAttnArgs {
   const void* q;
@@ -237,7 +234,6 @@ struct PagedAcceptArgs {
 };
 
 hipError_t launch_paged_plan(const PagedPlanArgs& a);
-hipError_t launch_paged_tree(const PagedTreeArgs& a);
 hipError_t launch_paged_accept(const PagedAcceptArgs& a);
 hipError_t launch_paged_attention(const PagedAttnArgs& a);
 hipError_t launch_paged_append(const PagedAppendArgs& a);

@@ -243,7 +243,7 @@ def paged_plan(page_table, q_lengths, kv_lengths, n_tokens, heads, kv_heads, pag
     cached tokens directly; (n_tokens) int32 on the GPU or a host list. A row then sees the tokens cached
     before the step, those on its path, and itself. At most 256 new tokens of a sequence form a tree; those
     of a longer one follow each other whatever `tree` holds (host lists that say otherwise are refused,
-    device ones are not read; there, what names no earlier token counts as -1). Another launch."""
+    device ones are not read; there, what names no earlier token counts as -1)."""
     device = _one_device(page_table)
     if device.index != _current_device():  # launches and allocations go to the tensors' device
         with torch.cuda.device(device):
@@ -269,15 +269,17 @@ def paged_plan(page_table, q_lengths, kv_lengths, n_tokens, heads, kv_heads, pag
     plan._capture = attention._capture_id() if torch._C._cuda_isCurrentStreamCapturing() else None
     plan._step = _lib.PagedStep(page_table.data_ptr(), plan.words.data_ptr(), n_tokens, n_seqs, width,
                                 page_size, heads, kv_heads)
-    check(lib().va_paged_plan(plan._step, q_lengths.data_ptr(), kv_lengths.data_ptr(), n_words,
-                              plan._stream), "va_paged_plan")
-    plan._tree = plan._paths = None
-    if parents is not None:
-        n_words = _tree_words(n_seqs, n_tokens, heads, kv_heads, page_size, width)
-        plan._paths = torch.empty(n_words, dtype=torch.int32, device=device)
-        plan._tree = plan._paths.data_ptr()
-        check(lib().va_paged_tree(plan._step, parents.data_ptr(), plan._tree, n_words, plan._stream),
-              "va_paged_tree")
+    if parents is None:
+        plan._tree = plan._paths = None
+        check(lib().va_paged_plan(plan._step, q_lengths.data_ptr(), kv_lengths.data_ptr(), n_words,
+                                  plan._stream), "va_paged_plan")
+        return plan
+    tree_words = _tree_words(n_seqs, n_tokens, heads, kv_heads, page_size, width)
+    plan._paths = torch.empty(tree_words, dtype=torch.int32, device=device)
+    plan._tree = plan._paths.data_ptr()
+    check(lib().va_paged_plan_tree(plan._step, q_lengths.data_ptr(), kv_lengths.data_ptr(), n_words,
+                                   parents.data_ptr(), plan._tree, tree_words, plan._stream),
+          "va_paged_plan_tree")
     return plan
 
 

@@ -391,8 +391,8 @@ int va_pages_compact(void* pages, int64_t outer, int32_t n_pages, int32_t kv_hea
  * (at least Hkv page_size, under 2^31): the row's values are its numbers times 2^(e - 127). e is the smallest
  * from 27 on that brings the row's largest finite number to 448 or less; what is not finite is held as
  * not a number. Strides are in elements (multiples of 8; of 16 for VA_E4M3).
- * `tree` is NULL (the new tokens of every sequence follow each other) or what va_paged_tree wrote:
- * va_paged_tree_words int32 of device memory, 16-byte aligned, for the plan that it was given with.
+ * `tree` is NULL (the new tokens of every sequence follow each other) or what va_paged_plan_tree wrote beside
+ * the plan: va_paged_tree_words int32 of device memory, 16-byte aligned.
  * parents (n_tokens): of every row the number, among the new tokens of its sequence, of the one that it
  * follows (an earlier one); anything else: it follows the cached rows directly. A row then sees the rows
  * cached before the step, the tokens on its path and itself; its position, which it is rotated by, is
@@ -411,8 +411,9 @@ typedef struct va_paged_pages {
   int32_t dtype;
 } va_paged_pages;
 int va_paged_tree_words(const va_paged_step* step, int64_t* words);
-int va_paged_tree(const va_paged_step* step, const int32_t* parents, int32_t* tree,
-                  int64_t tree_words, void* stream);
+int va_paged_plan_tree(const va_paged_step* step, const int32_t* q_lengths, const int32_t* kv_lengths,
+                       int64_t plan_words, const int32_t* parents, int32_t* tree,
+                       int64_t tree_words, void* stream);
 
 /* va_paged_append into pages of either kind; out_dtype is q_out's type (that of 16-bit pages). */
 int va_paged_append_pages(const va_paged_step* step, const int32_t* tree, const void* q, const void* k,

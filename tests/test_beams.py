@@ -62,13 +62,17 @@ def test_tree_arguments_are_checked():
     assert L.va_paged_tree_words(None, ctypes.byref(words)) == _lib.VA_EINVAL
     assert L.va_paged_tree_words(step(p), None) == _lib.VA_EINVAL
     assert L.va_paged_tree_words(step(p, hq=13), ctypes.byref(words)) == _lib.VA_ESHAPE
-    need = 8 * 8 + 8
-    for args, code in (((step(p), None, p, need, None), _lib.VA_EINVAL), ((step(p), p, None, need, None), _lib.VA_EINVAL),
-                       ((step(p), p + 2, p, need, None), _lib.VA_EINVAL), ((step(p), p, p + 4, need, None), _lib.VA_EINVAL),
-                       ((step(p), p, p, need - 1, None), _lib.VA_ECAPACITY),
-                       ((step(p, page_size=20), p, p, need, None), _lib.VA_ESHAPE),
-                       ((step(p, n_tokens=0), None, None, 0, None), _lib.VA_OK)):
-        assert L.va_paged_tree(*args) == code
+    need, room = 8 * 8 + 8, 1 << 30
+    for args, code in (((step(p), p, p, room, None, p, need, None), _lib.VA_EINVAL),
+                       ((step(p), p, p, room, p, None, need, None), _lib.VA_EINVAL),
+                       ((step(p), p, p, room, p + 2, p, need, None), _lib.VA_EINVAL),
+                       ((step(p), p, p, room, p, p + 4, need, None), _lib.VA_EINVAL),
+                       ((step(p), None, p, room, p, p, need, None), _lib.VA_EINVAL),
+                       ((step(p), p, p, 8, p, p, need, None), _lib.VA_ECAPACITY),
+                       ((step(p), p, p, room, p, p, need - 1, None), _lib.VA_ECAPACITY),
+                       ((step(p, page_size=20), p, p, room, p, p, need, None), _lib.VA_ESHAPE),
+                       ((step(p, n_tokens=0), None, None, 0, None, None, 0, None), _lib.VA_OK)):
+        assert L.va_paged_plan_tree(*args) == code
 
 
 @pytest.mark.parametrize("at,value,code", [

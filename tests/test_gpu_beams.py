@@ -268,6 +268,10 @@ def test_refusals():
         select_beams(logits.float().requires_grad_(), scores, 4)
     with pytest.raises(RuntimeError, match="no backward"):
         select_beams(logits, scores.clone().requires_grad_(), 4)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(logits.float(), torch.ones(12, 100, device="cuda"))
+        with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            select_beams(dual, scores, 4)
     got = select_beams(logits[:0], scores[:0], 4)
     assert [x.shape for x in got] == [(0, 4)] * 3
     cache = PagedCache(1, 8, 16, 1, 4, 64)
