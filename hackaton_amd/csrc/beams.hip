@@ -9,11 +9,12 @@
 // numbers, and the best numbers in them. Scores are formed and compared in 64 bits, score + (number - log
 // of the sum): a rounding to 32 would make ties of continuations that are not as good.
 //
-// The first kernel is bounded by memory, and for 16-bit numbers nearly as much by its arithmetic (a power of
-// two, 16 cycles of a wave, and six other instructions a number): 512 rows of 150,016 numbers (154 MB) 34 us,
-// 4.6 TB/s; of 75,008 fp32 numbers, as many bytes, 30 us. 1, 2 and 4 pieces on their way and 1024 to 8192
-// work-groups measured 34 to 47. The second kernel is bounded by the latency of its steps: 9 us for a prompt
-// of four beams, 11 us for 64 of eight (13.8 and 33.7 with 256 threads, which computed each key twice).
+// The first kernel is bounded by memory, and for 16-bit numbers nearly as much by its arithmetic (a
+// power of two, 16 cycles of a wave, and six other instructions a number): 512 rows of 150,016 numbers
+// (154 MB) 34 us, 4.6 TB/s; of 75,008 fp32 numbers, as many bytes, 30 us. 1, 2 and 4 pieces on their
+// way and 1024 to 8192 work-groups measured 34 to 47. The second kernel is bounded by the latency of
+// its steps: 9 us for a prompt of four beams, 11 us for 64 of eight (13.8 and 33.7 with 256 threads,
+// which computed each key twice).
 #include <climits>
 #include <type_traits>
 
@@ -57,8 +58,8 @@ struct Numbers {
 
 // The same on the way: 16-bit numbers that begin in the middle of a word (ODD) are loaded as the words that
 // they lie in, from the number before them to the one behind them, and shifted when they are used (512 rows
-// of 150,001: 36 us, 39 with loads that straddle words). Not by cells that begin elsewhere: rows that hold the
-// same numbers have the same sum to the last bit, or equal scores would be no ties.
+// of 150,001: 36 us, 39 with loads that straddle words). Not by cells that begin elsewhere: rows that
+// hold the same numbers have the same sum to the last bit, or equal scores would be no ties.
 template <int DT, bool ODD>
 struct Coming {
   Numbers<DT> x;
@@ -104,11 +105,11 @@ __device__ inline float wave_max_last(float x) {
   return dpp_max<0x143, 0xc>(x);  // row_bcast 31: lane 31 to rows 2, 3
 }
 
-// Exponentials are powers of two, number * kLog2e less the reference of the largest number so far. Up to 2^16
-// that is largest * kLog2e rounded, so that a power costs a fused multiply-add and one rounding, of a
-// difference; from there on, where that rounding would count, the product itself: differences of numbers
-// are taken first. kLog2e, rounded, stands for the base: the second kernel divides by it, so a shift of all
-// numbers shifts the result.
+// Exponentials are powers of two, number * kLog2e less the reference of the largest number so far. Up
+// to 2^16 that is largest * kLog2e rounded, so that a power costs a fused multiply-add and one
+// rounding, of a difference; from there on, where that rounding would count, the product itself:
+// differences of numbers are taken first. kLog2e, rounded, stands for the base: the second kernel
+// divides by it, so a shift of all numbers shifts the result.
 __device__ inline bool far_out(float largest) { return fabsf(largest) >= 65536.f; }
 // Power of two by which a sum over the reference of `was` has to be multiplied for that of `is`.
 __device__ inline float rescale(float was, float is) {
@@ -424,8 +425,8 @@ __global__ __launch_bounds__(PT) void beams_pick_kernel(BeamsArgs a) {
   }
   in_order(s, n, s_runs, [&](int i) { return i / l.cells * kBeamsVocab + i % l.cells * l.cell; });
 
-  // the best runs in them where their numbers are too many, then the numbers. Each thread takes kNumbers at a
-  // time. Index of a number: beam * 2^18 + token (of a run: its first number's).
+  // the best runs in them where their numbers are too many, then the numbers. Each thread takes
+  // kNumbers at a time. Index of a number: beam * 2^18 + token (of a run: its first number's).
   auto see = [&](int at, float (&x)[kNumbers]) {  // numbers from `at` on; returns how many there are
     const int beam = at / kBeamsVocab, token = at % kBeamsVocab, some = min(a.vocab - token, kNumbers);
     if (some <= 0) return 0;

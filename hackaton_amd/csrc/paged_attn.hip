@@ -85,9 +85,9 @@ __device__ inline int last_at_most(const int* v, int n, int x) {
 // ------------------------------------------------------------------------------------------------
 // trees
 // ------------------------------------------------------------------------------------------------
-// The paths of a sequence's new tokens by doubling (after round r a token knows the 2^r next ones on its way to
-// the root, and the one behind them), a work-group per sequence. Bounded by the latency of its first loads
-// and the rounds' barriers.
+// The paths of a sequence's new tokens by doubling (after round r a token knows the 2^r next ones on
+// its way to the root, and the one behind them), a work-group per sequence. Bounded by the latency of
+// its first loads and the rounds' barriers.
 static_assert(PT == kTreeTokens && PT <= 256, "a thread per token; eight bits of a sequence's number");
 struct TreeLds {
   uint32_t path[PT][kTreeWords + 1];
@@ -127,8 +127,14 @@ __device__ inline void tree_paths(const PagedPlanArgs& a, TreeLds& lds, int firs
   positions[first + tid] = pos0 + depth;
 }
 
-// Rows of a merge record: one where few rows have many parts, which are then shared out in it. (16 trees of 32
-// tokens on 500 to 16,000, up to 26 parts: 11 us with one row each.)
+// x / by for x >= 0, by > 0. (The division of 64 bits is a hundred instructions, in the one wave of a
+// SIMD.)
+__device__ inline long long quotient(long long x, long long by) {
+  return ((x | by) >> 32) == 0 ? (long long)((uint32_t)x / (uint32_t)by) : x / by;
+}
+
+// Rows of a merge record: one where few rows have many parts, which are then shared out in it. (16
+// trees of 32 tokens on 500 to 16,000, up to 26 parts: 11 us with one row each.)
 __device__ inline int merged_rows(bool few, int parts) { return parts <= (few ? 8 : 32) ? 8 : 1; }
 
 // The first `writers` work-groups write the items, as many the merge records, the others place the rows.
@@ -143,8 +149,8 @@ __device__ inline int merged_rows(bool few, int parts) { return parts <= (few ? 
 // XCD i mod 8: with a multiple of 8 items per tile, the tiles that read the same keys run on one XCD
 // and find them in its L2, so the parts are rounded down to that where there are enough of them
 // (128 new tokens on 32,768, 28/4 heads: 9 parts per tile and head 85 us, 8 parts 80 us).
-// With a tree and one sequence per thread, `n_seqs` more work-groups take a sequence's paths each (64 answers of 24
-// drafted tokens: 4 us in a launch of their own).
+// With a tree and one sequence per thread, `n_seqs` more work-groups take a sequence's paths each (64
+// answers of 24 drafted tokens: 4 us in a launch of their own).
 template <int SPT, bool TREE>  // sequences per thread
 __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int writers, int placers) {
   constexpr int S = PT * SPT;
@@ -217,14 +223,15 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
   // (lengths that pass the rows are cut there, which may change a tile's kind: such a step is not split)
   const bool split =
       a.max_keys > kPagedWholeKeys && ((long long)sums[1] << 15) + sums[0] <= a.n_tokens;
-  int chunks[2];
-  // parts of prompt tiles that are as many as the card has places (few-row tiles behind them fill the places
-  // that shorter ones leave)
+  int chunks[2] = {INT_MAX / 2, INT_MAX / 2};
+  // parts of prompt tiles that are as many as the card has places (few-row tiles behind them fill the
+  // places that shorter ones leave)
   const long long its = (long long)sums[2] * a.hkv;
   const long long many = min(max(sums[3] == 0 ? its : its / 2, (long long)kPagedManyParts / 4),
                              (long long)a.layout.many_parts);
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
+  for (int k = 0; k < 2 && split; ++k) {
+    if (sums[2 + k] == 0) continue;  // (no such tile)
     const long long items = (long long)sums[2 + k] * a.hkv;
     const long long all = k == 1         ? kPagedFewParts - max(0LL, many - kPagedManyParts)
                           : sums[3] == 0 ? a.layout.many_base
@@ -236,9 +243,10 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
     // tokens, 32/8 heads, makes 2^32. Rounded up and added to a range it stays below 2^31.)
     const long long least =
         k == 1 ? kPagedFewKeys
-               : min(max(keys * a.hkv / kPagedShortItems, (long long)kPagedFewKeys), (long long)kPagedManyKeys);
-    const long long share = split ? min(max((keys * a.hkv + parts - 1) / parts, least), (long long)(INT_MAX / 2))
-                                  : INT_MAX / 2;
+               : min(max(quotient(keys * a.hkv, kPagedShortItems), (long long)kPagedFewKeys),
+                     (long long)kPagedManyKeys);
+    const long long share =
+        min(max(quotient(keys * a.hkv + parts - 1, parts), least), (long long)(INT_MAX / 2));
     chunks[k] = (int)((share + kPagedChunkKeys - 1) / kPagedChunkKeys * kPagedChunkKeys);
   }
   const int aligned = 8 / (a.hkv % 8 == 0 ? 8 : a.hkv % 4 == 0 ? 4 : a.hkv % 2 == 0 ? 2 : 1);
@@ -277,9 +285,9 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
     for (int k = 0; k < 4; ++k) x[k] += own[i][k];
   }
   __syncthreads();
-  // Prompt tiles of unequal ranges, more than the card has places and nothing behind them: the sequences with the
-  // longest ranges first, so that what starts last is short (64 trees on 64 to 8192 tokens 78 -> 58 us for
-  // 1 us here; up to PT sequences, by counting).
+  // Prompt tiles of unequal ranges, more than the card has places and nothing behind them: the
+  // sequences with the longest ranges first, so that what starts last is short (64 trees on 64 to 8192
+  // tokens 78 -> 58 us for 1 us here; up to PT sequences, by counting).
   bool sorted = false;
   if constexpr (SPT == 1) {
     sorted = n[0] > kPagedManyParts && n[1] == 0 && n[2] > 0;
@@ -782,10 +790,10 @@ __device__ inline void few_rows(const PagedAttnArgs& a, const Item& it, lds_u16*
 
 // 8-bit pages. Keys: lane (row, hi) of the operand loads its row's 16-byte pieces 2 i + hi, i = 0..3; piece
 // i serves two products, whose k slots 8 hi + 0..7 are then numbers 16 (2 i + hi) + 8 half + 0..7 of a row,
-// in the queries too. Values: 16 numbers of row 8 j + lane / 8 per lane and load, turned into 16-bit rows of
-// the wave's own LDS tile. A tile's loads are issued when the registers of the one before are free: keys
-// after its products, values after their rows are in LDS, so that 8 KB per wave are in flight but for the
-// conversions.
+// in the queries too. Values: 16 numbers of row 8 j + lane / 8 per lane and load, turned into 16-bit
+// rows of the wave's own LDS tile. A tile's loads are issued when the registers of the one before are
+// free: keys after its products, values after their rows are in LDS, so that 8 KB per wave are in
+// flight but for the conversions.
 template <class E>
 __device__ inline u32x4 numbers8(uint32_t lo, uint32_t hi, float power) {
   return u32x4{E::from_e4m3(lo, power, false), E::from_e4m3(lo, power, true),
@@ -889,8 +897,9 @@ __device__ inline void few_rows8(const PagedAttnArgs& a, const Item& it, lds_u16
       for (int j = 0; j < 8; ++j)
         s[0] = E::mfma(numbers8<E>(kr[j >> 1][2 * (j & 1)], kr[j >> 1][2 * (j & 1) + 1], power), qf[j], s[0]);
     }
-    // (behind the last tile too, where no page is: loads under a condition would all be waited for before the
-    // next tile's first use; with keys loaded as device memory, eight answers of 700 11.6 -> 11.0 us, four of 512 9.3 -> 9.0)
+    // (behind the last tile too, where no page is: loads under a condition would all be waited for
+    // before the next tile's first use; with keys loaded as device memory, eight answers of 700 11.6 ->
+    // 11.0 us, four of 512 9.3 -> 9.0)
     locate(t + NW, i + 1);
     fetch_keys(t + NW);
     u32x4 pf[1][2];
@@ -932,9 +941,9 @@ __device__ inline void many_rows(const PagedAttnArgs& a, const Item& it, lds_u16
   // numbers of its next 64 tiles are in its lanes.
   const Head rows(a, it, head, P8 ? D : D * 2);
   int pages = 0, tc = 0;
-  // 8-bit pages: a wave fetches 4 GROUPS rows of K and of V into registers (16 numbers of row 8 j + lane / 8
-  // per lane and load; the powers of K rows in lanes 0 to 15, of V rows in lanes 16 to 31) and places them
-  // as 16-bit rows in their stage.
+  // 8-bit pages: a wave fetches 4 GROUPS rows of K and of V into registers (16 numbers of row 8 j +
+  // lane / 8 per lane and load; the powers of K rows in lanes 0 to 15, of V rows in lanes 16 to 31) and
+  // places them as 16-bit rows in their stage.
   constexpr int PIECES = 4 * GROUPS / 8;
   u32x4 kr[PIECES], vr[PIECES];
   uint32_t ex = 0;
@@ -1206,8 +1215,8 @@ __global__ __launch_bounds__(Shape<W>::THREADS, 2) void paged_attn_kernel(PagedA
   }
 }
 
-// Parts of split key ranges: a record of 8 rows has 32 lanes (4 elements each) per row, one of a single row and
-// many parts shares the parts out to the 8 groups of 32 lanes.
+// Parts of split key ranges: a record of 8 rows has 32 lanes (4 elements each) per row, one of a single
+// row and many parts shares the parts out to the 8 groups of 32 lanes.
 struct Sum {
   float m, l;
   f32x4 o;

@@ -23,30 +23,30 @@ constexpr int kPagedChunkKeys = 64;  // key ranges are split at multiples of thi
 // for the others. us with 4 / 8 waves: 2 x 2048 tokens, 12/2 heads (388 tiles) 51 / 42; 4096 tokens
 // (386) 88 / 72; 8 x 300 on 700 (240) 27.5 / 26; two chunks of 512 beside 62 answers, 28/4 heads (492) 60 /
 // 59; 2 x 1024 on 500 (456) 46.5 / 47.5; 3 x 1024 (684) 62 / 67; 4 x 1024 (912) 78 / 82; four chunks of
-// 2048 623 / 680; 64 answers of 64 to 8192 tokens 30.4 / 32.0, 16 of 1500 12.1 / 12.8, four of 512 7.9 / 7.5.
-// Steps of few prompt tiles over ranges that are split take 4 waves too, and twice the parts: two work-groups
-// of a CU wait for different barriers. us, 8 waves and 256 parts / 4 and 512, 28/4 heads: 16 trees of 24 on 4000 75
-// / 53, 8 of 48 to 64 on 28,672 to 32,768 305 / 268, 512 new tokens on 8192 98 / 86, on 4096 55 / 55, 1024 new
-// ones (the table's bound 228) on 4096 106 / 106, 8 x 300 on 700, 12/2 heads (240) 29 / 39.
+// 2048 623 / 680; 64 answers of 64 to 8192 tokens 30.4 / 32.0, 16 of 1500 12.1 / 12.8, four of 512 7.9
+// / 7.5. Steps of few prompt tiles over ranges that are split take 4 waves too, and twice the parts:
+// two work-groups of a CU wait for different barriers. us, 8 waves and 256 parts / 4 and 512, 28/4
+// heads: 16 trees of 24 on 4000 75 / 53, 8 of 48 to 64 on 28,672 to 32,768 305 / 268, 512 new tokens on
+// 8192 98 / 86, on 4096 55 / 55, 1024 new ones (the table's bound 228) on 4096 106 / 106, 8 x 300 on
+// 700, 12/2 heads (240) 29 / 39.
 constexpr int kPagedWideTiles = 512, kPagedSplitTiles = 200;
 // Parts that a step's keys are split into, by kind of tile, the shortest part (but a range's last) and
 // the longest table row that is never split. us at 384 / 512 / 1024 few-row parts: 64 answers of 64 to
 // 8192 tokens, 12/2 heads 34 / 30 / 32, four of 65,536, 28/4 heads 103 / 97 / 100; shortest few-row part
 // 128 / 256 / 512: one answer of 8192 9.0 / 9.8 / 11.5, 16 of 1500 13.4 / 12.1 / 12.6. At 256 / 512
-// prompt parts: two chunks of 512 beside 62 answers 57 / 76, 128 new tokens on 32,768 80 / 94; shortest
-// prompt part 256 / 512 / 704: 300 new tokens on 1000 16.8 / 17.7 / 20.4, two of 64 on 8000 26.9 / 27.0 /
-// 27.8, where 256 would make twice the parts and room for the merge. Four answers of 512, table rows of
-// 576: split 8.5, whole 7.9 and a launch less.
-// Prompt tiles that are as many as the card has places (tiles x heads) are split where they are longer than the
-// average one, into up to kPagedMostParts parts: 64 trees of 24 tokens on 64 to 8192, 28/4
-// heads (512 items) 162 -> 59 us and 3 more to merge, 16 chunks of 64 to 2048 on 64 to 16,384 349 -> 220. Where
-// answers follow, which fill the places that shorter items leave, at twice the average: two chunks of 512
-// beside 62 answers 58 us, 67 at the average. Steps of prompts of one length are not split by it. (What passes
-// kPagedManyParts, few-row tiles go without, so that the room for items is the same.)
+// prompt parts: two chunks of 512 beside 62 answers 57 / 76, 128 new tokens on 32,768 80 / 94. Four answers
+// of 512, table rows of 576: split 8.5, whole 7.9 and a launch less.
+// Prompt tiles that are as many as the card has places (tiles x heads) are split where they are longer
+// than the average one, into up to kPagedMostParts parts: 64 trees of 24 tokens on 64 to 8192, 28/4
+// heads (512 items) 162 -> 59 us and 3 more to merge, 16 chunks of 64 to 2048 on 64 to 16,384 349 ->
+// 220. Where answers follow, which fill the places that shorter items leave, at twice the average: two
+// chunks of 512 beside 62 answers 58 us, 67 at the average. Steps of prompts of one length are not
+// split by it. (What passes kPagedManyParts, few-row tiles go without, so that the room for items is
+// the same.)
 constexpr int kPagedFewParts = 512, kPagedManyParts = 256, kPagedMostParts = 512;
 // Prompt parts are shorter than kPagedManyKeys, down to kPagedFewKeys, while that makes no more than
-// kPagedShortItems of them (us with the merge, 512 / shorter: 300 new tokens on 700, 12/2 heads 19.6 / 16.5; with
-// 384 items 512 on 1536 23.3 / 27.3, two of 64 on 8000 25.3 / 28.0).
+// kPagedShortItems of them (us with the merge, 512 / shorter: 300 new tokens on 700, 12/2 heads 19.6 /
+// 16.5; with 384 items 512 on 1536 23.3 / 27.3, two of 64 on 8000 25.3 / 28.0).
 constexpr int kPagedFewKeys = 256, kPagedManyKeys = 512, kPagedShortItems = 192;
 constexpr int kPagedWholeKeys = 1024;
 constexpr int kPagedPadRows = 64;     // padding rows that one item zeroes
@@ -138,7 +138,6 @@ constexpr int kExpBias = 127, kExpMin = 27;
 constexpr int kTreeTokens = 256, kTreeWords = kTreeTokens / 32;
 constexpr int64_t tree_positions(int64_t n_tokens) { return n_tokens * kTreeWords; }
 inline int64_t tree_words(int64_t n_tokens) { return tree_positions(n_tokens) + up4(n_tokens); }
-
 
 struct PagedAttnArgs {
   const void* q;

@@ -342,7 +342,7 @@ def paged_append(q, k, v, cos, sin, k_pages, v_pages, plan, dtype=None):
     nothing; padding and positions outside the cos / sin table give zeros in q. Pages may be
     `QuantizedPages`: keys, rotated, and values go into them in 8 bits. `dtype` is then q's, fp16 or bf16
     (None: the projections' type, fp16 for fp32 ones)."""
-    keys, values = _split(k_pages)[0], _split(v_pages)[0]
+    (keys, k_exps), (values, v_exps) = _split(k_pages), _split(v_pages)
     device = _one_device(q, k, v, cos, sin, keys, values, plan.words)
     if device.index != _current_device():  # launches and allocations go to the tensors' device
         with torch.cuda.device(device):
@@ -358,10 +358,10 @@ def paged_append(q, k, v, cos, sin, k_pages, v_pages, plan, dtype=None):
     if not (q.dtype == k.dtype == v.dtype) or q.dtype not in _DTYPES:
         raise ValueError(f"q, k and v must share a dtype (fp16, bf16 or fp32), got {q.dtype}, "
                          f"{k.dtype}, {v.dtype}")
-    plain = plan._tree is None and keys is k_pages and values is v_pages  # 16 bits, no tree
+    plain = plan._tree is None and k_exps is None and v_exps is None  # 16 bits, no tree
     if dtype is None:
-        dtype = keys.dtype if keys is k_pages else q.dtype if q.dtype != torch.float32 else torch.float16
-    elif dtype not in (torch.float16, torch.bfloat16) or (keys is k_pages and dtype != keys.dtype):
+        dtype = keys.dtype if k_exps is None else q.dtype if q.dtype != torch.float32 else torch.float16
+    elif dtype not in (torch.float16, torch.bfloat16) or (k_exps is None and dtype != keys.dtype):
         raise ValueError(f"queries in {dtype} over pages in {keys.dtype}")
     if plain:
         out_dtype = _attn_dtype(k_pages)
@@ -409,19 +409,19 @@ def paged_attention(query, k_pages, v_pages, plan, scale):
     The same step gives the same bits; the same sequence in another step agrees to rounding. Pages may be
     `QuantizedPages`, under queries in fp16 or bf16: their values are multiplied as numbers of that type,
     exactly but for what passes fp16's range."""
-    keys, values = _split(k_pages)[0], _split(v_pages)[0]
+    (keys, k_exps), (values, v_exps) = _split(k_pages), _split(v_pages)
     device = _one_device(query, keys, values, plan.words)
     if device.index != _current_device():  # launches and allocations go to the tensors' device
         with torch.cuda.device(device):
             return paged_attention(query, k_pages, v_pages, plan, scale)
     _no_grad(query, keys, values)
     dtype = _attn_dtype(query)
-    if keys is k_pages and keys.dtype != query.dtype:
+    if k_exps is None and keys.dtype != query.dtype:
         raise ValueError(f"query in {query.dtype}, pages in {keys.dtype}")
     n, heads = plan.n_tokens, plan.heads
     if query.shape != (n, heads, HEAD_DIM):
         raise ValueError(f"query must be ({n}, {heads}, {HEAD_DIM}), got {tuple(query.shape)}")
-    plain = plan._tree is None and keys is k_pages and values is v_pages  # 16 bits, no tree
+    plain = plan._tree is None and k_exps is None and v_exps is None  # 16 bits, no tree
     if plain:
         k_stride, v_stride, n_pages = _pages_of(k_pages, v_pages, plan)
     else:
@@ -447,9 +447,8 @@ def paged_attention(query, k_pages, v_pages, plan, scale):
 # ------------------------------------------------------------------------------------------------
 # page bookkeeping
 # ------------------------------------------------------------------------------------------------
-def _pool_of(pages):
+def _pool_of(pages, exponents):
     """(layers * 2, n_pages, kv_heads, page_size) of a whole pool."""
-    pages, exponents = _split(pages)
     shape = pages.shape
     if len(shape) != 6 or shape[1] != 2 or shape[5] != HEAD_DIM:
         raise ValueError(f"pages must be (layers, 2, n_pages, kv_heads, page_size, {HEAD_DIM}), got "
@@ -466,13 +465,6 @@ def _pool_of(pages):
         raise ValueError(f"exponents must be {tuple(shape[:-1])}, contiguous, on {pages.device}, got "
                          f"{tuple(exponents.shape)}, strides {exponents.stride()} on {exponents.device}")
     return 2 * shape[0], shape[2], shape[3], _page_size(shape[4])
-
-
-def _pool_args(pages):
-    """(the library's suffix, the pool's addresses)."""
-    pages, exponents = _split(pages)
-    return ("", (pages.data_ptr(),)) if exponents is None else \
-        ("8", (pages.data_ptr(), exponents.data_ptr()))
 
 
 def _state_of(n_pages, table, lengths, refs, **more):
@@ -515,26 +507,29 @@ def remap_pages(pages, table, lengths, refs, parents=None, new_lengths=None):
     slot that ends in it if nobody else holds it, and the others get a copy of its filled rows, in
     every layer. Free pages are handed out in ascending order, slot after slot. shortfall (1): 0, or
     how many pages the pool or the table rows lack, in which case nothing changes."""
-    device = _one_device(_split(pages)[0], table, lengths, refs,
+    codes, exponents = _split(pages)
+    device = _one_device(codes, table, lengths, refs,
                          *(t for t in (parents, new_lengths) if t is not None))
     if device.index != _current_device():  # launches and allocations go to the tensors' device
         with torch.cuda.device(device):
             return remap_pages(pages, table, lengths, refs, parents, new_lengths)
-    _no_grad(_split(pages)[0])
-    outer, n_pages, kv_heads, page_size = _pool_of(pages)
+    _no_grad(codes)
+    outer, n_pages, kv_heads, page_size = _pool_of(codes, exponents)
     slots, width = _state_of(n_pages, table, lengths, refs, parents=parents, new_lengths=new_lengths)
     table_out, lengths_out, refs_out = (torch.empty_like(table), torch.empty_like(lengths),
                                         torch.empty_like(refs))
     shortfall = torch.empty(1, dtype=torch.int32, device=device)
     words = _scratch_words(slots, n_pages)
     scratch = torch.empty(words, dtype=torch.int32, device=device)
-    bits, pool = _pool_args(pages)
-    check(getattr(lib(), "va_pages_remap" + bits)(
-        *pool, outer, n_pages, kv_heads, page_size, HEAD_DIM, table.data_ptr(),
-        lengths.data_ptr(), refs.data_ptr(), None if parents is None else parents.data_ptr(),
-        None if new_lengths is None else new_lengths.data_ptr(), slots, width, table_out.data_ptr(),
-        lengths_out.data_ptr(), refs_out.data_ptr(), shortfall.data_ptr(), scratch.data_ptr(), words,
-        _current_stream(device.index)), "va_pages_remap" + bits)
+    rest = (outer, n_pages, kv_heads, page_size, HEAD_DIM, table.data_ptr(), lengths.data_ptr(),
+            refs.data_ptr(), None if parents is None else parents.data_ptr(),
+            None if new_lengths is None else new_lengths.data_ptr(), slots, width,
+            table_out.data_ptr(), lengths_out.data_ptr(), refs_out.data_ptr(), shortfall.data_ptr(),
+            scratch.data_ptr(), words, _current_stream(device.index))
+    if exponents is None:
+        check(lib().va_pages_remap(codes.data_ptr(), *rest), "va_pages_remap")
+    else:
+        check(lib().va_pages_remap8(codes.data_ptr(), exponents.data_ptr(), *rest), "va_pages_remap8")
     return table_out, lengths_out, refs_out, shortfall
 
 
@@ -543,23 +538,26 @@ def compact_pages(pages, table, lengths, refs):
     moves to the k-th free page below it, in every layer. Arguments as for `remap_pages`. Returns
     new (table, refs, live); live (1): how many pages are in use, all of them below that number. Pages
     that the program holds without a table row move too: a row of their own keeps track of them."""
-    device = _one_device(_split(pages)[0], table, lengths, refs)
+    codes, exponents = _split(pages)
+    device = _one_device(codes, table, lengths, refs)
     if device.index != _current_device():  # launches and allocations go to the tensors' device
         with torch.cuda.device(device):
             return compact_pages(pages, table, lengths, refs)
-    _no_grad(_split(pages)[0])
-    outer, n_pages, kv_heads, page_size = _pool_of(pages)
+    _no_grad(codes)
+    outer, n_pages, kv_heads, page_size = _pool_of(codes, exponents)
     slots, width = _state_of(n_pages, table, lengths, refs)
     table_out, refs_out = torch.empty_like(table), torch.empty_like(refs)
     live = torch.empty(1, dtype=torch.int32, device=device)
     words = _scratch_words(slots, n_pages)
     scratch = torch.empty(words, dtype=torch.int32, device=device)
-    bits, pool = _pool_args(pages)
-    check(getattr(lib(), "va_pages_compact" + bits)(
-        *pool, outer, n_pages, kv_heads, page_size, HEAD_DIM, table.data_ptr(),
-        lengths.data_ptr(), refs.data_ptr(), slots, width, table_out.data_ptr(), refs_out.data_ptr(),
-        live.data_ptr(), scratch.data_ptr(), words, _current_stream(device.index)),
-        "va_pages_compact" + bits)
+    rest = (outer, n_pages, kv_heads, page_size, HEAD_DIM, table.data_ptr(), lengths.data_ptr(),
+            refs.data_ptr(), slots, width, table_out.data_ptr(), refs_out.data_ptr(), live.data_ptr(),
+            scratch.data_ptr(), words, _current_stream(device.index))
+    if exponents is None:
+        check(lib().va_pages_compact(codes.data_ptr(), *rest), "va_pages_compact")
+    else:
+        check(lib().va_pages_compact8(codes.data_ptr(), exponents.data_ptr(), *rest),
+              "va_pages_compact8")
     return table_out, refs_out, live
 
 
@@ -571,14 +569,16 @@ def paged_accept(pages, plan, lengths, accepted):
     anything else: none stays. The rows that stay move together behind the tokens cached before, in order
     and in every layer; rows behind them hold what they held or what moved over them. Returns the lengths
     (sequences) int32; sequences without new tokens keep theirs. Pages past them are given back by
-    `remap_pages(pages, table, lengths, refs, None, new_lengths)` over the lengths of before the call."""
+    `remap_pages(pages, table, lengths, refs, None, new_lengths)` over the lengths of before the call.
+    The call belongs to its step: before the sequences are forked, reordered or stepped again, since it
+    follows the page table as it is and moves rows within pages that no other sequence may hold."""
     codes, exponents = _split(pages)
     device = _one_device(codes, plan.words, lengths, accepted)
     if device.index != _current_device():  # launches and allocations go to the tensors' device
         with torch.cuda.device(device):
             return paged_accept(pages, plan, lengths, accepted)
     _no_grad(codes)
-    outer, n_pages, kv_heads, page_size = _pool_of(pages)
+    outer, n_pages, kv_heads, page_size = _pool_of(codes, exponents)
     if (kv_heads, page_size) != (plan.kv_heads, plan.page_size):
         raise ValueError(f"pages of {page_size} rows of {kv_heads} heads, the plan's have "
                          f"{plan.page_size} of {plan.kv_heads}")
@@ -596,9 +596,10 @@ class PagedCache:
     """Keys and values of `layers` layers in one pool of `n_pages` pages, and up to `slots` sequences
     of at most `max_length` tokens (rounded up to whole pages) in it, in fp16, bf16 or, with
     `dtype=torch.float8_e4m3fn`, in 8 bits (`QuantizedPages`). State, all on the GPU: `pages` (8 bits: the
-    codes, and `exponents`), `table`, `lengths`, `refs`. Every call updates it in place on the current stream, so the calls of one
-    cache belong on one stream or in order across streams, and a captured step replays on the state it
-    finds. A call that lacks pages (or a step that lacks rows) changes nothing; `check()` reports it."""
+    codes, and `exponents`), `table`, `lengths`, `refs`. Every call updates it in place on the current
+    stream, so the calls of one cache belong on one stream or in order across streams, and a captured
+    step replays on the state it finds. A call that lacks pages (or a step that lacks rows) changes
+    nothing; `check()` reports it."""
 
     def __init__(self, layers, n_pages, page_size, kv_heads, slots, max_length,
                  dtype=torch.float16, device="cuda"):
@@ -690,7 +691,8 @@ class PagedCache:
     def accept(self, plan, accepted):
         """Of the last step's new tokens (`plan`: what `step` returned) those up to `accepted[s]` on its
         path stay, `paged_accept`; pages that are not needed any more are given back. accepted: (slots)
-        int32 tensor, or a dict {slot: number} (the other slots' new tokens go)."""
+        int32 tensor, or a dict {slot: number} (the other slots' new tokens go). Once per step, before
+        any other call that changes the slots."""
         accepted = self._slots(accepted, [-1] * self.slots)
         self.remap(None, paged_accept(self.pool, plan, self.lengths, accepted))
 
