@@ -302,21 +302,26 @@ def _pages_of(k_pages, v_pages, plan):
     return k_stride[0], v_stride[0], shape[0]
 
 
-def _exponents_of(pages, plan):
-    """Elements from one page's exponents to the next."""
-    codes, exponents = pages
-    if codes.dtype != torch.float8_e4m3fn or exponents.dtype != torch.float8_e8m0fnu:
+def _exponents_of(k_pages, v_pages, n_pages, plan):
+    """Elements from one page's exponents to the next, of keys and of values."""
+    (codes, k), (_, v) = k_pages, v_pages
+    if codes.dtype != torch.float8_e4m3fn or k.dtype != torch.float8_e8m0fnu or v.dtype != k.dtype:
         raise ValueError("8-bit pages are float8_e4m3fn codes and float8_e8m0fnu exponents, got "
-                         f"{codes.dtype} and {exponents.dtype}")
-    if exponents.device != codes.device:
-        raise ValueError(f"tensors on {codes.device} and {exponents.device}")
-    shape, stride = exponents.shape, exponents.stride()
-    if shape != codes.shape[:-1]:
-        raise ValueError(f"exponents must be {tuple(codes.shape[:-1])}, got {tuple(shape)}")
-    if stride[2] != 1 or (stride[1] != plan.page_size and plan.kv_heads != 1):
-        raise ValueError(f"every page's exponents must be contiguous, got strides {stride}")
-    least = plan.kv_heads * plan.page_size
-    return max(stride[0], least) if shape[0] <= 1 else stride[0]
+                         f"{codes.dtype} and {k.dtype}, {v.dtype}")
+    if k.device != codes.device or v.device != codes.device:
+        raise ValueError(f"tensors on {codes.device}, {k.device} and {v.device}")
+    kv_heads, page_size = plan.kv_heads, plan.page_size
+    shape = (n_pages, kv_heads, page_size)
+    if k.shape != shape or v.shape != shape:
+        raise ValueError(f"exponents must be {shape}, got {tuple(k.shape)} and {tuple(v.shape)}")
+    k_stride, v_stride = k.stride(), v.stride()
+    for stride in (k_stride, v_stride):
+        if stride[2] != 1 or (stride[1] != page_size and kv_heads != 1):
+            raise ValueError(f"every page's exponents must be contiguous, got strides {stride}")
+    if n_pages <= 1:
+        least = kv_heads * page_size
+        return max(k_stride[0], least), max(v_stride[0], least)
+    return k_stride[0], v_stride[0]
 
 
 def _layer(k_pages, v_pages, plan):
@@ -328,9 +333,9 @@ def _layer(k_pages, v_pages, plan):
     if k_exps is None:
         return _lib.PagedPages(k.data_ptr(), v.data_ptr(), None, None, k_stride, v_stride, 0, 0, n_pages,
                                _attn_dtype(k))
+    k_exp_stride, v_exp_stride = _exponents_of(k_pages, v_pages, n_pages, plan)
     return _lib.PagedPages(k.data_ptr(), v.data_ptr(), k_exps.data_ptr(), v_exps.data_ptr(), k_stride,
-                           v_stride, _exponents_of(k_pages, plan), _exponents_of(v_pages, plan), n_pages,
-                           _lib.VA_E4M3)
+                           v_stride, k_exp_stride, v_exp_stride, n_pages, _lib.VA_E4M3)
 
 
 def paged_append(q, k, v, cos, sin, k_pages, v_pages, plan, dtype=None):
