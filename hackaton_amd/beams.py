@@ -32,7 +32,8 @@ def select_beams(logits, scores, beams, count=None, ended=None, end_token=None):
     fp16, bf16 or fp32, rows next to each other or apart, vocab at most 2^18; rows g * beams to
     (g + 1) * beams - 1 are the beams (at most 64) of prompt g. scores (rows) fp32: the beams' sums of log
     probabilities so far (-inf: a beam that is not used yet). A continuation's score is its beam's plus
-    the token's log softmax, formed and compared in 64 bits; what is not a number counts as -inf.
+    the token's log softmax, formed and compared in 64 bits (the row's exponentials are summed in 32 by
+    every wave of a work-group, in 64 over them); what is not a number counts as -inf.
 
     Returns (scores (prompts, count) fp32, parents (prompts, count) int32: the row that each goes on from,
     tokens (prompts, count) int32), the best first, ties to the lowest row and token: the order of a
@@ -76,7 +77,7 @@ def select_beams(logits, scores, beams, count=None, ended=None, end_token=None):
     scores = scores.contiguous()
     if ended is not None:
         ended = ended.contiguous()
-    if count < 1:
+    if not 1 <= count < 1 << 20:
         raise ValueError(f"count must be 1 to 64, got {count}")
     out = torch.empty(groups, count, dtype=torch.float32, device=device)
     parents = torch.empty(groups, count, dtype=torch.int32, device=device)
@@ -85,7 +86,7 @@ def select_beams(logits, scores, beams, count=None, ended=None, end_token=None):
     check(lib().va_select_beams(
         logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0), groups, beams, vocab,
         scores.data_ptr(), None if ended is None else ended.data_ptr(),
-        0 if end_token is None else int(end_token), count, out.data_ptr(),
+        0 if end_token is None else max(-1, min(int(end_token), vocab)), count, out.data_ptr(),
         parents.data_ptr(), tokens.data_ptr(), ws.data_ptr(), nbytes, _current_stream(device.index)),
         "va_select_beams")
     return out, parents, tokens

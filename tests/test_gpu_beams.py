@@ -272,6 +272,11 @@ def test_refusals():
         dual = torch.autograd.forward_ad.make_dual(logits.float(), torch.ones(12, 100, device="cuda"))
         with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
             select_beams(dual, scores, 4)
+    # (what passes 32 bits is refused too, not cut to its low bits)
+    with pytest.raises(RuntimeError, match="end_token"):
+        select_beams(logits, scores, 4, 4, ended, 1 + (1 << 32))
+    with pytest.raises(ValueError, match="count"):
+        select_beams(logits, scores, 4, 4 + (1 << 32))
     got = select_beams(logits[:0], scores[:0], 4)
     assert [x.shape for x in got] == [(0, 4)] * 3
     cache = PagedCache(1, 8, 16, 1, 4, 64)
