@@ -67,8 +67,10 @@ static_assert(sizeof(Merge) == 4 * kPagedMergeWords, "merge words");
 
 // Tiles of a sequence with `rows` rows, and the keys that the row before `end` sees (pos0: the position
 // of the first one).
-__device__ inline int tiles_of(int rows) {
-  return rows <= kPagedFewRows ? (rows > 0) : (rows + kPagedTileRows - 1) / kPagedTileRows;
+__device__ inline int tiles_of(int rows, bool narrow) {
+  return narrow                  ? (rows + kPagedFewRows - 1) / kPagedFewRows
+         : rows <= kPagedFewRows ? (rows > 0)
+                                 : (rows + kPagedTileRows - 1) / kPagedTileRows;
 }
 __device__ inline int keys_of(int pos0, int end, int group) { return max(pos0 + (end - 1) / group + 1, 0); }
 // The last of n ascending numbers at or below x (the first one is).
@@ -161,6 +163,7 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
   __shared__ __attribute__((aligned(16))) uint32_t s_key[PT];
   __shared__ int s_at[PT], s_items[PT];  // (one sequence per thread: their order)
   const int tid = threadIdx.x, group = a.hq / a.hkv;
+  const bool narrow = a.layout.narrow;
   // Row offsets need sums of q; the split shares need, per kind (many rows, few rows), the tiles and
   // their keys, here from the lengths as they are given (cut to n_tokens one by one), which is no less
   // than what the rows make. Sums that could pass 32 bits go in pieces of 15 and 19 bits: 4096 sequences
@@ -176,7 +179,7 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
     q[i] = min(len, a.n_tokens);
     sum[0] += q[i] & 0x7fff;
     sum[1] += q[i] >> 15;
-    const int rows = q[i] * group, kind = rows <= kPagedFewRows, t = tiles_of(rows);
+    const int rows = q[i] * group, kind = narrow || rows <= kPagedFewRows, t = tiles_of(rows, narrow);
     const long long keys = (long long)t * kv;
     sum[2 + kind] += t;
 #pragma unroll
@@ -254,7 +257,7 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
   int own[SPT][4], longest_of[SPT];
 #pragma unroll
   for (int i = 0; i < SPT; ++i) {
-    const int s = tid * SPT + i, rows = n_rows[i], kind = rows <= kPagedFewRows;
+    const int s = tid * SPT + i, rows = n_rows[i], kind = narrow || rows <= kPagedFewRows;
     const int longest = rows > 0 ? keys_of(s_pos0[s], rows, group) : 0;
     int parts = max(1, (longest + chunks[kind] - 1) / chunks[kind]);
     if (kind == 0 && parts > aligned) parts -= parts % aligned;
@@ -263,7 +266,7 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
     if (parts > 1) parts = (longest + c - 1) / c;
     s_parts[s] = parts;
     s_chunk[s] = max(c, 1);
-    const int items = tiles_of(rows) * parts * a.hkv;
+    const int items = tiles_of(rows, narrow) * parts * a.hkv;
     longest_of[i] = kind == 0 ? longest : 0;
     own[i][0] = kind == 0 ? items : 0;
     own[i][1] = kind == 0 ? 0 : items;
@@ -321,14 +324,16 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlanArgs a, int wri
     const int j = many ? i : i - n[0], nth = last_at_most(before, a.n_seqs, j);
     const int s = SPT == 1 && many && sorted ? s_at[nth] : nth;
     const int rows = (s_cu[s + 1] - s_cu[s]) * group, parts = s_parts[s], chunk = s_chunk[s];
-    const int in = j - before[nth], per_tile = parts * a.hkv, tile = tiles_of(rows) - 1 - in / per_tile;
+    const int in = j - before[nth], per_tile = parts * a.hkv;
+    const int tile = tiles_of(rows, narrow) - 1 - in / per_tile;
     const int head = in % a.hkv, part = in % per_tile / a.hkv;
     Item it;
     it.token0 = s_cu[s];
     it.seq = s;
     it.pos0 = s_pos0[s];
-    it.row = tile * kPagedTileRows;
-    it.row_end = min(it.row + kPagedTileRows, rows);
+    const int each = narrow ? kPagedFewRows : kPagedTileRows;
+    it.row = tile * each;
+    it.row_end = min(it.row + each, rows);
     const int all = keys_of(it.pos0, it.row_end, group);
     it.key = part * chunk;
     it.key_end = parts == 1 ? all : min(it.key + chunk, all);

@@ -14,7 +14,7 @@ constexpr int kPageMin = 16, kPageMax = 256;
 
 // Work items of a step: rows (token, query head of the group) of one sequence and key/value head,
 // flattened token by token. Up to kPagedFewRows of them are one tile whose waves share the keys out;
-// more are tiles of kPagedTileRows, a strip of 32 per wave.
+// more are tiles of kPagedTileRows, a strip of 32 per wave (in short steps tiles of kPagedFewRows, see below).
 constexpr int kPagedFewRows = 32;
 constexpr int kPagedTileRows = 128;
 constexpr int kPagedChunkKeys = 64;  // key ranges are split at multiples of this
@@ -49,6 +49,15 @@ constexpr int kPagedFewParts = 512, kPagedManyParts = 256, kPagedMostParts = 512
 // 16.5; with 384 items 512 on 1536 23.3 / 27.3, two of 64 on 8000 25.3 / 28.0).
 constexpr int kPagedFewKeys = 256, kPagedManyKeys = 512, kPagedShortItems = 192;
 constexpr int kPagedWholeKeys = 1024;
+// Short steps: prompt tiles over table rows that are not split are of kPagedFewRows rows too, whose waves share
+// the keys out, where that makes no more items than there are CUs (8 waves each), or up to twice as many (4
+// waves, two work-groups per CU) of sequences of kPagedNarrowTiles such tiles or more. us, 128 rows / 32: four
+// trees of 16 on 512, 12/2 heads 14.6 / 10.6, 28/4 15.4 / 10.6; 32 of 16 on 800 19.6 / 17.3; 128 new tokens on
+// 800 19.5 / 12.3; two prompts of 512 (388 items) 14.1 / 11.7, one of 900 19.7 / 14.1, 8 x 64 on 600, 28/4 heads
+// (480) 17.8 / 16.1. Sequences of fewer tiles, which read their keys as often as more work-groups hold them:
+// 48 trees of 16 on 500 (384) 15.2 / 18.7, 24 x 32 on 900 (336) 21.3 / 23.1. (4 waves for up to 256 items: 8.6
+// for 9.3 at 64 new tokens on 200, 13.5 for 12.4 at 16 x 8 on 900.)
+constexpr int kPagedNarrowItems = 256, kPagedNarrowTiles = 8;
 constexpr int kPagedPadRows = 64;     // padding rows that one item zeroes
 
 // A step's plan, int32 words: cu (n_seqs + 1) row offsets of the sequences, the sequence (-1: padding)
@@ -59,10 +68,10 @@ struct PagedLayout {
   int64_t max_items, max_merges, max_part_rows;
   int many_parts;  // parts of prompt tiles at most, and
   int many_base;   // where there are fewer of them than that, and no few-row tiles
-  bool wide;
+  bool wide, narrow;
 };
 inline int64_t up4(int64_t x) { return (x + 3) & ~int64_t(3); }
-// Bounds: a sequence with rows makes one tile, and one more per full kPagedTileRows. A kind's parts have
+// Bounds: a sequence with rows makes one tile, and one more per full kPagedTileRows (kPagedFewRows if narrow). A kind's parts have
 // at least its total (tiles times the longest of the sequence) / its number of parts keys, so the
 // tiles of a sequence of n > 1 parts stand for more than n - 1 >= n / 2 of them each, and all split
 // tiles have at most twice as many parts; each part holds at most the kind's rows, and a row is in at
@@ -71,11 +80,15 @@ inline int64_t up4(int64_t x) { return (x + 3) & ~int64_t(3); }
 inline PagedLayout paged_layout(int64_t n_seqs, int64_t n_tokens, int64_t hq, int64_t hkv,
                                 int64_t max_keys) {
   PagedLayout l;
-  const int64_t tiles = (n_seqs < n_tokens ? n_seqs : n_tokens) + n_tokens * (hq / hkv) / kPagedTileRows;
-  const bool split = max_keys > kPagedWholeKeys;
-  const int64_t rows = n_tokens * hq;
-  const bool prompts = n_tokens > n_seqs, few = prompts && split && tiles * hkv <= kPagedSplitTiles;
-  l.wide = prompts && !few && tiles * hkv <= kPagedWideTiles;
+  const bool split = max_keys > kPagedWholeKeys, prompts = n_tokens > n_seqs;
+  const int64_t rows = n_tokens * hq, seqs = n_seqs < n_tokens ? n_seqs : n_tokens;
+  const int64_t short_tiles = n_tokens * (hq / hkv) / kPagedFewRows, short_items = (seqs + short_tiles) * hkv;
+  const bool fits = short_items <= kPagedNarrowItems;
+  l.narrow = prompts && !split &&
+             (fits || (short_items <= 2 * kPagedNarrowItems && short_tiles >= kPagedNarrowTiles * seqs));
+  const int64_t tiles = seqs + (l.narrow ? short_tiles : n_tokens * (hq / hkv) / kPagedTileRows);
+  const bool few = prompts && split && tiles * hkv <= kPagedSplitTiles;
+  l.wide = prompts && !few && (l.narrow ? fits : tiles * hkv <= kPagedWideTiles);
   const int64_t fit = n_tokens * (hq / hkv) / (kPagedFewRows + 1);  // (prompt tiles, of more rows each)
   const int64_t its = (fit < tiles ? fit : tiles) * hkv;
   const int64_t many = few || its > kPagedMostParts ? kPagedMostParts : its < kPagedManyParts ? kPagedManyParts : its;

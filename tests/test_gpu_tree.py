@@ -33,11 +33,11 @@ def case(bits, seed, q, kv, heads, kv_heads, dtype, ps, padding=0, width=None):
     return query, k.cuda(), v.cuda(), [torch.nan_to_num(x.double()) for x in (k, v)], table
 
 
-def check_tree(bits, trees, kv, heads, kv_heads, dtype, ps, padding=0):
+def check_tree(bits, trees, kv, heads, kv_heads, dtype, ps, padding=0, width=None):
     """trees: parents per sequence (empty: no new token)."""
     q = [len(t) for t in trees]
     banner("tree", bits, q[:20], kv[:20], heads, kv_heads, dtype, ps)
-    query, k, v, exact, table = case(bits, sum(kv) + heads, q, kv, heads, kv_heads, dtype, ps, padding)
+    query, k, v, exact, table = case(bits, sum(kv) + heads, q, kv, heads, kv_heads, dtype, ps, padding, width)
     n = sum(q) + padding
     parents = ints([p for t in trees for p in t] + [3] * padding)
     plan = paged_plan(table.cuda(), ints(q), ints(kv), n, heads, kv_heads, ps, parents)
