@@ -77,8 +77,9 @@ def _one_device(first, *tensors):
     device = first.device
     if not first.is_cuda:
         raise ValueError(f"the paged cache lives on the GPU only: got a tensor on {device}")
+    index = device.index
     for t in tensors:
-        if t.device != device:
+        if t.get_device() != index:  # (-1: not on a GPU)
             raise ValueError(f"tensors on {device} and {t.device}")
     return device
 
@@ -153,7 +154,7 @@ class PagedPlan:
 
     __slots__ = ("page_table", "words", "n_tokens", "n_seqs", "heads", "kv_heads", "page_size",
                  "workspace_bytes", "_step", "_page", "_strides", "_stream",
-                 "_capture", "_tree", "_paths")
+                 "_capture", "_tree", "_paths")  # (_tree: the address of the tree's words, _paths: in `words`)
 
     def _rows(self, which):
         rows = -(-self.n_tokens // 4) * 4
@@ -171,8 +172,8 @@ class PagedPlan:
         the tokens that come before it, cached ones and those on its path."""
         if self._tree is None:
             return self._rows(1)
-        at = self.n_tokens * (TREE_TOKENS // 32)
-        return self._paths[at:at + self.n_tokens]
+        at = self._paths + self.n_tokens * (TREE_TOKENS // 32)
+        return self.words[at:at + self.n_tokens]
 
     @property
     def places(self):
@@ -193,8 +194,6 @@ class PagedPlan:
             current = torch.cuda.current_stream()
             self.words.record_stream(current)
             self.page_table.record_stream(current)
-            if self._paths is not None:
-                self._paths.record_stream(current)
         return stream
 
 
@@ -264,7 +263,8 @@ def paged_plan(page_table, q_lengths, kv_lengths, n_tokens, heads, kv_heads, pag
     plan.heads, plan.kv_heads, plan.page_size = heads, kv_heads, page_size
     plan._page = (kv_heads, page_size, HEAD_DIM)
     plan._strides = (page_size * HEAD_DIM, HEAD_DIM, 1)
-    plan.words = torch.empty(n_words, dtype=torch.int32, device=device)
+    tree_words = 0 if parents is None else _tree_words(n_seqs, n_tokens, heads, kv_heads, page_size, width)
+    plan.words = torch.empty(n_words + tree_words, dtype=torch.int32, device=device)
     plan._stream = _current_stream(device.index)
     plan._capture = attention._capture_id() if torch._C._cuda_isCurrentStreamCapturing() else None
     plan._step = _lib.PagedStep(page_table.data_ptr(), plan.words.data_ptr(), n_tokens, n_seqs, width,
@@ -274,9 +274,7 @@ def paged_plan(page_table, q_lengths, kv_lengths, n_tokens, heads, kv_heads, pag
         check(lib().va_paged_plan(plan._step, q_lengths.data_ptr(), kv_lengths.data_ptr(), n_words,
                                   plan._stream), "va_paged_plan")
         return plan
-    tree_words = _tree_words(n_seqs, n_tokens, heads, kv_heads, page_size, width)
-    plan._paths = torch.empty(tree_words, dtype=torch.int32, device=device)
-    plan._tree = plan._paths.data_ptr()
+    plan._paths, plan._tree = n_words, plan._step.plan + 4 * n_words  # (whole pieces of 16 bytes)
     check(lib().va_paged_plan_tree(plan._step, q_lengths.data_ptr(), kv_lengths.data_ptr(), n_words,
                                    parents.data_ptr(), plan._tree, tree_words, plan._stream),
           "va_paged_plan_tree")
@@ -380,7 +378,7 @@ def paged_append(q, k, v, cos, sin, k_pages, v_pages, plan, dtype=None):
     cos, sin = _tables(cos[None] if by_row else cos, sin[None] if by_row else sin)
     if not by_row and cos.shape[0] not in (1, plan.n_seqs):
         raise ValueError(f"cos/sin for {cos.shape[0]} sequences, the plan has {plan.n_seqs}")
-    query = torch.empty((n, heads, HEAD_DIM), dtype=dtype, device=device)
+    query = torch.empty(n, heads, HEAD_DIM, dtype=dtype, device=device)
     if n == 0:
         return query
     if cos.shape[1] == 0:
@@ -432,7 +430,7 @@ def paged_attention(query, k_pages, v_pages, plan, scale):
     else:
         layer = _layer(k_pages, v_pages, plan)
     query = query.contiguous()
-    out = torch.empty((n, heads * HEAD_DIM), dtype=query.dtype, device=device)
+    out = torch.empty(n, heads * HEAD_DIM, dtype=query.dtype, device=device)
     if n == 0:
         return out
     nbytes = plan.workspace_bytes

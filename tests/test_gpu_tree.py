@@ -291,7 +291,7 @@ def test_a_graph_keeps_the_tree_that_it_reads():
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         out = paged_attention(query, k, v, plan, SCALE)
-    size = plan._paths.numel()
+    size = plan.words.numel()
     del plan
     fill = [torch.full((size,), 0, dtype=torch.int32, device="cuda") for _ in range(8)]
     for _ in range(3):
