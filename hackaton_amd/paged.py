@@ -615,6 +615,7 @@ class PagedCache:
             self.exponents = torch.empty(self.pages.shape[:-1], dtype=torch.float8_e8m0fnu, device=device)
         else:
             _attn_dtype(self.pages)
+        self._held = self._views()
         ints = {"dtype": torch.int32, "device": self.pages.device}
         self.table = torch.full((slots, width), -1, **ints)
         self.lengths = torch.zeros(slots, **ints)
@@ -632,15 +633,28 @@ class PagedCache:
         """All pages, as the page bookkeeping takes them."""
         return self.pages if self.exponents is None else QuantizedPages(self.pages, self.exponents)
 
-    def _of(self, layer, which):
-        pages = self.pages[layer, which]
-        return pages if self.exponents is None else QuantizedPages(pages, self.exponents[layer, which])
+    def _views(self):
+        """(pages, exponents, every layer's keys, its values): the layers as views, made once (made in every call,
+        two to four of them take as long as its kernel's launch)."""
+        def views(which):
+            codes = [self.pages[layer, which] for layer in range(self.pages.shape[0])]
+            if self.exponents is None:
+                return codes
+            return [QuantizedPages(x, self.exponents[layer, which]) for layer, x in enumerate(codes)]
+
+        return self.pages, self.exponents, views(0), views(1)
+
+    def _layer(self, layer, which):
+        held = self._held
+        if held[0] is not self.pages or held[1] is not self.exponents:  # (the program has set others)
+            held = self._held = self._views()
+        return held[which][layer]
 
     def keys(self, layer):
-        return self._of(layer, 0)
+        return self._layer(layer, 2)
 
     def values(self, layer):
-        return self._of(layer, 1)
+        return self._layer(layer, 3)
 
     def _slots(self, values, fill):
         """One int32 per slot: a device tensor as it is, or `fill` with a host dict's entries."""

@@ -206,3 +206,21 @@ def test_the_references_agree():
         for h in range(4):
             w = torch.softmax(rows[0][h // 2] @ query[j, h].double() * orc.SCALE, 0)
             assert torch.allclose(got[j, h], w @ rows[1][h // 2], atol=1e-12)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float8_e4m3fn])
+def test_layers_of_a_cache_are_views_of_its_pages(dtype):
+    cache = PagedCache(3, 8, 16, 2, 2, 64, dtype, device="cpu")
+    for _ in range(2):
+        for layer in (0, 2, -1):
+            for which, got in enumerate((cache.keys(layer), cache.values(layer))):
+                quantized = dtype == torch.float8_e4m3fn
+                pages, want = got.codes if quantized else got, cache.pages[layer, which]
+                assert pages.data_ptr() == want.data_ptr() and pages.shape == want.shape
+                assert pages.stride() == want.stride()
+                if quantized:
+                    assert got.exponents.data_ptr() == cache.exponents[layer, which].data_ptr()
+                    assert got.exponents.shape == cache.exponents[layer, which].shape
+        with pytest.raises(IndexError):
+            cache.keys(3)
+        cache.pages = torch.zeros_like(cache.pages)  # (others that the program sets are followed)
