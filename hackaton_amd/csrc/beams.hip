@@ -240,104 +240,109 @@ __global__ __launch_bounds__(T) void beams_read_kernel(BeamsArgs a) {
 // ------------------------------------------------------------------------------------------------
 // selection
 // ------------------------------------------------------------------------------------------------
-// A candidate: its score as a whole number of the same order (0: none) and its number.
+// A candidate: its score (not a number: -infinity) and its number; none: -infinity and INT_MAX, behind all.
 struct Pick {
-  uint64_t key;
+  double score;
   int index, pad;
 };
-__device__ inline bool before(uint64_t key, int index, uint64_t than, int than_index) {
-  return key > than || (key == than && index < than_index);
-}
-// 64-bit floats in order; not a number counts as -infinity.
-__device__ inline uint64_t key_of(double x) {
-  const uint64_t b = __builtin_bit_cast(uint64_t, x != x ? -__builtin_inf() : x == 0 ? 0.0 : x);
-  return b >> 63 ? ~b : b | 1ull << 63;
-}
-__device__ inline double value_of(uint64_t key) {
-  return __builtin_bit_cast(double, key >> 63 ? key & ~(1ull << 63) : ~key);
+__device__ inline bool before(double score, int index, double than, int than_index) {
+  return score > than || (score == than && index < than_index);
 }
 
 constexpr int PT = 1024, PW = PT / 64;  // threads and waves of a work-group that picks
 constexpr int kPool = 4096;             // candidates that pass the threshold, at most
 struct Picks {
-  Pick pool[kPool], best[64], out[kBeamsCount];
-  int rank[2][64];
+  Pick pool[kPool], best[64], out[kBeamsCount], least;
   int n;
 };
 
-// How many of v[0..n) come before v[lane]: the waves share them out, ranks add up in s.
-__device__ inline void count_before(const Pick* v, int n, const Pick& mine, int* rank) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// Over the 16 lanes of a row: the total, and the first in order, in all of them.
+template <int CTRL>
+__device__ inline int turned(int x) {  // (row_ror)
+  return __builtin_amdgcn_update_dpp(x, x, CTRL, 0xf, 0xf, false);
+}
+__device__ inline int row_sum(int x) {
+  x += turned<0x128>(x);
+  x += turned<0x124>(x);
+  x += turned<0x122>(x);
+  return x + turned<0x121>(x);
+}
+template <int CTRL>
+__device__ inline void first_of(double& score, int& index) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, score);
+  const uint32_t lo = (uint32_t)turned<CTRL>((int)(uint32_t)b), hi = (uint32_t)turned<CTRL>((int)(b >> 32));
+  const double x = __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+  const int i = turned<CTRL>(index);
+  if (before(x, i, score, index)) score = x, index = i;
+}
+// How many of v[0..n) come before `mine`, which the 16 lanes of a row have in common and share the others of.
+__device__ inline int count_before(const Pick* v, int n, const Pick& mine) {
   int r = 0;
 #pragma unroll 4
-  for (int j = wave; j < n; j += PW) {
+  for (int j = threadIdx.x & 15; j < n; j += 16) {
     const Pick p = v[j];
-    r += before(p.key, p.index, mine.key, mine.index);
+    r += before(p.score, p.index, mine.score, mine.index);
   }
-  if (r != 0) atomicAdd(&rank[lane], r);
+  return row_sum(r);
 }
 
-// The best `count` of all threads' E candidates (key 0: none), in order, to s.out; returns how many there
+// The best `count` of all threads' E candidates (a thread's in the order of their numbers), in order, to s.out; returns how many there
 // are. Each group of 16 threads brings its best one; the count-th best of those 64 is a bound that `count`
 // candidates reach, and only those of the groups whose best reaches it: at most 16 E count (and not more
 // than there are; the callers see to it that kPool is no less). They are then put in order by counting who
 // comes before. (A pool of more than 64 is slow, but takes scores whose best ones all lie with one
-// thread.)
+// thread.) Counts over 16 lanes in registers, and one LDS addition per wave: 1.3 us where additions per
+// candidate and of ranks took 2.3.
 template <int E>
-__device__ inline int select(Picks& s, int count, const uint64_t (&key)[E], const int (&index)[E]) {
-  const int tid = threadIdx.x, lane = tid & 63;
-  uint64_t top = 0;
-  int at = INT_MAX;
+__device__ inline int select(Picks& s, int count, const double (&score)[E], const int (&index)[E]) {
+  const int tid = threadIdx.x, group = tid >> 4;
+  double top = score[0];
+  int at = index[0];
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (key[e] != 0 && before(key[e], index[e], top, at)) top = key[e], at = index[e];
-#pragma unroll
-  for (int d = 1; d < 16; d *= 2) {
-    const uint64_t k = __shfl_xor((unsigned long long)top, d);
-    const int i = __shfl_xor(at, d);
-    if (before(k, i, top, at)) top = k, at = i;
-  }
+  for (int e = 1; e < E; ++e)
+    if (score[e] > top || at == INT_MAX) top = score[e], at = index[e];
+  first_of<0x128>(top, at);
+  first_of<0x124>(top, at);
+  first_of<0x122>(top, at);
+  first_of<0x121>(top, at);
   __syncthreads();  // (the pool and the counts may be in use from before)
-  if ((tid & 15) == 0) s.best[tid >> 4] = Pick{top, at, 0};
-  if (tid < 64) s.rank[0][tid] = s.rank[1][tid] = 0;
-  if (tid == 0) s.n = 0;
-  __syncthreads();
-  const Pick mine = s.best[lane];
-  count_before(s.best, 64, mine, s.rank[0]);
-  __syncthreads();
-  // (groups without a candidate are alike and rank behind the others)
-  const uint64_t found = __builtin_amdgcn_ballot_w64(s.rank[0][lane] == count - 1 && mine.key != 0);
-  uint64_t least = 0;
-  int last = INT_MAX;
-  if (found != 0) {
-    const Pick p = s.best[__builtin_ctzll(found)];
-    least = p.key;
-    last = p.index;
+  if ((tid & 15) == 0) s.best[group] = Pick{top, at, 0};
+  if (tid == 0) {
+    s.n = 0;
+    s.least = Pick{-__builtin_inf(), INT_MAX - 1, 0};  // (where fewer groups than `count` have a candidate)
   }
+  __syncthreads();
+  // (groups without a candidate are alike and come behind the others)
+  const int rank = count_before(s.best, 64, Pick{top, at, 0});
+  if (rank == count - 1 && at != INT_MAX && (tid & 15) == 0) s.least = Pick{top, at, 0};
+  __syncthreads();
+  const Pick least = s.least;
+  uint64_t hits[E];
+  int total = 0;
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (key[e] != 0 && !before(least, last, key[e], index[e])) {
-      const int n = atomicAdd(&s.n, 1);
-      if (n < kPool) s.pool[n] = Pick{key[e], index[e], 0};
+  for (int e = 0; e < E; ++e) {
+    hits[e] = __builtin_amdgcn_ballot_w64(!before(least.score, least.index, score[e], index[e]));
+    total += __builtin_popcountll(hits[e]);
+  }
+  if (total > 0) {  // (the same in all lanes)
+    int place = 0;
+    if ((tid & 63) == 0) place = atomicAdd(&s.n, total);
+    place = __builtin_amdgcn_readfirstlane(place);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (hits[e] == 0) continue;
+      const int n = place + __builtin_amdgcn_mbcnt_hi((uint32_t)(hits[e] >> 32),
+                                                      __builtin_amdgcn_mbcnt_lo((uint32_t)hits[e], 0));
+      if (hits[e] >> (tid & 63) & 1 && n < kPool) s.pool[n] = Pick{score[e], index[e], 0};
+      place += __builtin_popcountll(hits[e]);
     }
+  }
   __syncthreads();
   const int n = min(s.n, kPool);
-  if (n <= 64) {
-    const Pick p = s.pool[min(lane, n - 1)];
-    count_before(s.pool, n, p, s.rank[1]);
-    __syncthreads();
-    if (tid < n && s.rank[1][tid] < count) s.out[s.rank[1][tid]] = p;
-  } else {
-    for (int i = tid; i < n; i += PT) {
-      const Pick p = s.pool[i];
-      int r = 0;
-#pragma unroll 4
-      for (int j = 0; j < n; ++j) {
-        const Pick o = s.pool[j];
-        r += before(o.key, o.index, p.key, p.index);
-      }
-      if (r < count) s.out[r] = p;
-    }
+  for (int i = group; i - group < n; i += PT / 16) {  // (whole waves stay together)
+    const Pick p = s.pool[max(0, min(i, n - 1))];
+    const int r = count_before(s.pool, n, p);
+    if ((tid & 15) == 0 && i < n && r < count) s.out[r] = p;
   }
   __syncthreads();
   return min(n, count);
@@ -400,7 +405,8 @@ __global__ __launch_bounds__(PT) void beams_pick_kernel(BeamsArgs a) {
     }
   }
   __syncthreads();
-  auto score_of = [&](int beam, float x) { return key_of(s_score[beam] + ((double)x - s_sum[beam])); };
+  constexpr double none = -__builtin_inf();
+  auto score_of = [&](int beam, float x) { return fmax(s_score[beam] + ((double)x - s_sum[beam]), none); };
 
   // the best cells
   int n;
@@ -408,20 +414,20 @@ __global__ __launch_bounds__(PT) void beams_pick_kernel(BeamsArgs a) {
     // (quotients of small numbers: exact in fp32, half a unit to spare)
     const float inv = 1.f / (float)l.cells;
     const int end_cell = a.end_token / l.cell;
-    uint64_t key[CELLS];
+    double score[CELLS];
     int index[CELLS];
 #pragma unroll
     for (int e = 0; e < CELLS; ++e) {
       const int i = e * PT + tid;
-      index[e] = i;
-      key[e] = 0;
+      index[e] = i < cells ? i : INT_MAX;
+      score[e] = none;
       if (i < cells) {
         const int beam = (int)(((float)i + 0.5f) * inv);
         if (s_ended[beam]) top[e] = i - beam * l.cells == end_cell ? 0.f : -INFINITY;
-        key[e] = score_of(beam, top[e]);
+        score[e] = score_of(beam, top[e]);
       }
     }
-    n = select(s, min(a.count, cells), key, index);
+    n = select(s, min(a.count, cells), score, index);
   }
   in_order(s, n, s_runs, [&](int i) { return i / l.cells * kBeamsVocab + i % l.cells * l.cell; });
 
@@ -444,50 +450,53 @@ __global__ __launch_bounds__(PT) void beams_pick_kernel(BeamsArgs a) {
   if (n * (run / kNumbers) > PT || (16 * kNumbers * a.count > kPool && n * run > kPool)) {
     constexpr int RUNS = 64 * kBeamsCount / PT;
     const int part = run / 64;
-    uint64_t key[RUNS];
+    double score[RUNS];
     int index[RUNS];
 #pragma unroll
     for (int e = 0; e < RUNS; ++e) {
       const int i = e * PT + tid;
-      key[e] = 0;
-      index[e] = 0;
+      score[e] = none;
+      index[e] = INT_MAX;
       if (i < 64 * n) {
-        index[e] = s_runs[i >> 6] + (i & 63) * part;
+        const int at = s_runs[i >> 6] + (i & 63) * part;
         float best = -INFINITY;
         bool any = false;
         for (int k = 0; k < part; k += kNumbers) {
           float x[kNumbers];
-          const int some = see(index[e] + k, x);
+          const int some = see(at + k, x);
 #pragma unroll
           for (int j = 0; j < kNumbers; ++j)
             if (j < some) best = fmaxf(best, x[j]);
           any = any || some > 0;
         }
-        if (any) key[e] = score_of(index[e] / kBeamsVocab, best);
+        if (any) {
+          index[e] = at;
+          score[e] = score_of(at / kBeamsVocab, best);
+        }
       }
     }
-    n = select(s, a.count, key, index);
+    n = select(s, a.count, score, index);
     in_order(s, n, s_runs, [](int i) { return i; });
     run = part;
   }
   {
     const int shift = __builtin_ctz(run / kNumbers), loads = n << shift;
-    uint64_t key[kNumbers];
+    double score[kNumbers];
     int index[kNumbers];
     float x[kNumbers];
     const int at = tid < loads ? s_runs[tid >> shift] + (tid & ((1 << shift) - 1)) * kNumbers : 0;
     const int some = tid < loads ? see(at, x) : 0;
 #pragma unroll
     for (int e = 0; e < kNumbers; ++e) {
-      index[e] = at + e;
-      key[e] = e < some ? score_of(at / kBeamsVocab, x[e]) : 0;
+      index[e] = e < some ? at + e : INT_MAX;
+      score[e] = e < some ? score_of(at / kBeamsVocab, x[e]) : none;
     }
-    n = select(s, a.count, key, index);
+    n = select(s, a.count, score, index);
   }
   if (tid < a.count) {  // (n is count: there are no fewer numbers)
     const Pick p = s.out[min(tid, n - 1)];
     const int64_t at = (int64_t)blockIdx.x * a.count + tid;
-    a.scores_out[at] = (float)value_of(p.key);
+    a.scores_out[at] = (float)p.score;
     a.parents_out[at] = first + p.index / kBeamsVocab;
     a.tokens_out[at] = p.index % kBeamsVocab;
   }
