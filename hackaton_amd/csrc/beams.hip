@@ -12,9 +12,10 @@
 // The first kernel is bounded by memory, and for 16-bit numbers nearly as much by its arithmetic (a
 // power of two, 16 cycles of a wave, and six other instructions a number): 512 rows of 150,016 numbers
 // (154 MB) 34 us, 4.6 TB/s; of 75,008 fp32 numbers, as many bytes, 30 us. 1, 2 and 4 pieces on their
-// way and 1024 to 8192 work-groups measured 34 to 47. The second kernel is bounded by the latency of
-// its steps: 9 us for a prompt of four beams, 11 us for 64 of eight (13.8 and 33.7 with 256 threads,
-// which computed each key twice).
+// way and 1024 to 8192 work-groups measured 34 to 47. The second kernel is bounded by the latency of its dozen
+// steps between barriers, some 0.45 us each, and of its first loads (1.7 and 1.1): 8.2 us for a prompt of four
+// beams, 10.2 us for 64 of eight (with scores compared as whole numbers and ranks added up in LDS 8.8 and
+// 11.2; with 256 threads 13.8 and 33.7; with one copy of the code for all picks 8.9 and 12.8).
 #include <climits>
 #include <type_traits>
 
@@ -291,8 +292,7 @@ __device__ inline int count_before(const Pick* v, int n, const Pick& mine) {
 // candidates reach, and only those of the groups whose best reaches it: at most 16 E count (and not more
 // than there are; the callers see to it that kPool is no less). They are then put in order by counting who
 // comes before. (A pool of more than 64 is slow, but takes scores whose best ones all lie with one
-// thread.) Counts over 16 lanes in registers, and one LDS addition per wave: 1.3 us where additions per
-// candidate and of ranks took 2.3.
+// thread.) Sums over 16 lanes stay in registers.
 template <int E>
 __device__ inline int select(Picks& s, int count, const double (&score)[E], const int (&index)[E]) {
   const int tid = threadIdx.x, group = tid >> 4;
