@@ -29,7 +29,11 @@ constexpr int kPagedChunkKeys = 64;  // key ranges are split at multiples of thi
 // heads: 16 trees of 24 on 4000 75 / 53, 8 of 48 to 64 on 28,672 to 32,768 305 / 268, 512 new tokens on
 // 8192 98 / 86, on 4096 55 / 55, 1024 new ones (the table's bound 228) on 4096 106 / 106, 8 x 300 on
 // 700, 12/2 heads (240) 29 / 39.
-constexpr int kPagedWideTiles = 512, kPagedSplitTiles = 200;
+// Sequences of a few tiles each, as long as each other, that are more items than CUs, take 4 waves: with 8 the
+// last ones begin when the first have ended. us, 8 / 4: 36 trees of 24 on 500, 28/4 heads (288 items) 29.4 / 21.4, 40
+// on 1200 52 / 40, 100 on 1500, 12/2 heads (400) 64 / 50; 32 on 64 to 8192, 28/4 heads (256) 40 / 45; prompts of
+// kPagedLongTiles tiles and more differ in their tiles' ranges (above).
+constexpr int kPagedWideTiles = 512, kPagedSplitTiles = 200, kPagedWidePlaces = 256, kPagedLongTiles = 4;
 // Parts that a step's keys are split into, by kind of tile, the shortest part (but a range's last) and
 // the longest table row that is never split. us at 384 / 512 / 1024 few-row parts: 64 answers of 64 to
 // 8192 tokens, 12/2 heads 34 / 30 / 32, four of 65,536, 28/4 heads 103 / 97 / 100; shortest few-row part
@@ -88,7 +92,9 @@ inline PagedLayout paged_layout(int64_t n_seqs, int64_t n_tokens, int64_t hq, in
              (fits || (short_items <= 2 * kPagedNarrowItems && short_tiles >= kPagedNarrowTiles * seqs));
   const int64_t tiles = seqs + (l.narrow ? short_tiles : n_tokens * (hq / hkv) / kPagedTileRows);
   const bool few = prompts && split && tiles * hkv <= kPagedSplitTiles;
-  l.wide = prompts && !few && (l.narrow ? fits : tiles * hkv <= kPagedWideTiles);
+  const int64_t each = seqs == 0 ? 0 : (n_tokens * (hq / hkv) + seqs * kPagedTileRows - 1) / (seqs * kPagedTileRows);
+  const bool placed = seqs * each * hkv <= kPagedWidePlaces || each >= kPagedLongTiles;
+  l.wide = prompts && !few && (l.narrow ? fits : tiles * hkv <= kPagedWideTiles && placed);
   const int64_t fit = n_tokens * (hq / hkv) / (kPagedFewRows + 1);  // (prompt tiles, of more rows each)
   const int64_t its = (fit < tiles ? fit : tiles) * hkv;
   const int64_t many = few || its > kPagedMostParts ? kPagedMostParts : its < kPagedManyParts ? kPagedManyParts : its;
