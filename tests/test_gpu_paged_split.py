@@ -8,6 +8,7 @@ import torch
 from hackaton_amd import paged_plan
 from tests import paged8_oracle as o8
 from tests.test_gpu_paged import banner, check_attention, ints
+from tests.test_gpu_paged8 import check_attention as check_attention8
 from tests.test_gpu_paged_edges import check_lists, lists_of, long_plan
 from tests.test_gpu_tree import check_tree
 
@@ -118,3 +119,29 @@ def test_trees_of_many_sequences(n_seqs):
     sizes[3], sizes[n_seqs // 2], sizes[-1] = 60, 256, 257
     trees = [o8.random_tree(rng, n, 9) for n in sizes]
     check_tree(16, trees, [n + int(rng.integers(0, 30)) for n in sizes], 2, 1, FP16, 16, padding=300)
+
+
+# 240 tiles x heads, and 204: 8 waves a tile, over ranges that are split
+WIDE = [([900, 40, 700], [1800, 2100, 700], 16, 16), ([700, 3, 820, 1], [1500, 2300, 830, 1900], 14, 14)]
+
+
+@pytest.mark.parametrize("q,kv,heads,kv_heads", WIDE)
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+def test_attention_of_8_waves_over_split_ranges(q, kv, heads, kv_heads, dtype):
+    check_attention(q, kv, heads, kv_heads, dtype, 32, padding=3)
+    check_attention8(q, kv, heads, kv_heads, dtype, 32, padding=3)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_trees_of_8_waves_over_split_ranges(bits):
+    past, rng = [1500, 300, 20, 900, 0, 64, 1100, 600], np.random.default_rng(3)
+    check_tree(bits, [o8.random_tree(rng, 100, 6) for _ in past], [100 + p for p in past], 28, 4, BF16, 16)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_trees_that_are_more_than_the_places_of_8_waves(bits):
+    """37 sequences of two tiles of four heads, in ranges that are split and that are not."""
+    for past, count in ((500, 37), (1100, 37)):
+        rng = np.random.default_rng(past)
+        check_tree(bits, [o8.random_tree(rng, 19, 6) for _ in range(count)], [past + 19 + s for s in range(count)], 28, 4,
+                   FP16, 16, width=80)
