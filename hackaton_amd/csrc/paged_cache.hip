@@ -427,13 +427,13 @@ __global__ __launch_bounds__(T) void accept_kernel(PagedAcceptArgs a) {
     for (int w = kTreeWords - 1; w >= 0; --w)
       if (~words[w] != 0) moved = min(kept, 32 * w + __builtin_ctz(~words[w]));
   }
-  if (tid == 0 && o == 0) {
-    const int had = a.lengths[s];
-    a.lengths_out[s] = count == 0 ? had : max(had - count, 0) + kept;
-  }
+  // The place of the first new token as the plan has it: where the rows lie. (`lengths` may count tokens that
+  // the step had no rows for, or that pass the table row.)
+  const int pos0 = count > 0 ? a.plan[a.layout.pos + first] : 0;
+  if (tid == 0 && o == 0) a.lengths_out[s] = count > 0 ? max(pos0 + kept, 0) : a.lengths[s];
   if (!some || chain || moved >= kept || o >= a.outer) return;  // (the same in all threads)
   __syncthreads();
-  const int pos0 = a.plan[a.layout.pos + first], ps = 1 << a.page_shift;
+  const int ps = 1 << a.page_shift;
   if (tid < kept) {  // pages of the path's rows and of their new places
     const int32_t* row = a.table + (long)s * a.width;
     const int from = pos0 + s_path[tid], to = pos0 + tid;

@@ -571,7 +571,8 @@ def paged_accept(pages, plan, lengths, accepted):
     tokens, the new ones included; accepted (sequences) int32: the number of a new token of the sequence,
     anything else: none stays. The rows that stay move together behind the tokens cached before, in order
     and in every layer; rows behind them hold what they held or what moved over them. Returns the lengths
-    (sequences) int32; sequences without new tokens keep theirs. Pages past them are given back by
+    (sequences) int32, up to the last row that stays, by the plan's places (which end with the step's rows and
+    the table row); sequences without rows in the step keep theirs. Pages past them are given back by
     `remap_pages(pages, table, lengths, refs, None, new_lengths)` over the lengths of before the call.
     The call belongs to its step: before the sequences are forked, reordered or stepped again, since it
     follows the page table as it is and moves rows within pages that no other sequence may hold."""

@@ -433,7 +433,8 @@ int va_paged_attention_pages(const va_paged_step* step, const int32_t* tree, con
  * sequence that stays; the ones on its path stay with it and their rows, in every one of the `outer`
  * (keys and values of every layer) x n_pages pages, move together behind the cached rows, in order;
  * anything else: none stays. lengths (n_seqs): the cached tokens, the new ones included; lengths_out
- * those that stay. Rows behind them keep what they held or what moved over them. `pages` as in
+ * those that stay: up to the last such row, by the plan's places; a sequence without rows in the step keeps
+ * its length. Rows behind them keep what they held or what moved over them. `pages` as in
  * va_pages_remap, or 8-bit rows with their exponents (outer, n_pages, kv_heads, page_size). */
 int va_paged_accept(const va_paged_step* step, const int32_t* tree, void* pages, uint8_t* exps,
                     int64_t outer, int32_t n_pages, int32_t kv_heads, int32_t head_dim,
