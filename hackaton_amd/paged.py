@@ -635,27 +635,37 @@ class PagedCache:
         return self.pages if self.exponents is None else QuantizedPages(self.pages, self.exponents)
 
     def _views(self):
-        """(pages, exponents, every layer's keys, its values): the layers as views, made once (made in every call,
-        two to four of them take as long as its kernel's launch)."""
+        """The layers as views, made once (made in every call, two to four of them take as long as its kernel's
+        launch): every layer's keys, its values, and what they are views of, with the memory it was set to."""
         def views(which):
             codes = [self.pages[layer, which] for layer in range(self.pages.shape[0])]
             if self.exponents is None:
                 return codes
             return [QuantizedPages(x, self.exponents[layer, which]) for layer, x in enumerate(codes)]
 
-        return self.pages, self.exponents, views(0), views(1)
+        held = [t if t is None else (t, t.detach(), t.dtype) for t in (self.pages, self.exponents)]
+        return views(0), views(1), *held
 
     def _layer(self, layer, which):
         held = self._held
-        if held[0] is not self.pages or held[1] is not self.exponents:  # (the program has set others)
+        pages, as_set, dtype = held[2]
+        # (the program has set other pages, or the same tensor to other memory, sizes or another type)
+        if pages is not self.pages or not pages.is_set_to(as_set) or pages.dtype is not dtype:
             held = self._held = self._views()
+        elif held[3] is None:
+            if self.exponents is not None:
+                held = self._held = self._views()
+        else:
+            exponents, as_set, dtype = held[3]
+            if exponents is not self.exponents or not exponents.is_set_to(as_set) or exponents.dtype is not dtype:
+                held = self._held = self._views()
         return held[which][layer]
 
     def keys(self, layer):
-        return self._layer(layer, 2)
+        return self._layer(layer, 0)
 
     def values(self, layer):
-        return self._layer(layer, 3)
+        return self._layer(layer, 1)
 
     def _slots(self, values, fill):
         """One int32 per slot: a device tensor as it is, or `fill` with a host dict's entries."""
