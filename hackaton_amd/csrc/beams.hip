@@ -112,8 +112,10 @@ __device__ inline float wave_max_last(float x) {
 // differences of numbers are taken first. kLog2e, rounded, stands for the base: the second kernel
 // divides by it, so a shift of all numbers shifts the result.
 __device__ inline bool far_out(float largest) { return fabsf(largest) >= 65536.f; }
-// Power of two by which a sum over the reference of `was` has to be multiplied for that of `is`.
+// Power of two by which a sum over the reference of `was` has to be multiplied for that of `is`. (References are
+// the rounded products: their difference may not become a multiply-add of an unrounded one.)
 __device__ inline float rescale(float was, float is) {
+#pragma clang fp contract(off)
   const float a = was * kLog2e, b = is * kLog2e;
   const float d = far_out(is) ? (far_out(was) ? (was - is) * kLog2e : __builtin_fmaf(-is, kLog2e, a))
                               : (far_out(was) ? __builtin_fmaf(was, kLog2e, -b) : a - b);
