@@ -14,17 +14,24 @@
 //
 // Both copy pages straight from memory into LDS (16 rows of a page per wave and step, so a page border
 // never falls into a copy), rows past the end of the range as zeros: what earlier sequences left in a
-// page is never read. S^T = K Q^T has one row's scores in a lane and its half-wave partner; O^T += V^T
+// page is not read (in 8-bit pages it may be, see below). S^T = K Q^T has one row's scores in a lane and its half-wave partner; O^T += V^T
 // P^T reads V^T from the row-major tile with transposed LDS reads. A tile's rows are stored in groups of
 // 4 (1 KB, one copy instruction) 1088 bytes apart, chunk c of row r at c ^ (r & 3), so that both reads
 // touch all banks.
 //
-// 8-bit pages: an e4m3 number times a power of two is a 16-bit number exactly (four significant bits), so
+// 8-bit pages: an e4m3 number times a power of two is a 16-bit number exactly (four significant bits), in fp16 but
+// for its range: past 65504 it is infinite, and below 2^-14 it is rounded to a multiple of 2^-24 (rows of
+// numbers around 10^-4 lose digits of their smaller ones, rows around 10^-6 keep a few steps). So
 // rows are turned into 16-bit ones on the way, two numbers and their power by one instruction, and the
 // products are those of 16-bit pages. Copies go through registers: a wave turns its share of a tile into
 // LDS rows while the next tile's loads are in flight. Few rows take keys as the matrix operand straight
 // from memory (a lane holds a key's numbers in memory's order, the queries follow it) and only the values,
 // which the product needs transposed, through LDS.
+// Few rows load whole tiles of 32 keys and their exponents without bounds: bytes behind the range's end, of page 0
+// where there is no page, and one tile more behind the last. All lie in the pool (a pool without pages takes
+// another path), and none counts: the scores of keys behind the end are replaced by the mask, codes of missing pages
+// by zeros, values behind the end read as zeros by the descriptor, and an exponent byte of 255 stands for a
+// finite power, so that zero times it is zero.
 //
 // Trees of new tokens: the tiles that reach past the cached rows read, for every row, the bits of the
 // tokens on its path (tree_paths) instead of comparing places.

@@ -40,7 +40,8 @@ class QuantizedPages(NamedTuple):
     (..., n_pages, kv_heads, page_size) float8_e8m0fnu. A row's values are its codes times its power of
     two, the smallest from 2^-100 on that brings the row's largest finite number to 448 or less; numbers
     are rounded once, to nearest even, and what is not finite is held as not a number. A row takes 129
-    bytes instead of 256. One layer's keys or values for `paged_append` and `paged_attention`, the whole
+    bytes instead of 256. (`paged_append` writes exponent bytes of 27 to 247. Rows that a program writes itself
+    may have 1 to 254: 0 and 255, 2^-127 and not a number to `dequantize`, mean nothing to the attention.) One layer's keys or values for `paged_append` and `paged_attention`, the whole
     pool (layers, 2, ...) for the page bookkeeping."""
 
     codes: torch.Tensor
@@ -404,14 +405,14 @@ def paged_attention(query, k_pages, v_pages, plan, scale):
     """Every new token attends to its sequence's keys at positions up to its own. query
     (n_tokens, heads, 128) in the pages' type; returns (n_tokens, heads * 128), zeros for padding and
     for rows that see no key. Key/value heads are shared by heads / kv_heads query heads each. What a
-    page holds behind its sequence's end is never read. (Keys that a row does not see never reach it,
+    page holds behind its sequence's end never reaches a result. (Keys that a row does not see never reach it,
     whatever they hold. Values that are infinite or not a number do where they lie in a 64-key tile that
     another of the 32 rows computed together sees, rows being pairs of a token and a query head of the
     group: in rows of the same sequence up to 63 + ceil(31 kv_heads / heads) positions before their own;
     with a tree, places before or behind it: rows that do not see each other share tiles.)
     The same step gives the same bits; the same sequence in another step agrees to rounding. Pages may be
     `QuantizedPages`, under queries in fp16 or bf16: their values are multiplied as numbers of that type,
-    exactly but for what passes fp16's range."""
+    exactly but for fp16's range: past 65504 they are infinite, below 2^-14 multiples of 2^-24."""
     (keys, k_exps), (values, v_exps) = _split(k_pages), _split(v_pages)
     device = _one_device(query, keys, values, plan.words)
     if device.index != _current_device():  # launches and allocations go to the tensors' device

@@ -390,7 +390,8 @@ int va_pages_compact(void* pages, int64_t outer, int32_t n_pages, int32_t kv_hea
  * exponent byte e beside it in (n_pages, Hkv, page_size) bytes, k_exp_stride / v_exp_stride apart
  * (at least Hkv page_size, under 2^31): the row's values are its numbers times 2^(e - 127). e is the smallest
  * from 27 on that brings the row's largest finite number to 448 or less; what is not finite is held as
- * not a number. Strides are in elements (multiples of 8; of 16 for VA_E4M3).
+ * not a number. (Rows that a program writes itself may have e from 1 to 254; 0 and 255 mean nothing to the
+ * attention.) Strides are in elements (multiples of 8; of 16 for VA_E4M3).
  * `tree` is NULL (the new tokens of every sequence follow each other) or what va_paged_plan_tree wrote beside
  * the plan: va_paged_tree_words int32 of device memory, 16-byte aligned.
  * parents (n_tokens): of every row the number, among the new tokens of its sequence, of the one that it
@@ -423,7 +424,8 @@ int va_paged_append_pages(const va_paged_step* step, const int32_t* tree, const 
                           int32_t in_dtype, int32_t out_dtype, void* stream);
 
 /* va_paged_attention over pages of either kind; dtype is that of q and out (that of 16-bit pages). 8-bit
- * rows are multiplied as 16-bit numbers of that type: exactly, but for what passes VA_F16's range. */
+ * rows are multiplied as 16-bit numbers of that type: exactly, but for VA_F16's range (past 65504 they are
+ * infinite, below 2^-14 they are rounded to multiples of 2^-24). */
 int va_paged_attention_pages(const va_paged_step* step, const int32_t* tree, const void* q,
                              const va_paged_pages* pages, int32_t head_dim, float scale,
                              int32_t dtype, void* out, void* workspace, int64_t workspace_bytes,
