@@ -33,11 +33,14 @@ def select_beams(logits, scores, beams, count=None, ended=None, end_token=None):
     (g + 1) * beams - 1 are the beams (at most 64) of prompt g. scores (rows) fp32: the beams' sums of log
     probabilities so far (-inf: a beam that is not used yet). A continuation's score is its beam's plus
     the token's log softmax, formed and compared in 64 bits (the row's exponentials are summed in 32 by
-    every wave of a work-group, in 64 over them); what is not a number counts as -inf.
+    every wave of a work-group, in 64 over them); what is not a number counts as -inf. Tokens that are not allowed
+    are best masked with -inf: beside numbers past some 10^10 the logarithm of the sum loses digits, and a row
+    that holds nothing but fp32's or bf16's lowest number scores as its beam, for every token.
 
     Returns (scores (prompts, count) fp32, parents (prompts, count) int32: the row that each goes on from,
     tokens (prompts, count) int32), the best first, ties to the lowest row and token: the order of a
-    stable sort of all continuations. ended (rows) bool: beams that have ended; their logits are not read,
+    stable sort of all continuations, but for those of rows that differ whose scores are within the error of the rows'
+    sums (2.1e-5 at most at 32,000 tokens, 1.3e-4 at 2^18, both rows together). ended (rows) bool: beams that have ended; their logits are not read,
     they go on with `end_token` at their score, and at -inf with every other token. Nothing is read back,
     so a captured step follows its inputs. No backward: a choice has none, and the scores' is refused."""
     device = logits.device

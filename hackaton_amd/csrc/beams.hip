@@ -7,13 +7,16 @@
 // each of those cells would hold a better one, or one as good of a lower number, since cells are runs of
 // numbers in order. So a second kernel, a work-group per prompt, picks the best cells from their largest
 // numbers, and the best numbers in them. Scores are formed and compared in 64 bits, score + (number - log
-// of the sum): a rounding to 32 would make ties of continuations that are not as good.
+// of the sum): a rounding to 32 would make ties of continuations that are not as good. The sum itself is off by
+// what a wave's additions in fp32 lose, (8 ceil(vocab / 2048) + 48) 2^-24 of it at most: the order is exact within a
+// row and between rows of the same numbers; continuations of other rows whose scores are closer than twice that may
+// change places.
 //
 // The first kernel is bounded by memory, and for 16-bit numbers nearly as much by its arithmetic (a
 // power of two, 16 cycles of a wave, and six other instructions a number): 512 rows of 150,016 numbers
 // (154 MB) 34 us, 4.6 TB/s; of 75,008 fp32 numbers, as many bytes, 30 us. 1, 2 and 4 pieces on their
-// way and 1024 to 8192 work-groups measured 34 to 47. The second kernel is bounded by the latency of its dozen
-// steps between barriers, some 0.45 us each, and of its first loads (1.7 and 1.1): 8.2 us for a prompt of four
+// way and 1024 to 8192 work-groups measured 34 to 47. The second kernel is, for ordinary logits and counts of 16 or
+// so (see select), bounded by the latency of its dozen steps between barriers, some 0.45 us each, and of its first loads (1.7 and 1.1): 8.2 us for a prompt of four
 // beams, 10.2 us for 64 of eight (with scores compared as whole numbers and ranks added up in LDS 8.8 and
 // 11.2; with 256 threads 13.8 and 33.7; with one copy of the code for all picks 8.9 and 12.8).
 #include <climits>
@@ -293,8 +296,13 @@ __device__ inline int count_before(const Pick* v, int n, const Pick& mine) {
 // are. Each group of 16 threads brings its best one; the count-th best of those 64 is a bound that `count`
 // candidates reach, and only those of the groups whose best reaches it: at most 16 E count (and not more
 // than there are; the callers see to it that kPool is no less). They are then put in order by counting who
-// comes before. (A pool of more than 64 is slow, but takes scores whose best ones all lie with one
-// thread.) Sums over 16 lanes stay in registers.
+// comes before, n^2 reads of LDS for a pool of n. Ordinary logits leave little more than `count`. Where the count-th
+// best group's best is -infinity, or equal to others, order goes by number alone and whole groups pass: 129, 516 and
+// 1032 candidates where all beams of a prompt have ended, at 1 beam and count 2, 4 and 8, 8 and 16; counts near the
+// 64 groups have a bound that many pass in any case. A work-group is then as slow as its pool (us a call of 32,000
+// fp16 numbers a row, ordinary / a prompt all of whose beams have ended / equal logits / 10 allowed tokens): 64 prompts
+// of 4 beams, count 8, 15.9 / 43 / 94 / 45, of 8, count 16, 20 / 119 / 353 / 130; 16 of 32, count 64, 135 / 241 / 244 /
+// 249, and 1164 where every other beam has ended. Sums over 16 lanes stay in registers.
 template <int E>
 __device__ inline int select(Picks& s, int count, const double (&score)[E], const int (&index)[E]) {
   const int tid = threadIdx.x, group = tid >> 4;

@@ -465,7 +465,11 @@ int va_pages_compact8(void* pages, uint8_t* exps, int64_t outer, int32_t n_pages
  * -infinity. Outputs (groups, count), best first, ties to the lowest row and token: scores, rows that they
  * continue (among all rows) and tokens. ended (a byte per row, may be NULL): rows that are not 0 have
  * ended; their logits are not read, they go on with end_token at their score, and as -infinity with every
- * other token. The order is that of a full sort of all continuations. Deterministic. Workspace:
+ * other token. The order is that of a full sort of all continuations, exactly within a row and between rows of
+ * the same numbers; a row's exponentials are added in fp32 by every wave, so that its sum is off by
+ * (8 ceil(vocab / 2048) + 48) 2^-24 of it at most, and continuations of other rows whose scores are closer than
+ * twice that may change places. A row of nothing but fp32's or bf16's lowest number scores as its beam (its sum's
+ * logarithm vanishes beside it in 64 bits): what is not allowed is -infinity. Deterministic. Workspace:
  * va_select_beams_workspace bytes, 16-byte aligned; calls that may overlap need one each. No counterpart in
  * the reference (its generation goes through transformers). */
 int va_select_beams_workspace(int64_t groups, int32_t beams, int32_t vocab, int64_t* bytes);
