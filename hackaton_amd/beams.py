@@ -40,9 +40,9 @@ def select_beams(logits, scores, beams, count=None, ended=None, end_token=None):
     Returns (scores (prompts, count) fp32, parents (prompts, count) int32: the row that each goes on from,
     tokens (prompts, count) int32), the best first, ties to the lowest row and token: the order of a
     stable sort of all continuations, but for those of rows that differ whose scores are within the error of the rows'
-    sums (2.1e-5 at most at 32,000 tokens, 1.3e-4 at 2^18, both rows together). ended (rows) bool: beams that have ended; their logits are not read,
-    they go on with `end_token` at their score, and at -inf with every other token. Nothing is read back,
-    so a captured step follows its inputs. No backward: a choice has none, and the scores' is refused."""
+    sums (2.1e-5 at most at 32,000 tokens, 1.3e-4 at 2^18, both rows together). ended (rows) bool: beams
+    that have ended; their logits are not read, they go on with `end_token` at their score, and at -inf with
+    every other token. Nothing is read back, so a captured step follows its inputs. No backward: a choice has none, and the scores' is refused."""
     device = logits.device
     if not logits.is_cuda:
         raise ValueError(f"the selection runs on the GPU only: got a tensor on {device}")

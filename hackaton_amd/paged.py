@@ -41,7 +41,8 @@ class QuantizedPages(NamedTuple):
     two, the smallest from 2^-100 on that brings the row's largest finite number to 448 or less; numbers
     are rounded once, to nearest even, and what is not finite is held as not a number. A row takes 129
     bytes instead of 256. (`paged_append` writes exponent bytes of 27 to 247. Rows that a program writes itself
-    may have 1 to 254: 0 and 255, 2^-127 and not a number to `dequantize`, mean nothing to the attention.) One layer's keys or values for `paged_append` and `paged_attention`, the whole
+    may have 1 to 254: 0 and 255, 2^-127 and not a number to `dequantize`, mean nothing to the attention.)
+    One layer's keys or values for `paged_append` and `paged_attention`, the whole
     pool (layers, 2, ...) for the page bookkeeping."""
 
     codes: torch.Tensor
